@@ -8,11 +8,12 @@ group of consecutive input features):
 * ``moe``     a mixture-of-experts layer for a few tokens: router, the k best
               experts of each token, their gated feed-forward, weighted sum
 
-The format: ``W[n, k] = code[n, k] * scale[n, k // group]``; a code is held as
-``code + 8`` in 4 bits, eight in a 32-bit word in the order of input features
-0, 2, 4, 6, 1, 3, 5, 7 from the lowest bits; a row is padded to a multiple of 32
-features with code 0; scales are bf16 with at most five significant bits, so
-that ``code * scale`` is a bf16 number.
+The format: ``W[n, k] = code[n, k] * scale[n, k // group]``; a row is padded with
+zeros to a multiple of 128 features.  A code is held as ``code + 8`` in 4 bits,
+eight in a 32-bit word in the order of features 0, 2, 4, 6, 1, 3, 5, 7 from the
+lowest bits.  Of the 16 words of 128 features, word 4 a + b holds the eight
+features from 32 b + 8 a on.  Scales are bf16 with at most five significant
+bits, so that ``code * scale`` is a bf16 number.
 """
 
 import math
@@ -97,40 +98,41 @@ def _round5(s):
     return b.view(torch.float32)
 
 
-def _pad_last(x, to):
-    return torch.nn.functional.pad(x, (0, to - x.shape[-1]))
+def _padded(k):
+    return -(-k // 128) * 128
 
 
 def _groups(w, group):
-    """[..., k] -> [..., ceil(k / group), group], zeros behind the end."""
-    n = -(-w.shape[-1] // group)
-    return _pad_last(w, n * group).unflatten(-1, (n, group))
+    """[..., k] -> [..., padded k / group, group], zeros behind the end."""
+    k = w.shape[-1]
+    if k % 128:
+        w = torch.nn.functional.pad(w, (0, _padded(k) - k))
+    return w.unflatten(-1, (-1, group))
 
 
 def _quantise(w, group, wide=torch.float64):
-    """fp32 weight -> codes as whole numbers [..., k] and fp32 scales; the quotients in `wide`."""
+    """fp32 weight -> codes as whole numbers [..., padded k] and fp32 scales; the quotients in `wide`."""
     g = _groups(w, group)
     amax = g.abs().amax(-1)
     s = _round5(amax / 7).clamp_min(_SCALE_MIN)
     c = torch.round(g.to(wide) / s.unsqueeze(-1).to(wide)).clamp(-7, 7)
-    return c.to(torch.int8).flatten(-2)[..., : w.shape[-1]], s
+    return c.to(torch.int8).flatten(-2), s
 
 
 def _pack(codes):
-    k = codes.shape[-1]
-    u = _pad_last(codes, -(-k // 32) * 32).add(8).to(torch.uint8)
-    u = u.unflatten(-1, (-1, 4, 2)).transpose(-1, -2).flatten(-2)  # nibbles of each word, lowest first
-    return (u[..., 0::2] | (u[..., 1::2] << 4)).flatten(-2)
+    u = codes.add(8).to(torch.uint8).unflatten(-1, (-1, 4, 4, 4, 2))  # [block, b, a, pair, odd]
+    u = u.transpose(-4, -3).transpose(-2, -1).flatten(-5)  # [block, a, b, odd, pair]: nibbles, lowest first
+    return u[..., 0::2] | (u[..., 1::2] << 4)
 
 
-def _unpack(q, k):
-    nib = torch.stack((q & 15, q >> 4), -1).flatten(-2)
-    return nib.unflatten(-1, (-1, 2, 4)).transpose(-1, -2).flatten(-3)[..., :k].to(torch.int8) - 8
+def _unpack(q):
+    nib = torch.stack((q & 15, q >> 4), -1).flatten(-2).unflatten(-1, (-1, 4, 4, 2, 4))
+    return nib.transpose(-4, -3).transpose(-2, -1).flatten(-5).to(torch.int8) - 8
 
 
 def _values(q, s, k, group, dtype):
     """The weight that codes and scales stand for, as `dtype`."""
-    g = _groups(_unpack(q, k).to(dtype), group) * s.to(dtype).unsqueeze(-1)
+    g = _unpack(q).to(dtype).unflatten(-1, (-1, group)) * s.to(dtype).unsqueeze(-1)
     return g.flatten(-2)[..., :k]
 
 
@@ -184,7 +186,7 @@ def prepare(case, seed):
 def _plain_quant(st):
     c = st["case"]
     codes, s = _quantise(st["w"].float(), c["group"])
-    g = _groups(codes.float(), c["group"]) * s.unsqueeze(-1)
+    g = codes.float().unflatten(-1, (-1, c["group"])) * s.unsqueeze(-1)
     return dict(scale=s.to(torch.bfloat16), values=g.flatten(-2)[..., : c["k"]].to(st["w"].dtype))
 
 
@@ -256,7 +258,7 @@ def run(state):
 
 # ------------------------------------------------------------------- work
 def _weight_bytes(rows, k, group):
-    return rows * (-(-k // 32) * 16 + 2 * -(-k // group))
+    return rows * _padded(k) // 2 + rows * 2 * (_padded(k) // group)
 
 
 def work(case):
@@ -276,14 +278,14 @@ def work(case):
 
 # ------------------------------------------------------------------ exact
 def _exact_values(q, s, k, group):
-    """The weight in fp64, from the format's definition: one word of eight codes at a time."""
-    words = q.contiguous().view(torch.int32)
-    order = (0, 2, 4, 6, 1, 3, 5, 7)
-    w = torch.empty(*words.shape, 8, dtype=torch.float64, device=q.device)
-    for nibble, feature in enumerate(order):
-        w[..., feature] = ((words >> (4 * nibble)) & 15).double() - 8.0
-    w = w.flatten(-2)[..., :k]
-    return w * s.double().repeat_interleave(group, dim=-1)[..., :k]
+    """The weight in fp64, from the format's definition: one nibble of one word of each block at a time."""
+    words = q.contiguous().view(torch.int32).unflatten(-1, (-1, 16))
+    w = torch.empty(*words.shape[:-1], 128, dtype=torch.float64, device=q.device)
+    for word in range(16):
+        first = 32 * (word % 4) + 8 * (word // 4)
+        for nibble, feature in enumerate((0, 2, 4, 6, 1, 3, 5, 7)):
+            w[..., first + feature] = ((words[..., word] >> (4 * nibble)) & 15).double() - 8.0
+    return (w.flatten(-2) * s.double().repeat_interleave(group, dim=-1))[..., :k]
 
 
 def exact(case, seed):
@@ -292,8 +294,8 @@ def exact(case, seed):
     if case["op"] == "quant":
         w = st["w"].double()
         n, k = w.shape
-        scale = torch.zeros(n, -(-k // group), dtype=torch.float64, device=w.device)
-        for j in range(scale.shape[1]):
+        scale = torch.zeros(n, _padded(k) // group, dtype=torch.float64, device=w.device)
+        for j in range(-(-k // group)):
             scale[:, j] = w[:, j * group:(j + 1) * group].abs().amax(1) / 7.0
         mant, exp = torch.frexp(scale)
         scale = torch.ldexp(torch.round(mant * 32.0) / 32.0, exp).clamp_min(_SCALE_MIN)  # torch.round: ties to even
