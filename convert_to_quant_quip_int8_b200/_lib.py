@@ -34,7 +34,7 @@ QI8_Q_TOKEN, QI8_Q_BLOCK, QI8_Q_GELU = 0, 1, 0x100
 QI8_S_NONE, QI8_S_SCALAR, QI8_S_ROW, QI8_S_ROW_KBLOCK, QI8_S_TILE128 = 0, 1, 2, 3, 4
 QI8_MAX_PEERS = 8
 # epilogue activation
-QI8_ACT_NONE, QI8_ACT_GELU = 0, 1
+QI8_ACT_NONE, QI8_ACT_GELU, QI8_ACT_SILU = 0, 1, 2
 # weight requant schemes
 QI8_REQ_ROW, QI8_REQ_GLOBAL, QI8_REQ_BLOCK = 0, 1, 2
 
@@ -85,6 +85,12 @@ SIGNATURES = {
     "qi8_ipc_open": (_I, [_P, _I64, ctypes.POINTER(_P)]),
     "qi8_ipc_close": (_I, [_P, _I64]),
     "qi8_peer_barrier": (_I, [_P, _I, _I, _P]),
+    "qi8_quant_weight_i4": (_I, [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P]),
+    "qi8_dequant_i4": (_I, [_P, _P, _I64, _I64, _I, _P, _I, _I64, _P]),
+    "qi8_gemm_w4": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _I, _P, _I, _P, _I, _I64, _P]),
+    "qi8_moe_w4_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I]),
+    "qi8_moe_w4": (_I, [_P, _I, _I64, _I64, _I64, _P, _I, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _I, _P, _I64,
+                        _P, _I64, _P]),
 }
 
 _lib = None

@@ -17,6 +17,7 @@ dispatch order.  Differences, all on the hot path:
   layout;
 * ``QuIPHadamardINT8Layout`` (new) consumes transformed-space checkpoints
   (``sign_row`` / ``sign_col`` / ``hadamard_size_*``) as a W8A8 linear;
+* ``GroupWiseINT4Layout`` (new) holds weights of 4 bits with group scales;
 * ``F.linear`` reaches the linear handlers through ``__torch_function__``
   (in the reference it decomposes into ``t`` + ``mm`` before dispatch).
 """
@@ -373,6 +374,30 @@ class QuIPHadamardINT8Layout(QuantizedLayout):
         return qtensor._qdata, p["scale"], p["sign_row"], p["sign_col"]
 
 
+class GroupWiseINT4Layout(QuantizedLayout):
+    """Weight [..., N, K] of 4-bit codes with one bf16 scale per (row, group of
+    ``group_size`` input features); no counterpart in the reference.  ``_qdata``
+    is the packed uint8 [..., N, Kp/2].  ``linear`` keeps the activations in
+    bf16 / fp16 and is meant for single tokens (see int4_kernels)."""
+
+    @classmethod
+    def quantize(cls, tensor, scale=None, group_size=128, **kwargs):
+        if scale is not None:
+            raise NotImplementedError("static (pre-computed) group scales are not supported")
+        qdata, scale = ops.quant_weight_i4(tensor, group_size)
+        return qdata, {"scale": scale, "group_size": group_size, "in_features": tensor.shape[-1],
+                       "orig_dtype": tensor.dtype}
+
+    @staticmethod
+    def dequantize(qdata, scale, group_size, in_features, orig_dtype, **kwargs):
+        return ops.dequant_i4(qdata, scale, in_features, group_size, orig_dtype)
+
+    @classmethod
+    def get_plain_tensors(cls, qtensor):
+        p = qtensor._layout_params
+        return qtensor._qdata, p["scale"], p["group_size"], p["in_features"]
+
+
 QUANT_ALGOS = {
     "int8_blockwise": {
         "storage_t": torch.int8,
@@ -382,6 +407,14 @@ QUANT_ALGOS = {
         "group_size": 128,
         "asymmetric_layout": True,
     },
+    "int4_groupwise": {
+        "storage_t": torch.uint8,
+        "required_parameters": {"weight_scale"},
+        "optional_parameters": set(),
+        "comfy_tensor_layout": "GroupWiseINT4Layout",
+        "group_size": 128,
+        "asymmetric_layout": False,
+    },
 }
 
 LAYOUTS = {
@@ -389,6 +422,7 @@ LAYOUTS = {
     "TensorWiseINT8Layout": TensorWiseINT8Layout,
     "AxisWiseINT8Layout": AxisWiseINT8Layout,
     "QuIPHadamardINT8Layout": QuIPHadamardINT8Layout,
+    "GroupWiseINT4Layout": GroupWiseINT4Layout,
 }
 
 
@@ -563,6 +597,18 @@ def quip_hadamard_linear(func, args, kwargs):
     y_had = ops.gemm_i8(xq, q, xs, L.QI8_S_ROW, scale.reshape(-1), L.QI8_S_ROW, None, torch.float32)
     y = ops.unrotate_rows(y_had, s_u, N, bias, x.dtype)
     return y.reshape(*x.shape[:-1], N)
+
+
+@register_layout_op(torch.ops.aten.linear.default, "GroupWiseINT4Layout")
+def int4_linear(func, args, kwargs):
+    """4-bit weight, 16-bit activations: ``x W^T + bias`` with fp32 sums."""
+    x, weight = args[0], args[1]
+    bias = args[2] if len(args) > 2 else kwargs.get("bias")
+    if not isinstance(weight, QuantizedTensor) or isinstance(x, QuantizedTensor):
+        return QuantizedTensor._dequant_and_fallback(func, args, kwargs)
+    q, scale, group_size, in_features = GroupWiseINT4Layout.get_plain_tensors(weight)
+    assert x.shape[-1] == in_features, f"input has {x.shape[-1]} features, weight expects {in_features}"
+    return ops.gemm_w4(x, q, scale, group_size, bias)
 
 
 def quip_hadamard_weight(q_rot: torch.Tensor, scale: torch.Tensor, sign_row: torch.Tensor, sign_col: torch.Tensor,

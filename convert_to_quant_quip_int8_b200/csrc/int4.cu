@@ -1,0 +1,403 @@
+// Weights of 4 bits with group scales (format: int4.cuh): quantization,
+// dequantization and the linear layer of a few tokens.
+//
+//   scale = max(round5(amax(|w| over the group) / 7), 2^-100)
+//   code  = rint(w / scale), ties to even, in [-7, 7]
+//
+// round5 keeps five significant bits (ties to even): a code has three, so
+// code * scale is exact in bf16 and every product downstream multiplies the
+// weight that dequantization reports.  The scale is at most 1/32 off amax / 7,
+// which leaves |w| / scale < 7.25: no code is clipped by more than a quarter
+// step.  A group that holds an infinity or a NaN gets scale NaN and code 0, so
+// it reads back as NaN as a whole.
+#include <cstdint>
+#include <type_traits>
+
+#include "common.cuh"
+#include "int4.cuh"
+
+namespace qi8 {
+namespace {
+
+// ------------------------------------------------------------ quantization
+// One thread per word of eight features, groups of 4, 8 or 16 neighbouring
+// lanes.  Threads walk the words of the whole matrix in memory order of w; the
+// (row, word) pair advances by a constant step without a division.
+constexpr int Q_THREADS = 256;
+
+struct Walk {
+  int64_t row;
+  int word;  // of the row, in feature order
+  int64_t step_row;
+  int step_word;
+  int words;  // per row
+  __device__ __forceinline__ Walk(int64_t at, int64_t step, int words_) : words(words_) {
+    row = at / words;
+    word = (int)(at - row * words);
+    step_row = step / words;
+    step_word = (int)(step - step_row * words);
+  }
+  __device__ __forceinline__ void advance() {
+    row += step_row;
+    word += step_word;
+    if (word >= words) {
+      word -= words;
+      ++row;
+    }
+  }
+};
+
+// Position inside the row's words of the word that starts at feature 8 j.
+__device__ __forceinline__ int word_slot(int j) {
+  return (j & ~15) | ((j & 3) << 2) | ((j >> 2) & 3);
+}
+
+template <typename T, bool VEC>
+__device__ __forceinline__ void load8(const T* row, int k, int K, float (&v)[8]) {
+  if constexpr (sizeof(T) == 4) {
+    if (VEC && k + 8 <= K) {
+      const float4 a = __ldg(reinterpret_cast<const float4*>(row + k));
+      const float4 b = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
+      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+      return;
+    }
+  } else if (VEC && k + 8 <= K) {
+    const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + k));
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const T lo = reinterpret_cast<const T*>(&w[i])[0], hi = reinterpret_cast<const T*>(&w[i])[1];
+      v[2 * i] = Elem<T>::to_f32(lo);
+      v[2 * i + 1] = Elem<T>::to_f32(hi);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? Elem<T>::to_f32(row[k + i]) : 0.0f;
+}
+
+// Positive finite fp32 to five significant bits, ties to even.
+__device__ __forceinline__ float round5(float s) {
+  uint32_t b = __float_as_uint(s);
+  b = (b + 0x3FFFFu + ((b >> 19) & 1u)) & ~0x7FFFFu;
+  return __uint_as_float(b);
+}
+
+// rint(w / s) + 8 for |w / s| < 7.5, ties to even, in the low nibble.
+// q = w * (1 / s) is off by less than 2^-21.  For 16-bit weights a quotient
+// that is no tie is at least 2^-13 away from one (numerator and denominator
+// have 11 and 5 bits), so rounding q to multiples of 2^-17 first -- adding 96,
+// where that is the spacing of fp32 -- restores exact ties and moves nothing
+// across one.  fp32 weights compare the remainder, which fma leaves exact.
+template <typename T>
+__device__ __forceinline__ uint32_t code_bits(float w, float s, float inv) {
+  if constexpr (sizeof(T) == 2) {
+    const float t = fmaf(w, inv, 96.0f);
+    return __float_as_uint(__fadd_rn(t, 12582912.0f - 96.0f + 8.0f));
+  } else {
+    float q = rintf(w * inv);
+    const float e = fmaf(-q, s, w), h = 0.5f * s, a = fabsf(e);
+    if (a > h || (a == h && ((int)q & 1))) q += e > 0.0f ? 1.0f : -1.0f;
+    return (uint32_t)((int)q + 8);
+  }
+}
+
+template <typename T, int G, bool VEC>
+__global__ void __launch_bounds__(Q_THREADS)
+quant_i4_kernel(const T* __restrict__ w, int64_t ld, int64_t rows, int K, int Kp, uint32_t* __restrict__ q,
+                __nv_bfloat16* __restrict__ scale) {
+  constexpr int LANES = G / 8;  // of a group
+  const int words = Kp / 8;
+  // rows * words is a multiple of 16: a group's lanes are all in or all out
+  for (Walk at((int64_t)blockIdx.x * Q_THREADS + threadIdx.x, (int64_t)gridDim.x * Q_THREADS, words); ;
+       at.advance()) {
+    const bool in = at.row < rows;
+    if (!__any_sync(0xffffffffu, in)) break;
+    float v[8];
+    if (in) load8<T, VEC>(w + at.row * ld, at.word * 8, K, v);
+    else
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
+    uint32_t m = 0;  // as bits: NaN counts above infinity
+#pragma unroll
+    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
+#pragma unroll
+    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+    const bool finite = m < 0x7f800000u;
+    const float s = fmaxf(round5(__fdiv_rn(__uint_as_float(finite ? m : 0u), 7.0f)), 0x1p-100f);
+    const float inv = __frcp_rn(s);
+    uint32_t word = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      // nibble order 0, 2, 4, 6, 1, 3, 5, 7
+      const uint32_t u = code_bits<T>(v[i], s, inv) & 15u;
+      word |= u << (4 * ((i >> 1) + 4 * (i & 1)));
+    }
+    if (in) {
+      q[at.row * words + word_slot(at.word)] = finite ? word : 0x88888888u;
+      if ((at.word & (LANES - 1)) == 0)
+        scale[at.row * (Kp / G) + at.word / LANES] =
+            finite ? __float2bfloat16_rn(s) : __ushort_as_bfloat16((unsigned short)0x7fffu);
+    }
+  }
+}
+
+// ---------------------------------------------------------- dequantization
+template <typename T, int G, bool VEC>
+__global__ void __launch_bounds__(Q_THREADS)
+dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restrict__ scale, int64_t rows, int K, int Kp,
+                  T* __restrict__ out, int64_t ld) {
+  const int words = Kp / 8;
+  for (Walk at((int64_t)blockIdx.x * Q_THREADS + threadIdx.x, (int64_t)gridDim.x * Q_THREADS, words);
+       at.row < rows; at.advance()) {
+    const int k = at.word * 8;
+    if (k >= K) continue;
+    const uint32_t w = __ldg(q + at.row * words + word_slot(at.word));
+    const float s = __bfloat162float(scale[at.row * (Kp / G) + k / G]);
+    T* o = out + at.row * ld + k;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const uint32_t u = (w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u;
+      v[i] = (__uint_as_float(0x4B000000u | u) - 8388616.0f) * s;  // 2^23 + u - (2^23 + 8)
+    }
+    if (VEC && k + 8 <= K) {
+      if constexpr (sizeof(T) == 4) {
+        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+      } else {
+        alignas(16) T h[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) h[i] = Elem<T>::from_f32(v[i]);
+        *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(h);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (k + i < K) o[i] = Elem<T>::from_f32(v[i]);
+    }
+  }
+}
+
+// ------------------------------------------------- linear, a few tokens
+// y[t, n] = sum_k W[n, k] x[t, k] + bias[n] for up to 8 NT tokens a block.
+// Bound by the weight's bytes: each block takes 16 MT weight rows, its warps
+// the 128-feature blocks in turn, and the MMAs (m16n8k16, tokens as the 8
+// columns) keep the arithmetic per weight at the unpacking alone.  fp32 sums
+// per warp, joined in shared memory in the order of the warps.
+constexpr int LIN_WARPS = 8;
+
+struct LinArgs {
+  const uint16_t* x;
+  int64_t ld_x;
+  const uint8_t* q;
+  const __nv_bfloat16* scale;
+  const void* bias;
+  int bias_dtype;
+  void* out;
+  int64_t ld_out;
+  int out_dtype;
+  int M, N, K, KB;  // KB = Kp / 128
+};
+
+template <typename T, int G, int MT, int NT, bool VEC>
+__global__ void __launch_bounds__(LIN_WARPS * 32)
+w4_rows_kernel(const LinArgs p) {
+  __shared__ float red[LIN_WARPS][8 * NT][16 * MT + 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, a = lane & 3;
+  const int n0 = blockIdx.x * 16 * MT;
+  const int t0 = blockIdx.y * 8 * NT;
+
+  const uint8_t* q[2 * MT];
+  const __nv_bfloat16* sc[2 * MT];
+#pragma unroll
+  for (int r = 0; r < 2 * MT; ++r) {
+    const int n = min(n0 + (r >> 1) * 16 + (r & 1) * 8 + g, p.N - 1);  // rows past the end are read as the last
+    q[r] = p.q + (int64_t)n * p.KB * 64 + a * 16;
+    sc[r] = p.scale + (int64_t)n * p.KB * (W4_BLOCK / G);
+  }
+  const uint16_t* x[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int t = t0 + nt * 8 + g;
+    x[nt] = t < p.M ? p.x + (int64_t)t * p.ld_x : nullptr;
+  }
+
+  float sum[MT][NT][4] = {};
+  W4Frag<G, MT> cur, next;
+  int kb = warp;
+  if (kb < p.KB)
+#pragma unroll
+    for (int r = 0; r < 2 * MT; ++r) cur.load(r, q[r] + (int64_t)kb * 64, sc[r] + kb * (W4_BLOCK / G));
+  for (; kb < p.KB; kb += LIN_WARPS) {
+    const int nx = kb + LIN_WARPS;
+    if (nx < p.KB)
+#pragma unroll
+      for (int r = 0; r < 2 * MT; ++r) next.load(r, q[r] + (int64_t)nx * 64, sc[r] + nx * (W4_BLOCK / G));
+    w4_block<T, G, MT, NT>(cur, sum, [&](int nt, int b) {
+      return x[nt] ? ld_act8<VEC>(x[nt], kb * W4_BLOCK + b * 32 + a * 8, p.K) : make_uint4(0, 0, 0, 0);
+    });
+    cur = next;
+  }
+
+#pragma unroll
+  for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        red[warp][nt * 8 + 2 * a + (i & 1)][mt * 16 + g + 8 * (i >> 1)] = sum[mt][nt][i];
+  __syncthreads();
+  for (int i = threadIdx.x; i < 16 * MT * 8 * NT; i += LIN_WARPS * 32) {
+    const int r = i % (16 * MT), c = i / (16 * MT);
+    const int n = n0 + r, t = t0 + c;
+    if (n >= p.N || t >= p.M) continue;
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < LIN_WARPS; ++w) y += red[w][c][r];
+    if (p.bias) y += load_as_f32(p.bias, p.bias_dtype, n);
+    store_from_f32(p.out, p.out_dtype, (int64_t)t * p.ld_out + n, y);
+  }
+}
+
+template <typename F>
+int with_group(int group, F&& f) {
+  switch (group) {
+    case 32: return f(std::integral_constant<int, 32>{});
+    case 64: return f(std::integral_constant<int, 64>{});
+    case 128: return f(std::integral_constant<int, 128>{});
+    default: return fail(QI8_ESHAPE, "group_size must be 32, 64 or 128, got %d", group);
+  }
+}
+template <typename F>
+int with_float(int dtype, F&& f) {
+  switch (dtype) {
+    case QI8_BF16: return f(__nv_bfloat16{});
+    case QI8_F16: return f(__half{});
+    case QI8_F32: return f(float{});
+    default: return fail(QI8_EDTYPE, "bf16, fp16 or fp32 required, got dtype code %d", dtype);
+  }
+}
+template <typename F>
+int with_bool(bool b, F&& f) {
+  return b ? f(std::true_type{}) : f(std::false_type{});
+}
+
+int q_grid(int64_t words) {
+  const int64_t need = (words + Q_THREADS - 1) / Q_THREADS;
+  const int64_t cap = (int64_t)sm_count() * 8;  // eight blocks of 256 threads fill an SM
+  return (int)(need < cap ? need : cap);
+}
+
+int check_weight(const void* q, const void* scale, int64_t rows, int64_t K) {
+  QI8_REQUIRE(rows >= 0 && rows < (1LL << 40) && K > 0 && K <= (1 << 24), QI8_ESHAPE,
+              "4-bit weight of %lld rows, %lld features", (long long)rows, (long long)K);
+  QI8_REQUIRE(rows == 0 || (q && scale), QI8_EINVAL, "null pointer");
+  QI8_REQUIRE(aligned16(q) && aligned16(scale), QI8_EALIGN, "4-bit codes and scales must be 16-byte aligned");
+  return QI8_OK;
+}
+
+}  // namespace
+}  // namespace qi8
+
+using namespace qi8;
+
+extern "C" int qi8_quant_weight_i4(const void* w, int w_dtype, int64_t rows, int64_t K, int64_t ld_w, int group,
+                                   uint8_t* q_out, void* scale_out, void* stream) {
+  QI8_REQUIRE(device_ok(), QI8_EUNSUPPORTED, "no sm_100 device current");
+  if (int rc = check_weight(q_out, scale_out, rows, K)) return rc;
+  QI8_REQUIRE(rows == 0 || w, QI8_EINVAL, "null pointer");
+  QI8_REQUIRE(ld_w >= K, QI8_ESHAPE, "row stride %lld below the row's %lld elements", (long long)ld_w, (long long)K);
+  const int Kp = (int)w4_padded(K);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return with_group(group, [&](auto G) {
+    return with_float(w_dtype, [&](auto t) {
+      using T = decltype(t);
+      if (rows == 0) return (int)QI8_OK;
+      return with_bool(aligned16(w) && ld_w * sizeof(T) % 16 == 0, [&](auto vec) {
+        quant_i4_kernel<T, decltype(G)::value, decltype(vec)::value><<<q_grid(rows * (Kp / 8)), Q_THREADS, 0, st>>>(
+            static_cast<const T*>(w), ld_w, rows, (int)K, Kp, reinterpret_cast<uint32_t*>(q_out),
+            static_cast<__nv_bfloat16*>(scale_out));
+        return check_cuda(cudaGetLastError(), "quant_i4_kernel launch");
+      });
+    });
+  });
+}
+
+extern "C" int qi8_dequant_i4(const uint8_t* q, const void* scale, int64_t rows, int64_t K, int group, void* out,
+                              int out_dtype, int64_t ld_out, void* stream) {
+  QI8_REQUIRE(device_ok(), QI8_EUNSUPPORTED, "no sm_100 device current");
+  if (int rc = check_weight(q, scale, rows, K)) return rc;
+  QI8_REQUIRE(rows == 0 || out, QI8_EINVAL, "null pointer");
+  QI8_REQUIRE(ld_out >= K, QI8_ESHAPE, "row stride %lld below the row's %lld elements", (long long)ld_out,
+              (long long)K);
+  const int Kp = (int)w4_padded(K);
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return with_group(group, [&](auto G) {
+    return with_float(out_dtype, [&](auto t) {
+      using T = decltype(t);
+      if (rows == 0) return (int)QI8_OK;
+      return with_bool(aligned16(out) && ld_out * sizeof(T) % 16 == 0, [&](auto vec) {
+        dequant_i4_kernel<T, decltype(G)::value, decltype(vec)::value><<<q_grid(rows * (Kp / 8)), Q_THREADS, 0, st>>>(
+            reinterpret_cast<const uint32_t*>(q), static_cast<const __nv_bfloat16*>(scale), rows, (int)K, Kp,
+            static_cast<T*>(out), ld_out);
+        return check_cuda(cudaGetLastError(), "dequant_i4_kernel launch");
+      });
+    });
+  });
+}
+
+namespace {
+
+template <typename T, int G, int MT, int NT>
+int launch_rows(const LinArgs& p, bool vec, cudaStream_t st) {
+  const dim3 grid((p.N + 16 * MT - 1) / (16 * MT), (p.M + 8 * NT - 1) / (8 * NT));
+  return with_bool(vec, [&](auto v) {
+    w4_rows_kernel<T, G, MT, NT, decltype(v)::value><<<grid, LIN_WARPS * 32, 0, st>>>(p);
+    return check_cuda(cudaGetLastError(), "w4_rows_kernel launch");
+  });
+}
+
+}  // namespace
+
+extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* q,
+                           const void* scale, int64_t N, int group, const void* bias, int bias_dtype, void* out,
+                           int out_dtype, int64_t ld_out, void* stream) {
+  QI8_REQUIRE(device_ok(), QI8_EUNSUPPORTED, "no sm_100 device current");
+  if (int rc = check_weight(q, scale, N, K)) return rc;
+  QI8_REQUIRE(x_dtype == QI8_BF16 || x_dtype == QI8_F16, QI8_EDTYPE, "activations must be bf16 or fp16");
+  QI8_REQUIRE(out_dtype == x_dtype || out_dtype == QI8_F32, QI8_EDTYPE,
+              "output dtype must be the activations' or fp32");
+  QI8_REQUIRE(!bias || bias_dtype == QI8_BF16 || bias_dtype == QI8_F16 || bias_dtype == QI8_F32, QI8_EDTYPE,
+              "bias must be bf16, fp16 or fp32");
+  QI8_REQUIRE(M >= 0 && M < (1 << 30) && N < (1 << 30), QI8_ESHAPE, "%lld tokens, %lld outputs", (long long)M,
+              (long long)N);
+  QI8_REQUIRE(ld_x >= K && ld_out >= N, QI8_ESHAPE, "row strides %lld, %lld below the rows' %lld, %lld elements",
+              (long long)ld_x, (long long)ld_out, (long long)K, (long long)N);
+  QI8_REQUIRE(M == 0 || N == 0 || (x && out), QI8_EINVAL, "null pointer");
+  if (int rc = with_group(group, [](auto) { return (int)QI8_OK; })) return rc;
+  if (M == 0 || N == 0) return QI8_OK;
+  const cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const bool vec = aligned16(x) && ld_x % 8 == 0 && K % 8 == 0;
+  LinArgs p{static_cast<const uint16_t*>(x), ld_x, q, static_cast<const __nv_bfloat16*>(scale), bias, bias_dtype,
+            out, ld_out, out_dtype, 0, (int)N, (int)K, (int)(w4_padded(K) / W4_BLOCK)};
+  // grid.y holds 65535 token tiles at most
+  for (int64_t m = 0; m < M; m += 32768) {
+    p.M = (int)(M - m < 32768 ? M - m : 32768);
+    const int rc = with_group(group, [&](auto G) {
+      constexpr int g = decltype(G)::value;
+      return with_bool(x_dtype == QI8_F16, [&](auto half) {
+        using T = std::conditional_t<decltype(half)::value, __half, __nv_bfloat16>;
+        if (p.M <= 8) return launch_rows<T, g, 1, 1>(p, vec, st);
+        if (p.M <= 16) return launch_rows<T, g, 2, 2>(p, vec, st);
+        return launch_rows<T, g, 2, 4>(p, vec, st);
+      });
+    });
+    if (rc) return rc;
+    p.x += p.M * ld_x;
+    p.out = static_cast<uint8_t*>(p.out) + p.M * ld_out * elem_size(out_dtype);
+  }
+  return QI8_OK;
+}

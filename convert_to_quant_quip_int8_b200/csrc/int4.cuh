@@ -1,0 +1,158 @@
+// The 4-bit weight format and the tensor-core step on it.
+//
+//   W[n, k] = (u[n, k] - 8) * scale[n, k / group],   group 32, 64 or 128
+//
+// Rows are padded to Kp, a multiple of 128 features (code 0, u = 8); q holds
+// Kp / 2 bytes per row, scale (bf16) Kp / group values per row.
+//
+// * Eight codes share a 32-bit word, from the lowest nibble in the order of
+//   features 0, 2, 4, 6, 1, 3, 5, 7: (word >> 4 i) & 0x000f000f is then the
+//   pair of features (2 i, 2 i + 1) in the two halves of a register, where a
+//   16-bit MMA operand wants them.  OR-ing a float's exponent above the
+//   nibbles gives 128 + u (bf16) or 1024 + u (fp16); one packed subtraction
+//   leaves the code itself.  1.4 instructions per weight, nothing rounded.
+// * Of the 16 words of a 128-feature block, word 4 a + b holds features
+//   32 b + 8 a .. + 7.  A thread of an m16n8k16 quad (a = lane % 4) loads its
+//   four words as 16 bytes, and word b of the quad covers exactly the 32
+//   features of group block b: no MMA step mixes two groups, so the scales
+//   stay out of the operands and multiply the fp32 sums.
+#pragma once
+
+#include <type_traits>
+
+#include "common.cuh"
+
+namespace qi8 {
+
+constexpr int W4_BLOCK = 128;  // features per block of 16 words (64 bytes)
+
+inline int64_t w4_padded(int64_t k) { return (k + W4_BLOCK - 1) / W4_BLOCK * W4_BLOCK; }
+
+// (a & b) | c in one instruction
+__device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xEA;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+
+// The codes of one word as four packed pairs of T, features in order.
+template <typename T>
+__device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t (&p)[4]) {
+  if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
+    const uint32_t off = 0x64086408u;  // 1024 + 8
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = and_or(w >> (4 * i), 0x000f000fu, 0x64006400u);
+      asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(v), "r"(off));
+    }
+  } else {
+    const uint32_t off = 0x43084308u;  // 128 + 8
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t v = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
+      asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(v), "r"(off));
+    }
+  }
+}
+
+// D[16, 8] += A[16, 16] B[16, 8], 16-bit operands, fp32 sums.
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                         uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+  else
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Weights are read once: keep them out of L1, which the activations use.
+__device__ __forceinline__ uint4 ld_stream(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int b) {
+  return b == 0 ? v.x : b == 1 ? v.y : b == 2 ? v.z : v.w;
+}
+
+// Eight consecutive features of an activation row from feature k on, zero from
+// K on.  VEC: the row starts on a 16-byte boundary and K is a multiple of 8.
+template <bool VEC>
+__device__ __forceinline__ uint4 ld_act8(const uint16_t* row, int k, int K) {
+  if constexpr (VEC) return k < K ? __ldg(reinterpret_cast<const uint4*>(row + k)) : make_uint4(0, 0, 0, 0);
+  else {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t lo = k + 2 * i < K ? __ldg(row + k + 2 * i) : 0;
+      const uint32_t hi = k + 2 * i + 1 < K ? __ldg(row + k + 2 * i + 1) : 0;
+      w[i] = lo | (hi << 16);
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+  }
+}
+
+// A thread's weights of one 128-feature block for MT tiles of 16 rows: rows
+// g and g + 8 of each tile (g = lane / 4), and those rows' scales.
+template <int G, int MT>
+struct W4Frag {
+  static constexpr int NS = W4_BLOCK / G;  // scales per row and block
+  uint4 w[2 * MT];
+  uint2 s[2 * MT];  // NS bf16 values in the low halves first
+
+  __device__ __forceinline__ void load(int r, const uint8_t* q, const __nv_bfloat16* sc) {
+    w[r] = ld_stream(q);
+    if (NS == 4) s[r] = __ldg(reinterpret_cast<const uint2*>(sc));
+    else if (NS == 2) s[r].x = __ldg(reinterpret_cast<const uint32_t*>(sc));
+    else s[r].x = __ldg(reinterpret_cast<const unsigned short*>(sc));
+  }
+  __device__ __forceinline__ float scale(int r, int j) const {
+    const uint32_t v = j < 2 ? s[r].x : s[r].y;
+    return __uint_as_float((j & 1) ? (v & 0xffff0000u) : (v << 16));
+  }
+};
+
+// sum[mt][nt] += W X^T over one 128-feature block: lane (g, a) gets rows g
+// (elements 0, 1) and g + 8 (2, 3), columns 2 a and 2 a + 1.  act(nt, b)
+// returns features 32 b + 8 a .. + 7 of the activation row of column 8 nt + g.
+template <typename T, int G, int MT, int NT, typename Act>
+__device__ __forceinline__ void w4_block(const W4Frag<G, MT>& f, float (&sum)[MT][NT][4], Act&& act) {
+  float d[MT][NT][4];
+#pragma unroll
+  for (int b = 0; b < 4; ++b) {
+    uint4 x[NT];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) x[nt] = act(nt, b);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+      uint32_t p[4], r[4];
+      w4_unpack<T>(word_of(f.w[2 * mt], b), p);
+      w4_unpack<T>(word_of(f.w[2 * mt + 1], b), r);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        if (b * 32 % G == 0) d[mt][nt][0] = d[mt][nt][1] = d[mt][nt][2] = d[mt][nt][3] = 0.0f;
+        mma16816<T>(d[mt][nt], p[0], r[0], p[1], r[1], x[nt].x, x[nt].y);
+        mma16816<T>(d[mt][nt], p[2], r[2], p[3], r[3], x[nt].z, x[nt].w);
+      }
+      if ((b + 1) * 32 % G == 0) {
+        const int j = b * 32 / G;
+        const float s0 = f.scale(2 * mt, j), s1 = f.scale(2 * mt + 1, j);
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          sum[mt][nt][0] = fmaf(d[mt][nt][0], s0, sum[mt][nt][0]);
+          sum[mt][nt][1] = fmaf(d[mt][nt][1], s0, sum[mt][nt][1]);
+          sum[mt][nt][2] = fmaf(d[mt][nt][2], s1, sum[mt][nt][2]);
+          sum[mt][nt][3] = fmaf(d[mt][nt][3], s1, sum[mt][nt][3]);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace qi8

@@ -471,6 +471,149 @@ def ldlq_finish(q: torch.Tensor, scale: torch.Tensor, cols: torch.Tensor, want_d
     return deq, qs
 
 
+# ---------------------------------------------------------------------------
+# weights of 4 bits with group scales (format: include/qi8.h)
+# ---------------------------------------------------------------------------
+
+_I4_GROUPS = (32, 64, 128)
+
+
+def _i4_padded(k: int) -> int:
+    """Features per row of a 4-bit weight: ``k`` rounded up to whole 128s."""
+    return -(-k // 128) * 128
+
+
+def _one_device(x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> torch.device:
+    L.require_cuda(x, *tensors)
+    dev = x.device
+    for t in tensors:
+        assert t is None or t.device == dev, f"tensors on {dev} and {t.device}"
+    return dev
+
+
+def _launch(dev: torch.device, what: str, fn, *args) -> None:
+    """Calls a libqi8 entry point on ``dev`` and its current stream."""
+    if dev.index == torch.cuda.current_device():
+        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if rc:
+        L.check(rc, what)
+
+
+def _check_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int, dims: int) -> None:
+    """``q`` uint8 [..., N, Kp/2] and ``scale`` bf16 [..., N, Kp/group] of a weight with ``k`` input features."""
+    if q.dtype != torch.uint8 or scale.dtype != torch.bfloat16:
+        raise TypeError(f"4-bit weights are uint8 codes and bfloat16 scales, got {q.dtype} and {scale.dtype}")
+    assert group in _I4_GROUPS, f"group_size must be 32, 64 or 128, got {group}"
+    kp = _i4_padded(k)
+    assert q.dim() == dims and q.shape[-1] * 2 == kp, \
+        f"4-bit codes of shape {tuple(q.shape)}: expected {dims} dimensions and {kp // 2} bytes a row for {k} features"
+    assert scale.shape[:-1] == q.shape[:-1] and scale.shape[-1] * group == kp, \
+        f"scales of shape {tuple(scale.shape)} for codes of shape {tuple(q.shape)} and group_size {group}"
+    assert q.is_contiguous() and scale.is_contiguous(), "4-bit codes and scales must be contiguous"
+
+
+def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
+    """Inference only: a result without a gradient must not pass for one with it."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError("4-bit operators have no backward pass: call them under torch.no_grad() or on "
+                                   "detached tensors")
+
+
+def quant_weight_i4(w: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
+    """4-bit codes and group scales of ``w`` [..., N, K]: ``(q uint8 [..., N, Kp/2], scale bf16 [..., N, Kp/group])``."""
+    dev = _one_device(w)
+    _no_grad(w)
+    dt = L.dtype_code(w.dtype)
+    if dt not in (L.QI8_BF16, L.QI8_F16, L.QI8_F32):
+        raise TypeError(f"weights must be bfloat16, float16 or float32, got {w.dtype}")
+    assert w.dim() >= 2 and w.shape[-1] > 0, f"weight of shape {tuple(w.shape)}: expected [..., N, K] with K > 0"
+    assert group in _I4_GROUPS, f"group_size must be 32, 64 or 128, got {group}"
+    w2 = w if w.dim() == 2 else w.reshape(-1, w.shape[-1])
+    if w2.stride(1) != 1 or w2.stride(0) < w2.shape[1]:
+        w2 = w2.contiguous()
+    rows, k = w2.shape
+    kp = _i4_padded(k)
+    q = torch.empty(*w.shape[:-1], kp // 2, dtype=torch.uint8, device=dev)
+    s = torch.empty(*w.shape[:-1], kp // group, dtype=torch.bfloat16, device=dev)
+    _launch(dev, "qi8_quant_weight_i4", L.load().qi8_quant_weight_i4, w2.data_ptr(), dt, rows, k,
+            max(w2.stride(0), k), group, q.data_ptr(), s.data_ptr())
+    return q, s
+
+
+def dequant_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int = 128,
+               out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """The weight [..., N, k] that 4-bit codes and scales stand for."""
+    dev = _one_device(q, scale)
+    _check_i4(q, scale, k, group, q.dim())
+    assert q.dim() >= 2, f"4-bit codes of shape {tuple(q.shape)}: expected [..., N, Kp/2]"
+    dt = L.dtype_code(out_dtype)
+    if dt not in (L.QI8_BF16, L.QI8_F16, L.QI8_F32):
+        raise TypeError(f"output dtype must be bfloat16, float16 or float32, got {out_dtype}")
+    out = torch.empty(*q.shape[:-1], k, dtype=out_dtype, device=dev)
+    _launch(dev, "qi8_dequant_i4", L.load().qi8_dequant_i4, q.data_ptr(), scale.data_ptr(), out.numel() // k, k,
+            group, out.data_ptr(), dt, k)
+    return out
+
+
+def gemm_w4(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, group: int = 128,
+            bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    """``x [..., K] W^T + bias`` with the 4-bit weight ``q`` [N, Kp/2], ``scale`` [N, Kp/group]."""
+    dev = _one_device(x, q, scale, bias)
+    _no_grad(x, bias)
+    k = x.shape[-1]
+    _check_i4(q, scale, k, group, 2)
+    n = q.shape[0]
+    x2 = x if x.dim() == 2 else x.reshape(-1, k)
+    if x2.stride(1) != 1 or x2.stride(0) < k:
+        x2 = x2.contiguous()
+    m = x2.shape[0]
+    if bias is not None:
+        assert bias.dim() == 1 and bias.shape[0] == n, f"Bias must be 1D with length {n}, got shape {tuple(bias.shape)}"
+        bias = bias.contiguous()
+    out = torch.empty(m, n, dtype=out_dtype or x.dtype, device=dev)
+    _launch(dev, "qi8_gemm_w4", L.load().qi8_gemm_w4, x2.data_ptr(), L.dtype_code(x.dtype), m, k,
+            max(x2.stride(0), k), q.data_ptr(), scale.data_ptr(), n, group, None if bias is None else bias.data_ptr(),
+            0 if bias is None else L.dtype_code(bias.dtype), out.data_ptr(), L.dtype_code(out.dtype), n)
+    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
+
+
+def moe_w4(x: torch.Tensor, router: torch.Tensor, q13: torch.Tensor, s13: torch.Tensor, q2: torch.Tensor,
+           s2: torch.Tensor, top_k: int, group: int = 128, renormalize: bool = True,
+           act: int = L.QI8_ACT_SILU) -> torch.Tensor:
+    """A mixture-of-experts layer on ``x`` [..., H] with 4-bit experts: ``router`` [E, H], ``q13``/``s13`` of
+    [E, 2 I, H] (gate rows above up rows), ``q2``/``s2`` of [E, H, I]."""
+    dev = _one_device(x, router, q13, s13, q2, s2)
+    _no_grad(x, router)
+    h = x.shape[-1]
+    _check_i4(q13, s13, h, group, 3)
+    e, i2 = q13.shape[:2]
+    assert i2 % 2 == 0, f"gate and up weights of {i2} rows: expected as many of each"
+    i = i2 // 2
+    _check_i4(q2, s2, i, group, 3)
+    assert tuple(q2.shape[:2]) == (e, h), f"down weights of shape {tuple(q2.shape)}: expected [{e}, {h}, ...]"
+    assert tuple(router.shape) == (e, h), f"router of shape {tuple(router.shape)}: expected [{e}, {h}]"
+    assert router.is_contiguous(), "router must be contiguous"
+    x2 = x if x.dim() == 2 else x.reshape(-1, h)
+    if x2.stride(1) != 1 or x2.stride(0) < h:
+        x2 = x2.contiguous()
+    t = x2.shape[0]
+    lib = L.load()
+    nbytes = lib.qi8_moe_w4_workspace_bytes(t, h, e, i, top_k)
+    if nbytes == 0:
+        L.check(L.QI8_ESHAPE, "qi8_moe_w4")
+    out = torch.empty(t, h, dtype=x.dtype, device=dev)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+    _launch(dev, "qi8_moe_w4", lib.qi8_moe_w4, x2.data_ptr(), L.dtype_code(x.dtype), t, h, max(x2.stride(0), h),
+            router.data_ptr(), L.dtype_code(router.dtype), e, q13.data_ptr(), s13.data_ptr(), i, q2.data_ptr(),
+            s2.data_ptr(), group, top_k, int(bool(renormalize)), act, out.data_ptr(), h, ws.data_ptr(), nbytes)
+    return out if x.dim() == 2 else out.view(x.shape)
+
+
 def device_status(reset: bool = True) -> None:
     """Raise if a kernel's bounded wait expired since the last check."""
     L.check(L.load().qi8_device_status(int(reset)), "device status")

@@ -75,8 +75,8 @@ enum {
   QI8_S_TILE128 = 4    /* [rows/128, K/128]: per 128x128 weight tile (comfy block weight) */
 };
 
-/* GEMM epilogue activation */
-enum { QI8_ACT_NONE = 0, QI8_ACT_GELU = 1 };
+/* GEMM epilogue activation (SILU: the expert layer's gate only) */
+enum { QI8_ACT_NONE = 0, QI8_ACT_GELU = 1, QI8_ACT_SILU = 2 };
 
 /* weight requantization schemes (converters/quip_int8.py:1614-1669) */
 enum { QI8_REQ_ROW = 0, QI8_REQ_GLOBAL = 1, QI8_REQ_BLOCK = 2 };
@@ -408,6 +408,47 @@ QI8_API int qi8_peer_barrier(uint32_t* const* flags, int world, int rank, void* 
 QI8_API int qi8_requant_weight(const void* w, int w_dtype, int64_t M, int64_t N, int64_t ld_w, int requant,
                                int block, int8_t* q_out, float* scale_out, void* workspace,
                                int64_t workspace_bytes, void* stream);
+
+/* ---- Weights of 4 bits with group scales (no counterpart in the reference).
+   W[n, k] = (u - 8) * scale[n, k / group], group 32, 64 or 128.  Rows are
+   padded to Kp = K rounded up to a multiple of 128 features (code 0).
+   q [rows, Kp / 2] uint8: eight codes per 32-bit word, from the lowest nibble
+   in the order of features 0, 2, 4, 6, 1, 3, 5, 7; of the 16 words of a
+   128-feature block, word 4 a + b holds features 32 b + 8 a .. + 7.
+   scale [rows, Kp / group] bf16.  Both 16-byte aligned. */
+
+/* scale = max(amax / 7 rounded to five significant bits, 2^-100) per (row,
+   group), code = rint(w / scale) (ties to even), so code * scale is exact in
+   bf16.  A group with an infinity or a NaN gets scale NaN, code 0.
+   w [rows, K] bf16 / f16 / f32, row stride ld_w. */
+QI8_API int qi8_quant_weight_i4(const void* w, int w_dtype, int64_t rows, int64_t K, int64_t ld_w, int group,
+                                uint8_t* q_out, void* scale_out, void* stream);
+
+/* out [rows, K] (row stride ld_out) = code * scale as bf16 / f16 / f32. */
+QI8_API int qi8_dequant_i4(const uint8_t* q, const void* scale, int64_t rows, int64_t K, int group, void* out,
+                           int out_dtype, int64_t ld_out, void* stream);
+
+/* y [M, N] = x [M, K] W^T + bias with the 4-bit weight W [N, K], fp32 sums.
+   x bf16 / f16 (row stride ld_x); y of the same type or f32 (row stride
+   ld_out); bias (or null) [N] bf16 / f16 / f32. */
+QI8_API int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* q,
+                        const void* scale, int64_t N, int group, const void* bias, int bias_dtype, void* out,
+                        int out_dtype, int64_t ld_out, void* stream);
+
+/* A mixture-of-experts layer, x [T, H] -> out [T, H] (bf16 / f16):
+     l = x router^T (64-bit sums), the top_k largest per token (equal ones:
+     lowest expert first), p = softmax(l) on them (over their sum when
+     renormalize != 0), y = sum_e p_e D_e (act(G_e x) * (U_e x)).
+   router [E, H] of x's type or f32; q13 / s13: [E, 2 I, H] (G_e above U_e),
+   q2 / s2: [E, H, I], 4-bit weights as above; act QI8_ACT_SILU or
+   QI8_ACT_GELU (erf).  E <= 1024, top_k <= min(E, 64).  Tokens run 64 at a
+   time.  workspace >= qi8_moe_w4_workspace_bytes(...), 16-byte aligned, its
+   contents do not matter; calls that overlap need one each. */
+QI8_API int64_t qi8_moe_w4_workspace_bytes(int64_t T, int64_t H, int64_t E, int64_t I, int top_k);
+QI8_API int qi8_moe_w4(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ld_x, const void* router,
+                       int router_dtype, int64_t E, const uint8_t* q13, const void* s13, int64_t I,
+                       const uint8_t* q2, const void* s2, int group, int top_k, int renormalize, int act, void* out,
+                       int64_t ld_out, void* workspace, int64_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

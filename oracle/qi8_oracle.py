@@ -754,3 +754,70 @@ def lpt_partition(costs, n_parts: int):
         parts[j].append(i)
         loads[j] += costs[i]
     return [sorted(p) for p in parts]
+
+
+# --------------------------------------------------------------------------
+# Weights of 4 bits with group scales (no counterpart in the reference; the
+# format is stated in include/qi8.h)
+# --------------------------------------------------------------------------
+
+def i4_padded(k: int) -> int:
+    return -(-k // 128) * 128
+
+
+def i4_positions(k: int) -> Tuple[np.ndarray, np.ndarray]:
+    """For every feature of a padded row: the byte that holds its code and the
+    code's shift in that byte.  Eight features share a 32-bit word, nibbles in
+    the order 0, 2, 4, 6, 1, 3, 5, 7; word 4 a + b of a 128-feature block starts
+    at feature 32 b + 8 a."""
+    f = np.arange(i4_padded(k))
+    block, b, a, e = f // 128, f % 128 // 32, f % 32 // 8, f % 8
+    nibble = e // 2 + 4 * (e % 2)
+    return block * 64 + (4 * a + b) * 4 + nibble // 2, 4 * (nibble % 2)
+
+
+def i4_quantize(w: np.ndarray, group: int) -> Tuple[np.ndarray, np.ndarray]:
+    """``(codes int8 [N, Kp], scale float64 [N, Kp / group])`` of a weight [N, K],
+    in fp64: ``scale = max(amax / 7 to five significant bits, 2^-100)``,
+    ``code = rint(w / scale)``; a group that is not finite gets NaN and 0."""
+    w = np.asarray(w, dtype=np.float64)
+    wp = np.zeros((w.shape[0], i4_padded(w.shape[1])))
+    wp[:, :w.shape[1]] = w
+    g = wp.reshape(w.shape[0], -1, group)
+    finite = np.isfinite(g).all(-1)
+    g = np.where(finite[..., None], g, 0.0)
+    mant, exp = np.frexp(np.abs(g).max(-1) / 7.0)
+    scale = np.maximum(np.ldexp(np.rint(mant * 32.0) / 32.0, exp), 2.0 ** -100)
+    codes = np.rint(g / scale[..., None]).astype(np.int8)
+    return codes.reshape(w.shape[0], -1), np.where(finite, scale, np.nan)
+
+
+def i4_pack(codes: np.ndarray) -> np.ndarray:
+    """Codes [N, Kp] in [-8, 7] -> packed uint8 [N, Kp / 2]."""
+    byte, shift = i4_positions(codes.shape[1])
+    q = np.zeros((codes.shape[0], codes.shape[1] // 2), np.uint8)
+    for half in (0, 4):
+        at = shift == half
+        q[:, byte[at]] |= ((codes[:, at].astype(np.int16) + 8) << half).astype(np.uint8)
+    return q
+
+
+def i4_unpack(q: np.ndarray) -> np.ndarray:
+    """Packed uint8 [N, Kp / 2] -> codes int8 [N, Kp]."""
+    byte, shift = i4_positions(2 * q.shape[1])
+    return ((q[:, byte] >> shift.astype(np.uint8)) & 15).astype(np.int8) - 8
+
+
+def i4_values(q: np.ndarray, scale: np.ndarray, k: int, group: int) -> np.ndarray:
+    """The weight [N, k] in fp64."""
+    return (i4_unpack(q) * np.repeat(np.asarray(scale, np.float64), group, axis=1))[:, :k]
+
+
+def moe_route(logits: np.ndarray, top_k: int, renormalize: bool) -> np.ndarray:
+    """Weights [T, E] (0 where an expert is not chosen) of fp64 logits [T, E]."""
+    out = np.zeros_like(logits)
+    for t, row in enumerate(logits):
+        best = sorted(range(len(row)), key=lambda e: (-row[e], e))[:top_k]
+        p = np.exp(row - row.max())
+        out[t, best] = p[best] / (p[best].sum() if renormalize else p.sum())
+    return out
