@@ -87,7 +87,8 @@ SIGNATURES = {
     "qi8_peer_barrier": (_I, [_P, _I, _I, _P]),
     "qi8_quant_weight_i4": (_I, [_P, _I, _I64, _I64, _I64, _I, _P, _P, _P]),
     "qi8_dequant_i4": (_I, [_P, _P, _I64, _I64, _I, _P, _I, _I64, _P]),
-    "qi8_gemm_w4": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _I, _P, _I, _P, _I, _I64, _P]),
+    "qi8_gemm_w4_workspace_bytes": (_I64, [_P, _I64, _I64, _I64]),
+    "qi8_gemm_w4": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _I, _P, _I, _P, _I, _I64, _P, _I64, _P]),
     "qi8_moe_w4_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I]),
     "qi8_moe_w4": (_I, [_P, _I, _I64, _I64, _I64, _P, _I, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _I, _P, _I64,
                         _P, _I64, _P]),

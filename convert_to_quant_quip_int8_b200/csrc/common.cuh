@@ -45,6 +45,10 @@ enum : unsigned int {
   ST_GEMM_EPILOGUE = 1u << 2,
   ST_GEMM_DRAIN = 1u << 3,
   ST_PEER_BARRIER = 1u << 4,
+  ST_W4_PRODUCER = 1u << 5,
+  ST_W4_UNPACK = 1u << 6,
+  ST_W4_MMA = 1u << 7,
+  ST_W4_EPILOGUE = 1u << 8,
 };
 
 // ---------------------------------------------------------- conversions

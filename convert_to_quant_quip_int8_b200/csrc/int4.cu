@@ -188,19 +188,6 @@ dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restric
 // per warp, joined in shared memory in the order of the warps.
 constexpr int LIN_WARPS = 8;
 
-struct LinArgs {
-  const uint16_t* x;
-  int64_t ld_x;
-  const uint8_t* q;
-  const __nv_bfloat16* scale;
-  const void* bias;
-  int bias_dtype;
-  void* out;
-  int64_t ld_out;
-  int out_dtype;
-  int M, N, K, KB;  // KB = Kp / 128
-};
-
 template <typename T, int G, int MT, int NT, bool VEC>
 __global__ void __launch_bounds__(LIN_WARPS * 32)
 w4_rows_kernel(const LinArgs p) {
@@ -259,6 +246,16 @@ w4_rows_kernel(const LinArgs p) {
     for (int w = 0; w < LIN_WARPS; ++w) y += red[w][c][r];
     if (p.bias) y += load_as_f32(p.bias, p.bias_dtype, n);
     store_from_f32(p.out, p.out_dtype, (int64_t)t * p.ld_out + n, y);
+  }
+}
+
+// Activation rows onto 16-byte boundaries, the last 16 bytes filled with zeros:
+// TMA takes no others.
+__global__ void align_rows_kernel(const uint16_t* __restrict__ x, int64_t ld_x, int K, uint4* __restrict__ out,
+                                  int vecs, int64_t total) {
+  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t t = i / vecs;
+    out[i] = ld_act8<false>(x + t * ld_x, (int)(i - t * vecs) * 8, K);
   }
 }
 
@@ -362,9 +359,22 @@ int launch_rows(const LinArgs& p, bool vec, cudaStream_t st) {
 
 }  // namespace
 
+namespace {
+// tokens from which the tcgen05 kernel takes over
+constexpr int64_t W4_TILES_FROM = 17;
+
+bool act_aligned(const void* x, int64_t K, int64_t ld_x) { return aligned16(x) && ld_x % 8 == 0 && K % 8 == 0; }
+}  // namespace
+
+extern "C" int64_t qi8_gemm_w4_workspace_bytes(const void* x, int64_t M, int64_t K, int64_t ld_x) {
+  if (M < W4_TILES_FROM || act_aligned(x, K, ld_x)) return 0;
+  return M * ((K + 7) / 8) * 16;
+}
+
 extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* q,
                            const void* scale, int64_t N, int group, const void* bias, int bias_dtype, void* out,
-                           int out_dtype, int64_t ld_out, void* stream) {
+                           int out_dtype, int64_t ld_out, void* workspace, int64_t workspace_bytes,
+                           void* stream) {
   QI8_REQUIRE(device_ok(), QI8_EUNSUPPORTED, "no sm_100 device current");
   if (int rc = check_weight(q, scale, N, K)) return rc;
   QI8_REQUIRE(x_dtype == QI8_BF16 || x_dtype == QI8_F16, QI8_EDTYPE, "activations must be bf16 or fp16");
@@ -380,24 +390,30 @@ extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int
   if (int rc = with_group(group, [](auto) { return (int)QI8_OK; })) return rc;
   if (M == 0 || N == 0) return QI8_OK;
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
-  const bool vec = aligned16(x) && ld_x % 8 == 0 && K % 8 == 0;
+  const bool vec = act_aligned(x, K, ld_x);
   LinArgs p{static_cast<const uint16_t*>(x), ld_x, q, static_cast<const __nv_bfloat16*>(scale), bias, bias_dtype,
             out, ld_out, out_dtype, 0, (int)N, (int)K, (int)(w4_padded(K) / W4_BLOCK)};
-  // grid.y holds 65535 token tiles at most
-  for (int64_t m = 0; m < M; m += 32768) {
-    p.M = (int)(M - m < 32768 ? M - m : 32768);
-    const int rc = with_group(group, [&](auto G) {
-      constexpr int g = decltype(G)::value;
-      return with_bool(x_dtype == QI8_F16, [&](auto half) {
-        using T = std::conditional_t<decltype(half)::value, __half, __nv_bfloat16>;
-        if (p.M <= 8) return launch_rows<T, g, 1, 1>(p, vec, st);
-        if (p.M <= 16) return launch_rows<T, g, 2, 2>(p, vec, st);
-        return launch_rows<T, g, 2, 4>(p, vec, st);
-      });
-    });
-    if (rc) return rc;
-    p.x += p.M * ld_x;
-    p.out = static_cast<uint8_t*>(p.out) + p.M * ld_out * elem_size(out_dtype);
+  p.M = (int)M;
+  if (M >= W4_TILES_FROM) {
+    if (const int64_t need = qi8_gemm_w4_workspace_bytes(x, M, K, ld_x)) {
+      QI8_REQUIRE(workspace && workspace_bytes >= need, QI8_ESHAPE, "workspace of %lld bytes, %lld needed",
+                  (long long)workspace_bytes, (long long)need);
+      QI8_REQUIRE(aligned16(workspace), QI8_EALIGN, "workspace must be 16-byte aligned");
+      const int vecs = (int)((K + 7) / 8);
+      align_rows_kernel<<<q_grid(M * vecs), Q_THREADS, 0, st>>>(p.x, ld_x, p.K, static_cast<uint4*>(workspace), vecs,
+                                                                M * vecs);
+      if (int rc = check_cuda(cudaGetLastError(), "align_rows_kernel launch")) return rc;
+      p.x = static_cast<const uint16_t*>(workspace);
+      p.ld_x = vecs * 8;
+    }
+    return gemm_w4_tiles(p, x_dtype, group, st);
   }
-  return QI8_OK;
+  return with_group(group, [&](auto G) {
+    constexpr int g = decltype(G)::value;
+    return with_bool(x_dtype == QI8_F16, [&](auto half) {
+      using T = std::conditional_t<decltype(half)::value, __half, __nv_bfloat16>;
+      if (p.M <= 8) return launch_rows<T, g, 1, 1>(p, vec, st);
+      return launch_rows<T, g, 2, 2>(p, vec, st);
+    });
+  });
 }

@@ -28,6 +28,23 @@ constexpr int W4_BLOCK = 128;  // features per block of 16 words (64 bytes)
 
 inline int64_t w4_padded(int64_t k) { return (k + W4_BLOCK - 1) / W4_BLOCK * W4_BLOCK; }
 
+// One linear layer on a 4-bit weight: y [M, N] = x [M, K] W^T + bias.
+struct LinArgs {
+  const uint16_t* x;
+  int64_t ld_x;
+  const uint8_t* q;
+  const __nv_bfloat16* scale;
+  const void* bias;
+  int bias_dtype;
+  void* out;
+  int64_t ld_out;
+  int out_dtype;
+  int M, N, K, KB;  // KB = Kp / 128
+};
+
+// The tcgen05 kernel (gemm_w4.cu): x rows start on 16-byte boundaries.
+int gemm_w4_tiles(const LinArgs& p, int x_dtype, int group, cudaStream_t st);
+
 // (a & b) | c in one instruction
 __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;

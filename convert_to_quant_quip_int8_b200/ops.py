@@ -484,20 +484,27 @@ def _i4_padded(k: int) -> int:
 
 
 def _one_device(x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> torch.device:
-    L.require_cuda(x, *tensors)
     dev = x.device
-    for t in tensors:
-        assert t is None or t.device == dev, f"tensors on {dev} and {t.device}"
+    for t in (x, *tensors):
+        if t is not None and (not t.is_cuda or t.device != dev):
+            L.require_cuda(x, *tensors)
+            raise AssertionError(f"tensors on {dev} and {t.device}")
     return dev
+
+
+# the current stream of a device as a plain pointer: a tenth of the cost of a Stream object
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
+    (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
 
 def _launch(dev: torch.device, what: str, fn, *args) -> None:
     """Calls a libqi8 entry point on ``dev`` and its current stream."""
-    if dev.index == torch.cuda.current_device():
-        rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    index = dev.index
+    if index == torch.cuda.current_device():
+        rc = fn(*args, _raw_stream(index))
     else:
         with torch.cuda.device(dev):
-            rc = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = fn(*args, _raw_stream(index))
     if rc:
         L.check(rc, what)
 
@@ -508,10 +515,11 @@ def _check_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int, dims: in
         raise TypeError(f"4-bit weights are uint8 codes and bfloat16 scales, got {q.dtype} and {scale.dtype}")
     assert group in _I4_GROUPS, f"group_size must be 32, 64 or 128, got {group}"
     kp = _i4_padded(k)
-    assert q.dim() == dims and q.shape[-1] * 2 == kp, \
-        f"4-bit codes of shape {tuple(q.shape)}: expected {dims} dimensions and {kp // 2} bytes a row for {k} features"
-    assert scale.shape[:-1] == q.shape[:-1] and scale.shape[-1] * group == kp, \
-        f"scales of shape {tuple(scale.shape)} for codes of shape {tuple(q.shape)} and group_size {group}"
+    shape = q.shape
+    assert len(shape) == dims and shape[-1] * 2 == kp, \
+        f"4-bit codes of shape {tuple(shape)}: expected {dims} dimensions and {kp // 2} bytes a row for {k} features"
+    assert scale.shape == (*shape[:-1], kp // group), \
+        f"scales of shape {tuple(scale.shape)} for codes of shape {tuple(shape)} and group_size {group}"
     assert q.is_contiguous() and scale.is_contiguous(), "4-bit codes and scales must be contiguous"
 
 
@@ -565,21 +573,33 @@ def gemm_w4(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, group: int = 
     """``x [..., K] W^T + bias`` with the 4-bit weight ``q`` [N, Kp/2], ``scale`` [N, Kp/group]."""
     dev = _one_device(x, q, scale, bias)
     _no_grad(x, bias)
-    k = x.shape[-1]
+    shape = x.shape
+    k = shape[-1]
     _check_i4(q, scale, k, group, 2)
     n = q.shape[0]
-    x2 = x if x.dim() == 2 else x.reshape(-1, k)
-    if x2.stride(1) != 1 or x2.stride(0) < k:
-        x2 = x2.contiguous()
+    x2 = x if len(shape) == 2 else x.reshape(-1, k)
     m = x2.shape[0]
+    ld, inner = x2.stride()
+    if inner != 1 or ld < k:
+        if m > 1 or inner != 1:
+            x2 = x2.contiguous()
+        ld = k
+    bias_ptr, bias_dt = None, 0
     if bias is not None:
         assert bias.dim() == 1 and bias.shape[0] == n, f"Bias must be 1D with length {n}, got shape {tuple(bias.shape)}"
         bias = bias.contiguous()
+        bias_ptr, bias_dt = bias.data_ptr(), L.dtype_code(bias.dtype)
     out = torch.empty(m, n, dtype=out_dtype or x.dtype, device=dev)
-    _launch(dev, "qi8_gemm_w4", L.load().qi8_gemm_w4, x2.data_ptr(), L.dtype_code(x.dtype), m, k,
-            max(x2.stride(0), k), q.data_ptr(), scale.data_ptr(), n, group, None if bias is None else bias.data_ptr(),
-            0 if bias is None else L.dtype_code(bias.dtype), out.data_ptr(), L.dtype_code(out.dtype), n)
-    return out if x.dim() == 2 else out.view(*x.shape[:-1], n)
+    lib = L.load()
+    x_ptr, ws_ptr, nbytes = x2.data_ptr(), None, 0
+    if k & 7 or ld & 7 or x_ptr & 15:
+        nbytes = lib.qi8_gemm_w4_workspace_bytes(x_ptr, m, k, ld)
+        if nbytes:
+            ws = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+            ws_ptr = ws.data_ptr()
+    _launch(dev, "qi8_gemm_w4", lib.qi8_gemm_w4, x_ptr, L.dtype_code(x.dtype), m, k, ld, q.data_ptr(),
+            scale.data_ptr(), n, group, bias_ptr, bias_dt, out.data_ptr(), L.dtype_code(out.dtype), n, ws_ptr, nbytes)
+    return out if len(shape) == 2 else out.view(*shape[:-1], n)
 
 
 def moe_w4(x: torch.Tensor, router: torch.Tensor, q13: torch.Tensor, s13: torch.Tensor, q2: torch.Tensor,

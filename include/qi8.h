@@ -430,10 +430,14 @@ QI8_API int qi8_dequant_i4(const uint8_t* q, const void* scale, int64_t rows, in
 
 /* y [M, N] = x [M, K] W^T + bias with the 4-bit weight W [N, K], fp32 sums.
    x bf16 / f16 (row stride ld_x); y of the same type or f32 (row stride
-   ld_out); bias (or null) [N] bf16 / f16 / f32. */
+   ld_out); bias (or null) [N] bf16 / f16 / f32.  Activations whose rows do
+   not start on 16-byte boundaries (or K % 8 != 0) are copied to such rows in
+   the workspace when there are more than a few tokens:
+   qi8_gemm_w4_workspace_bytes bytes (0 otherwise), 16-byte aligned. */
+QI8_API int64_t qi8_gemm_w4_workspace_bytes(const void* x, int64_t M, int64_t K, int64_t ld_x);
 QI8_API int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* q,
                         const void* scale, int64_t N, int group, const void* bias, int bias_dtype, void* out,
-                        int out_dtype, int64_t ld_out, void* stream);
+                        int out_dtype, int64_t ld_out, void* workspace, int64_t workspace_bytes, void* stream);
 
 /* A mixture-of-experts layer, x [T, H] -> out [T, H] (bf16 / f16):
      l = x router^T (64-bit sums), the top_k largest per token (equal ones:

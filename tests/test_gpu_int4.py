@@ -257,8 +257,9 @@ def test_linear_writes_its_columns_alone(m):
     q, s, _ = weight(33, 100, 32, seed=13)
     x = randn(m, 100, seed=14, dtype=BF)
     out = torch.full((m + 2, 50), 3.0, dtype=BF, device="cuda")
+    ws = torch.empty(m * 208, dtype=torch.uint8, device="cuda")  # 100 features: rows are copied to 104
     L.check(L.load().qi8_gemm_w4(x.data_ptr(), L.QI8_BF16, m, 100, 100, q.data_ptr(), s.data_ptr(), 33, 32, None, 0,
-                                 out.data_ptr(), L.QI8_BF16, 50, L.stream_ptr()))
+                                 out.data_ptr(), L.QI8_BF16, 50, ws.data_ptr(), ws.numel(), L.stream_ptr()))
     assert torch.equal(out[:m, :33], I4.int4_linear(x, q, s, 32))
     assert (out[m:] == 3).all() and (out[:, 33:] == 3).all()
 
