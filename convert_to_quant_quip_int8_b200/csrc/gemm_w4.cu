@@ -6,15 +6,20 @@
 // The weight rows are the MMA's M (128 TMEM lanes), the tokens its N, so that
 // one kernel serves 17 tokens and a long prompt.  Roles of a block:
 //   warps 0..3    epilogue: TMEM -> registers -> y (thread = weight row)
-//   warps 4..11   unpacking, two groups of four warps that take the
-//                 128-feature blocks in turn (thread = weight row): 64 bytes of
-//                 codes -> code * scale in 16 bits -> the 128-byte-swizzled A
-//                 operand in shared memory
-//   warp 12       TMA producer of the activations
-//   warp 13       TMEM allocation, MMA issue (one thread)
-// A ring of SLOTS slots holds 64 features each (128 x 64 weights, BN x 64
-// activations); a slot is full when TMA has written its bytes and the four
-// warps of the unpacking group have arrived.
+//   warps 4..19   unpacking, four groups of four warps (thread = weight row):
+//                 half of a 128-feature block, 32 bytes of codes -> code *
+//                 scale in 16 bits -> 32 TMEM columns of the A operand
+//   warps 20, 22  TMA producers: activations, codes
+//   warp 21       TMEM allocation, MMA issue (one thread)
+// The A operand lives in TMEM.  In shared memory it cost the stores and the
+// fence to the async proxy (800 to 1900 cycles a block, counted with clock64) and
+// its reads (66 cycles for each MMA of 16 features, whatever the tokens).
+// Rings: codes (stages of two blocks), activations, operand slots of 128
+// features.  A slot costs the issuing thread 500 cycles of waits and commits
+// whatever is in it: slots of 64 features were slower.  A group fills about every
+// other slot of the sequence and had waited for slot n - 3 - SLOTS or a later one
+// to be consumed before it waits for slot n: with SLOTS >= 3 the parity it waits
+// for cannot be that of slot n - 2 SLOTS.  Codes are unpacked before the wait.
 //
 // code * scale is exact in bf16 when the scale has five significant bits, as
 // qi8_quant_weight_i4 writes it; scales with more are rounded here, half a step
@@ -24,7 +29,9 @@
 //
 // Few tiles: a cluster of S blocks splits K and joins its fp32 sums through
 // distributed shared memory in the order of the ranks, each block finishing
-// 1 / S of the tile's tokens.
+// 1 / S of the tile's tokens.  (Tiles of N / SMs rows over all of K instead:
+// 17 x 4096 x 4096 took 25 us against 14, 100 x 4096 x 10240 45 against 25.)
+// With very few tiles they have 64 rows: 100 x 512 x 4096 11 us, not 14.
 //
 // Every wait is bounded; on expiry the role sets a status bit, all roles leave
 // their loops, copies and MMAs in flight are drained and TMEM is freed.
@@ -40,25 +47,33 @@ namespace {
 namespace w4tc {
 
 constexpr int BM = 128;
-constexpr int EPI_WARPS = 4, UNPACK_WARP0 = 4, PRODUCER = 12, ISSUER = 13;
-constexpr int THREADS = 14 * 32;
-constexpr int A_BYTES = BM * 128;  // 64 features in 16 bits
+constexpr int EPI_WARPS = 4, UNPACK_WARP0 = 4, PRODUCER = 20, ISSUER = 21, CODES = 22;
+constexpr int UNPACK_WARPS = 16;
+constexpr int THREADS = 23 * 32;
+constexpr int SLOTS = 4;     // of the weight operand, 128 features each
+constexpr int A_COLS = 64;   // TMEM columns of one: two 16-bit features per column
+constexpr int SEG = 2;       // 128-feature blocks per stage of the code ring: 128 bytes per row
+constexpr int CODE_BARS = 8; // code stages at most
 
 template <int BN> struct Cfg {
-  static constexpr int SLOTS = BN == 256 ? 4 : BN == 128 ? 3 : BN == 64 ? 4 : 5;
-  static constexpr int OCC = BN == 256 ? 1 : 2;  // blocks per SM
-  static constexpr int B_BYTES = BN * 128;
-  static constexpr int SLOT_BYTES = A_BYTES + B_BYTES;
-  static constexpr int SMEM = 1024 + SLOTS * SLOT_BYTES + 192;
-  static constexpr uint32_t TMEM_COLS = 2 * BN;  // two accumulators
-  static_assert(OCC * SMEM <= 232448 && BN * 512 <= SLOTS * SLOT_BYTES, "shared memory");
-  static_assert((2 * SLOTS + 5) * 8 + 16 <= 192, "barriers");
+  static constexpr int X_SLOTS = BN == 256 ? 3 : BN == 128 ? 5 : BN == 64 ? 8 : 12;
+  static constexpr int CODE_BYTES = (BN == 256 ? 32 : BN == 32 ? 96 : 64) * 1024;
+  static constexpr int X_BYTES = BN * 256;
+  static constexpr int RING = X_SLOTS * X_BYTES + CODE_BYTES;
+  static constexpr int BARS = 2 * (SLOTS + X_SLOTS + CODE_BARS) + 5;
+  static constexpr int SMEM = 1024 + RING + BARS * 8 + 16;
+  static constexpr int ACCS = BN == 256 ? 1 : 2;  // accumulators that fit beside the weight slots
+  static_assert(SMEM <= 232448 && (BN + 64) * 512 <= RING, "shared memory; the sums of a split tile");
+  static_assert(ACCS * BN + SLOTS * A_COLS <= 512, "tensor memory");
 };
+constexpr uint32_t TMEM_COLS = 512;
 
 struct Args {
   LinArgs l;
-  int n_tiles, t_tiles;  // of 128 weight rows, of BN tokens
+  int rows;              // weight rows per tile, at most 128
+  int n_tiles, t_tiles;  // of `rows` weight rows, of BN tokens
   int split;             // blocks per tile (cluster size)
+  int code_stages;       // stages of the code ring
   unsigned int* status;
 };
 
@@ -69,27 +84,38 @@ __host__ __device__ constexpr uint32_t idesc(int bn) {
   return (1u << 4) | (f << 7) | (f << 10) | ((uint32_t)(bn >> 3) << 17) | ((uint32_t)(BM >> 4) << 24);
 }
 
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
+// A in TMEM, B in shared memory
+__device__ __forceinline__ void mma_f16(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accum) {
   asm volatile(
       "{\n\t.reg .pred p;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accum)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(accum)
       : "memory");
 }
-
-__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+// 32 columns of the warp's 32 lanes
+__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&r)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16, "
+      "%17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(addr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
 }
-__device__ __forceinline__ void st_cluster_f32(uint32_t addr, float v) {
-  asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
-}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 bytes: a whole sector per thread
-__device__ __forceinline__ void ld_codes(uint4& a, uint4& b, const uint8_t* p) {
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
-               : "=r"(a.x), "=r"(a.y), "=r"(a.z), "=r"(a.w), "=r"(b.x), "=r"(b.y), "=r"(b.z), "=r"(b.w)
-               : "l"(p));
+__device__ __forceinline__ uint2 ld_shared8(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
+               : "memory");
 }
 
 // fp16 only: the power of two that brings the row's largest finite scale to
@@ -123,30 +149,43 @@ __device__ __forceinline__ uint32_t mul_pair(uint32_t a, uint32_t b) {
 }
 
 template <typename T, int G, int BN>
-__global__ void __launch_bounds__(THREADS, Cfg<BN>::OCC)
-gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ CUtensorMap tmQ,
+               const __grid_constant__ Args p) {
   using C = Cfg<BN>;
-  constexpr int SLOTS = C::SLOTS;
+  constexpr int X_SLOTS = C::X_SLOTS, ACCS = C::ACCS;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
   const uint32_t base = (raw + 1023u) & ~1023u;
-  const uint32_t sA = base, sB = base + SLOTS * A_BYTES;
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + (base - raw) + SLOTS * C::SLOT_BYTES);
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * SLOTS + 5);
+  const uint32_t sX = base, sQ = base + X_SLOTS * C::X_BYTES;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem_raw + (base - raw) + C::RING);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + C::BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
   auto empty_bar = [&](int s) { return smem_u32(bars + SLOTS + s); };
   auto tfull_bar = [&](int b) { return smem_u32(bars + 2 * SLOTS + b); };
   auto tempty_bar = [&](int b) { return smem_u32(bars + 2 * SLOTS + 2 + b); };
   const uint32_t drain_bar = smem_u32(bars + 2 * SLOTS + 4);
+  auto qfull_bar = [&](int s) { return smem_u32(bars + 2 * SLOTS + 5 + s); };
+  auto qempty_bar = [&](int s) { return smem_u32(bars + 2 * SLOTS + 5 + CODE_BARS + s); };
+  auto xfull_bar = [&](int s) { return smem_u32(bars + 2 * (SLOTS + CODE_BARS) + 5 + s); };
+  auto xempty_bar = [&](int s) { return smem_u32(bars + 2 * (SLOTS + CODE_BARS) + 5 + X_SLOTS + s); };
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int split = p.split;
   const int rank = split > 1 ? (int)cta_rank() : 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(full_bar(s), 1 + 4);
+      mbar_init(full_bar(s), 8);  // warps of two groups
       mbar_init(empty_bar(s), 1);
+    }
+    for (int s = 0; s < X_SLOTS; ++s) {
+      mbar_init(xfull_bar(s), 1);
+      mbar_init(xempty_bar(s), 1);
+    }
+    for (int s = 0; s < CODE_BARS; ++s) {
+      mbar_init(qfull_bar(s), 1);
+      mbar_init(qempty_bar(s), UNPACK_WARPS);
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(tfull_bar(b), 1);
@@ -158,20 +197,23 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
   }
   if (warp == ISSUER) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
-                 "r"(C::TMEM_COLS)
+                 "r"(TMEM_COLS)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   if (warp == PRODUCER && lane == 0) tma_prefetch_desc(&tmX);
+  if (warp == CODES && lane == 0) tma_prefetch_desc(&tmQ);
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
-  const uint32_t tmem_base = *tmem_slot;
+  const uint32_t tmem_base = *tmem_slot, tmem_a = tmem_base + (uint32_t)(ACCS * BN);
 
   // tiles of this block, 128-feature blocks of each
   const int tiles = p.n_tiles * p.t_tiles;
   const int tile0 = blockIdx.x / split, tile_step = gridDim.x / split;
   const int kb0 = (int)((int64_t)p.l.KB * rank / split), kb1 = (int)((int64_t)p.l.KB * (rank + 1) / split);
+
+  const int kn = kb1 - kb0;
 
   if (warp == PRODUCER) {
     if (lane == 0) {
@@ -180,45 +222,79 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
       bool ok = true;
       for (int tile = tile0; ok && tile < tiles; tile += tile_step) {
         const int t0 = (tile / p.n_tiles) * BN;
-        for (int kb = 2 * kb0; kb < 2 * kb1; ++kb) {
-          if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, ST_W4_PRODUCER, WAIT_LIMIT_NS)) {
+        for (int kb = kb0; kb < kb1; ++kb) {
+          if (!mbar_wait(xempty_bar(s), ph ^ 1u, abort_flag, p.status, ST_W4_PRODUCER, WAIT_LIMIT_NS)) {
             ok = false;
             break;
           }
-          mbar_arrive_expect_tx(full_bar(s), C::B_BYTES);
-          tma_load_2d(sB + s * C::B_BYTES, &tmX, kb * 64, t0, full_bar(s));
+          mbar_arrive_expect_tx(xfull_bar(s), C::X_BYTES);
+          tma_load_2d(sX + s * C::X_BYTES, &tmX, kb * 128, t0, xfull_bar(s));
+          tma_load_2d(sX + s * C::X_BYTES + C::X_BYTES / 2, &tmX, kb * 128 + 64, t0, xfull_bar(s));
           issued |= 1u << s;
           issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
-          if (++s == SLOTS) s = 0, ph ^= 1u;
+          if (++s == X_SLOTS) s = 0, ph ^= 1u;
         }
       }
       // the last copies land before the block exits, also when nobody reads them any more
       if (!ok)
-        for (int t = 0; t < SLOTS; ++t)
-          if (issued & (1u << t)) drain_wait(full_bar(t), (issued_ph >> t) & 1u);
+        for (int t = 0; t < X_SLOTS; ++t)
+          if (issued & (1u << t)) drain_wait(xfull_bar(t), (issued_ph >> t) & 1u);
     }
+  } else if (warp == CODES) {
+    int s = 0;
+    uint32_t ph = 0, issued = 0, issued_ph = 0;
+    bool ok = true;
+    for (int tile = tile0; ok && tile < tiles; tile += tile_step) {
+      const int n0 = (tile % p.n_tiles) * p.rows;
+      const int rows = min(p.rows, p.l.N - n0);
+      for (int kb = kb0; kb < kb1; kb += SEG) {
+        if (!warp_wait(qempty_bar(s), ph ^ 1u, abort_flag, p.status, ST_W4_PRODUCER, WAIT_LIMIT_NS)) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {  // past a split's range too: the box is whole
+          mbar_arrive_expect_tx(qfull_bar(s), (uint32_t)(p.rows * SEG) * 64u);
+          tma_load_2d(sQ + (uint32_t)(s * p.rows * SEG * 64), &tmQ, kb * 16, n0, qfull_bar(s));
+        }
+        for (int r = lane; r < rows; r += 32)
+          prefetch_l2(p.l.scale + ((int64_t)(n0 + r) * p.l.KB + kb) * (W4_BLOCK / G));
+        issued |= 1u << s;
+        issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
+        if (++s == p.code_stages) s = 0, ph ^= 1u;
+      }
+    }
+    if (!ok)
+      for (int t = 0; t < p.code_stages; ++t)
+        if (issued & (1u << t)) drain_wait(qfull_bar(t), (issued_ph >> t) & 1u);
   } else if (warp == ISSUER) {
     if (lane == 0) {
-      int s = 0, unit = 0;
-      uint32_t ph = 0;
+      int xs = 0, unit = 0;
+      uint32_t xph = 0;
+      unsigned seq = 0;  // blocks so far, over all tiles
       bool ok = true;
       for (int tile = tile0; ok && tile < tiles; tile += tile_step, ++unit) {
-        const int buf = unit & 1;
-        if (!mbar_wait(tempty_bar(buf), ((unit >> 1) & 1) ^ 1u, abort_flag, p.status, ST_W4_MMA, WAIT_LIMIT_NS)) break;
+        const int buf = unit % ACCS;
+        if (!mbar_wait(tempty_bar(buf), ((unit / ACCS) & 1) ^ 1u, abort_flag, p.status, ST_W4_MMA, WAIT_LIMIT_NS))
+          break;
         tc_fence_after();
         const uint32_t d = tmem_base + (uint32_t)(buf * BN);
-        for (int kb = 2 * kb0; kb < 2 * kb1; ++kb) {
-          if (!mbar_wait(full_bar(s), ph, abort_flag, p.status, ST_W4_MMA, WAIT_LIMIT_NS)) {
+        for (int kb = 0; kb < kn; ++kb, ++seq) {
+          const int s = seq % SLOTS;
+          if (!mbar_wait(xfull_bar(xs), xph, abort_flag, p.status, ST_W4_MMA, WAIT_LIMIT_NS) ||
+              !mbar_wait(full_bar(s), (seq / SLOTS) & 1u, abort_flag, p.status, ST_W4_MMA, WAIT_LIMIT_NS)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          const uint64_t da = sw128_desc(sA + s * A_BYTES), db = sw128_desc(sB + s * C::B_BYTES);
+          const uint32_t a = tmem_a + (uint32_t)(s * A_COLS);
+          const uint64_t db = sw128_desc(sX + xs * C::X_BYTES);
 #pragma unroll
-          for (int k = 0; k < 4; ++k)
-            mma_f16(d, da + (uint64_t)(2 * k), db + (uint64_t)(2 * k), idesc<T>(BN), kb > 2 * kb0 || k > 0);
+          for (int k = 0; k < 8; ++k)  // 16 features each: 8 columns of A, 32 bytes of a swizzled half of B
+            mma_f16(d, a + 8 * k, db + (uint64_t)((k >> 2) * (C::X_BYTES / 2 / 16) + (k & 3) * 2), idesc<T>(BN),
+                    kb > 0 || k > 0);
           tc_commit(empty_bar(s));
-          if (++s == SLOTS) s = 0, ph ^= 1u;
+          tc_commit(xempty_bar(xs));
+          if (++xs == X_SLOTS) xs = 0, xph ^= 1u;
         }
         if (ok) tc_commit(tfull_bar(buf));
       }
@@ -227,69 +303,76 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
     }
     __syncwarp();
   } else if (warp >= UNPACK_WARP0) {
-    const int group = (warp - UNPACK_WARP0) >> 2;
+    // group g of four warps unpacks half g % 2 of block g / 2 of every code stage
+    const int g = (warp - UNPACK_WARP0) >> 2, half = g & 1, which = g >> 1;
     const int row = ((warp & 3) << 5) + lane;
-    const uint32_t a_row = sA + row * 128;
-    const uint32_t swz = (uint32_t)(row & 7);
-    int s = 2 * group;  // this group's first slot of the ring
-    uint32_t ph = 0;
-    int block = 0;  // blocks before this tile, over all tiles
+    const bool warp_live = ((warp & 3) << 5) < p.rows;  // lanes of the MMA past the tile's rows hold what they hold
+    const uint32_t swz = (uint32_t)(row & 7) << 4;      // 128-byte swizzle of the codes
+    const uint32_t q_row = sQ + min(row, p.rows - 1) * 128 + half * 8;
+    const uint32_t a_row = tmem_a + ((uint32_t)((warp & 3) * 32) << 16) + (uint32_t)(half * 32);
+    int qs = 0;
+    uint32_t qph = 0;
+    unsigned before = 0;  // blocks before this tile, over all tiles
     bool ok = true;
-    const int kn = kb1 - kb0;
-    for (int tile = tile0; ok && tile < tiles; tile += tile_step, block += kn) {
-      const int64_t n = min((tile % p.n_tiles) * BM + row, p.l.N - 1);  // rows past the end are read as the last
-      const uint8_t* q = p.l.q + (n * p.l.KB + kb0) * 64;
+    for (int tile = tile0; ok && tile < tiles; tile += tile_step, before += kn) {
+      const int64_t n = min((tile % p.n_tiles) * p.rows + row, p.l.N - 1);  // rows past the end: any scale
       const __nv_bfloat16* sc = p.l.scale + (n * p.l.KB + kb0) * (W4_BLOCK / G);
       float shift = 1.0f;
       if constexpr (std::is_same<T, __half>::value)
         shift = __uint_as_float(row_shift(sc, kn * (W4_BLOCK / G)) << 23);
-      // word 4 a + b of the block in w[a].b
-      uint4 w[4], next[4];
-      uint2 f, fn;
-      auto load = [&](int kb, uint4 (&v)[4], uint2& sv) {
-        ld_codes(v[0], v[1], q + kb * 64);
-        ld_codes(v[2], v[3], q + kb * 64 + 32);
-        const __nv_bfloat16* sp = sc + kb * (W4_BLOCK / G);
-        if (G == 32) sv = __ldg(reinterpret_cast<const uint2*>(sp));
-        else if (G == 64) sv.x = __ldg(reinterpret_cast<const uint32_t*>(sp));
-        else sv.x = __ldg(reinterpret_cast<const unsigned short*>(sp));
+      auto load_scales = [&](int kb) -> uint32_t {  // of this half block
+        if (kb >= kn) return 0;
+        if (G == 32) return __ldg(reinterpret_cast<const uint32_t*>(sc + kb * 4 + half * 2));
+        return __ldg(reinterpret_cast<const unsigned short*>(G == 64 ? sc + kb * 2 + half : sc + kb));
       };
-      int kb = (block & 1) ^ group;  // blocks alternate between the groups, across tiles too
-      if (kb < kn) load(kb, w, f);
-      for (; kb < kn; kb += 2) {
-        if (kb + 2 < kn) load(kb + 2, next, fn);
+      uint32_t f0 = load_scales(which), f1 = load_scales(which + SEG);
+      for (int kb = which; kb - which < kn; kb += SEG) {
+        const uint32_t f = f0;
+        f0 = f1;
+        f1 = load_scales(kb + 2 * SEG);
+        if (!warp_wait(qfull_bar(qs), qph, abort_flag, p.status, ST_W4_UNPACK, WAIT_LIMIT_NS)) {
+          ok = false;
+          break;
+        }
+        // words 4 a + 2 half and the next of the block, unpacked before the slot is there to take them
+        uint32_t v[32];
+        const bool have = kb < kn;  // the last stage may have one block
+        if (have && warp_live) {
+          const uint32_t at = q_row + (uint32_t)(qs * p.rows * 128);
+          uint2 w[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, ST_W4_UNPACK, WAIT_LIMIT_NS)) {
-            ok = false;
-            break;
-          }
-          const uint32_t dst = a_row + s * A_BYTES;
+          for (int a = 0; a < 4; ++a) w[a] = ld_shared8(at + (((uint32_t)(which * 4 + a) << 4) ^ swz));
 #pragma unroll
-          for (int bb = 0; bb < 2; ++bb) {
-            const int b = 2 * h + bb, j = b * 32 / G;
-            const uint32_t sv = j < 2 ? f.x : f.y;
-            const uint32_t sp = scale_pair<T>(__uint_as_float((j & 1) ? (sv & 0xffff0000u) : (sv << 16)), shift);
+          for (int b = 0; b < 2; ++b) {
+            const uint32_t sp =
+                scale_pair<T>(__uint_as_float(G == 32 && b == 1 ? (f & 0xffff0000u) : (f << 16)), shift);
 #pragma unroll
             for (int a = 0; a < 4; ++a) {
-              uint32_t v[4];
-              w4_unpack<T>(word_of(w[a], b), v);
+              uint32_t u[4];
+              w4_unpack<T>(b ? w[a].y : w[a].x, u);
 #pragma unroll
-              for (int i = 0; i < 4; ++i) v[i] = mul_pair<T>(v[i], sp);
-              st_shared16(dst + (((uint32_t)(bb * 4 + a) ^ swz) << 4), v[0], v[1], v[2], v[3]);
+              for (int e = 0; e < 4; ++e) v[16 * b + 4 * a + e] = mul_pair<T>(u[e], sp);
             }
           }
-          asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-          __syncwarp();
-          if (lane == 0) mbar_arrive(full_bar(s));
-          if (++s == SLOTS) s = 0, ph ^= 1u;
         }
-        if (!ok) break;
-        s += 2;  // the other group's slots
-        if (s >= SLOTS) s -= SLOTS, ph ^= 1u;
-#pragma unroll
-        for (int a = 0; a < 4; ++a) w[a] = next[a];
-        f = fn;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(qempty_bar(qs));
+        if (++qs == p.code_stages) qs = 0, qph ^= 1u;
+        if (!have) break;
+        const unsigned seq = before + kb;
+        const int s = seq % SLOTS;
+        if (!warp_wait(empty_bar(s), ((seq / SLOTS) & 1u) ^ 1u, abort_flag, p.status, ST_W4_UNPACK, WAIT_LIMIT_NS)) {
+          ok = false;
+          break;
+        }
+        if (warp_live) {
+          tc_fence_after();
+          tmem_st32(a_row + (uint32_t)(s * A_COLS), v);
+          tmem_wait_st();
+          tc_fence_before();
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(full_bar(s));
       }
     }
   } else {
@@ -297,16 +380,16 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
     int unit = 0;
     const uint32_t lanes = (uint32_t)(warp * 32) << 16;
     for (int tile = tile0; tile < tiles; tile += tile_step, ++unit) {
-      const int n = (tile % p.n_tiles) * BM + warp * 32 + lane;
+      const int r0 = warp * 32 + lane, n = (tile % p.n_tiles) * p.rows + r0;
       const int t0 = (tile / p.n_tiles) * BN;
-      const int buf = unit & 1;
+      const int buf = unit % ACCS;
       float unshift = 1.0f;
       if constexpr (std::is_same<T, __half>::value)
         unshift = __uint_as_float(
             (254u - row_shift(p.l.scale + ((int64_t)min(n, p.l.N - 1) * p.l.KB + kb0) * (W4_BLOCK / G),
                               (kb1 - kb0) * (W4_BLOCK / G))) << 23);
       const float bias = p.l.bias && n < p.l.N ? load_as_f32(p.l.bias, p.l.bias_dtype, n) : 0.0f;
-      if (!mbar_wait(tfull_bar(buf), (unit >> 1) & 1, abort_flag, p.status, ST_W4_EPILOGUE, WAIT_LIMIT_NS)) break;
+      if (!warp_wait(tfull_bar(buf), (unit / ACCS) & 1, abort_flag, p.status, ST_W4_EPILOGUE, WAIT_LIMIT_NS)) break;
       tc_fence_after();
       if (split == 1) {
         const int t1 = min(BN, p.l.M - t0);
@@ -316,7 +399,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
           uint32_t r[32];
           tmem_ld32(tmem_base + lanes + (uint32_t)(buf * BN + c), r);
           tmem_wait_ld();
-          if (n < p.l.N) {
+          if (r0 < p.rows && n < p.l.N) {
             const int64_t at = (int64_t)(t0 + c) * p.l.ld_out + n;
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
@@ -341,8 +424,9 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
     cluster_sync();
     tc_fence_after();
     const int tile = tile0;
-    const int t0 = (tile / p.n_tiles) * BN, n0 = (tile % p.n_tiles) * BM;
+    const int t0 = (tile / p.n_tiles) * BN, n0 = (tile % p.n_tiles) * p.rows;
     const int t1 = min(BN, p.l.M - t0);
+    const int per = ((BN + split - 1) / split + 3) & ~3, pitch = per + 4;  // columns per rank; padded against conflicts
     if (warp < EPI_WARPS && !*abort_flag) {
       const uint32_t lanes = (uint32_t)(warp * 32) << 16;
       const int row = warp * 32 + lane;
@@ -351,19 +435,21 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
         unshift = __uint_as_float(
             (254u - row_shift(p.l.scale + ((int64_t)min(n0 + row, p.l.N - 1) * p.l.KB + kb0) * (W4_BLOCK / G),
                               (kb1 - kb0) * (W4_BLOCK / G))) << 23);
+      // rank d finishes columns [d per, (d + 1) per); its blocks of sums are [source][row][pitch]
 #pragma unroll 1
       for (int c = 0; c < t1; c += 32) {
         uint32_t r[32];
         tmem_ld32(tmem_base + lanes + (uint32_t)c, r);
         tmem_wait_ld();
+        if (row < p.rows) {
+          int d = c / per, at = c - d * per;
 #pragma unroll
-        for (int j = 0; j < 32; ++j) {
-          const int col = c + j;
-          // column col belongs to rank col % split, at [source][col / split][row]
-          const int dst = col % split, slot = rank * ((BN + split - 1) / split) + col / split;
-          if (col < t1)
-            st_cluster_f32(mapa(base + (uint32_t)((slot * BM + row) * 4), (uint32_t)dst),
-                           __uint_as_float(r[j]) * unshift);
+          for (int j = 0; j < 32; j += 4) {
+            st_cluster_f32x4(mapa(base + (uint32_t)(((rank * BM + row) * pitch + at) * 4), (uint32_t)d),
+                             __uint_as_float(r[j]) * unshift, __uint_as_float(r[j + 1]) * unshift,
+                             __uint_as_float(r[j + 2]) * unshift, __uint_as_float(r[j + 3]) * unshift);
+            if ((at += 4) >= per) at -= per, ++d;
+          }
         }
       }
     }
@@ -372,13 +458,12 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
     cluster_sync();
     tc_fence_after();
     const float* part = reinterpret_cast<const float*>(smem_raw + (base - raw));
-    const int per = (BN + split - 1) / split;
     for (int i = threadIdx.x; i < per * BM; i += THREADS) {
       const int row = i & (BM - 1), c = i / BM;
-      const int col = c * split + rank, n = n0 + row;
-      if (col >= t1 || n >= p.l.N) continue;
+      const int col = rank * per + c, n = n0 + row;
+      if (col >= t1 || row >= p.rows || n >= p.l.N) continue;
       float y = 0.0f;
-      for (int r = 0; r < split; ++r) y += part[(r * per + c) * BM + row];
+      for (int r = 0; r < split; ++r) y += part[(r * BM + row) * pitch + c];
       if (p.l.bias) y += load_as_f32(p.l.bias, p.l.bias_dtype, n);
       const int64_t at = (int64_t)(t0 + col) * p.l.ld_out + n;
       if (p.l.out_dtype == QI8_F32) static_cast<float*>(p.l.out)[at] = y;
@@ -390,7 +475,7 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const Args p) {
   __syncthreads();
   if (warp == ISSUER) {
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(C::TMEM_COLS)
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem_base), "r"(TMEM_COLS)
                  : "memory");
   }
 }
@@ -410,34 +495,29 @@ int activation_map(CUtensorMap* map, const LinArgs& p, bool half, int bn) {
   return QI8_OK;
 }
 
+template <typename T, int G, int BN> struct Key {};
+
 template <typename T, int G, int BN>
 int launch(const LinArgs& l, cudaStream_t st) {
   using C = Cfg<BN>;
   auto kern = gemm_w4_kernel<T, G, BN>;
-  int dev = 0;
-  if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
-  static bool set[64];
-  if (dev >= 64 || !set[dev]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM),
-                            "cudaFuncSetAttribute"))
-      return rc;
-    if (dev < 64) set[dev] = true;
+  if (int rc = allow_smem<Key<T, G, BN>>(kern, C::SMEM)) return rc;
+  const int sms = sm_count();
+  Args p{l, BM, (l.N + BM - 1) / BM, (l.M + BN - 1) / BN, 1, 2, device_status_ptr()};
+  if ((int64_t)p.n_tiles * p.t_tiles * 16 <= sms) {  // splits of K fill the SMs up to eightfold
+    p.rows = BM / 2;
+    p.n_tiles = (l.N + p.rows - 1) / p.rows;
   }
-  CUtensorMap map;
-  if (int rc = activation_map(&map, l, std::is_same<T, __half>::value, BN)) return rc;
-  Args p{l, (l.N + BM - 1) / BM, (l.M + BN - 1) / BN, 1, device_status_ptr()};
   const int64_t tiles = (int64_t)p.n_tiles * p.t_tiles;
   QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
-  const int sms = sm_count(), seats = sms * C::OCC;
-  // blocks per tile: the split with the least work on the fullest SM, while all
-  // blocks are resident at once and each has a few blocks of K
-  int64_t best = (tiles + sms - 1) / sms * 64;
-  for (int s = 2; s <= 8 && tiles * s <= seats && p.l.KB >= 2 * s; ++s) {
-    const int64_t cost = (tiles * s + sms - 1) / sms * 64 / s + 2;  // and a little for joining
-    if (cost < best) best = cost, p.split = s;
-  }
+  while (p.split < 8 && tiles * (p.split + 1) <= sms && p.l.KB >= 2 * (p.split + 1)) ++p.split;
+  p.code_stages = C::CODE_BYTES / (p.rows * SEG * 64);
+  if (p.code_stages > CODE_BARS) p.code_stages = CODE_BARS;
+  CUtensorMap map, codes;
+  if (int rc = activation_map(&map, l, std::is_same<T, __half>::value, BN)) return rc;
+  if (int rc = code_map(&codes, l.q, l.N, l.KB, SEG, p.rows, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : tiles < seats ? tiles : seats));
+  cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : tiles < sms ? tiles : sms));
   cfg.blockDim = dim3(THREADS);
   cfg.dynamicSmemBytes = C::SMEM;
   cfg.stream = st;
@@ -447,7 +527,7 @@ int launch(const LinArgs& l, cudaStream_t st) {
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, map, p), "gemm_w4_kernel launch");
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, map, codes, p), "gemm_w4_kernel launch");
 }
 
 template <typename T, int G>

@@ -209,7 +209,7 @@ w4_rows_kernel(const LinArgs p) {
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt) {
     const int t = t0 + nt * 8 + g;
-    x[nt] = t < p.M ? p.x + (int64_t)t * p.ld_x : nullptr;
+    x[nt] = p.x + (int64_t)min(t, p.M - 1) * p.ld_x + (VEC ? 8 * a : 0);  // columns past the end repeat the last
   }
 
   float sum[MT][NT][4] = {};
@@ -223,9 +223,14 @@ w4_rows_kernel(const LinArgs p) {
     if (nx < p.KB)
 #pragma unroll
       for (int r = 0; r < 2 * MT; ++r) next.load(r, q[r] + (int64_t)nx * 64, sc[r] + nx * (W4_BLOCK / G));
-    w4_block<T, G, MT, NT>(cur, sum, [&](int nt, int b) {
-      return x[nt] ? ld_act8<VEC>(x[nt], kb * W4_BLOCK + b * 32 + a * 8, p.K) : make_uint4(0, 0, 0, 0);
-    });
+    if (VEC && (kb + 1) * W4_BLOCK <= p.K)
+      w4_block<T, G, MT, NT>(cur, sum, [&](int nt, int b) {
+        return __ldg(reinterpret_cast<const uint4*>(x[nt] + kb * W4_BLOCK + b * 32));
+      });
+    else
+      w4_block<T, G, MT, NT>(cur, sum, [&](int nt, int b) {
+        return ld_act8<VEC>(x[nt] - (VEC ? 8 * a : 0), kb * W4_BLOCK + b * 32 + a * 8, p.K);
+      });
     cur = next;
   }
 

@@ -42,6 +42,21 @@ struct LinArgs {
   int M, N, K, KB;  // KB = Kp / 128
 };
 
+// Lets a kernel have `smem` bytes of shared memory, once per device (Key: a type
+// of the kernel's own).
+template <typename Key, typename F>
+int allow_smem(F* kern, int smem) {
+  static bool done[64];
+  int dev = 0;
+  if (int rc = check_cuda(cudaGetDevice(&dev), "cudaGetDevice")) return rc;
+  if (dev < 64 && done[dev]) return QI8_OK;
+  if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem),
+                          "cudaFuncSetAttribute"))
+    return rc;
+  if (dev < 64) done[dev] = true;
+  return QI8_OK;
+}
+
 // The tcgen05 kernel (gemm_w4.cu): x rows start on 16-byte boundaries.
 int gemm_w4_tiles(const LinArgs& p, int x_dtype, int group, cudaStream_t st);
 
@@ -125,6 +140,9 @@ struct W4Frag {
 
   __device__ __forceinline__ void load(int r, const uint8_t* q, const __nv_bfloat16* sc) {
     w[r] = ld_stream(q);
+    load_scale(r, sc);
+  }
+  __device__ __forceinline__ void load_scale(int r, const __nv_bfloat16* sc) {
     if (NS == 4) s[r] = __ldg(reinterpret_cast<const uint2*>(sc));
     else if (NS == 2) s[r].x = __ldg(reinterpret_cast<const uint32_t*>(sc));
     else s[r].x = __ldg(reinterpret_cast<const unsigned short*>(sc));

@@ -13,10 +13,14 @@
 // Four launches, bound by the bytes of the experts in use:
 //   moe_logits_kernel  one warp per (expert, token quad)
 //   moe_route_kernel   one block: the choice, its weights, tokens by expert
-//   moe_up_kernel      one block per (expert, 16 rows of G and of U); h = act(g) * u
-//   moe_down_kernel    one block per 16 rows of y: every expert in use, all
-//                      tokens; its sums never leave the block, so nothing is
-//                      added atomically and the result does not depend on order
+//   moe_up_kernel      streaming engine (w4_stream.cuh): tasks are 16 rows of G
+//                      and of U of one expert, h = act(g) * u
+//   moe_down_kernel    streaming engine: a block takes a share of y's rows and
+//                      goes through every expert in use; its sums never leave the
+//                      block, so nothing is added atomically and the result does
+//                      not depend on order
+// An expert's tokens come in chunks of up to `cap` pairs (token, choice): as many
+// as the MMA columns of a task hold.
 //
 // h is held as two bf16 numbers (value and remainder, 16 significant bits
 // together): rounding it to one would cost as much accuracy as the output's
@@ -27,6 +31,7 @@
 
 #include "common.cuh"
 #include "int4.cuh"
+#include "w4_stream.cuh"
 
 namespace qi8 {
 namespace {
@@ -37,12 +42,12 @@ constexpr int MOE_MAX_EXPERTS = 1024;
 
 // What the route kernel leaves for the others, in the workspace.
 struct Route {
-  int* n_used;                    // experts with tokens
-  int* expert;                    // [used] which
-  int* first;                     // [used] its first pair
-  unsigned long long* mask;       // [used] its tokens
-  int* token;                     // [pair]
-  float* weight;                  // [pair]
+  int* n_chunks;  // of all experts with tokens, in the experts' order
+  int* expert;    // [chunk]
+  int* first;     // [chunk] its first pair
+  int* count;     // [chunk] its pairs
+  int* token;     // [pair]
+  float* weight;  // [pair]
 };
 
 struct MoeArgs {
@@ -59,6 +64,9 @@ struct MoeArgs {
   int dtype;
   int T, H, E, I, top_k;
   int renorm, act;
+  int cap;         // pairs per chunk
+  int height;      // rows of y per tile of the down product
+  unsigned int* status;
   double* logits;  // [T, E]
   __nv_bfloat16* h;  // [pair][2][Ip]
   Route r;
@@ -161,29 +169,29 @@ moe_route_kernel(const MoeArgs p) {
 
   // experts with tokens, in order: warp 0 runs over all of them
   if (warp == 0) {
-    int used = 0, pairs = 0;
+    int chunks = 0, pairs = 0;
     for (int e0 = 0; e0 < p.E; e0 += 32) {
       const int e = e0 + lane;
-      const unsigned long long m = e < p.E ? mask[e] : 0;
-      const int n = __popcll(m);
-      int before = n;  // inclusive sum over the lanes
+      const int n = e < p.E ? __popcll(mask[e]) : 0, nc = (n + p.cap - 1) / p.cap;
+      int pair_end = n, chunk_end = nc;  // inclusive sums over the lanes
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, before, o);
-        if (lane >= o) before += v;
+        const int a = __shfl_up_sync(0xffffffffu, pair_end, o), b = __shfl_up_sync(0xffffffffu, chunk_end, o);
+        if (lane >= o) pair_end += a, chunk_end += b;
       }
-      const unsigned some = __ballot_sync(0xffffffffu, m != 0);
-      if (m) {
-        const int at = used + __popc(some & ((1u << lane) - 1));
-        first[e] = pairs + before - n;
-        p.r.expert[at] = e;
-        p.r.first[at] = first[e];
-        p.r.mask[at] = m;
+      if (n) {
+        first[e] = pairs + pair_end - n;
+        for (int c = 0; c < nc; ++c) {
+          const int at = chunks + chunk_end - nc + c;
+          p.r.expert[at] = e;
+          p.r.first[at] = first[e] + c * p.cap;
+          p.r.count[at] = min(p.cap, n - c * p.cap);
+        }
       }
-      used += __popc(some);
-      pairs += __shfl_sync(0xffffffffu, before, 31);
+      chunks += __shfl_sync(0xffffffffu, chunk_end, 31);
+      pairs += __shfl_sync(0xffffffffu, pair_end, 31);
     }
-    if (lane == 0) *p.r.n_used = used;
+    if (lane == 0) *p.r.n_chunks = chunks;
   }
   __syncthreads();
   for (int i = threadIdx.x; i < p.T * p.top_k; i += blockDim.x) {
@@ -200,178 +208,145 @@ __device__ __forceinline__ float gate_act(float g, int act) {
   return g / (1.0f + expf(-g));
 }
 
-// Tokens c0 .. of the block's expert, eight times NT of them.
-template <typename T, int G, int NT, bool VEC>
-__device__ __forceinline__ void up_tokens(const MoeArgs& p, int e, int row0, int pair0, int count,
-                                          float (*red)[2][8 * NT][17]) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int g = lane >> 2, a = lane & 3;
-  const int KB = (p.H + W4_BLOCK - 1) / W4_BLOCK;
-  const uint8_t* q[4];
-  const __nv_bfloat16* sc[4];
-#pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int i = min(row0 + (r & 1) * 8 + g, p.I - 1);
-    const int64_t n = ((int64_t)e * 2 + (r >> 1)) * p.I + i;  // gate rows, then up rows
-    q[r] = p.q13 + n * KB * 64 + a * 16;
-    sc[r] = p.s13 + n * KB * (W4_BLOCK / G);
+// Tasks: (chunk, 16 rows of I), chunk-major, an equal share for every block.
+template <typename T_, int G_, int NT_, bool VEC_>
+struct UpJob {
+  using T = T_;
+  static constexpr int G = G_, MT = 2, NT = NT_, W = 16;
+  static constexpr bool VEC = VEC_;
+  const MoeArgs& p;
+  int tiles;
+  int lo, hi;
+  __device__ __forceinline__ explicit UpJob(const MoeArgs& p_) : p(p_) {
+    tiles = (p.I + 15) / 16;
+    const int64_t all = (int64_t)*p.r.n_chunks * tiles;  // below 2^28
+    lo = (int)(all * blockIdx.x / gridDim.x);
+    hi = (int)(all * (blockIdx.x + 1) / gridDim.x);
   }
-  const uint16_t* x[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int c = nt * 8 + g;
-    x[nt] = c < count ? p.x + (int64_t)p.r.token[pair0 + c] * p.ld_x : nullptr;
+  __device__ __forceinline__ int tasks() const { return hi - lo; }
+  __device__ __forceinline__ int KB() const { return (p.H + W4_BLOCK - 1) / W4_BLOCK; }
+  __device__ __forceinline__ int K() const { return p.H; }
+  __device__ __forceinline__ int height() const { return 16; }
+  __device__ __forceinline__ int rows() const { return 2 * p.E * p.I; }
+  __device__ __forceinline__ const __nv_bfloat16* scales() const { return p.s13; }
+  __device__ __forceinline__ int chunk(int j) const { return (lo + j) / tiles; }
+  __device__ __forceinline__ int first_row(int j) const { return (lo + j) % tiles * 16; }
+  // gate rows, then up rows; a tile that passes the end of one reads what follows, for nothing
+  __device__ __forceinline__ int row(int j, int mt) const {
+    return (2 * p.r.expert[chunk(j)] + mt) * p.I + first_row(j);
   }
-  float sum[2][NT][4] = {};
-  W4Frag<G, 2> cur, next;
-  int kb = warp;
-  if (kb < KB)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) cur.load(r, q[r] + (int64_t)kb * 64, sc[r] + kb * (W4_BLOCK / G));
-  for (; kb < KB; kb += MOE_WARPS) {
-    const int nx = kb + MOE_WARPS;
-    if (nx < KB)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) next.load(r, q[r] + (int64_t)nx * 64, sc[r] + nx * (W4_BLOCK / G));
-    w4_block<T, G, 2, NT>(cur, sum, [&](int nt, int b) {
-      return x[nt] ? ld_act8<VEC>(x[nt], kb * W4_BLOCK + b * 32 + a * 8, p.H) : make_uint4(0, 0, 0, 0);
-    });
-    cur = next;
+  __device__ __forceinline__ const uint16_t* activation(int j, int col) const {
+    const int c = chunk(j);
+    return p.x + (int64_t)p.r.token[p.r.first[c] + min(col, p.r.count[c] - 1)] * p.ld_x;
   }
+  __device__ __forceinline__ void finish(int j, const float* sums, int tid) const {
+    constexpr int TILE = stream::Cfg<MT, NT, W>::TILE;
+    const int c = chunk(j), i0 = first_row(j), count = p.r.count[c];
+    const int Ip = (p.I + W4_BLOCK - 1) / W4_BLOCK * W4_BLOCK;
+    __nv_bfloat16* h = p.h + (int64_t)p.r.first[c] * 2 * Ip + i0;
+    for (int i = tid; i < 16 * count; i += stream::FINISH_WARPS * 32) {
+      const int r = i & 15, col = i >> 4;
+      float gv = 0.0f, uv = 0.0f;
 #pragma unroll
-  for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) red[warp][mt][nt * 8 + 2 * a + (i & 1)][g + 8 * (i >> 1)] = sum[mt][nt][i];
-  __syncthreads();
-  const int Ip = (p.I + W4_BLOCK - 1) / W4_BLOCK * W4_BLOCK;
-  for (int i = threadIdx.x; i < 16 * 8 * NT; i += MOE_WARPS * 32) {
-    const int r = i & 15, c = i >> 4;
-    if (c >= count) continue;
-    float gv = 0.0f, uv = 0.0f;
-#pragma unroll
-    for (int w = 0; w < MOE_WARPS; ++w) gv += red[w][0][c][r], uv += red[w][1][c][r];
-    const float v = row0 + r < p.I ? gate_act(gv, p.act) * uv : 0.0f;
-    const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-    const float rest = v - __bfloat162float(hi);
-    __nv_bfloat16* h = p.h + (int64_t)(pair0 + c) * 2 * Ip + row0 + r;
-    h[0] = hi;
-    h[Ip] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);  // an infinite or NaN value is in hi alone
+      for (int w = 0; w < W; ++w) {
+        gv += sums[w * MT * TILE + col * stream::COL_PITCH + r];
+        uv += sums[(w * MT + 1) * TILE + col * stream::COL_PITCH + r];
+      }
+      const float v = i0 + r < p.I ? gate_act(gv, p.act) * uv : 0.0f;
+      const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+      const float rest = v - __bfloat162float(hi);
+      h[(int64_t)col * 2 * Ip + r] = hi;
+      // an infinite or NaN value is in hi alone
+      h[(int64_t)col * 2 * Ip + Ip + r] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
+    }
+    // zeros from the last rows to the padded end of h
+    if (i0 + 16 >= p.I)
+      for (int i = tid; i < (Ip - i0 - 16) * count * 2; i += stream::FINISH_WARPS * 32)
+        h[(int64_t)(i % (2 * count)) * Ip + 16 + i / (2 * count)] = __float2bfloat16_rn(0.0f);
   }
-  __syncthreads();
-}
+  __device__ __forceinline__ void finish_all(int) const {}
+};
 
-template <typename T, int G, bool VEC>
-__global__ void __launch_bounds__(MOE_WARPS * 32)
-moe_up_kernel(const MoeArgs p) {
-  __shared__ __align__(16) unsigned char red[MOE_WARPS * 2 * 16 * 17 * sizeof(float)];
-  if ((int)blockIdx.y >= *p.r.n_used) return;
-  const int e = p.r.expert[blockIdx.y], pair0 = p.r.first[blockIdx.y];
-  const int count = __popcll(p.r.mask[blockIdx.y]);
-  const int row0 = blockIdx.x * 16;
-  for (int c = 0; c < count; c += 16) {
-    if (count - c <= 8)
-      up_tokens<T, G, 1, VEC>(p, e, row0, pair0 + c, count - c, reinterpret_cast<float(*)[2][8][17]>(red));
-    else
-      up_tokens<T, G, 2, VEC>(p, e, row0, pair0 + c, min(count - c, 16), reinterpret_cast<float(*)[2][16][17]>(red));
-  }
+template <typename T, int G, int NT, bool VEC>
+__global__ void __launch_bounds__(stream::Cfg<2, NT, 16>::THREADS, 1)
+moe_up_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ MoeArgs p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  UpJob<T, G, NT, VEC> job(p);
+  stream::run(job, &codes, smem, p.status);
 }
 
 // ------------------------------------------------------------------- down
-// Columns 2 j and 2 j + 1 of the MMA are value and remainder of pair j.
+// Tasks: (tile of the block's rows, chunk).  Columns 2 j and 2 j + 1 of the MMA
+// are value and remainder of pair j.
+template <int G_, int NT_>
+struct DownJob {
+  using T = __nv_bfloat16;
+  static constexpr int G = G_, MT = 1, NT = NT_, W = 16;
+  static constexpr bool VEC = true;
+  const MoeArgs& p;
+  float (*y)[17];  // [token][row]
+  int chunks, r0, r1, tiles;
+  __device__ __forceinline__ DownJob(const MoeArgs& p_, float (*y_)[17]) : p(p_), y(y_) {
+    chunks = *p.r.n_chunks;
+    r0 = (int)((int64_t)p.H * blockIdx.x / gridDim.x);
+    r1 = (int)((int64_t)p.H * (blockIdx.x + 1) / gridDim.x);
+    tiles = (r1 - r0 + p.height - 1) / p.height;
+  }
+  __device__ __forceinline__ int tasks() const { return tiles * chunks; }
+  __device__ __forceinline__ int KB() const { return (p.I + W4_BLOCK - 1) / W4_BLOCK; }
+  __device__ __forceinline__ int K() const { return KB() * W4_BLOCK; }
+  __device__ __forceinline__ int height() const { return p.height; }
+  __device__ __forceinline__ int rows() const { return p.E * p.H; }
+  __device__ __forceinline__ const __nv_bfloat16* scales() const { return p.s2; }
+  // the last tile of a block may overlap the one before, or pass the block's first row
+  __device__ __forceinline__ int first_row(int j) const { return max(min(r0 + j / chunks * p.height, r1 - p.height), 0); }
+  __device__ __forceinline__ int row(int j, int) const { return p.r.expert[j % chunks] * p.H + first_row(j); }
+  __device__ __forceinline__ const uint16_t* activation(int j, int col) const {
+    const int c = j % chunks;
+    return reinterpret_cast<const uint16_t*>(p.h) +
+           ((int64_t)p.r.first[c] * 2 + min(col, 2 * p.r.count[c] - 1)) * K();
+  }
+  __device__ __forceinline__ void finish(int j, const float* sums, int tid) const {
+    constexpr int TILE = stream::Cfg<MT, NT, W>::TILE;
+    const int c = j % chunks, first = p.r.first[c];
+    for (int i = tid; i < 16 * p.r.count[c]; i += stream::FINISH_WARPS * 32) {
+      const int r = i & 15, pair = i >> 4;  // pairs of a chunk are of different tokens
+      float v = 0.0f;
+#pragma unroll
+      for (int w = 0; w < W; ++w) {
+        const float* s = sums + w * TILE + 2 * pair * stream::COL_PITCH + r;
+        v += s[0] + s[stream::COL_PITCH];
+      }
+      float* at = &y[p.r.token[first + pair]][r];
+      *at = fmaf(p.r.weight[first + pair], v, *at);
+    }
+    if (c < chunks - 1) return;
+    stream::finish_sync();
+    for (int i = tid; i < 16 * p.T; i += stream::FINISH_WARPS * 32) {
+      const int r = i & 15, t = i >> 4, n = first_row(j) + r;
+      if (r < p.height && n >= r0 && n < r1) store_from_f32(p.out, p.dtype, (int64_t)t * p.ld_out + n, y[t][r]);
+      y[t][r] = 0.0f;
+    }
+  }
+  __device__ __forceinline__ void finish_all(int) const {}
+};
+
 template <int G, int NT>
-__device__ __forceinline__ void down_pairs(const MoeArgs& p, const uint8_t* const (&q)[2],
-                                           const __nv_bfloat16* const (&sc)[2], int kb0, int kb1, int pair0, int count,
-                                           float (*ysum)[17]) {
-  const int lane = threadIdx.x & 31;
-  const int g = lane >> 2, a = lane & 3;
-  const int Ip = (p.I + W4_BLOCK - 1) / W4_BLOCK * W4_BLOCK;
-  const uint16_t* x[NT];
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int c = nt * 8 + g;
-    x[nt] = c < 2 * count ? reinterpret_cast<const uint16_t*>(p.h) + ((int64_t)pair0 * 2 + c) * Ip : nullptr;
-  }
-  float sum[1][NT][4] = {};
-  W4Frag<G, 1> cur, next;
-#pragma unroll
-  for (int r = 0; r < 2; ++r) cur.load(r, q[r] + (int64_t)kb0 * 64, sc[r] + kb0 * (W4_BLOCK / G));
-  for (int kb = kb0; kb < kb1; ++kb) {
-    if (kb + 1 < kb1)
-#pragma unroll
-      for (int r = 0; r < 2; ++r)
-        next.load(r, q[r] + (int64_t)(kb + 1) * 64, sc[r] + (kb + 1) * (W4_BLOCK / G));
-    w4_block<__nv_bfloat16, G, 1, NT>(cur, sum, [&](int nt, int b) {
-      return x[nt] ? *reinterpret_cast<const uint4*>(x[nt] + kb * W4_BLOCK + b * 32 + a * 8) : make_uint4(0, 0, 0, 0);
-    });
-    cur = next;
-  }
-#pragma unroll
-  for (int nt = 0; nt < NT; ++nt) {
-    const int j = nt * 4 + a;
-    if (j < count) {
-      float* y = ysum[p.r.token[pair0 + j]];
-      const float w = p.r.weight[pair0 + j];
-      y[g] = fmaf(w, sum[0][nt][0] + sum[0][nt][1], y[g]);
-      y[g + 8] = fmaf(w, sum[0][nt][2] + sum[0][nt][3], y[g + 8]);
-    }
-  }
-  __syncwarp();
-}
-
-template <int G>
-__global__ void __launch_bounds__(MOE_WARPS * 32)
-moe_down_kernel(const MoeArgs p) {
-  extern __shared__ unsigned char dyn[];
-  float(*ysum)[17] = reinterpret_cast<float(*)[17]>(dyn);  // [warp][token][16]
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int n0 = blockIdx.x * 16;
-  for (int i = threadIdx.x; i < MOE_WARPS * p.T * 17; i += MOE_WARPS * 32) ysum[0][i] = 0.0f;
-  __syncthreads();
-
-  const int KB = (p.I + W4_BLOCK - 1) / W4_BLOCK;
-  const int64_t items = (int64_t)*p.r.n_used * KB;  // (expert, block of I), split evenly over the warps
-  int64_t at = items * warp / MOE_WARPS;
-  const int64_t end = items * (warp + 1) / MOE_WARPS;
-  while (at < end) {
-    const int u = (int)(at / KB), kb0 = (int)(at - (int64_t)u * KB);
-    const int kb1 = (int)min((int64_t)KB, kb0 + (end - at));
-    const int e = p.r.expert[u], pair0 = p.r.first[u], count = __popcll(p.r.mask[u]);
-    const uint8_t* q[2];
-    const __nv_bfloat16* sc[2];
-#pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      const int64_t n = (int64_t)e * p.H + min(n0 + r * 8 + (lane >> 2), p.H - 1);
-      q[r] = p.q2 + n * KB * 64 + (lane & 3) * 16;
-      sc[r] = p.s2 + n * KB * (W4_BLOCK / G);
-    }
-    float(*mine)[17] = ysum + warp * p.T;
-    for (int c = 0; c < count; c += 16) {
-      const int left = count - c;
-      if (left <= 4) down_pairs<G, 1>(p, q, sc, kb0, kb1, pair0 + c, left, mine);
-      else if (left <= 8) down_pairs<G, 2>(p, q, sc, kb0, kb1, pair0 + c, left, mine);
-      else down_pairs<G, 4>(p, q, sc, kb0, kb1, pair0 + c, min(left, 16), mine);
-    }
-    at += kb1 - kb0;
-  }
-  __syncthreads();
-  for (int i = threadIdx.x; i < p.T * 16; i += MOE_WARPS * 32) {
-    const int t = i >> 4, r = i & 15;
-    if (n0 + r >= p.H) continue;
-    float y = 0.0f;
-#pragma unroll
-    for (int w = 0; w < MOE_WARPS; ++w) y += ysum[w * p.T + t][r];
-    store_from_f32(p.out, p.dtype, (int64_t)t * p.ld_out + n0 + r, y);
-  }
+__global__ void __launch_bounds__(stream::Cfg<1, NT, 16>::THREADS, 1)
+moe_down_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ MoeArgs p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  float(*y)[17] = reinterpret_cast<float(*)[17]>(smem + stream::Cfg<1, NT, 16>::SMEM);  // behind the engine's
+  for (int i = threadIdx.x; i < p.T * 17; i += blockDim.x) y[0][i] = 0.0f;  // seen after the engine's first barrier
+  DownJob<G, NT> job(p, y);
+  stream::run(job, &codes, smem, p.status);
 }
 
 // --------------------------------------------------------------- workspace
 struct Layout {
-  int64_t logits, h, n_used, expert, first, mask, token, weight, bytes;
+  int64_t logits, h, n_chunks, expert, first, count, token, weight, bytes;
 };
 Layout layout(int64_t T, int64_t E, int64_t I, int64_t k) {
-  const int64_t pairs = T * k, used = pairs < E ? pairs : E;
+  const int64_t pairs = T * k;  // and never more chunks
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t here = at;
@@ -381,31 +356,57 @@ Layout layout(int64_t T, int64_t E, int64_t I, int64_t k) {
   Layout l;
   l.logits = take(T * E * 8);
   l.h = take(pairs * 2 * w4_padded(I) * 2);
-  l.mask = take(used * 8);
-  l.n_used = take(4);
-  l.expert = take(used * 4);
-  l.first = take(used * 4);
+  l.n_chunks = take(4);
+  l.expert = take(pairs * 4);
+  l.first = take(pairs * 4);
+  l.count = take(pairs * 4);
   l.token = take(pairs * 4);
   l.weight = take(pairs * 4);
   l.bytes = at;
   return l;
 }
 
+template <typename Tag, typename K>
+int launch_stream(K kern, int threads, int smem, int grid, const CUtensorMap& codes, const MoeArgs& p,
+                  cudaStream_t st, const char* what) {
+  if (int rc = allow_smem<Tag>(kern, smem)) return rc;
+  kern<<<grid, threads, smem, st>>>(codes, p);
+  return check_cuda(cudaGetLastError(), what);
+}
+
+// NTU, NTD: columns of eight for gate and up (one per pair), for down (two per pair)
+template <typename T, int G, int NTU, int NTD, bool VEC>
+int run_up_down(MoeArgs p, cudaStream_t st) {
+  using CU = stream::Cfg<2, NTU, 16>;
+  using CD = stream::Cfg<1, NTD, 16>;
+  constexpr int y_bytes = MOE_TOKENS * 17 * 4;
+  static_assert(CU::SMEM <= 232448 && CD::SMEM + y_bytes <= 232448, "shared memory");
+  const int KU = (int)(w4_padded(p.H) / W4_BLOCK), KD = (int)(w4_padded(p.I) / W4_BLOCK);
+  CUtensorMap up, down;
+  if (int rc = code_map(&up, p.q13, (int64_t)2 * p.E * p.I, KU, KU < stream::SEG ? KU : stream::SEG, 16)) return rc;
+  if (int rc = launch_stream<UpJob<T, G, NTU, VEC>>(moe_up_kernel<T, G, NTU, VEC>, CU::THREADS, CU::SMEM, sm_count(),
+                                                    up, p, st, "moe_up_kernel launch"))
+    return rc;
+  const int need = (p.H + 3) / 4;  // at least four rows a block
+  const int grid = need < sm_count() ? need : sm_count();
+  p.height = stream::tile_height((p.H + grid - 1) / grid, 1);
+  if (int rc = code_map(&down, p.q2, (int64_t)p.E * p.H, KD, KD < stream::SEG ? KD : stream::SEG, p.height)) return rc;
+  return launch_stream<DownJob<G, NTD>>(moe_down_kernel<G, NTD>, CD::THREADS, CD::SMEM + y_bytes, grid, down, p, st,
+                                        "moe_down_kernel launch");
+}
+
 template <typename T, int G>
 int run_experts(const MoeArgs& p, cudaStream_t st) {
-  const int64_t pairs = (int64_t)p.T * p.top_k;
-  const unsigned used = (unsigned)(pairs < p.E ? pairs : p.E);
-  const unsigned Ip = (unsigned)w4_padded(p.I);
-  const dim3 grid(Ip / 16, used);
-  if (aligned16(p.x) && p.ld_x % 8 == 0 && p.H % 8 == 0) moe_up_kernel<T, G, true><<<grid, MOE_WARPS * 32, 0, st>>>(p);
-  else moe_up_kernel<T, G, false><<<grid, MOE_WARPS * 32, 0, st>>>(p);
-  if (int rc = check_cuda(cudaGetLastError(), "moe_up_kernel launch")) return rc;
-  moe_down_kernel<G><<<(p.H + 15) / 16, MOE_WARPS * 32, MOE_WARPS * p.T * 17 * sizeof(float), st>>>(p);
-  return check_cuda(cudaGetLastError(), "moe_down_kernel launch");
+  const bool vec = aligned16(p.x) && p.ld_x % 8 == 0 && p.H % 8 == 0;
+  if (p.cap == 4) return vec ? run_up_down<T, G, 1, 1, true>(p, st) : run_up_down<T, G, 1, 1, false>(p, st);
+  if (p.cap == 8) return vec ? run_up_down<T, G, 1, 2, true>(p, st) : run_up_down<T, G, 1, 2, false>(p, st);
+  return vec ? run_up_down<T, G, 2, 4, true>(p, st) : run_up_down<T, G, 2, 4, false>(p, st);
 }
 
 template <typename T>
-int run_chunk(const MoeArgs& p, int group, cudaStream_t st) {
+int run_chunk(MoeArgs p, int group, cudaStream_t st) {
+  // an expert has at most T pairs, T top_k / E on average
+  p.cap = p.T <= 4 ? 4 : p.T <= 8 || p.T * p.top_k <= 6 * p.E ? 8 : 16;
   const dim3 grid((p.E + MOE_WARPS - 1) / MOE_WARPS, (p.T + LOGIT_TOKENS - 1) / LOGIT_TOKENS);
   if (p.router_dtype == QI8_F32) moe_logits_kernel<T, float><<<grid, MOE_WARPS * 32, 0, st>>>(p);
   else moe_logits_kernel<T, T><<<grid, MOE_WARPS * 32, 0, st>>>(p);
@@ -422,6 +423,8 @@ constexpr int MOE_MAX_TOP = 64;  // choices of 64 tokens fit the route kernel's 
 int check_sizes(int64_t T, int64_t H, int64_t E, int64_t I, int top_k) {
   QI8_REQUIRE(T >= 0 && T < (1 << 30) && H > 0 && H <= (1 << 20) && I > 0 && I <= (1 << 20), QI8_ESHAPE,
               "%lld tokens of %lld features, experts of %lld", (long long)T, (long long)H, (long long)I);
+  QI8_REQUIRE(2 * E * I < (1LL << 31) && E * H < (1LL << 31), QI8_ESHAPE, "%lld experts of %lld x %lld: too many rows",
+              (long long)E, (long long)I, (long long)H);
   QI8_REQUIRE(E > 0 && E <= MOE_MAX_EXPERTS, QI8_ESHAPE, "%lld experts: 1 to %d are supported", (long long)E,
               MOE_MAX_EXPERTS);
   QI8_REQUIRE(top_k > 0 && top_k <= E && top_k <= MOE_MAX_TOP, QI8_ESHAPE,
@@ -463,10 +466,10 @@ extern "C" int qi8_moe_w4(const void* x, int x_dtype, int64_t T, int64_t H, int6
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   MoeArgs p{static_cast<const uint16_t*>(x), ld_x, router, router_dtype, q13,
             static_cast<const __nv_bfloat16*>(s13), q2, static_cast<const __nv_bfloat16*>(s2), out, ld_out, x_dtype,
-            0, (int)H, (int)E, (int)I, top_k, renormalize != 0, act,
+            0, (int)H, (int)E, (int)I, top_k, renormalize != 0, act, 0, 0, device_status_ptr(),
             reinterpret_cast<double*>(ws + l.logits), reinterpret_cast<__nv_bfloat16*>(ws + l.h),
-            {reinterpret_cast<int*>(ws + l.n_used), reinterpret_cast<int*>(ws + l.expert),
-             reinterpret_cast<int*>(ws + l.first), reinterpret_cast<unsigned long long*>(ws + l.mask),
+            {reinterpret_cast<int*>(ws + l.n_chunks), reinterpret_cast<int*>(ws + l.expert),
+             reinterpret_cast<int*>(ws + l.first), reinterpret_cast<int*>(ws + l.count),
              reinterpret_cast<int*>(ws + l.token), reinterpret_cast<float*>(ws + l.weight)}};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int64_t t = 0; t < T; t += MOE_TOKENS) {
