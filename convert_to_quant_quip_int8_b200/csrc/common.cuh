@@ -28,7 +28,7 @@ bool device_ok();
 #define QI8_CUDA(expr) \
   do { int _rc = ::qi8::check_cuda((expr), #expr); if (_rc) return _rc; } while (0)
 
-inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+__host__ __device__ inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline int elem_size(int dtype) {
   switch (dtype) {
     case QI8_BF16: case QI8_F16: return 2;

@@ -10,17 +10,18 @@
 // is D_e.  Up to 64 tokens run together, so that an expert's weights are read
 // once for all of its tokens; longer inputs take several turns.
 //
-// Four launches, bound by the bytes of the experts in use:
-//   moe_logits_kernel  one warp per (expert, token quad)
-//   moe_route_kernel   one block: the choice, its weights, tokens by expert
-//   moe_up_kernel      streaming engine (w4_stream.cuh): tasks are 16 rows of G
-//                      and of U of one expert, h = act(g) * u
-//   moe_down_kernel    streaming engine: a block takes a share of y's rows and
-//                      goes through every expert in use; its sums never leave the
-//                      block, so nothing is added atomically and the result does
-//                      not depend on order
+// Five launches, bound by the bytes of the experts in use; each starts while the
+// one before it drains (programmatic dependent launch):
+//   moe_logits_kernel   a block per expert and eight tokens
+//   moe_route_kernel    one block: the choice, its weights, tokens by expert
+//   moe_expert_kernel   gate and up: 16 rows of G and of U per warp, h = act(g) * u
+//   moe_expert_kernel   down: 32 rows of D per warp, fp32 rows per (token, choice)
+//   moe_combine_kernel  y = sum of a token's rows with its weights, in the order of
+//                       the choices: no atomics, the same bits every time
 // An expert's tokens come in chunks of up to `cap` pairs (token, choice): as many
-// as the MMA columns of a task hold.
+// as the MMA columns of a task hold.  The warps of a block share a chunk; they
+// split K where blocks would be few, the rows otherwise (the activations then come
+// from L2 once per block, not once per warp).
 //
 // h is held as two bf16 numbers (value and remainder, 16 significant bits
 // together): rounding it to one would cost as much accuracy as the output's
@@ -31,7 +32,6 @@
 
 #include "common.cuh"
 #include "int4.cuh"
-#include "w4_stream.cuh"
 
 namespace qi8 {
 namespace {
@@ -47,7 +47,8 @@ struct Route {
   int* first;     // [chunk] its first pair
   int* count;     // [chunk] its pairs
   int* token;     // [pair]
-  float* weight;  // [pair]
+  int* pair;      // [token][choice]
+  float* weight;  // [token][choice]
 };
 
 struct MoeArgs {
@@ -65,46 +66,71 @@ struct MoeArgs {
   int T, H, E, I, top_k;
   int renorm, act;
   int cap;         // pairs per chunk
-  int height;      // rows of y per tile of the down product
-  unsigned int* status;
   double* logits;  // [T, E]
   __nv_bfloat16* h;  // [pair][2][Ip]
+  float* part;       // [pair][Hp], Hp = H to a multiple of 4
   Route r;
 };
 
 // ------------------------------------------------------------------ router
 // The choice of experts has to be that of the exact logits, so the sums are
 // fp64 (products of 16- or 24-bit factors are exact in it).
-constexpr int LOGIT_TOKENS = 4;
+constexpr int LOGIT_TOKENS = 8;
 
+// Eight values from k on as fp64, zeros from n on.
 template <typename T>
-__device__ __forceinline__ double elem64(const T* p, int64_t i) {
-  return (double)Elem<T>::to_f32(p[i]);
+__device__ __forceinline__ void load8_f64(const T* row, bool vec, int k, int n, double (&v)[8]) {
+  if (vec && k + 8 <= n) {
+    alignas(16) T b[8];
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i)
+      reinterpret_cast<uint4*>(b)[i] = __ldg(reinterpret_cast<const uint4*>(row + k) + i);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (double)Elem<T>::to_f32(b[i]);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = k + i < n ? (double)Elem<T>::to_f32(row[k + i]) : 0.0;
+  }
 }
 
 template <typename T, typename R>
 __global__ void __launch_bounds__(MOE_WARPS * 32)
 moe_logits_kernel(const MoeArgs p) {
-  const int lane = threadIdx.x & 31;
-  const int e = blockIdx.x * MOE_WARPS + (threadIdx.x >> 5);
-  if (e >= p.E) return;
-  const int t0 = blockIdx.y * LOGIT_TOKENS;
+  __shared__ double part[LOGIT_TOKENS][MOE_WARPS];
+  pdl_launch_dependents();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int e = blockIdx.x, t0 = blockIdx.y * LOGIT_TOKENS;
+  const int tokens = min(LOGIT_TOKENS, p.T - t0);
   const R* w = static_cast<const R*>(p.router) + (int64_t)e * p.H;
-  const T* x = reinterpret_cast<const T*>(p.x);
+  const T* x = reinterpret_cast<const T*>(p.x) + (int64_t)t0 * p.ld_x;
+  const bool wvec = aligned16(p.router) && (int64_t)p.H * sizeof(R) % 16 == 0;
+  const bool xvec = aligned16(p.x) && p.ld_x % 8 == 0;
   double acc[LOGIT_TOKENS] = {};
-  for (int k = lane; k < p.H; k += 32) {
-    const double r = elem64(w, k);
+  for (int k = threadIdx.x * 8; k < p.H; k += MOE_WARPS * 256) {
+    double r[8];
+    load8_f64(w, wvec, k, p.H, r);
 #pragma unroll
-    for (int j = 0; j < LOGIT_TOKENS; ++j) {
-      const int t = min(t0 + j, p.T - 1);
-      acc[j] = fma(elem64(x, (int64_t)t * p.ld_x + k), r, acc[j]);
+    for (int t = 0; t < LOGIT_TOKENS; ++t) {
+      if (t >= tokens) break;
+      double v[8];
+      load8_f64(x + t * p.ld_x, xvec, k, p.H, v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) acc[t] = fma(v[i], r[i], acc[t]);
     }
   }
 #pragma unroll
-  for (int j = 0; j < LOGIT_TOKENS; ++j) {
+  for (int t = 0; t < LOGIT_TOKENS; ++t) {
+    if (t >= tokens) break;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) acc[j] += __shfl_xor_sync(0xffffffffu, acc[j], o);
-    if (lane == 0 && t0 + j < p.T) p.logits[(int64_t)(t0 + j) * p.E + e] = acc[j];
+    for (int o = 16; o > 0; o >>= 1) acc[t] += __shfl_xor_sync(0xffffffffu, acc[t], o);
+    if (lane == 0) part[t][warp] = acc[t];
+  }
+  __syncthreads();
+  if (threadIdx.x < tokens) {
+    double sum = 0.0;
+#pragma unroll
+    for (int i = 0; i < MOE_WARPS; ++i) sum += part[threadIdx.x][i];
+    p.logits[(int64_t)(t0 + threadIdx.x) * p.E + e] = sum;
   }
 }
 
@@ -115,55 +141,69 @@ __device__ __forceinline__ unsigned long long order_key(double v) {
   return b < 0 ? ~(unsigned long long)b : (unsigned long long)b | 0x8000000000000000ull;
 }
 
+__device__ __forceinline__ double order_value(unsigned long long key) {
+  return __longlong_as_double((long long)(key >> 63 ? key & 0x7fffffffffffffffull : ~key));
+}
+
+// One warp chooses for token t; lane l holds the keys of experts l, l + 32, ...
+template <int PER_LANE>
+__device__ __forceinline__ void choose(const MoeArgs& p, int t, int lane, unsigned long long* mask, int* ids,
+                                       float* wts) {
+  const double* l = p.logits + (int64_t)t * p.E;
+  unsigned long long key[PER_LANE];
+#pragma unroll
+  for (int i = 0; i < PER_LANE; ++i) key[i] = i * 32 + lane < p.E ? order_key(l[i * 32 + lane]) : 0;
+  double top = 0.0;
+  float total = 0.0f, mine = 0.0f, mine2 = 0.0f;  // of choices lane and lane + 32
+  for (int j = 0; j < p.top_k; ++j) {
+    unsigned long long best = 0;
+    int at = 0;
+#pragma unroll
+    for (int i = 0; i < PER_LANE; ++i)
+      if (key[i] > best) best = key[i], at = i;  // the lowest expert of the lane among equal ones
+    const unsigned hi = __reduce_max_sync(0xffffffffu, (unsigned)(best >> 32));
+    const bool in_hi = (unsigned)(best >> 32) == hi;
+    const unsigned lo = __reduce_max_sync(0xffffffffu, in_hi ? (unsigned)best : 0u);
+    const bool in = in_hi && (unsigned)best == lo;
+    const int e = (int)__reduce_min_sync(0xffffffffu, in ? (unsigned)(at * 32 + lane) : 0xffffffffu);
+    const unsigned long long won = (unsigned long long)hi << 32 | lo;
+    const double v = won == ~0ull ? __longlong_as_double(0x7ff8000000000000ll) : order_value(won);
+    if (j == 0) top = v;
+    if (in && at * 32 + lane == e) {
+#pragma unroll
+      for (int i = 0; i < PER_LANE; ++i)
+        if (i == at) key[i] = 0;
+      atomicOr(&mask[e], 1ull << t);
+      ids[t * p.top_k + j] = e;
+    }
+    const float w = expf((float)(v - top));
+    total += w;
+    if ((j & 31) == lane) (j < 32 ? mine : mine2) = w;
+  }
+  if (!p.renorm) {
+    total = 0.0f;
+    for (int e = lane; e < p.E; e += 32) total += expf((float)(l[e] - top));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
+  }
+  if (lane < p.top_k) wts[t * p.top_k + lane] = mine / total;
+  if (lane + 32 < p.top_k) wts[t * p.top_k + lane + 32] = mine2 / total;
+}
+
 __global__ void __launch_bounds__(512)
 moe_route_kernel(const MoeArgs p) {
   __shared__ unsigned long long mask[MOE_MAX_EXPERTS];
   __shared__ int first[MOE_MAX_EXPERTS];
-  extern __shared__ unsigned char dyn[];  // per (token, choice): expert, weight
-  int* ids = reinterpret_cast<int*>(dyn);
-  float* wts = reinterpret_cast<float*>(ids + p.T * p.top_k);
+  extern __shared__ int ids[];  // [token][choice]
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   for (int e = threadIdx.x; e < p.E; e += blockDim.x) mask[e] = 0;
   __syncthreads();
-
+  pdl_wait();
+  pdl_launch_dependents();
   for (int t = warp; t < p.T; t += warps) {
-    const double* l = p.logits + (int64_t)t * p.E;
-    // each choice is the greatest (logit, lower expert first) below the last one
-    unsigned long long last_key = ~0ull;
-    int last_e = -1;
-    double top = 0.0;
-    for (int j = 0; j < p.top_k; ++j) {
-      unsigned long long best = 0;
-      int best_e = 0x7fffffff;
-      for (int e = lane; e < p.E; e += 32) {
-        const unsigned long long key = order_key(l[e]);
-        const bool below = key < last_key || (key == last_key && e > last_e);
-        if (below && (key > best || (key == best && e < best_e))) best = key, best_e = e;
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        const unsigned long long ok = __shfl_xor_sync(0xffffffffu, best, o);
-        const int oe = __shfl_xor_sync(0xffffffffu, best_e, o);
-        if (ok > best || (ok == best && oe < best_e)) best = ok, best_e = oe;
-      }
-      last_key = best;
-      last_e = best_e;
-      if (j == 0) top = l[best_e];
-      if (lane == 0) {
-        ids[t * p.top_k + j] = best_e;
-        atomicOr(&mask[best_e], 1ull << t);
-      }
-    }
-    __syncwarp();
-    float total = 0.0f;
-    if (p.renorm)
-      for (int j = lane; j < p.top_k; j += 32) total += expf((float)(l[ids[t * p.top_k + j]] - top));
-    else
-      for (int e = lane; e < p.E; e += 32) total += expf((float)(l[e] - top));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xffffffffu, total, o);
-    for (int j = lane; j < p.top_k; j += 32)
-      wts[t * p.top_k + j] = expf((float)(l[ids[t * p.top_k + j]] - top)) / total;
+    if (p.E <= 64) choose<2>(p, t, lane, mask, ids, p.r.weight);
+    else if (p.E <= 256) choose<8>(p, t, lane, mask, ids, p.r.weight);
+    else choose<32>(p, t, lane, mask, ids, p.r.weight);
   }
   __syncthreads();
 
@@ -198,7 +238,7 @@ moe_route_kernel(const MoeArgs p) {
     const int t = i / p.top_k, e = ids[i];
     const int at = first[e] + __popcll(mask[e] & ((1ull << t) - 1));
     p.r.token[at] = t;
-    p.r.weight[at] = wts[i];
+    p.r.pair[i] = at;
   }
 }
 
@@ -208,144 +248,150 @@ __device__ __forceinline__ float gate_act(float g, int act) {
   return g / (1.0f + expf(-g));
 }
 
-// Tasks: (chunk, 16 rows of I), chunk-major, an equal share for every block.
-template <typename T_, int G_, int NT_, bool VEC_>
-struct UpJob {
-  using T = T_;
-  static constexpr int G = G_, MT = 2, NT = NT_, W = 16;
-  static constexpr bool VEC = VEC_;
-  const MoeArgs& p;
-  int tiles;
-  int lo, hi;
-  __device__ __forceinline__ explicit UpJob(const MoeArgs& p_) : p(p_) {
-    tiles = (p.I + 15) / 16;
-    const int64_t all = (int64_t)*p.r.n_chunks * tiles;  // below 2^28
-    lo = (int)(all * blockIdx.x / gridDim.x);
-    hi = (int)(all * (blockIdx.x + 1) / gridDim.x);
-  }
-  __device__ __forceinline__ int tasks() const { return hi - lo; }
-  __device__ __forceinline__ int KB() const { return (p.H + W4_BLOCK - 1) / W4_BLOCK; }
-  __device__ __forceinline__ int K() const { return p.H; }
-  __device__ __forceinline__ int height() const { return 16; }
-  __device__ __forceinline__ int rows() const { return 2 * p.E * p.I; }
-  __device__ __forceinline__ const __nv_bfloat16* scales() const { return p.s13; }
-  __device__ __forceinline__ int chunk(int j) const { return (lo + j) / tiles; }
-  __device__ __forceinline__ int first_row(int j) const { return (lo + j) % tiles * 16; }
-  // gate rows, then up rows; a tile that passes the end of one reads what follows, for nothing
-  __device__ __forceinline__ int row(int j, int mt) const {
-    return (2 * p.r.expert[chunk(j)] + mt) * p.I + first_row(j);
-  }
-  __device__ __forceinline__ const uint16_t* activation(int j, int col) const {
-    const int c = chunk(j);
-    return p.x + (int64_t)p.r.token[p.r.first[c] + min(col, p.r.count[c] - 1)] * p.ld_x;
-  }
-  __device__ __forceinline__ void finish(int j, const float* sums, int tid) const {
-    constexpr int TILE = stream::Cfg<MT, NT, W>::TILE;
-    const int c = chunk(j), i0 = first_row(j), count = p.r.count[c];
-    const int Ip = (p.I + W4_BLOCK - 1) / W4_BLOCK * W4_BLOCK;
-    __nv_bfloat16* h = p.h + (int64_t)p.r.first[c] * 2 * Ip + i0;
-    for (int i = tid; i < 16 * count; i += stream::FINISH_WARPS * 32) {
-      const int r = i & 15, col = i >> 4;
-      float gv = 0.0f, uv = 0.0f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        gv += sums[w * MT * TILE + col * stream::COL_PITCH + r];
-        uv += sums[(w * MT + 1) * TILE + col * stream::COL_PITCH + r];
-      }
-      const float v = i0 + r < p.I ? gate_act(gv, p.act) * uv : 0.0f;
-      const __nv_bfloat16 hi = __float2bfloat16_rn(v);
-      const float rest = v - __bfloat162float(hi);
-      h[(int64_t)col * 2 * Ip + r] = hi;
-      // an infinite or NaN value is in hi alone
-      h[(int64_t)col * 2 * Ip + Ip + r] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);
-    }
-    // zeros from the last rows to the padded end of h
-    if (i0 + 16 >= p.I)
-      for (int i = tid; i < (Ip - i0 - 16) * count * 2; i += stream::FINISH_WARPS * 32)
-        h[(int64_t)(i % (2 * count)) * Ip + 16 + i / (2 * count)] = __float2bfloat16_rn(0.0f);
-  }
-  __device__ __forceinline__ void finish_all(int) const {}
-};
-
-template <typename T, int G, int NT, bool VEC>
-__global__ void __launch_bounds__(stream::Cfg<2, NT, 16>::THREADS, 1)
-moe_up_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ MoeArgs p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  UpJob<T, G, NT, VEC> job(p);
-  stream::run(job, &codes, smem, p.status);
+// h of column `col` and row i0 + r of a chunk, as value and remainder.
+__device__ __forceinline__ void store_h(const MoeArgs& p, __nv_bfloat16* h, int Ip, int col, int i, float g, float u) {
+  const float v = i < p.I ? gate_act(g, p.act) * u : 0.0f;  // zeros to the padded end
+  const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+  const float rest = v - __bfloat162float(hi);
+  h[(int64_t)col * 2 * Ip + i] = hi;
+  h[((int64_t)col * 2 + 1) * Ip + i] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);  // infinities, NaN: hi alone
 }
 
-// ------------------------------------------------------------------- down
-// Tasks: (tile of the block's rows, chunk).  Columns 2 j and 2 j + 1 of the MMA
-// are value and remainder of pair j.
-template <int G_, int NT_>
-struct DownJob {
-  using T = __nv_bfloat16;
-  static constexpr int G = G_, MT = 1, NT = NT_, W = 16;
-  static constexpr bool VEC = true;
-  const MoeArgs& p;
-  float (*y)[17];  // [token][row]
-  int chunks, r0, r1, tiles;
-  __device__ __forceinline__ DownJob(const MoeArgs& p_, float (*y_)[17]) : p(p_), y(y_) {
-    chunks = *p.r.n_chunks;
-    r0 = (int)((int64_t)p.H * blockIdx.x / gridDim.x);
-    r1 = (int)((int64_t)p.H * (blockIdx.x + 1) / gridDim.x);
-    tiles = (r1 - r0 + p.height - 1) / p.height;
-  }
-  __device__ __forceinline__ int tasks() const { return tiles * chunks; }
-  __device__ __forceinline__ int KB() const { return (p.I + W4_BLOCK - 1) / W4_BLOCK; }
-  __device__ __forceinline__ int K() const { return KB() * W4_BLOCK; }
-  __device__ __forceinline__ int height() const { return p.height; }
-  __device__ __forceinline__ int rows() const { return p.E * p.H; }
-  __device__ __forceinline__ const __nv_bfloat16* scales() const { return p.s2; }
-  // the last tile of a block may overlap the one before, or pass the block's first row
-  __device__ __forceinline__ int first_row(int j) const { return max(min(r0 + j / chunks * p.height, r1 - p.height), 0); }
-  __device__ __forceinline__ int row(int j, int) const { return p.r.expert[j % chunks] * p.H + first_row(j); }
-  __device__ __forceinline__ const uint16_t* activation(int j, int col) const {
-    const int c = j % chunks;
-    return reinterpret_cast<const uint16_t*>(p.h) +
-           ((int64_t)p.r.first[c] * 2 + min(col, 2 * p.r.count[c] - 1)) * K();
-  }
-  __device__ __forceinline__ void finish(int j, const float* sums, int tid) const {
-    constexpr int TILE = stream::Cfg<MT, NT, W>::TILE;
-    const int c = j % chunks, first = p.r.first[c];
-    for (int i = tid; i < 16 * p.r.count[c]; i += stream::FINISH_WARPS * 32) {
-      const int r = i & 15, pair = i >> 4;  // pairs of a chunk are of different tokens
-      float v = 0.0f;
-#pragma unroll
-      for (int w = 0; w < W; ++w) {
-        const float* s = sums + w * TILE + 2 * pair * stream::COL_PITCH + r;
-        v += s[0] + s[stream::COL_PITCH];
-      }
-      float* at = &y[p.r.token[first + pair]][r];
-      *at = fmaf(p.r.weight[first + pair], v, *at);
-    }
-    if (c < chunks - 1) return;
-    stream::finish_sync();
-    for (int i = tid; i < 16 * p.T; i += stream::FINISH_WARPS * 32) {
-      const int r = i & 15, t = i >> 4, n = first_row(j) + r;
-      if (r < p.height && n >= r0 && n < r1) store_from_f32(p.out, p.dtype, (int64_t)t * p.ld_out + n, y[t][r]);
-      y[t][r] = 0.0f;
-    }
-  }
-  __device__ __forceinline__ void finish_all(int) const {}
-};
+// One chunk of tokens against the rows of one expert.
+// UP:   tile 0 of a warp is 16 rows of G, tile 1 the same of U; columns are pairs.
+// down: two tiles of 16 rows of D; columns 2 j, 2 j + 1 are value and remainder of
+//       pair j, so that a thread holds both.
+// RW warps side by side over the rows, KW over the 128-feature blocks of K.
+template <typename T, int G, int NT, int RW, bool VEC, bool UP>
+__global__ void __launch_bounds__(MOE_WARPS * 32, NT == 1 ? 2 : 1)
+moe_expert_kernel(const MoeArgs p) {
+  constexpr int KW = MOE_WARPS / RW, NS = W4_BLOCK / G;
+  __shared__ float red[KW > 1 ? KW : 1][KW > 1 ? 2 : 1][KW > 1 ? 8 * NT : 1][KW > 1 ? 17 : 1];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, a = lane & 3;
+  const int rw = warp % RW, kw = warp / RW;
+  pdl_wait();
+  pdl_launch_dependents();
+  const int c = blockIdx.y;
+  if (c >= *p.r.n_chunks) return;
+  const int e = p.r.expert[c], first = p.r.first[c], count = p.r.count[c];
+  const int K = UP ? p.H : p.I, KB = (K + W4_BLOCK - 1) / W4_BLOCK;
+  const int Ip = (p.I + W4_BLOCK - 1) / W4_BLOCK * W4_BLOCK;
+  const int n0 = (blockIdx.x * RW + rw) * (UP ? 16 : 32);
+  const int rows = UP ? p.I : p.H;
+  if (KW == 1 && n0 >= (UP ? Ip : p.H)) return;
 
-template <int G, int NT>
-__global__ void __launch_bounds__(stream::Cfg<1, NT, 16>::THREADS, 1)
-moe_down_kernel(const __grid_constant__ CUtensorMap codes, const __grid_constant__ MoeArgs p) {
-  extern __shared__ __align__(128) uint8_t smem[];
-  float(*y)[17] = reinterpret_cast<float(*)[17]>(smem + stream::Cfg<1, NT, 16>::SMEM);  // behind the engine's
-  for (int i = threadIdx.x; i < p.T * 17; i += blockDim.x) y[0][i] = 0.0f;  // seen after the engine's first barrier
-  DownJob<G, NT> job(p, y);
-  stream::run(job, &codes, smem, p.status);
+  const uint8_t* q[4];
+  const __nv_bfloat16* sc[4];
+#pragma unroll
+  for (int r = 0; r < 4; ++r) {
+    const int n = min(n0 + (UP ? 0 : (r >> 1) * 16) + (r & 1) * 8 + g, rows - 1);  // rows past the end repeat the last
+    const int64_t row = UP ? ((int64_t)e * 2 + (r >> 1)) * p.I + n : (int64_t)e * p.H + n;
+    q[r] = (UP ? p.q13 : p.q2) + row * KB * 64 + a * 16;
+    sc[r] = (UP ? p.s13 : p.s2) + row * KB * NS;
+  }
+  const uint16_t* x[NT];  // columns past the end repeat the last
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int col = nt * 8 + g;
+    if (UP) x[nt] = p.x + (int64_t)p.r.token[first + min(col, count - 1)] * p.ld_x + (VEC ? 8 * a : 0);
+    else x[nt] = reinterpret_cast<const uint16_t*>(p.h) + ((int64_t)first * 2 + min(col, 2 * count - 1)) * Ip + 8 * a;
+  }
+  float sum[2][NT][4] = {};
+  W4Frag<G, 2> cur, next;
+  int kb = kw;
+  if (kb < KB)
+#pragma unroll
+    for (int r = 0; r < 4; ++r) cur.load(r, q[r] + (int64_t)kb * 64, sc[r] + kb * NS);
+  for (; kb < KB; kb += KW) {
+    if (kb + KW < KB)
+#pragma unroll
+      for (int r = 0; r < 4; ++r) next.load(r, q[r] + (int64_t)(kb + KW) * 64, sc[r] + (kb + KW) * NS);
+    if (!UP || (VEC && (kb + 1) * W4_BLOCK <= K))
+      w4_block<T, G, 2, NT>(cur, sum, [&](int nt, int b) {
+        return *reinterpret_cast<const uint4*>(x[nt] + kb * W4_BLOCK + b * 32);
+      });
+    else
+      w4_block<T, G, 2, NT>(cur, sum, [&](int nt, int b) {
+        return ld_act8<VEC>(x[nt] - (VEC ? 8 * a : 0), kb * W4_BLOCK + b * 32 + a * 8, K);
+      });
+    cur = next;
+  }
+
+  const int64_t Hp = (p.H + 3) & ~3;
+  __nv_bfloat16* h = p.h + (int64_t)first * 2 * Ip;
+  float* part = p.part + (int64_t)first * Hp;
+  if constexpr (KW == 1) {
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int r = g + 8 * (i >> 1);
+        if constexpr (UP) {
+          const int col = nt * 8 + 2 * a + (i & 1);
+          if (col < count) store_h(p, h, Ip, col, n0 + r, sum[0][nt][i], sum[1][nt][i]);
+        } else if ((i & 1) == 0) {
+          const int pair = nt * 4 + a;
+          if (pair < count) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+              if (n0 + mt * 16 + r < p.H) part[pair * Hp + n0 + mt * 16 + r] = sum[mt][nt][i] + sum[mt][nt][i + 1];
+          }
+        }
+      }
+  } else {
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) red[kw][mt][nt * 8 + 2 * a + (i & 1)][g + 8 * (i >> 1)] = sum[mt][nt][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < (UP ? 16 : 32) * count; i += MOE_WARPS * 32) {
+      if constexpr (UP) {
+        const int r = i & 15, col = i >> 4;
+        float gv = 0.0f, uv = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) gv += red[w][0][col][r], uv += red[w][1][col][r];
+        if (n0 + r < Ip) store_h(p, h, Ip, col, n0 + r, gv, uv);
+      } else {
+        const int r = i & 15, mt = (i >> 4) & 1, pair = i >> 5, n = n0 + mt * 16 + r;
+        float v = 0.0f;
+#pragma unroll
+        for (int w = 0; w < KW; ++w) v += red[w][mt][2 * pair][r] + red[w][mt][2 * pair + 1][r];
+        if (n < p.H) part[pair * Hp + n] = v;
+      }
+    }
+  }
+}
+
+// ---------------------------------------------------------------- combine
+// Four features of y per thread.
+__global__ void __launch_bounds__(128)
+moe_combine_kernel(const MoeArgs p) {
+  pdl_wait();
+  const int64_t Hp = (p.H + 3) & ~3;
+  const int n = (blockIdx.x * 128 + threadIdx.x) * 4, t = blockIdx.y;
+  if (n >= p.H) return;
+  float y[4] = {};
+  for (int j = 0; j < p.top_k; ++j) {
+    const float w = p.r.weight[t * p.top_k + j];
+    const float4 v = *reinterpret_cast<const float4*>(p.part + p.r.pair[t * p.top_k + j] * Hp + n);
+    y[0] = fmaf(w, v.x, y[0]);
+    y[1] = fmaf(w, v.y, y[1]);
+    y[2] = fmaf(w, v.z, y[2]);
+    y[3] = fmaf(w, v.w, y[3]);
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (n + i < p.H) store_from_f32(p.out, p.dtype, (int64_t)t * p.ld_out + n + i, y[i]);
 }
 
 // --------------------------------------------------------------- workspace
 struct Layout {
-  int64_t logits, h, n_chunks, expert, first, count, token, weight, bytes;
+  int64_t logits, h, part, n_chunks, expert, first, count, token, pair, weight, bytes;
 };
-Layout layout(int64_t T, int64_t E, int64_t I, int64_t k) {
+Layout layout(int64_t T, int64_t H, int64_t E, int64_t I, int64_t k) {
   const int64_t pairs = T * k;  // and never more chunks
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -356,63 +402,81 @@ Layout layout(int64_t T, int64_t E, int64_t I, int64_t k) {
   Layout l;
   l.logits = take(T * E * 8);
   l.h = take(pairs * 2 * w4_padded(I) * 2);
+  l.part = take(pairs * ((H + 3) & ~3) * 4);
   l.n_chunks = take(4);
   l.expert = take(pairs * 4);
   l.first = take(pairs * 4);
   l.count = take(pairs * 4);
   l.token = take(pairs * 4);
+  l.pair = take(pairs * 4);
   l.weight = take(pairs * 4);
   l.bytes = at;
   return l;
 }
 
-template <typename Tag, typename K>
-int launch_stream(K kern, int threads, int smem, int grid, const CUtensorMap& codes, const MoeArgs& p,
-                  cudaStream_t st, const char* what) {
-  if (int rc = allow_smem<Tag>(kern, smem)) return rc;
-  kern<<<grid, threads, smem, st>>>(codes, p);
-  return check_cuda(cudaGetLastError(), what);
+// In stream order, but scheduled while the kernel before it drains: each waits in
+// pdl_wait for that one's results.
+template <typename... KArgs, typename... Args>
+int launch_after(void (*kern)(KArgs...), dim3 grid, int threads, size_t smem, cudaStream_t st, const char* what,
+                 const Args&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, args...), what);
+}
+
+template <typename T, int G, int NT, bool VEC, bool UP>
+int launch_expert(const MoeArgs& p, cudaStream_t st) {
+  const int64_t pairs = (int64_t)p.T * p.top_k;
+  const unsigned chunks = (unsigned)(pairs < p.E + pairs / p.cap ? pairs : p.E + pairs / p.cap);
+  const int rows = UP ? (int)w4_padded(p.I) : p.H, tile = UP ? 16 : 32;
+  const unsigned tiles = (unsigned)((rows + tile - 1) / tile);
+  // eight warps over the rows when that makes two blocks per SM
+  const int64_t used = pairs < p.E ? pairs : p.E;
+  if (used * (tiles / MOE_WARPS) >= 2 * sm_count())
+    return launch_after(moe_expert_kernel<T, G, NT, MOE_WARPS, VEC, UP>,
+                        dim3((tiles + MOE_WARPS - 1) / MOE_WARPS, chunks), MOE_WARPS * 32, 0, st,
+                        "moe_expert_kernel launch", p);
+  return launch_after(moe_expert_kernel<T, G, NT, 1, VEC, UP>, dim3(tiles, chunks), MOE_WARPS * 32, 0, st,
+                      "moe_expert_kernel launch", p);
 }
 
 // NTU, NTD: columns of eight for gate and up (one per pair), for down (two per pair)
-template <typename T, int G, int NTU, int NTD, bool VEC>
-int run_up_down(MoeArgs p, cudaStream_t st) {
-  using CU = stream::Cfg<2, NTU, 16>;
-  using CD = stream::Cfg<1, NTD, 16>;
-  constexpr int y_bytes = MOE_TOKENS * 17 * 4;
-  static_assert(CU::SMEM <= 232448 && CD::SMEM + y_bytes <= 232448, "shared memory");
-  const int KU = (int)(w4_padded(p.H) / W4_BLOCK), KD = (int)(w4_padded(p.I) / W4_BLOCK);
-  CUtensorMap up, down;
-  if (int rc = code_map(&up, p.q13, (int64_t)2 * p.E * p.I, KU, KU < stream::SEG ? KU : stream::SEG, 16)) return rc;
-  if (int rc = launch_stream<UpJob<T, G, NTU, VEC>>(moe_up_kernel<T, G, NTU, VEC>, CU::THREADS, CU::SMEM, sm_count(),
-                                                    up, p, st, "moe_up_kernel launch"))
+template <typename T, int G, int NTU, int NTD>
+int run_up_down(const MoeArgs& p, cudaStream_t st) {
+  const bool vec = aligned16(p.x) && p.ld_x % 8 == 0 && p.H % 8 == 0;
+  if (int rc = vec ? launch_expert<T, G, NTU, true, true>(p, st) : launch_expert<T, G, NTU, false, true>(p, st))
     return rc;
-  const int need = (p.H + 3) / 4;  // at least four rows a block
-  const int grid = need < sm_count() ? need : sm_count();
-  p.height = stream::tile_height((p.H + grid - 1) / grid, 1);
-  if (int rc = code_map(&down, p.q2, (int64_t)p.E * p.H, KD, KD < stream::SEG ? KD : stream::SEG, p.height)) return rc;
-  return launch_stream<DownJob<G, NTD>>(moe_down_kernel<G, NTD>, CD::THREADS, CD::SMEM + y_bytes, grid, down, p, st,
-                                        "moe_down_kernel launch");
+  return launch_expert<__nv_bfloat16, G, NTD, true, false>(p, st);
 }
 
 template <typename T, int G>
 int run_experts(const MoeArgs& p, cudaStream_t st) {
-  const bool vec = aligned16(p.x) && p.ld_x % 8 == 0 && p.H % 8 == 0;
-  if (p.cap == 4) return vec ? run_up_down<T, G, 1, 1, true>(p, st) : run_up_down<T, G, 1, 1, false>(p, st);
-  if (p.cap == 8) return vec ? run_up_down<T, G, 1, 2, true>(p, st) : run_up_down<T, G, 1, 2, false>(p, st);
-  return vec ? run_up_down<T, G, 2, 4, true>(p, st) : run_up_down<T, G, 2, 4, false>(p, st);
+  const int rc = p.cap == 4   ? run_up_down<T, G, 1, 1>(p, st)
+                 : p.cap == 8 ? run_up_down<T, G, 1, 2>(p, st)
+                              : run_up_down<T, G, 2, 4>(p, st);
+  if (rc) return rc;
+  return launch_after(moe_combine_kernel, dim3((p.H + 511) / 512, p.T), 128, 0, st, "moe_combine_kernel launch", p);
 }
 
 template <typename T>
 int run_chunk(MoeArgs p, int group, cudaStream_t st) {
   // an expert has at most T pairs, T top_k / E on average
-  p.cap = p.T <= 4 ? 4 : p.T <= 8 || p.T * p.top_k <= 6 * p.E ? 8 : 16;
-  const dim3 grid((p.E + MOE_WARPS - 1) / MOE_WARPS, (p.T + LOGIT_TOKENS - 1) / LOGIT_TOKENS);
+  const int pairs = p.T * p.top_k;
+  p.cap = p.T <= 4 || pairs <= 3 * p.E ? 4 : p.T <= 8 || pairs <= 6 * p.E ? 8 : 16;
+  const dim3 grid(p.E, (p.T + LOGIT_TOKENS - 1) / LOGIT_TOKENS);
   if (p.router_dtype == QI8_F32) moe_logits_kernel<T, float><<<grid, MOE_WARPS * 32, 0, st>>>(p);
   else moe_logits_kernel<T, T><<<grid, MOE_WARPS * 32, 0, st>>>(p);
   if (int rc = check_cuda(cudaGetLastError(), "moe_logits_kernel launch")) return rc;
-  moe_route_kernel<<<1, 512, p.T * p.top_k * 8, st>>>(p);
-  if (int rc = check_cuda(cudaGetLastError(), "moe_route_kernel launch")) return rc;
+  if (int rc = launch_after(moe_route_kernel, dim3(1), 512, p.T * p.top_k * 4, st, "moe_route_kernel launch", p))
+    return rc;
   if (group == 32) return run_experts<T, 32>(p, st);
   if (group == 64) return run_experts<T, 64>(p, st);
   return run_experts<T, 128>(p, st);
@@ -423,8 +487,6 @@ constexpr int MOE_MAX_TOP = 64;  // choices of 64 tokens fit the route kernel's 
 int check_sizes(int64_t T, int64_t H, int64_t E, int64_t I, int top_k) {
   QI8_REQUIRE(T >= 0 && T < (1 << 30) && H > 0 && H <= (1 << 20) && I > 0 && I <= (1 << 20), QI8_ESHAPE,
               "%lld tokens of %lld features, experts of %lld", (long long)T, (long long)H, (long long)I);
-  QI8_REQUIRE(2 * E * I < (1LL << 31) && E * H < (1LL << 31), QI8_ESHAPE, "%lld experts of %lld x %lld: too many rows",
-              (long long)E, (long long)I, (long long)H);
   QI8_REQUIRE(E > 0 && E <= MOE_MAX_EXPERTS, QI8_ESHAPE, "%lld experts: 1 to %d are supported", (long long)E,
               MOE_MAX_EXPERTS);
   QI8_REQUIRE(top_k > 0 && top_k <= E && top_k <= MOE_MAX_TOP, QI8_ESHAPE,
@@ -439,7 +501,7 @@ using namespace qi8;
 
 extern "C" int64_t qi8_moe_w4_workspace_bytes(int64_t T, int64_t H, int64_t E, int64_t I, int top_k) {
   if (check_sizes(T, H, E, I, top_k)) return 0;
-  return layout(T < MOE_TOKENS ? T : MOE_TOKENS, E, I, top_k).bytes;
+  return layout(T < MOE_TOKENS ? T : MOE_TOKENS, H, E, I, top_k).bytes;
 }
 
 extern "C" int qi8_moe_w4(const void* x, int x_dtype, int64_t T, int64_t H, int64_t ld_x, const void* router,
@@ -460,17 +522,19 @@ extern "C" int qi8_moe_w4(const void* x, int x_dtype, int64_t T, int64_t H, int6
   QI8_REQUIRE(x && router && q13 && s13 && q2 && s2 && out && workspace, QI8_EINVAL, "null pointer");
   QI8_REQUIRE(aligned16(q13) && aligned16(s13) && aligned16(q2) && aligned16(s2) && aligned16(workspace), QI8_EALIGN,
               "4-bit codes, scales and the workspace must be 16-byte aligned");
-  const Layout l = layout(T < MOE_TOKENS ? T : MOE_TOKENS, E, I, top_k);
+  const Layout l = layout(T < MOE_TOKENS ? T : MOE_TOKENS, H, E, I, top_k);
   QI8_REQUIRE(workspace_bytes >= l.bytes, QI8_ESHAPE, "workspace of %lld bytes, %lld needed",
               (long long)workspace_bytes, (long long)l.bytes);
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   MoeArgs p{static_cast<const uint16_t*>(x), ld_x, router, router_dtype, q13,
             static_cast<const __nv_bfloat16*>(s13), q2, static_cast<const __nv_bfloat16*>(s2), out, ld_out, x_dtype,
-            0, (int)H, (int)E, (int)I, top_k, renormalize != 0, act, 0, 0, device_status_ptr(),
+            0, (int)H, (int)E, (int)I, top_k, renormalize != 0, act, 0,
             reinterpret_cast<double*>(ws + l.logits), reinterpret_cast<__nv_bfloat16*>(ws + l.h),
+            reinterpret_cast<float*>(ws + l.part),
             {reinterpret_cast<int*>(ws + l.n_chunks), reinterpret_cast<int*>(ws + l.expert),
              reinterpret_cast<int*>(ws + l.first), reinterpret_cast<int*>(ws + l.count),
-             reinterpret_cast<int*>(ws + l.token), reinterpret_cast<float*>(ws + l.weight)}};
+             reinterpret_cast<int*>(ws + l.token), reinterpret_cast<int*>(ws + l.pair),
+             reinterpret_cast<float*>(ws + l.weight)}};
   const cudaStream_t st = static_cast<cudaStream_t>(stream);
   for (int64_t t = 0; t < T; t += MOE_TOKENS) {
     p.T = (int)(T - t < MOE_TOKENS ? T - t : MOE_TOKENS);
