@@ -213,26 +213,16 @@ w4_rows_kernel(const LinArgs p) {
   }
 
   float sum[MT][NT][4] = {};
-  W4Frag<G, MT> cur, next;
-  int kb = warp;
-  if (kb < p.KB)
-#pragma unroll
-    for (int r = 0; r < 2 * MT; ++r) cur.load(r, q[r] + (int64_t)kb * 64, sc[r] + kb * (W4_BLOCK / G));
-  for (; kb < p.KB; kb += LIN_WARPS) {
-    const int nx = kb + LIN_WARPS;
-    if (nx < p.KB)
-#pragma unroll
-      for (int r = 0; r < 2 * MT; ++r) next.load(r, q[r] + (int64_t)nx * 64, sc[r] + nx * (W4_BLOCK / G));
+  w4_blocks<G, MT>(q, sc, warp, LIN_WARPS, p.KB, [&](int kb, const W4Frag<G, MT>& f) {
     if (VEC && (kb + 1) * W4_BLOCK <= p.K)
-      w4_block<T, G, MT, NT>(cur, sum, [&](int nt, int b) {
+      w4_block<T, G, MT, NT>(f, sum, [&](int nt, int b) {
         return __ldg(reinterpret_cast<const uint4*>(x[nt] + kb * W4_BLOCK + b * 32));
       });
     else
-      w4_block<T, G, MT, NT>(cur, sum, [&](int nt, int b) {
+      w4_block<T, G, MT, NT>(f, sum, [&](int nt, int b) {
         return ld_act8<VEC>(x[nt] - (VEC ? 8 * a : 0), kb * W4_BLOCK + b * 32 + a * 8, p.K);
       });
-    cur = next;
-  }
+  });
 
 #pragma unroll
   for (int mt = 0; mt < MT; ++mt)

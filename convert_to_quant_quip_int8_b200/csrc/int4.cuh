@@ -134,24 +134,65 @@ __device__ __forceinline__ uint4 ld_act8(const uint16_t* row, int k, int K) {
 // g and g + 8 of each tile (g = lane / 4), and those rows' scales.
 template <int G, int MT>
 struct W4Frag {
-  static constexpr int NS = W4_BLOCK / G;  // scales per row and block
   uint4 w[2 * MT];
-  uint2 s[2 * MT];  // NS bf16 values in the low halves first
+  uint2 s[2 * MT];  // 128 / G bf16 values, the first in the low half
 
-  __device__ __forceinline__ void load(int r, const uint8_t* q, const __nv_bfloat16* sc) {
-    w[r] = ld_stream(q);
-    load_scale(r, sc);
-  }
-  __device__ __forceinline__ void load_scale(int r, const __nv_bfloat16* sc) {
-    if (NS == 4) s[r] = __ldg(reinterpret_cast<const uint2*>(sc));
-    else if (NS == 2) s[r].x = __ldg(reinterpret_cast<const uint32_t*>(sc));
-    else s[r].x = __ldg(reinterpret_cast<const unsigned short*>(sc));
-  }
   __device__ __forceinline__ float scale(int r, int j) const {
     const uint32_t v = j < 2 ? s[r].x : s[r].y;
     return __uint_as_float((j & 1) ? (v & 0xffff0000u) : (v << 16));
   }
 };
+
+// Calls body(kb, fragment) for the 128-feature blocks first, first + step, ...
+// below end.  q, sc: the thread's rows (codes from its 16 bytes of a block on).
+// Codes are loaded one block ahead.  Scales are loaded four blocks at a time, one
+// block by each lane of a quad, and handed round by shuffles: a load that touches
+// eight rows takes L1 eight cycles, as many as a row's codes.
+template <int G, int MT, typename Body>
+__device__ __forceinline__ void w4_blocks(const uint8_t* const (&q)[2 * MT], const __nv_bfloat16* const (&sc)[2 * MT],
+                                          int first, int step, int end, Body&& body) {
+  constexpr int NS = W4_BLOCK / G;
+  const int a = threadIdx.x & 3;
+  W4Frag<G, MT> f;
+  uint4 next[2 * MT];
+  uint2 s[2 * MT], s_next[2 * MT];
+  auto load_scales = [&](int kb, uint2 (&v)[2 * MT]) {
+    kb += a * step;
+    if (kb >= end) return;
+#pragma unroll
+    for (int r = 0; r < 2 * MT; ++r) {
+      const __nv_bfloat16* at = sc[r] + kb * NS;
+      if (NS == 4) v[r] = __ldg(reinterpret_cast<const uint2*>(at));
+      else if (NS == 2) v[r].x = __ldg(reinterpret_cast<const uint32_t*>(at));
+      else v[r].x = __ldg(reinterpret_cast<const unsigned short*>(at));
+    }
+  };
+  if (first < end) {
+#pragma unroll
+    for (int r = 0; r < 2 * MT; ++r) next[r] = ld_stream(q[r] + (int64_t)first * 64);
+    load_scales(first, s_next);
+  }
+  for (int base = first; base < end; base += 4 * step) {
+#pragma unroll
+    for (int r = 0; r < 2 * MT; ++r) s[r] = s_next[r];
+    load_scales(base + 4 * step, s_next);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int kb = base + u * step;
+      if (kb >= end) break;
+#pragma unroll
+      for (int r = 0; r < 2 * MT; ++r) {
+        f.w[r] = next[r];
+        f.s[r].x = __shfl_sync(0xffffffffu, s[r].x, u, 4);
+        if (NS == 4) f.s[r].y = __shfl_sync(0xffffffffu, s[r].y, u, 4);
+      }
+      if (kb + step < end)
+#pragma unroll
+        for (int r = 0; r < 2 * MT; ++r) next[r] = ld_stream(q[r] + (int64_t)(kb + step) * 64);
+      body(kb, f);
+    }
+  }
+}
 
 // sum[mt][nt] += W X^T over one 128-feature block: lane (g, a) gets rows g
 // (elements 0, 1) and g + 8 (2, 3), columns 2 a and 2 a + 1.  act(nt, b)

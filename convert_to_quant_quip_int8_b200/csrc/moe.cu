@@ -263,7 +263,7 @@ __device__ __forceinline__ void store_h(const MoeArgs& p, __nv_bfloat16* h, int 
 //       pair j, so that a thread holds both.
 // RW warps side by side over the rows, KW over the 128-feature blocks of K.
 template <typename T, int G, int NT, int RW, bool VEC, bool UP>
-__global__ void __launch_bounds__(MOE_WARPS * 32, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(MOE_WARPS * 32, NT == 4 ? 1 : 2)
 moe_expert_kernel(const MoeArgs p) {
   constexpr int KW = MOE_WARPS / RW, NS = W4_BLOCK / G;
   __shared__ float red[KW > 1 ? KW : 1][KW > 1 ? 2 : 1][KW > 1 ? 8 * NT : 1][KW > 1 ? 17 : 1];
@@ -298,25 +298,16 @@ moe_expert_kernel(const MoeArgs p) {
     else x[nt] = reinterpret_cast<const uint16_t*>(p.h) + ((int64_t)first * 2 + min(col, 2 * count - 1)) * Ip + 8 * a;
   }
   float sum[2][NT][4] = {};
-  W4Frag<G, 2> cur, next;
-  int kb = kw;
-  if (kb < KB)
-#pragma unroll
-    for (int r = 0; r < 4; ++r) cur.load(r, q[r] + (int64_t)kb * 64, sc[r] + kb * NS);
-  for (; kb < KB; kb += KW) {
-    if (kb + KW < KB)
-#pragma unroll
-      for (int r = 0; r < 4; ++r) next.load(r, q[r] + (int64_t)(kb + KW) * 64, sc[r] + (kb + KW) * NS);
+  w4_blocks<G, 2>(q, sc, kw, KW, KB, [&](int kb, const W4Frag<G, 2>& f) {
     if (!UP || (VEC && (kb + 1) * W4_BLOCK <= K))
-      w4_block<T, G, 2, NT>(cur, sum, [&](int nt, int b) {
+      w4_block<T, G, 2, NT>(f, sum, [&](int nt, int b) {
         return *reinterpret_cast<const uint4*>(x[nt] + kb * W4_BLOCK + b * 32);
       });
     else
-      w4_block<T, G, 2, NT>(cur, sum, [&](int nt, int b) {
+      w4_block<T, G, 2, NT>(f, sum, [&](int nt, int b) {
         return ld_act8<VEC>(x[nt] - (VEC ? 8 * a : 0), kb * W4_BLOCK + b * 32 + a * 8, K);
       });
-    cur = next;
-  }
+  });
 
   const int64_t Hp = (p.H + 3) & ~3;
   __nv_bfloat16* h = p.h + (int64_t)first * 2 * Ip;
