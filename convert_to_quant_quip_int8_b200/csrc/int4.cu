@@ -186,10 +186,15 @@ dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restric
 // the 128-feature blocks in turn, and the MMAs (m16n8k16, tokens as the 8
 // columns) keep the arithmetic per weight at the unpacking alone.  fp32 sums
 // per warp, joined in shared memory in the order of the warps.
+// Measured for 1 x 65536 x 8192: 63 us, 4.4 TB/s (0.67 of the copy rate); issue
+// slots 59 %, ALU (the unpacking) 49 %, half of the stalls wait for memory.  64
+// registers, four blocks per SM: three blocks take 72 us, five with spills 78; two
+// and four blocks of codes ahead 76 and 83.  With few blocks per SM a deep
+// lookahead helps instead: 1 x 4096 x 4096 6.5 -> 5.4 us.
 constexpr int LIN_WARPS = 8;
 
-template <typename T, int G, int MT, int NT, bool VEC>
-__global__ void __launch_bounds__(LIN_WARPS * 32)
+template <typename T, int G, int MT, int NT, int AHEAD, bool VEC>
+__global__ void __launch_bounds__(LIN_WARPS * 32, NT == 1 && AHEAD == 1 ? 4 : 1)
 w4_rows_kernel(const LinArgs p) {
   __shared__ float red[LIN_WARPS][8 * NT][16 * MT + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -197,13 +202,20 @@ w4_rows_kernel(const LinArgs p) {
   const int n0 = blockIdx.x * 16 * MT;
   const int t0 = blockIdx.y * 8 * NT;
 
-  const uint8_t* q[2 * MT];
-  const __nv_bfloat16* sc[2 * MT];
+  const uint8_t* q[MT];
+  const __nv_bfloat16* sc[MT];
+  uint32_t qo[2 * MT], so[2 * MT];
 #pragma unroll
-  for (int r = 0; r < 2 * MT; ++r) {
-    const int n = min(n0 + (r >> 1) * 16 + (r & 1) * 8 + g, p.N - 1);  // rows past the end are read as the last
-    q[r] = p.q + (int64_t)n * p.KB * 64 + a * 16;
-    sc[r] = p.scale + (int64_t)n * p.KB * (W4_BLOCK / G);
+  for (int mt = 0; mt < MT; ++mt) {
+    const int64_t n = min(n0 + mt * 16, p.N - 1);
+    q[mt] = p.q + n * p.KB * 64;
+    sc[mt] = p.scale + n * p.KB * (W4_BLOCK / G);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t r = (uint32_t)(min((int)n + i * 8 + g, p.N - 1) - (int)n);  // rows past the end are read as the last
+      qo[2 * mt + i] = r * (uint32_t)p.KB * 64u + a * 16u;
+      so[2 * mt + i] = r * (uint32_t)p.KB * (W4_BLOCK / G);
+    }
   }
   const uint16_t* x[NT];
 #pragma unroll
@@ -213,7 +225,7 @@ w4_rows_kernel(const LinArgs p) {
   }
 
   float sum[MT][NT][4] = {};
-  w4_blocks<G, MT>(q, sc, warp, LIN_WARPS, p.KB, [&](int kb, const W4Frag<G, MT>& f) {
+  w4_blocks<G, MT, AHEAD>(q, sc, qo, so, warp, LIN_WARPS, p.KB, [&](int kb, const W4Frag<G, MT>& f) {
     if (VEC && (kb + 1) * W4_BLOCK <= p.K)
       w4_block<T, G, MT, NT>(f, sum, [&](int nt, int b) {
         return __ldg(reinterpret_cast<const uint4*>(x[nt] + kb * W4_BLOCK + b * 32));
@@ -343,11 +355,11 @@ extern "C" int qi8_dequant_i4(const uint8_t* q, const void* scale, int64_t rows,
 
 namespace {
 
-template <typename T, int G, int MT, int NT>
+template <typename T, int G, int MT, int NT, int AHEAD>
 int launch_rows(const LinArgs& p, bool vec, cudaStream_t st) {
   const dim3 grid((p.N + 16 * MT - 1) / (16 * MT), (p.M + 8 * NT - 1) / (8 * NT));
   return with_bool(vec, [&](auto v) {
-    w4_rows_kernel<T, G, MT, NT, decltype(v)::value><<<grid, LIN_WARPS * 32, 0, st>>>(p);
+    w4_rows_kernel<T, G, MT, NT, AHEAD, decltype(v)::value><<<grid, LIN_WARPS * 32, 0, st>>>(p);
     return check_cuda(cudaGetLastError(), "w4_rows_kernel launch");
   });
 }
@@ -407,8 +419,10 @@ extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int
     constexpr int g = decltype(G)::value;
     return with_bool(x_dtype == QI8_F16, [&](auto half) {
       using T = std::conditional_t<decltype(half)::value, __half, __nv_bfloat16>;
-      if (p.M <= 8) return launch_rows<T, g, 1, 1>(p, vec, st);
-      return launch_rows<T, g, 2, 2>(p, vec, st);
+      if (p.M > 8) return launch_rows<T, g, 2, 2, 2>(p, vec, st);
+      // few blocks per SM: more of each warp's own in flight
+      if (p.N <= 32 * sm_count()) return launch_rows<T, g, 1, 1, 4>(p, vec, st);
+      return launch_rows<T, g, 1, 1, 1>(p, vec, st);
     });
   });
 }

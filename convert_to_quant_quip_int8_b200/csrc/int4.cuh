@@ -144,34 +144,38 @@ struct W4Frag {
 };
 
 // Calls body(kb, fragment) for the 128-feature blocks first, first + step, ...
-// below end.  q, sc: the thread's rows (codes from its 16 bytes of a block on).
-// Codes are loaded one block ahead.  Scales are loaded four blocks at a time, one
+// below end.  Row r of the thread (r / 2: tile, r % 2: g or g + 8) has its codes at
+// q + qo[r] (from its 16 bytes of a block on) and its scales at sc + so[r]: a base
+// that is the same for all threads and 32-bit offsets, which spare registers.
+// Codes are loaded AHEAD (1, 2 or 4) blocks ahead.  Scales are loaded four blocks at a time, one
 // block by each lane of a quad, and handed round by shuffles: a load that touches
 // eight rows takes L1 eight cycles, as many as a row's codes.
-template <int G, int MT, typename Body>
-__device__ __forceinline__ void w4_blocks(const uint8_t* const (&q)[2 * MT], const __nv_bfloat16* const (&sc)[2 * MT],
-                                          int first, int step, int end, Body&& body) {
+template <int G, int MT, int AHEAD, typename Body>
+__device__ __forceinline__ void w4_blocks(const uint8_t* const (&q)[MT], const __nv_bfloat16* const (&sc)[MT],
+                                          const uint32_t (&qo)[2 * MT], const uint32_t (&so)[2 * MT], int first,
+                                          int step, int end, Body&& body) {
   constexpr int NS = W4_BLOCK / G;
   const int a = threadIdx.x & 3;
   W4Frag<G, MT> f;
-  uint4 next[2 * MT];
+  uint4 next[AHEAD][2 * MT];
   uint2 s[2 * MT], s_next[2 * MT];
   auto load_scales = [&](int kb, uint2 (&v)[2 * MT]) {
     kb += a * step;
     if (kb >= end) return;
 #pragma unroll
     for (int r = 0; r < 2 * MT; ++r) {
-      const __nv_bfloat16* at = sc[r] + kb * NS;
+      const __nv_bfloat16* at = sc[r >> 1] + (so[r] + (uint32_t)(kb * NS));
       if (NS == 4) v[r] = __ldg(reinterpret_cast<const uint2*>(at));
       else if (NS == 2) v[r].x = __ldg(reinterpret_cast<const uint32_t*>(at));
       else v[r].x = __ldg(reinterpret_cast<const unsigned short*>(at));
     }
   };
-  if (first < end) {
+  load_scales(first, s_next);
 #pragma unroll
-    for (int r = 0; r < 2 * MT; ++r) next[r] = ld_stream(q[r] + (int64_t)first * 64);
-    load_scales(first, s_next);
-  }
+  for (int i = 0; i < AHEAD; ++i)
+    if (first + i * step < end)
+#pragma unroll
+      for (int r = 0; r < 2 * MT; ++r) next[i][r] = ld_stream(q[r >> 1] + (qo[r] + (uint32_t)(first + i * step) * 64u));
   for (int base = first; base < end; base += 4 * step) {
 #pragma unroll
     for (int r = 0; r < 2 * MT; ++r) s[r] = s_next[r];
@@ -182,13 +186,13 @@ __device__ __forceinline__ void w4_blocks(const uint8_t* const (&q)[2 * MT], con
       if (kb >= end) break;
 #pragma unroll
       for (int r = 0; r < 2 * MT; ++r) {
-        f.w[r] = next[r];
+        f.w[r] = next[u % AHEAD][r];
         f.s[r].x = __shfl_sync(0xffffffffu, s[r].x, u, 4);
         if (NS == 4) f.s[r].y = __shfl_sync(0xffffffffu, s[r].y, u, 4);
       }
-      if (kb + step < end)
+      if (kb + AHEAD * step < end)
 #pragma unroll
-        for (int r = 0; r < 2 * MT; ++r) next[r] = ld_stream(q[r] + (int64_t)(kb + step) * 64);
+        for (int r = 0; r < 2 * MT; ++r) next[u % AHEAD][r] = ld_stream(q[r >> 1] + (qo[r] + (uint32_t)(kb + AHEAD * step) * 64u));
       body(kb, f);
     }
   }

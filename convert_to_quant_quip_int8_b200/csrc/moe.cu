@@ -281,14 +281,21 @@ moe_expert_kernel(const MoeArgs p) {
   const int rows = UP ? p.I : p.H;
   if (KW == 1 && n0 >= (UP ? Ip : p.H)) return;
 
-  const uint8_t* q[4];
-  const __nv_bfloat16* sc[4];
+  const uint8_t* q[2];
+  const __nv_bfloat16* sc[2];
+  uint32_t qo[4], so[4];
+  const int b0 = min(blockIdx.x * RW * (UP ? 16 : 32), rows - 1);  // the block's first row
 #pragma unroll
-  for (int r = 0; r < 4; ++r) {
-    const int n = min(n0 + (UP ? 0 : (r >> 1) * 16) + (r & 1) * 8 + g, rows - 1);  // rows past the end repeat the last
-    const int64_t row = UP ? ((int64_t)e * 2 + (r >> 1)) * p.I + n : (int64_t)e * p.H + n;
-    q[r] = (UP ? p.q13 : p.q2) + row * KB * 64 + a * 16;
-    sc[r] = (UP ? p.s13 : p.s2) + row * KB * NS;
+  for (int mt = 0; mt < 2; ++mt) {
+    const int64_t row = UP ? ((int64_t)e * 2 + mt) * p.I + b0 : (int64_t)e * p.H + b0;
+    q[mt] = (UP ? p.q13 : p.q2) + row * KB * 64;
+    sc[mt] = (UP ? p.s13 : p.s2) + row * KB * NS;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t r = (uint32_t)(min(n0 + (UP ? 0 : mt * 16) + i * 8 + g, rows - 1) - b0);  // past the end: the last
+      qo[2 * mt + i] = r * (uint32_t)KB * 64u + a * 16u;
+      so[2 * mt + i] = r * (uint32_t)KB * NS;
+    }
   }
   const uint16_t* x[NT];  // columns past the end repeat the last
 #pragma unroll
@@ -298,7 +305,7 @@ moe_expert_kernel(const MoeArgs p) {
     else x[nt] = reinterpret_cast<const uint16_t*>(p.h) + ((int64_t)first * 2 + min(col, 2 * count - 1)) * Ip + 8 * a;
   }
   float sum[2][NT][4] = {};
-  w4_blocks<G, 2>(q, sc, kw, KW, KB, [&](int kb, const W4Frag<G, 2>& f) {
+  w4_blocks<G, 2, 1>(q, sc, qo, so, kw, KW, KB, [&](int kb, const W4Frag<G, 2>& f) {
     if (!UP || (VEC && (kb + 1) * W4_BLOCK <= K))
       w4_block<T, G, 2, NT>(f, sum, [&](int nt, int b) {
         return *reinterpret_cast<const uint4*>(x[nt] + kb * W4_BLOCK + b * 32);
