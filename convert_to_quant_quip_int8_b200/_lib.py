@@ -121,6 +121,27 @@ def load() -> ctypes.CDLL:
     return _lib
 
 
+_call = None
+
+
+def fast_call():
+    """The host-side shortcut of the 4-bit operators (csrc/call.cpp), bound to
+    libqi8; ``None`` where it was not built for this interpreter and torch."""
+    global _call
+    if _call is None:
+        lib = load()
+        try:
+            from . import _call as mod
+        except ImportError:
+            _call = False
+        else:
+            mod.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
+                lib.qi8_quant_weight_i4, lib.qi8_dequant_i4, lib.qi8_gemm_w4, lib.qi8_moe_w4,
+                lib.qi8_moe_w4_workspace_bytes)))
+            _call = mod
+    return _call or None
+
+
 def last_error() -> str:
     return load().qi8_last_error().decode(errors="replace")
 

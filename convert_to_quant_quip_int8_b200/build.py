@@ -16,6 +16,7 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libqi8.so")
+CALL = os.path.join(PKG, "_call.so")
 BUILD_DIR = os.path.join(PKG, "_build")
 
 NVCC_FLAGS = [
@@ -81,5 +82,30 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     return LIB
 
 
+def build_call(force: bool = False, verbose: bool = False) -> str:
+    """Compile ``_call.so`` (csrc/call.cpp, host code against torch's C++ headers) if it is out of date."""
+    src = os.path.join(CSRC, "call.cpp")
+    deps = [src, os.path.join(os.path.dirname(PKG), "include", "qi8.h")]
+    if not force and os.path.exists(CALL) and os.path.getmtime(CALL) > max(os.path.getmtime(d) for d in deps):
+        return CALL
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    inc, lib = os.path.join(root, "include"), os.path.join(root, "lib")
+    cuda = os.path.join(os.path.dirname(os.path.dirname(nvcc_path())), "include")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-shared", "-std=c++17", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + inc,
+           "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + cuda,
+           "-I" + sysconfig.get_paths()["include"], src, "-o", CALL + ".tmp", "-L" + lib, "-lc10", "-lc10_cuda",
+           "-ltorch_cpu", "-ltorch_python"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(CALL + ".tmp", CALL)
+    return CALL
+
+
 if __name__ == "__main__":
+    build_call(force="--force" in sys.argv, verbose=True)
     print(build(force="--force" in sys.argv, verbose=True, ptxas_verbose="-v" in sys.argv))

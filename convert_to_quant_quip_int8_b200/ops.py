@@ -492,6 +492,12 @@ def _one_device(x: torch.Tensor, *tensors: Optional[torch.Tensor]) -> torch.devi
     return dev
 
 
+def _fast(name: str, *args):
+    """The shortcut's result for arguments that need no conversion; ``None`` for all others, errors among them."""
+    fast = L.fast_call() if L._call is None else L._call
+    return getattr(fast, name)(*args) if fast else None
+
+
 # the current stream of a device as a plain pointer: a tenth of the cost of a Stream object
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else \
     (lambda index: torch.cuda.current_stream(index).cuda_stream)
@@ -534,6 +540,9 @@ def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
 
 def quant_weight_i4(w: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
     """4-bit codes and group scales of ``w`` [..., N, K]: ``(q uint8 [..., N, Kp/2], scale bf16 [..., N, Kp/group])``."""
+    pair = _fast("quant_weight_i4", w, group)
+    if pair is not None:
+        return pair
     dev = _one_device(w)
     _no_grad(w)
     dt = L.dtype_code(w.dtype)
@@ -556,6 +565,9 @@ def quant_weight_i4(w: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, to
 def dequant_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int = 128,
                out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """The weight [..., N, k] that 4-bit codes and scales stand for."""
+    out = _fast("dequant_i4", q, scale, k, group, out_dtype)
+    if out is not None:
+        return out
     dev = _one_device(q, scale)
     _check_i4(q, scale, k, group, q.dim())
     assert q.dim() >= 2, f"4-bit codes of shape {tuple(q.shape)}: expected [..., N, Kp/2]"
@@ -571,6 +583,10 @@ def dequant_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int = 128,
 def gemm_w4(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, group: int = 128,
             bias: Optional[torch.Tensor] = None, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
     """``x [..., K] W^T + bias`` with the 4-bit weight ``q`` [N, Kp/2], ``scale`` [N, Kp/group]."""
+    if out_dtype is None:
+        out = _fast("gemm_w4", x, q, scale, group, bias)
+        if out is not None:
+            return out
     dev = _one_device(x, q, scale, bias)
     _no_grad(x, bias)
     shape = x.shape
@@ -607,6 +623,9 @@ def moe_w4(x: torch.Tensor, router: torch.Tensor, q13: torch.Tensor, s13: torch.
            act: int = L.QI8_ACT_SILU) -> torch.Tensor:
     """A mixture-of-experts layer on ``x`` [..., H] with 4-bit experts: ``router`` [E, H], ``q13``/``s13`` of
     [E, 2 I, H] (gate rows above up rows), ``q2``/``s2`` of [E, H, I]."""
+    out = _fast("moe_w4", x, router, q13, s13, q2, s2, top_k, group, bool(renormalize), act)
+    if out is not None:
+        return out
     dev = _one_device(x, router, q13, s13, q2, s2)
     _no_grad(x, router)
     h = x.shape[-1]

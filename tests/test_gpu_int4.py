@@ -551,3 +551,29 @@ def test_decode_step_of_a_quantized_block(t):
     v2 = I4.weight_dequant_int4(q2, s2, i, group, F32).double()
     close(m, *moe_reference(a, router, v13, v2, 2, True, "silu"))
     close(y, m.double() @ vo.T, ACC * (m.double().abs() @ vo.abs().T))
+
+
+def test_shortcut_and_python_path_agree(monkeypatch):
+    """The wrappers' host-side shortcut computes what they compute without it, and leaves the rest to them."""
+    assert L.fast_call() is not None, "csrc/call.cpp is not built"
+    w = randn(3, 40, 300, seed=1, dtype=BF)
+    x, b = randn(2, 5, 300, seed=2, dtype=BF), randn(40, seed=3)
+    mx, router, q13, s13, _, q2, s2, _ = moe_case(7, 6, 2, 256, 64, 64, BF, seed=4)
+
+    def calls():
+        q, s = I4.weight_quant_int4(w, 64)
+        return [q, s, I4.weight_dequant_int4(q, s, 300, 64, BF), I4.int4_linear(x, q[0], s[0], 64, b),
+                I4.int4_linear(x[0], q[0], s[0], 64), I4.moe_int4(mx, router, q13, s13, q2, s2, 2, 64, False, "gelu"),
+                I4.moe_int4(mx.view(1, 7, 256), router.float(), q13, s13, q2, s2, 2, 64)]
+
+    fast = calls()
+    f = L.fast_call()
+    q, s = fast[0][0].contiguous(), fast[1][0].contiguous()
+    xg = x.clone().requires_grad_()
+    for args in ((x[..., ::2], q, s, 64, None), (x, q, s, 128, None), (x.float(), q, s, 64, None),
+                 (xg, q, s, 64, None), (x, q, s, 64, b[:39]), (x.cpu(), q, s, 64, None), (x, q.cpu(), s, 64, None),
+                 (x, q, s, 64, b.double()), (x[0, 0], q, s, 64, None), (x[:, :0], q, s, 64, None)):
+        assert f.gemm_w4(*args) is None
+    monkeypatch.setattr(L, "_call", False)
+    for a, c in zip(fast, calls()):
+        assert a.shape == c.shape and a.dtype == c.dtype and torch.equal(a, c)
