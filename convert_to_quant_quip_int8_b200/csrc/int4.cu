@@ -20,37 +20,38 @@ namespace qi8 {
 namespace {
 
 // ------------------------------------------------------------ quantization
-// One thread per word of eight features, groups of 4, 8 or 16 neighbouring
-// lanes.  Threads walk the words of the whole matrix in memory order of w; the
-// (row, word) pair advances by a constant step without a division.
+// A thread handles 16 bytes of codes: words 4 a .. 4 a + 3 of a 128-feature block,
+// which are features 32 b + 8 a .. + 7 for b = 0 .. 3.  The quad a = 0 .. 3 covers
+// the block, so a group of 32 is the quad's maximum for one b, larger groups
+// combine b's in the thread.  Four loads of 16 bytes per thread and step keep HBM
+// busy (one word per thread and step: 31 us for each of 10240 x 4096 bf16 to codes
+// and back, four: see the launches).  Threads walk the matrix in the order of the
+// codes; the (row, piece) pair advances by a constant step without a division.
 constexpr int Q_THREADS = 256;
 
 struct Walk {
   int64_t row;
-  int word;  // of the row, in feature order
+  int piece;  // of the row, 32 features each
   int64_t step_row;
-  int step_word;
-  int words;  // per row
-  __device__ __forceinline__ Walk(int64_t at, int64_t step, int words_) : words(words_) {
-    row = at / words;
-    word = (int)(at - row * words);
-    step_row = step / words;
-    step_word = (int)(step - step_row * words);
+  int step_piece;
+  int pieces;  // per row, a multiple of 4
+  __device__ __forceinline__ Walk(int64_t at, int64_t step, int pieces_) : pieces(pieces_) {
+    row = at / pieces;
+    piece = (int)(at - row * pieces);
+    step_row = step / pieces;
+    step_piece = (int)(step - step_row * pieces);
   }
   __device__ __forceinline__ void advance() {
     row += step_row;
-    word += step_word;
-    if (word >= words) {
-      word -= words;
+    piece += step_piece;
+    if (piece >= pieces) {
+      piece -= pieces;
       ++row;
     }
   }
+  // first feature of word b
+  __device__ __forceinline__ int feature(int b) const { return (piece >> 2) * 128 + 32 * b + 8 * (piece & 3); }
 };
-
-// Position inside the row's words of the word that starts at feature 8 j.
-__device__ __forceinline__ int word_slot(int j) {
-  return (j & ~15) | ((j & 3) << 2) | ((j >> 2) & 3);
-}
 
 template <typename T, bool VEC>
 __device__ __forceinline__ void load8(const T* row, int k, int K, float (&v)[8]) {
@@ -107,38 +108,52 @@ template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 quant_i4_kernel(const T* __restrict__ w, int64_t ld, int64_t rows, int K, int Kp, uint32_t* __restrict__ q,
                 __nv_bfloat16* __restrict__ scale) {
-  constexpr int LANES = G / 8;  // of a group
-  const int words = Kp / 8;
-  // rows * words is a multiple of 16: a group's lanes are all in or all out
-  for (Walk at((int64_t)blockIdx.x * Q_THREADS + threadIdx.x, (int64_t)gridDim.x * Q_THREADS, words); ;
+  constexpr int NS = W4_BLOCK / G, PER = 4 / NS;  // groups per block, words of a group in this thread
+  const int pieces = Kp / 32;
+  // rows * pieces is a multiple of 4: a quad is all in or all out
+  for (Walk at((int64_t)blockIdx.x * Q_THREADS + threadIdx.x, (int64_t)gridDim.x * Q_THREADS, pieces); ;
        at.advance()) {
     const bool in = at.row < rows;
     if (!__any_sync(0xffffffffu, in)) break;
-    float v[8];
-    if (in) load8<T, VEC>(w + at.row * ld, at.word * 8, K, v);
-    else
+    float v[4][8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) v[i] = 0.0f;
-    uint32_t m = 0;  // as bits: NaN counts above infinity
+    for (int b = 0; b < 4; ++b) {
+      if (in) load8<T, VEC>(w + at.row * ld, at.feature(b), K, v[b]);
+      else
 #pragma unroll
-    for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[i]) & 0x7fffffffu);
-#pragma unroll
-    for (int o = LANES / 2; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const bool finite = m < 0x7f800000u;
-    const float s = fmaxf(round5(__fdiv_rn(__uint_as_float(finite ? m : 0u), 7.0f)), 0x1p-100f);
-    const float inv = __frcp_rn(s);
-    uint32_t word = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      // nibble order 0, 2, 4, 6, 1, 3, 5, 7
-      const uint32_t u = code_bits<T>(v[i], s, inv) & 15u;
-      word |= u << (4 * ((i >> 1) + 4 * (i & 1)));
+        for (int i = 0; i < 8; ++i) v[b][i] = 0.0f;
     }
-    if (in) {
-      q[at.row * words + word_slot(at.word)] = finite ? word : 0x88888888u;
-      if ((at.word & (LANES - 1)) == 0)
-        scale[at.row * (Kp / G) + at.word / LANES] =
-            finite ? __float2bfloat16_rn(s) : __ushort_as_bfloat16((unsigned short)0x7fffu);
+    uint32_t word[4], scales[NS];
+#pragma unroll
+    for (int j = 0; j < NS; ++j) {
+      uint32_t m = 0;  // as bits: NaN counts above infinity
+#pragma unroll
+      for (int b = j * PER; b < (j + 1) * PER; ++b)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[b][i]) & 0x7fffffffu);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const bool finite = m < 0x7f800000u;
+      const float s = fmaxf(round5(__fdiv_rn(__uint_as_float(finite ? m : 0u), 7.0f)), 0x1p-100f);
+      const float inv = __frcp_rn(s);
+      scales[j] = finite ? __float_as_uint(s) >> 16 : 0x7fffu;  // five significant bits: exact in bf16
+#pragma unroll
+      for (int b = j * PER; b < (j + 1) * PER; ++b) {
+        uint32_t c = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)  // nibble order 0, 2, 4, 6, 1, 3, 5, 7
+          c |= (code_bits<T>(v[b][i], s, inv) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
+        word[b] = finite ? c : 0x88888888u;
+      }
+    }
+    if (!in) continue;
+    reinterpret_cast<uint4*>(q)[at.row * pieces + at.piece] = make_uint4(word[0], word[1], word[2], word[3]);
+    if ((at.piece & 3) == 0) {
+      __nv_bfloat16* s = scale + at.row * (Kp / G) + (at.piece >> 2) * NS;
+      if constexpr (NS == 4)
+        *reinterpret_cast<uint2*>(s) = make_uint2(scales[0] | scales[1] << 16, scales[2] | scales[3] << 16);
+      else if constexpr (NS == 2) *reinterpret_cast<uint32_t*>(s) = scales[0] | scales[1] << 16;
+      else *reinterpret_cast<unsigned short*>(s) = (unsigned short)scales[0];
     }
   }
 }
@@ -148,34 +163,40 @@ template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restrict__ scale, int64_t rows, int K, int Kp,
                   T* __restrict__ out, int64_t ld) {
-  const int words = Kp / 8;
-  for (Walk at((int64_t)blockIdx.x * Q_THREADS + threadIdx.x, (int64_t)gridDim.x * Q_THREADS, words);
+  constexpr int NS = W4_BLOCK / G;
+  const int pieces = Kp / 32;
+  for (Walk at((int64_t)blockIdx.x * Q_THREADS + threadIdx.x, (int64_t)gridDim.x * Q_THREADS, pieces);
        at.row < rows; at.advance()) {
-    const int k = at.word * 8;
-    if (k >= K) continue;
-    const uint32_t w = __ldg(q + at.row * words + word_slot(at.word));
-    const float s = __bfloat162float(scale[at.row * (Kp / G) + k / G]);
-    T* o = out + at.row * ld + k;
-    float v[8];
+    const uint4 w = __ldg(reinterpret_cast<const uint4*>(q) + at.row * pieces + at.piece);
+    const __nv_bfloat16* sc = scale + at.row * (Kp / G) + (at.piece >> 2) * NS;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t u = (w >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u;
-      v[i] = (__uint_as_float(0x4B000000u | u) - 8388616.0f) * s;  // 2^23 + u - (2^23 + 8)
-    }
-    if (VEC && k + 8 <= K) {
-      if constexpr (sizeof(T) == 4) {
-        reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
-      } else {
-        alignas(16) T h[8];
+    for (int b = 0; b < 4; ++b) {
+      const int k = at.feature(b);
+      if (k >= K) break;
+      const float s = __bfloat162float(sc[b * NS / 4]);
+      const uint32_t c = word_of(w, b);
+      T* o = out + at.row * ld + k;
+      float v[8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) h[i] = Elem<T>::from_f32(v[i]);
-        *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(h);
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t u = (c >> (4 * ((i >> 1) + 4 * (i & 1)))) & 15u;
+        v[i] = (__uint_as_float(0x4B000000u | u) - 8388616.0f) * s;  // 2^23 + u - (2^23 + 8)
       }
-    } else {
+      if (VEC && k + 8 <= K) {
+        if constexpr (sizeof(T) == 4) {
+          reinterpret_cast<float4*>(o)[0] = make_float4(v[0], v[1], v[2], v[3]);
+          reinterpret_cast<float4*>(o)[1] = make_float4(v[4], v[5], v[6], v[7]);
+        } else {
+          alignas(16) T h[8];
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (k + i < K) o[i] = Elem<T>::from_f32(v[i]);
+          for (int i = 0; i < 8; ++i) h[i] = Elem<T>::from_f32(v[i]);
+          *reinterpret_cast<uint4*>(o) = *reinterpret_cast<const uint4*>(h);
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+          if (k + i < K) o[i] = Elem<T>::from_f32(v[i]);
+      }
     }
   }
 }
@@ -321,7 +342,7 @@ extern "C" int qi8_quant_weight_i4(const void* w, int w_dtype, int64_t rows, int
       using T = decltype(t);
       if (rows == 0) return (int)QI8_OK;
       return with_bool(aligned16(w) && ld_w * sizeof(T) % 16 == 0, [&](auto vec) {
-        quant_i4_kernel<T, decltype(G)::value, decltype(vec)::value><<<q_grid(rows * (Kp / 8)), Q_THREADS, 0, st>>>(
+        quant_i4_kernel<T, decltype(G)::value, decltype(vec)::value><<<q_grid(rows * (Kp / 32)), Q_THREADS, 0, st>>>(
             static_cast<const T*>(w), ld_w, rows, (int)K, Kp, reinterpret_cast<uint32_t*>(q_out),
             static_cast<__nv_bfloat16*>(scale_out));
         return check_cuda(cudaGetLastError(), "quant_i4_kernel launch");
@@ -344,7 +365,7 @@ extern "C" int qi8_dequant_i4(const uint8_t* q, const void* scale, int64_t rows,
       using T = decltype(t);
       if (rows == 0) return (int)QI8_OK;
       return with_bool(aligned16(out) && ld_out * sizeof(T) % 16 == 0, [&](auto vec) {
-        dequant_i4_kernel<T, decltype(G)::value, decltype(vec)::value><<<q_grid(rows * (Kp / 8)), Q_THREADS, 0, st>>>(
+        dequant_i4_kernel<T, decltype(G)::value, decltype(vec)::value><<<q_grid(rows * (Kp / 32)), Q_THREADS, 0, st>>>(
             reinterpret_cast<const uint32_t*>(q), static_cast<const __nv_bfloat16*>(scale), rows, (int)K, Kp,
             static_cast<T*>(out), ld_out);
         return check_cuda(cudaGetLastError(), "dequant_i4_kernel launch");
