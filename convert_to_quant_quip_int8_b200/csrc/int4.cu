@@ -24,8 +24,8 @@ namespace {
 // which are features 32 b + 8 a .. + 7 for b = 0 .. 3.  The quad a = 0 .. 3 covers
 // the block, so a group of 32 is the quad's maximum for one b, larger groups
 // combine b's in the thread.  Four loads of 16 bytes per thread and step keep HBM
-// busy (one word per thread and step: 31 us for each of 10240 x 4096 bf16 to codes
-// and back, four: see the launches).  Threads walk the matrix in the order of the
+// busy (10240 x 4096 bf16 to codes and back: 62 us with one word per thread and
+// step, 40 with four; 20 each).  Threads walk the matrix in the order of the
 // codes; the (row, piece) pair advances by a constant step without a division.
 constexpr int Q_THREADS = 256;
 
@@ -104,6 +104,81 @@ __device__ __forceinline__ uint32_t code_bits(float w, float s, float inv) {
   }
 }
 
+// Words of 16-bit weights: pairs as they lie in memory, absolute values compared
+// as pairs of 16-bit integers, codes joined by multiply-adds (1 instruction per
+// weight for each; 10240 x 4096 bf16 take 20 us, 28 as fp32 values, 16 at the copy rate).
+template <typename T> struct Piece16 {
+  uint4 r[4];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const T* row, int b, int k, int K) {
+    const uint16_t* raw = reinterpret_cast<const uint16_t*>(row);
+    if (VEC && k + 8 <= K) r[b] = __ldg(reinterpret_cast<const uint4*>(raw + k));
+    else r[b] = ld_act8<false>(raw, k, K);
+  }
+  __device__ __forceinline__ void clear(int b) { r[b] = make_uint4(0, 0, 0, 0); }
+  // largest magnitude of words [b0, b1), as bits of fp32 (NaN above infinity)
+  __device__ __forceinline__ uint32_t amax(int b0, int b1) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int b = b0; b < b1; ++b)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint32_t a = word_of(r[b], i) & 0x7fff7fffu;
+        asm("max.u16x2 %0, %0, %1;" : "+r"(m) : "r"(a));
+      }
+    const uint32_t top = max(m >> 16, m & 0xffffu);
+    if constexpr (std::is_same<T, __half>::value)
+      return top >= 0x7c00u ? 0x7f800000u : __float_as_uint(__half2float(__ushort_as_half((unsigned short)top)));
+    else return top << 16;
+  }
+  __device__ __forceinline__ uint32_t codes(int b, float, float inv) const {
+    // code_bits is 0x4B400000 + code + 8; the constants' sum over the nibbles comes off at the end
+    uint32_t c = 0u - (0x4B400000u + 0xB4000000u + 0x40000000u);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint32_t w = word_of(r[b], i);
+      float lo, hi;
+      if constexpr (std::is_same<T, __half>::value) {
+        lo = __half2float(__ushort_as_half((unsigned short)(w & 0xffffu)));
+        hi = __half2float(__ushort_as_half((unsigned short)(w >> 16)));
+      } else {
+        lo = __uint_as_float(w << 16);
+        hi = __uint_as_float(w & 0xffff0000u);
+      }
+      c += code_bits<T>(lo, 0.0f, inv) * (1u << (4 * i));
+      c += code_bits<T>(hi, 0.0f, inv) * (1u << (4 * i + 16));
+    }
+    return c;
+  }
+};
+// Words of fp32 weights.
+struct Piece32 {
+  float v[4][8];
+  template <bool VEC>
+  __device__ __forceinline__ void load(const float* row, int b, int k, int K) {
+    load8<float, VEC>(row, k, K, v[b]);
+  }
+  __device__ __forceinline__ void clear(int b) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[b][i] = 0.0f;
+  }
+  __device__ __forceinline__ uint32_t amax(int b0, int b1) const {
+    uint32_t m = 0;
+#pragma unroll
+    for (int b = b0; b < b1; ++b)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[b][i]) & 0x7fffffffu);
+    return m;
+  }
+  __device__ __forceinline__ uint32_t codes(int b, float s, float inv) const {
+    uint32_t c = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)  // nibble order 0, 2, 4, 6, 1, 3, 5, 7
+      c |= (code_bits<float>(v[b][i], s, inv) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
+    return c;
+  }
+};
+
 template <typename T, int G, bool VEC>
 __global__ void __launch_bounds__(Q_THREADS)
 quant_i4_kernel(const T* __restrict__ w, int64_t ld, int64_t rows, int K, int Kp, uint32_t* __restrict__ q,
@@ -115,22 +190,16 @@ quant_i4_kernel(const T* __restrict__ w, int64_t ld, int64_t rows, int K, int Kp
        at.advance()) {
     const bool in = at.row < rows;
     if (!__any_sync(0xffffffffu, in)) break;
-    float v[4][8];
+    std::conditional_t<sizeof(T) == 4, Piece32, Piece16<T>> v;
 #pragma unroll
     for (int b = 0; b < 4; ++b) {
-      if (in) load8<T, VEC>(w + at.row * ld, at.feature(b), K, v[b]);
-      else
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[b][i] = 0.0f;
+      if (in) v.template load<VEC>(w + at.row * ld, b, at.feature(b), K);
+      else v.clear(b);
     }
     uint32_t word[4], scales[NS];
 #pragma unroll
     for (int j = 0; j < NS; ++j) {
-      uint32_t m = 0;  // as bits: NaN counts above infinity
-#pragma unroll
-      for (int b = j * PER; b < (j + 1) * PER; ++b)
-#pragma unroll
-        for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(v[b][i]) & 0x7fffffffu);
+      uint32_t m = v.amax(j * PER, (j + 1) * PER);
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
       m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
       const bool finite = m < 0x7f800000u;
@@ -138,13 +207,7 @@ quant_i4_kernel(const T* __restrict__ w, int64_t ld, int64_t rows, int K, int Kp
       const float inv = __frcp_rn(s);
       scales[j] = finite ? __float_as_uint(s) >> 16 : 0x7fffu;  // five significant bits: exact in bf16
 #pragma unroll
-      for (int b = j * PER; b < (j + 1) * PER; ++b) {
-        uint32_t c = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)  // nibble order 0, 2, 4, 6, 1, 3, 5, 7
-          c |= (code_bits<T>(v[b][i], s, inv) & 15u) << (4 * ((i >> 1) + 4 * (i & 1)));
-        word[b] = finite ? c : 0x88888888u;
-      }
+      for (int b = j * PER; b < (j + 1) * PER; ++b) word[b] = finite ? v.codes(b, s, inv) : 0x88888888u;
     }
     if (!in) continue;
     reinterpret_cast<uint4*>(q)[at.row * pieces + at.piece] = make_uint4(word[0], word[1], word[2], word[3]);
