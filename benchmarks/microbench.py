@@ -6,6 +6,7 @@
     python benchmarks/microbench.py gemm_stack  # K2 on the Flux / T5 stacks' largest linears
     python benchmarks/microbench.py convert  # K4 QuIP conversion
     python benchmarks/microbench.py ldlq     # default converter: fp64 Hinv factorization, LDLQ pass
+    python benchmarks/microbench.py int4     # 4-bit weights: quantization, linear, mixture of experts
     python benchmarks/microbench.py gemm_ksweep  # K2 plain GEMM over K at fixed M, N
 
 Each case is timed with CUDA events around one launch, median of ``--iters``
@@ -109,6 +110,37 @@ def gemm_cases(run, dev):
                                              L.QI8_S_SCALAR, None, 0, L.ptr(out), L.QI8_F32, N, L.QI8_ACT_NONE,
                                              L.stream_ptr(dev))))
     res[f"k2_scalar_onepass_{M}x{N}x{K}"] = [us, 2 * M * N * K / us / 1e6]
+    return res
+
+
+def int4_cases(run, dev):
+    """4-bit weights at the sizes of a text encoder layer: [us, GB/s of weights], prompts [us, TFLOP/s]."""
+    res = {}
+    w = (torch.randn(10240, 4096, device=dev) * 0.02).to(torch.bfloat16)
+    q, s = ops.quant_weight_i4(w)
+    nbytes = q.numel() + 2 * s.numel()
+    us = run(lambda: ops.quant_weight_i4(w))
+    res["i4_quant_10240x4096"] = [us, (w.numel() * 2 + nbytes) / us / 1e3]
+    us = run(lambda: ops.dequant_i4(q, s, 4096))
+    res["i4_dequant_10240x4096"] = [us, (w.numel() * 2 + nbytes) / us / 1e3]
+    for T in (1, 8, 16, 64, 128):
+        x = torch.randn(T, 4096, device=dev).to(torch.bfloat16)
+        us = run(lambda: ops.gemm_w4(x, q, s))
+        res[f"w4_linear_{T}x10240x4096"] = [us, nbytes / us / 1e3]
+    for T in (512, 4096):
+        x = torch.randn(T, 4096, device=dev).to(torch.bfloat16)
+        us = run(lambda: ops.gemm_w4(x, q, s))
+        res[f"w4_linear_{T}x10240x4096"] = [us, 2 * T * w.numel() / us / 1e6]
+    e, h, i, k = 64, 4096, 1536, 8
+    q13, s13 = ops.quant_weight_i4((torch.randn(e, 2 * i, h, device=dev) * 0.02).to(torch.bfloat16))
+    q2, s2 = ops.quant_weight_i4((torch.randn(e, h, i, device=dev) * 0.02).to(torch.bfloat16))
+    router = (torch.randn(e, h, device=dev) * h ** -0.5).to(torch.bfloat16)
+    one = (q13.numel() + 2 * s13.numel() + q2.numel() + 2 * s2.numel()) // e
+    for T in (1, 4, 16, 64):
+        x = torch.randn(T, h, device=dev).to(torch.bfloat16)
+        us = run(lambda: ops.moe_w4(x, router, q13, s13, q2, s2, k))
+        used = (x.float() @ router.float().t()).topk(k).indices.unique().numel()
+        res[f"w4_moe_{T}_top{k}_of_{e}x{i}"] = [us, used * one / us / 1e3]
     return res
 
 
@@ -220,7 +252,7 @@ def gemm_ksweep_cases(run, dev):
 
 CASES = {"rotate": rotate_cases, "quant": quant_cases, "gemm": gemm_cases, "gemm_stack": gemm_stack_cases,
          "gemm_tile": gemm_tile_cases,
-         "convert": convert_cases, "ldlq": ldlq_cases, "gemm_ksweep": gemm_ksweep_cases}
+         "int4": int4_cases, "convert": convert_cases, "ldlq": ldlq_cases, "gemm_ksweep": gemm_ksweep_cases}
 
 
 def main(argv=None):

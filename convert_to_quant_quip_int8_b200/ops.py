@@ -539,12 +539,12 @@ def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
 
 
 def quant_weight_i4(w: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
-    """4-bit codes and group scales of ``w`` [..., N, K]: ``(q uint8 [..., N, Kp/2], scale bf16 [..., N, Kp/group])``."""
+    """4-bit codes and group scales of ``w`` [..., N, K] (a parameter is read as it is, like the int8 quantizers do):
+    ``(q uint8 [..., N, Kp/2], scale bf16 [..., N, Kp/group])``."""
     pair = _fast("quant_weight_i4", w, group)
     if pair is not None:
         return pair
     dev = _one_device(w)
-    _no_grad(w)
     dt = L.dtype_code(w.dtype)
     if dt not in (L.QI8_BF16, L.QI8_F16, L.QI8_F32):
         raise TypeError(f"weights must be bfloat16, float16 or float32, got {w.dtype}")

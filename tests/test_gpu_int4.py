@@ -336,6 +336,13 @@ def test_layout_through_flinear():
         assert torch.equal(F.linear(x.clone().requires_grad_(), wq, b), y)
 
 
+def test_a_models_parameter_quantizes():
+    w = torch.nn.Parameter(randn(40, 300, scale=0.02, dtype=BF))
+    a = QuantizedTensor.from_float(w, "GroupWiseINT4Layout")
+    b = QuantizedTensor.from_float(w.detach(), "GroupWiseINT4Layout")
+    assert torch.equal(a._qdata, b._qdata) and not a._layout_params["scale"].requires_grad
+
+
 def test_linear_refusals():
     q, s, _ = weight(40, 256, 64)
     x = randn(3, 256, dtype=BF)
