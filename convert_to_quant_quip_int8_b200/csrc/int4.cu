@@ -274,11 +274,14 @@ dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restric
 // slots 59 %, ALU (the unpacking) 49 %, half of the stalls wait for memory.  64
 // registers, four blocks per SM: three blocks take 72 us, five with spills 78; two
 // and four blocks of codes ahead 76 and 83.  With few blocks per SM a deep
-// lookahead helps instead: 1 x 4096 x 4096 6.5 -> 5.4 us.
+// lookahead helps instead: 1 x 4096 x 4096 6.5 -> 5.4 us.  9 to 16 tokens pair two
+// tiles of rows in a warp, which halves the loads of activations: 16 x 32768 x 4096
+// 31 us, 37 unpaired with the lookahead; with few blocks it is the other way round,
+// 16 x 4096 x 10240 13 us and 18.
 constexpr int LIN_WARPS = 8;
 
 template <typename T, int G, int MT, int NT, int AHEAD, bool VEC>
-__global__ void __launch_bounds__(LIN_WARPS * 32, NT == 1 && AHEAD == 1 ? 4 : 1)
+__global__ void __launch_bounds__(LIN_WARPS * 32, NT == 2 ? 2 : AHEAD == 1 ? 4 : 1)
 w4_rows_kernel(const LinArgs p) {
   __shared__ float red[LIN_WARPS][8 * NT][16 * MT + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -503,10 +506,10 @@ extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int
     constexpr int g = decltype(G)::value;
     return with_bool(x_dtype == QI8_F16, [&](auto half) {
       using T = std::conditional_t<decltype(half)::value, __half, __nv_bfloat16>;
-      if (p.M > 8) return launch_rows<T, g, 2, 2, 2>(p, vec, st);
-      // few blocks per SM: more of each warp's own in flight
-      if (p.N <= 32 * sm_count()) return launch_rows<T, g, 1, 1, 4>(p, vec, st);
-      return launch_rows<T, g, 1, 1, 1>(p, vec, st);
+      // few blocks per SM: more of each warp's own in flight, and no rows paired in a warp
+      const bool few = p.N <= 32 * sm_count();
+      if (p.M > 8) return few ? launch_rows<T, g, 1, 2, 4>(p, vec, st) : launch_rows<T, g, 2, 2, 1>(p, vec, st);
+      return few ? launch_rows<T, g, 1, 1, 4>(p, vec, st) : launch_rows<T, g, 1, 1, 1>(p, vec, st);
     });
   });
 }
