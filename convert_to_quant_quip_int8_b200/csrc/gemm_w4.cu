@@ -11,12 +11,14 @@
 //                 scale in 16 bits -> 32 TMEM columns of the A operand
 //   warps 20, 22  TMA producers: activations, codes
 //   warp 21       TMEM allocation, MMA issue (one thread)
-// The A operand lives in TMEM.  In shared memory it cost the stores and the
-// fence to the async proxy (800 to 1900 cycles a block, counted with clock64) and
-// its reads (66 cycles for each MMA of 16 features, whatever the tokens).
+// The A operand lives in TMEM: in shared memory its stores and their fence to the
+// async proxy took 800 to 1900 cycles a block (counted with clock64), here 140.
+// What bounds the kernel is the MMAs, about 64 cycles for each M = 128, K = 16
+// step up to 128 tokens, and as many more cycles a block of the issuing lane's
+// waits and commits (slots of 64 features were slower for that).  4096 x 10240 x
+// 4096 takes 248 us (1.39 PFLOP/s, 0.84 of measured), 100 x 10240 x 4096 26 us.
 // Rings: codes (stages of two blocks), activations, operand slots of 128
-// features.  A slot costs the issuing thread 500 cycles of waits and commits
-// whatever is in it: slots of 64 features were slower.  A group fills about every
+// features.  A group fills about every
 // other slot of the sequence and had waited for slot n - 3 - SLOTS or a later one
 // to be consumed before it waits for slot n: with SLOTS >= 3 the parity it waits
 // for cannot be that of slot n - 2 SLOTS.  Codes are unpacked before the wait.
@@ -118,15 +120,33 @@ __device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float a, float b
                : "memory");
 }
 
-// fp16 only: the power of two that brings the row's largest finite scale to
-// [2^12, 2^13), as the exponent field of the factor.
-__device__ __forceinline__ uint32_t row_shift(const __nv_bfloat16* scale, int count) {
-  uint32_t top = 13;
-  for (int i = 0; i < count; ++i) {
-    const uint32_t e = (__bfloat16_as_ushort(scale[i]) >> 7) & 0xffu;
-    if (e < 255) top = max(top, e);
+// fp16 only: the power of two that brings a row's largest finite scale to
+// [2^12, 2^13), as the exponent field of the factor, for row n0 + lane.  The warp
+// reads its 32 rows together, a row's scales side by side: a row per lane instead
+// touched 32 lines with every load and took 570 us for 4096 x 10240 x 4096 with
+// groups of 32, four rows at a time 369.
+__device__ __forceinline__ uint32_t row_shift(const __nv_bfloat16* scale, int n0, int n_rows, int pitch, int first,
+                                              int count, int lane) {
+  uint32_t top[32], mine = 13;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) top[r] = 13;
+  for (int i = lane; i < count; i += 32) {
+    uint32_t e[32];  // 32 loads in flight
+#pragma unroll
+    for (int r = 0; r < 32; ++r)
+      e[r] = __bfloat16_as_ushort(scale[(int64_t)min(n0 + r, n_rows - 1) * pitch + first + i]);
+#pragma unroll
+    for (int r = 0; r < 32; ++r) {
+      e[r] = (e[r] >> 7) & 0xffu;
+      if (e[r] < 255) top[r] = max(top[r], e[r]);
+    }
   }
-  return 266u - top;
+#pragma unroll
+  for (int r = 0; r < 32; ++r) {
+    const uint32_t m = __reduce_max_sync(0xffffffffu, top[r]);
+    if (r == lane) mine = m;
+  }
+  return 266u - mine;
 }
 
 // One scale as a packed pair of T.
@@ -319,7 +339,9 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
       const __nv_bfloat16* sc = p.l.scale + (n * p.l.KB + kb0) * (W4_BLOCK / G);
       float shift = 1.0f;
       if constexpr (std::is_same<T, __half>::value)
-        shift = __uint_as_float(row_shift(sc, kn * (W4_BLOCK / G)) << 23);
+        shift = __uint_as_float(row_shift(p.l.scale, (tile % p.n_tiles) * p.rows + ((warp & 3) << 5), p.l.N,
+                                          p.l.KB * (W4_BLOCK / G), kb0 * (W4_BLOCK / G), kn * (W4_BLOCK / G), lane)
+                                << 23);
       auto load_scales = [&](int kb) -> uint32_t {  // of this half block
         if (kb >= kn) return 0;
         if (G == 32) return __ldg(reinterpret_cast<const uint32_t*>(sc + kb * 4 + half * 2));
@@ -385,9 +407,10 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
       const int buf = unit % ACCS;
       float unshift = 1.0f;
       if constexpr (std::is_same<T, __half>::value)
-        unshift = __uint_as_float(
-            (254u - row_shift(p.l.scale + ((int64_t)min(n, p.l.N - 1) * p.l.KB + kb0) * (W4_BLOCK / G),
-                              (kb1 - kb0) * (W4_BLOCK / G))) << 23);
+        unshift = __uint_as_float((254u - row_shift(p.l.scale, (tile % p.n_tiles) * p.rows + warp * 32, p.l.N,
+                                                    p.l.KB * (W4_BLOCK / G), kb0 * (W4_BLOCK / G),
+                                                    kn * (W4_BLOCK / G), lane))
+                                  << 23);
       const float bias = p.l.bias && n < p.l.N ? load_as_f32(p.l.bias, p.l.bias_dtype, n) : 0.0f;
       if (!warp_wait(tfull_bar(buf), (unit / ACCS) & 1, abort_flag, p.status, ST_W4_EPILOGUE, WAIT_LIMIT_NS)) break;
       tc_fence_after();
@@ -427,14 +450,14 @@ gemm_w4_kernel(const __grid_constant__ CUtensorMap tmX, const __grid_constant__ 
     const int t0 = (tile / p.n_tiles) * BN, n0 = (tile % p.n_tiles) * p.rows;
     const int t1 = min(BN, p.l.M - t0);
     const int per = ((BN + split - 1) / split + 3) & ~3, pitch = per + 4;  // columns per rank; padded against conflicts
-    if (warp < EPI_WARPS && !*abort_flag) {
+    if (warp < EPI_WARPS && __all_sync(0xffffffffu, !*abort_flag)) {
       const uint32_t lanes = (uint32_t)(warp * 32) << 16;
       const int row = warp * 32 + lane;
       float unshift = 1.0f;
       if constexpr (std::is_same<T, __half>::value)
-        unshift = __uint_as_float(
-            (254u - row_shift(p.l.scale + ((int64_t)min(n0 + row, p.l.N - 1) * p.l.KB + kb0) * (W4_BLOCK / G),
-                              (kb1 - kb0) * (W4_BLOCK / G))) << 23);
+        unshift = __uint_as_float((254u - row_shift(p.l.scale, n0 + warp * 32, p.l.N, p.l.KB * (W4_BLOCK / G),
+                                                    kb0 * (W4_BLOCK / G), kn * (W4_BLOCK / G), lane))
+                                  << 23);
       // rank d finishes columns [d per, (d + 1) per); its blocks of sums are [source][row][pitch]
 #pragma unroll 1
       for (int c = 0; c < t1; c += 32) {
@@ -530,6 +553,8 @@ int launch(const LinArgs& l, cudaStream_t st) {
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, map, codes, p), "gemm_w4_kernel launch");
 }
 
+// The narrowest MMA that holds all tokens, up to 256: narrower tiles of the same
+// tokens would unpack the weight once for each.
 template <typename T, int G>
 int pick(const LinArgs& l, cudaStream_t st) {
   if (l.M <= 32) return launch<T, G, 32>(l, st);
