@@ -4,7 +4,7 @@
 //   y[t, n] = sum_k W[n, k] x[t, k] + bias[n]
 //
 // The weight rows are the MMA's M (128 TMEM lanes), the tokens its N, so that
-// one kernel serves 17 tokens and a long prompt.  Roles of a block:
+// one kernel serves a batch of single tokens and a long prompt.  Roles of a block:
 //   warps 0..3    epilogue: TMEM -> registers -> y (thread = weight row)
 //   warps 4..19   unpacking, four groups of four warps (thread = weight row):
 //                 half of a 128-feature block, 32 bytes of codes -> code *

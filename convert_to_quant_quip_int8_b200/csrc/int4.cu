@@ -266,7 +266,8 @@ dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restric
 
 // ------------------------------------------------- linear, a few tokens
 // y[t, n] = sum_k W[n, k] x[t, k] + bias[n] for up to 8 NT tokens a block.
-// Bound by the weight's bytes: each block takes 16 MT weight rows, its warps
+// Bound by the weight's bytes (read again, mostly from L2, for every further 8 NT
+// tokens): each block takes 16 MT weight rows, its warps
 // the 128-feature blocks in turn, and the MMAs (m16n8k16, tokens as the 8
 // columns) keep the arithmetic per weight at the unpacking alone.  fp32 sums
 // per warp, joined in shared memory in the order of the warps.
@@ -281,7 +282,7 @@ dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restric
 constexpr int LIN_WARPS = 8;
 
 template <typename T, int G, int MT, int NT, int AHEAD, bool VEC>
-__global__ void __launch_bounds__(LIN_WARPS * 32, NT == 2 ? 2 : AHEAD == 1 ? 4 : 1)
+__global__ void __launch_bounds__(LIN_WARPS * 32, NT >= 2 ? 2 : AHEAD == 1 ? 4 : 1)
 w4_rows_kernel(const LinArgs p) {
   __shared__ float red[LIN_WARPS][8 * NT][16 * MT + 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -454,11 +455,17 @@ int launch_rows(const LinArgs& p, bool vec, cudaStream_t st) {
 }  // namespace
 
 namespace {
-// Tokens from which the tcgen05 kernel takes over.  With four column tiles the
-// rows kernel takes 20 us for 17 x 10240 x 4096 and 57 for 32 x 32768 x 4096, the
-// tcgen05 kernel 23 and 42; at 16 and 17 tokens of 10240 x 4096 they meet at 16
-// (two column tiles) and 23 us.
+// The tcgen05 kernel takes over at 17 tokens, but for small products: it costs
+// 8 us before its first result, and the rows kernel with 32 tokens a block reads a
+// small weight again from L2 for the next 32.  Rows against tcgen05: 4.3 and 8.7 us
+// for 64 x 2048 x 1024, 9.8 and 21 for 128 x 1024 x 4096, 13 and 17 for 256 x 2048 x
+// 1024; equal at 2^29 multiply-adds (64 x 4096 x 2048: 10.9 and 11.3), slower beyond
+// (64 x 4096 x 4096: 17.7 and 13.9; 32 x 32768 x 4096: 57 and 42) and where K is long
+// and the blocks are few (64 x 64 x 16384: 26 and 16, split over clusters).
 constexpr int64_t W4_TILES_FROM = 17;
+bool few_products(int64_t M, int64_t N, int64_t K) {
+  return M <= 4096 && K <= 8192 && M * N * K <= (1LL << 29);
+}
 
 bool act_aligned(const void* x, int64_t K, int64_t ld_x) { return aligned16(x) && ld_x % 8 == 0 && K % 8 == 0; }
 }  // namespace
@@ -491,7 +498,7 @@ extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int
   LinArgs p{static_cast<const uint16_t*>(x), ld_x, q, static_cast<const __nv_bfloat16*>(scale), bias, bias_dtype,
             out, ld_out, out_dtype, 0, (int)N, (int)K, (int)(w4_padded(K) / W4_BLOCK)};
   p.M = (int)M;
-  if (M >= W4_TILES_FROM) {
+  if (M >= W4_TILES_FROM) {  // aligned from here on, whichever kernel: the bits do not depend on where x lies
     if (const int64_t need = qi8_gemm_w4_workspace_bytes(x, M, K, ld_x)) {
       QI8_REQUIRE(workspace && workspace_bytes >= need, QI8_ESHAPE, "workspace of %lld bytes, %lld needed",
                   (long long)workspace_bytes, (long long)need);
@@ -503,7 +510,7 @@ extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int
       p.x = static_cast<const uint16_t*>(workspace);
       p.ld_x = vecs * 8;
     }
-    return gemm_w4_tiles(p, x_dtype, group, st);
+    if (!few_products(M, N, K)) return gemm_w4_tiles(p, x_dtype, group, st);
   }
   return with_group(group, [&](auto G) {
     constexpr int g = decltype(G)::value;
@@ -511,6 +518,7 @@ extern "C" int qi8_gemm_w4(const void* x, int x_dtype, int64_t M, int64_t K, int
       using T = std::conditional_t<decltype(half)::value, __half, __nv_bfloat16>;
       // few blocks per SM: more of each warp's own in flight, and no rows paired in a warp
       const bool few = p.N <= 32 * sm_count();
+      if (p.M >= W4_TILES_FROM) return launch_rows<T, g, 1, 4, 2>(p, true, st);  // rows padded to 16 bytes
       if (p.M > 8) return few ? launch_rows<T, g, 1, 2, 4>(p, vec, st) : launch_rows<T, g, 2, 2, 1>(p, vec, st);
       return few ? launch_rows<T, g, 1, 1, 4>(p, vec, st) : launch_rows<T, g, 1, 1, 1>(p, vec, st);
     });

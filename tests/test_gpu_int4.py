@@ -173,6 +173,68 @@ def test_linear(m, n, k, group, dtype):
     check_linear(m, n, k, group, dtype, dtype, seed=m + n + 1)
 
 
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,n,k,group", [
+    (17, 48, 8320, 32), (32, 130, 8328, 128), (33, 129, 8194, 64), (64, 1, 9000, 128), (65, 300, 8448, 32),
+    (100, 640, 8320, 128), (127, 257, 8320, 64), (128, 128, 16384, 32), (129, 7, 8200, 64), (200, 384, 8704, 128),
+    (257, 1000, 8321, 32), (40, 4104, 4096, 128), (300, 2100, 1024, 64), (520, 4096, 520, 32), (1100, 4112, 136, 128),
+    (24, 10240, 4096, 64)])
+def test_linear_beyond_the_small_products(m, n, k, group, dtype):
+    """More than 2^29 multiply-adds or 8192 features: tensor-core tiles, split over clusters where they are few."""
+    check_linear(m, n, k, group, dtype, None, seed=m + n)
+    check_linear(m, n, k, group, dtype, F32, seed=m + n + 1)
+
+
+@pytest.mark.parametrize("m", [20, 300])
+def test_linear_tiles_hold_what_the_small_products_hold(m):
+    """Non-finite values, scales of eight bits, wide scale ranges, strided rows, untouched columns, graphs at 8320
+    features."""
+    n, k, group = 72, 8320, 32
+    q, s, _ = weight(n, k, group, seed=11)
+    x = randn(m, k, seed=12, dtype=BF)
+    good = I4.int4_linear(x, q, s, group)
+    x2, s2 = x.clone(), s.clone()
+    x2[1, 7], x2[2, k - 1], s2[5, 1] = float("nan"), float("inf"), float("nan")
+    y = I4.int4_linear(x2, q, s2, group)
+    assert torch.isnan(y[1]).all() and torch.isnan(y[:, 5]).all() and not torch.isfinite(y[2]).any()
+    keep_m, keep_n = [i for i in range(m) if i not in (1, 2)], [i for i in range(n) if i != 5]
+    assert torch.equal(y[keep_m][:, keep_n], good[keep_m][:, keep_n])
+
+    big = randn(2 * m, k + 24, seed=5, dtype=BF)
+    for v in (big[:m, :k], big[:m, 1:k + 1], big[::2, 8:k + 8]):
+        assert torch.equal(I4.int4_linear(v, q, s, group), I4.int4_linear(v.contiguous(), q, s, group))
+
+    rng = np.random.default_rng(1)
+    codes = rng.integers(-8, 8, (n, k)).astype(np.int8)
+    qa = torch.from_numpy(O.i4_pack(codes)).cuda()
+    sa = (torch.rand(n, k // group, generator=torch.Generator().manual_seed(2)) * 0.01 + 1e-3).to(BF).cuda()
+    va = torch.from_numpy(O.i4_values(qa.cpu().numpy(), sa.double().cpu().numpy(), k, group)).cuda()
+    for dtype in (BF, HF):
+        xa = randn(m, k, seed=8, dtype=dtype)
+        mag = xa.double().abs() @ va.abs().T
+        close(I4.int4_linear(xa, qa, sa, group), xa.double() @ va.T, (ACC + torch.finfo(dtype).eps / 2) * mag)
+    codes = rng.integers(-7, 8, (n, k)).astype(np.int8)
+    scale = np.ldexp(rng.integers(16, 32, (n, k // group)) / 16.0, rng.integers(-20, -8, (n, k // group)))
+    qr = torch.from_numpy(O.i4_pack(codes)).cuda()
+    vr = torch.from_numpy(codes * np.repeat(scale, group, 1)).cuda()
+    xr = randn(m, k, seed=9, dtype=HF)
+    close(ops.gemm_w4(xr, qr, torch.from_numpy(scale).to(BF).cuda(), group, out_dtype=F32), xr.double() @ vr.T,
+          ACC * (xr.double().abs() @ vr.abs().T))
+
+    out = torch.full((m + 2, n + 9), 3.0, dtype=BF, device="cuda")
+    L.check(L.load().qi8_gemm_w4(x.data_ptr(), L.QI8_BF16, m, k, k, q.data_ptr(), s.data_ptr(), n, group, None, 0,
+                                 out.data_ptr(), L.QI8_BF16, n + 9, None, 0, L.stream_ptr()))
+    assert torch.equal(out[:m, :n], good) and (out[m:] == 3).all() and (out[:, n:] == 3).all()
+
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        z = I4.int4_linear(x, q, s, group)
+    for _ in range(2):
+        z.zero_()
+        graph.replay()
+        assert torch.equal(z, good)
+
+
 @pytest.mark.parametrize("m", [3, 40, 300])
 def test_linear_bias_and_output_types(m):
     q, s, v = weight(96, 256, 64)
