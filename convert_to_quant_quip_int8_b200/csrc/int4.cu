@@ -339,6 +339,7 @@ w4_rows_kernel(const LinArgs p) {
     float y = 0.0f;
 #pragma unroll
     for (int w = 0; w < LIN_WARPS; ++w) y += red[w][c][r];
+    y *= w4_unit<T>();
     if (p.bias) y += load_as_f32(p.bias, p.bias_dtype, n);
     store_from_f32(p.out, p.out_dtype, (int64_t)t * p.ld_out + n, y);
   }

@@ -67,8 +67,9 @@ __device__ __forceinline__ uint32_t and_or(uint32_t a, uint32_t b, uint32_t c) {
   return r;
 }
 
-// The codes of one word as four packed pairs of T, features in order.
-template <typename T>
+// The codes of one word as four packed pairs of T, features in order; bf16 codes
+// times 2^-10 if SMALL.
+template <typename T, bool SMALL = false>
 __device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t (&p)[4]) {
   if constexpr (sizeof(T) == 2 && std::is_same<T, __half>::value) {
     const uint32_t off = 0x64086408u;  // 1024 + 8
@@ -78,10 +79,11 @@ __device__ __forceinline__ void w4_unpack(uint32_t w, uint32_t (&p)[4]) {
       asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(v), "r"(off));
     }
   } else {
-    const uint32_t off = 0x43084308u;  // 128 + 8
+    // 128 + u - (128 + 8), or 2^-10 times that
+    const uint32_t base = SMALL ? 0x3e003e00u : 0x43004300u, off = base + 0x00080008u;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t v = and_or(w >> (4 * i), 0x000f000fu, 0x43004300u);
+      const uint32_t v = and_or(w >> (4 * i), 0x000f000fu, base);
       asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(p[i]) : "r"(v), "r"(off));
     }
   }
@@ -198,7 +200,16 @@ __device__ __forceinline__ void w4_blocks(const uint8_t* const (&q)[MT], const _
   }
 }
 
-// sum[mt][nt] += W X^T over one 128-feature block: lane (g, a) gets rows g
+// What the sums of w4_block have to be multiplied by.  bf16 activations reach to
+// the end of fp32's range: a group's sum of 128 codes of up to 8 times such a one
+// would pass it where the scaled result does not.  So codes enter the MMA times
+// 2^-10 (a power of two: nothing rounds), and a group's sum stays finite.
+template <typename T>
+constexpr float w4_unit() {
+  return std::is_same<T, __half>::value ? 1.0f : 1024.0f;
+}
+
+// w4_unit * sum[mt][nt] += W X^T over one 128-feature block: lane (g, a) gets rows g
 // (elements 0, 1) and g + 8 (2, 3), columns 2 a and 2 a + 1.  act(nt, b)
 // returns features 32 b + 8 a .. + 7 of the activation row of column 8 nt + g.
 template <typename T, int G, int MT, int NT, typename Act>
@@ -212,8 +223,8 @@ __device__ __forceinline__ void w4_block(const W4Frag<G, MT>& f, float (&sum)[MT
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
       uint32_t p[4], r[4];
-      w4_unpack<T>(word_of(f.w[2 * mt], b), p);
-      w4_unpack<T>(word_of(f.w[2 * mt + 1], b), r);
+      w4_unpack<T, true>(word_of(f.w[2 * mt], b), p);
+      w4_unpack<T, true>(word_of(f.w[2 * mt + 1], b), r);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         if (b * 32 % G == 0) d[mt][nt][0] = d[mt][nt][1] = d[mt][nt][2] = d[mt][nt][3] = 0.0f;

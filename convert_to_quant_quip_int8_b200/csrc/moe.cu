@@ -251,7 +251,8 @@ __device__ __forceinline__ float gate_act(float g, int act) {
 // h of column `col` and row i0 + r of a chunk, as value and remainder.
 __device__ __forceinline__ void store_h(const MoeArgs& p, __nv_bfloat16* h, int Ip, int col, int i, float g, float u) {
   const float v = i < p.I ? gate_act(g, p.act) * u : 0.0f;  // zeros to the padded end
-  const __nv_bfloat16 hi = __float2bfloat16_rn(v);
+  // next to fp32's largest numbers, where rounding would give an infinity, cut
+  const __nv_bfloat16 hi = fabsf(v) < 0x1.ffp127f ? __float2bfloat16_rn(v) : __float2bfloat16_rz(v);
   const float rest = v - __bfloat162float(hi);
   h[(int64_t)col * 2 * Ip + i] = hi;
   h[((int64_t)col * 2 + 1) * Ip + i] = __float2bfloat16_rn(isfinite(rest) ? rest : 0.0f);  // infinities, NaN: hi alone
@@ -266,6 +267,7 @@ template <typename T, int G, int NT, int RW, bool VEC, bool UP>
 __global__ void __launch_bounds__(MOE_WARPS * 32, NT == 4 ? 1 : 2)
 moe_expert_kernel(const MoeArgs p) {
   constexpr int KW = MOE_WARPS / RW, NS = W4_BLOCK / G;
+  constexpr float unit = w4_unit<T>();
   __shared__ float red[KW > 1 ? KW : 1][KW > 1 ? 2 : 1][KW > 1 ? 8 * NT : 1][KW > 1 ? 17 : 1];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, a = lane & 3;
@@ -327,13 +329,13 @@ moe_expert_kernel(const MoeArgs p) {
         const int r = g + 8 * (i >> 1);
         if constexpr (UP) {
           const int col = nt * 8 + 2 * a + (i & 1);
-          if (col < count) store_h(p, h, Ip, col, n0 + r, sum[0][nt][i], sum[1][nt][i]);
+          if (col < count) store_h(p, h, Ip, col, n0 + r, sum[0][nt][i] * unit, sum[1][nt][i] * unit);
         } else if ((i & 1) == 0) {
           const int pair = nt * 4 + a;
           if (pair < count) {
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
-              if (n0 + mt * 16 + r < p.H) part[pair * Hp + n0 + mt * 16 + r] = sum[mt][nt][i] + sum[mt][nt][i + 1];
+              if (n0 + mt * 16 + r < p.H) part[pair * Hp + n0 + mt * 16 + r] = (sum[mt][nt][i] + sum[mt][nt][i + 1]) * unit;
           }
         }
       }
@@ -351,13 +353,13 @@ moe_expert_kernel(const MoeArgs p) {
         float gv = 0.0f, uv = 0.0f;
 #pragma unroll
         for (int w = 0; w < KW; ++w) gv += red[w][0][col][r], uv += red[w][1][col][r];
-        if (n0 + r < Ip) store_h(p, h, Ip, col, n0 + r, gv, uv);
+        if (n0 + r < Ip) store_h(p, h, Ip, col, n0 + r, gv * unit, uv * unit);
       } else {
         const int r = i & 15, mt = (i >> 4) & 1, pair = i >> 5, n = n0 + mt * 16 + r;
         float v = 0.0f;
 #pragma unroll
         for (int w = 0; w < KW; ++w) v += red[w][mt][2 * pair][r] + red[w][mt][2 * pair + 1][r];
-        if (n < p.H) part[pair * Hp + n] = v;
+        if (n < p.H) part[pair * Hp + n] = v * unit;
       }
     }
   }

@@ -1,0 +1,122 @@
+"""More GPU tests of the 4-bit operators: the ends of their types, their variants for large layers, what they refuse.
+
+Weights are random codes in [-8, 7] and random scales, unpacked on the GPU by the
+oracle's table of positions.  Tolerances: a tensor-core step sums 16 products
+(exact in fp32) and its accumulator and is off by at most 17 * 2^-23 of the sum of
+absolute values S.  ``steps`` of them in one accumulator, and the few additions
+that join warps, groups or splits, are off by at most (17 steps + 264) * 2^-23 S:
+8 steps per group and up to 256 groups of a warp in the rows kernel, all steps
+of K in the tiles kernel.  The output is rounded once, half a step.
+"""
+
+import numpy as np
+import pytest
+import torch
+
+import oracle as O
+from convert_to_quant_quip_int8_b200 import ops
+from convert_to_quant_quip_int8_b200.comfy import int4_kernels as I4
+from test_gpu_int4 import close, moe_reference, randn
+
+pytestmark = pytest.mark.gpu
+
+BF, HF, F32 = torch.bfloat16, torch.float16, torch.float32
+
+
+@pytest.fixture(autouse=True)
+def _status():
+    yield
+    ops.device_status(reset=True)
+
+
+def bound_of(steps):
+    return (17 * steps + 264) * 2.0 ** -23
+
+
+def weight(n, k, group, seed=0, lead=(), exps=(-8, -5), bits=5):
+    """A packed random weight, scales of ``bits`` significant bits, and its fp64 values [*lead, n, k]."""
+    kp = O.i4_padded(k)
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    q = torch.randint(0, 256, (*lead, n, kp // 2), dtype=torch.uint8, device="cuda", generator=g)
+    shape = (*lead, n, kp // group)
+    mant = torch.randint(1 << (bits - 1), 1 << bits, shape, device="cuda", generator=g).double() / 2 ** (bits - 1)
+    s = torch.ldexp(mant, torch.randint(*exps, shape, device="cuda", generator=g)).to(BF)
+    byte, shift = (torch.from_numpy(a).cuda() for a in O.i4_positions(k))
+    v = ((q[..., byte] >> shift.to(torch.uint8)) & 15).double() - 8
+    v *= s.double().repeat_interleave(group, -1)
+    return q, s, v[..., :k]
+
+
+def check_linear(m, n, k, group, dtype, steps, seed=0, bias=False, **how):
+    q, s, v = weight(n, k, group, seed=seed, **how)
+    x = randn(m, k, seed=seed + 1, dtype=dtype)
+    b = randn(n, seed=seed + 2, scale=0.1, dtype=dtype) if bias else None
+    y = I4.int4_linear(x, q, s, group, b)
+    ref, mag = x.double() @ v.T, x.double().abs() @ v.abs().T
+    if b is not None:
+        ref += b.double()
+        mag += b.double().abs()
+    close(y, ref, bound_of(steps) * mag)
+    assert torch.equal(y, I4.int4_linear(x, q, s, group, b))
+
+
+# ------------------------------------------------------ the ends of the types
+@pytest.mark.parametrize("m,k", [(1, 384), (3, 384), (12, 384), (40, 384), (20, 8320), (300, 8320)])
+@pytest.mark.parametrize("group", [32, 128])
+def test_linear_of_the_largest_activations(m, k, group):
+    """bf16 activations up to the type's largest: a group's sum of code * x may pass fp32's range, the result does
+    not."""
+    q, s, v = weight(72, k, group, seed=m, exps=(-44, -40))
+    x = randn(m, k, seed=1, scale=1e38).clamp(-3.38e38, 3.38e38).to(BF)
+    x[0, :128] = torch.finfo(BF).max
+    y = I4.int4_linear(x, q, s, group)
+    close(y, x.double() @ v.T, bound_of(-(-k // 128) * 8) * (x.double().abs() @ v.abs().T))
+
+
+@pytest.mark.parametrize("m,k", [(1, 384), (12, 384), (40, 384), (20, 8320)])
+def test_linear_of_the_smallest_activations(m, k):
+    """Normal bf16 activations down to 2^-126: products stay exact.  The output's own rounding near its smallest
+    numbers is half of bf16's smallest step."""
+    q, s, v = weight(72, k, 32, seed=m, exps=(-4, 4))
+    x = torch.ldexp(randn(m, k, seed=1).clamp(-4, 4), torch.tensor(-123, device="cuda")).to(BF)
+    x[x.abs() < 2.0 ** -126] = 2.0 ** -126
+    y = I4.int4_linear(x, q, s, 32)
+    ref = x.double() @ v.T
+    steps = -(-k // 128) * 8
+    off = (y.double() - ref).abs()
+    mag = x.double().abs() @ v.abs().T
+    # sums held in units of 2^10 lose no more than fp32's smallest step, 2^-149, an addition: 17 to a tensor-core
+    # step, times a scale of up to 2^4
+    small = (17 * steps * 2 ** 4 + 264) * 2.0 ** -139
+    bound = bound_of(steps) * mag + small
+    # the output's half step: eps / 2 = 2^-8 of a normal number, 2^-134 of the smallest ones
+    assert (off <= bound + torch.finfo(BF).eps / 2 * (ref.abs() + bound) + 2.0 ** -134).all()
+
+
+@pytest.mark.parametrize("t", [1, 9, 40])
+def test_moe_of_the_largest_values(t):
+    """Activations up to bf16's largest, and h = act(g) * u near fp32's largest, against small scales."""
+    e, top_k, h, i, group = 6, 2, 256, 200, 128
+    q13, s13, v13 = weight(2 * i, h, group, seed=1, lead=(e,), exps=(-8, -7))
+    q2, s2, v2 = weight(h, i, group, seed=2, lead=(e,), exps=(-44, -42))
+    x = randn(t, h, seed=3, scale=1e38).clamp(-3.38e38, 3.38e38).to(BF)
+    router = randn(e, h, seed=4, scale=h ** -0.5) * 2.0 ** -126
+    # codes of rms 4.6, 256 of them with x of 1e38: g and u of rms 2^15 with scales of 1.5 * 2^-118, 2^61 with 2^-72
+    for exp in (-110, -64):
+        sc, vc = torch.ldexp(s13, torch.tensor(exp, device="cuda")), torch.ldexp(v13, torch.tensor(exp, device="cuda"))
+        y = I4.moe_int4(x, router, q13, sc, q2, s2, top_k, group)
+        ref, bound = moe_reference(x, router, vc, v2, top_k, True, "silu")
+        assert torch.isfinite(ref.to(BF)).all()
+        close(y, ref, bound)
+
+
+def test_moe_intermediate_next_to_the_end_of_fp32():
+    """h = 7.875 * 2^62 * 8.125 * 2^60 is less than half a step of bf16 below 2^128."""
+    q13 = torch.from_numpy(O.i4_pack(np.array([[7] + [0] * 127, [5] + [0] * 127], np.int8))).cuda()[None]
+    q2 = torch.from_numpy(O.i4_pack(np.array([[1] + [0] * 127], np.int8))).cuda()[None]
+    s13 = torch.tensor([1.125 * 2.0 ** 62, 1.625 * 2.0 ** 60], dtype=BF).view(1, 2, 1).expand(1, 2, 4).contiguous().cuda()
+    s2 = torch.full((1, 1, 4), 2.0 ** -20, dtype=BF, device="cuda")
+    x = torch.ones(1, 1, dtype=BF, device="cuda")
+    y = I4.moe_int4(x, x, q13, s13, q2, s2, 1, 32)
+    ref = torch.full((1, 1), 7.875 * 8.125 * 2.0 ** 102, dtype=torch.float64, device="cuda")
+    close(y, ref, 2.0 ** -16 * ref)
