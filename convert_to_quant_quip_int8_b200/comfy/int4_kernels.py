@@ -11,9 +11,10 @@ A weight [..., N, K] is held as ``q`` uint8 [..., N, Kp/2] and ``scale`` bf16
 [..., N, Kp/group_size], Kp being K rounded up to whole 128s (the order of the
 codes: include/qi8.h).  Scales have at most five significant bits, so that
 code * scale is exact in bf16.  Activations are bf16 or fp16 and stay so (no
-activation quantization); sums are fp32.  Inference only: inputs that require
-a gradient are refused while gradients are enabled (the quantizer reads a
-parameter as it is).
+activation quantization); sums are fp32.  Inference only: inputs, scales among
+them, that require a gradient are refused while gradients are enabled, and such
+that carry a forward-mode tangent always (the quantizer reads a parameter as it
+is).
 """
 
 from typing import Optional, Tuple

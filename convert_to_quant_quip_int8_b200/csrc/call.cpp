@@ -32,10 +32,10 @@ int64_t padded(int64_t k) { return (k + 127) / 128 * 128; }
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
 
-// On the current device, and nobody waits for its gradient.
+// On the current device, and nobody waits for its gradient or has given it a tangent.
 bool plain(const at::Tensor& t, int device) {
   return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == device &&
-         !(c10::GradMode::is_enabled() && t.requires_grad());
+         !(c10::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined();
 }
 
 // q [..., n, padded(k) / 2] and s [..., n, padded(k) / group], `dims` dimensions

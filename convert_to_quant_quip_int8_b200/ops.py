@@ -11,6 +11,7 @@ import math
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib as L
 
@@ -530,12 +531,13 @@ def _check_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int, dims: in
 
 
 def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
-    """Inference only: a result without a gradient must not pass for one with it."""
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                raise RuntimeError("4-bit operators have no backward pass: call them under torch.no_grad() or on "
-                                   "detached tensors")
+    """Inference only: a result without a gradient (or a tangent of forward mode, which no_grad does not turn off) must
+    not pass for one with it."""
+    grad = torch.is_grad_enabled()
+    for t in tensors:
+        if t is not None and ((grad and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None):
+            raise RuntimeError("4-bit operators have no backward pass and no forward mode: call them on detached "
+                               "tensors, or under torch.no_grad() if no input has a tangent")
 
 
 def quant_weight_i4(w: torch.Tensor, group: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
@@ -569,6 +571,7 @@ def dequant_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int = 128,
     if out is not None:
         return out
     dev = _one_device(q, scale)
+    _no_grad(scale)
     _check_i4(q, scale, k, group, q.dim())
     assert q.dim() >= 2, f"4-bit codes of shape {tuple(q.shape)}: expected [..., N, Kp/2]"
     dt = L.dtype_code(out_dtype)
@@ -588,7 +591,7 @@ def gemm_w4(x: torch.Tensor, q: torch.Tensor, scale: torch.Tensor, group: int = 
         if out is not None:
             return out
     dev = _one_device(x, q, scale, bias)
-    _no_grad(x, bias)
+    _no_grad(x, scale, bias)
     shape = x.shape
     k = shape[-1]
     _check_i4(q, scale, k, group, 2)
@@ -627,7 +630,7 @@ def moe_w4(x: torch.Tensor, router: torch.Tensor, q13: torch.Tensor, s13: torch.
     if out is not None:
         return out
     dev = _one_device(x, router, q13, s13, q2, s2)
-    _no_grad(x, router)
+    _no_grad(x, router, s13, s2)
     h = x.shape[-1]
     _check_i4(q13, s13, h, group, 3)
     e, i2 = q13.shape[:2]

@@ -12,6 +12,7 @@ of K in the tiles kernel.  The output is rounded once, half a step.
 import numpy as np
 import pytest
 import torch
+import torch.autograd.forward_ad as fwAD
 
 import oracle as O
 from convert_to_quant_quip_int8_b200 import ops
@@ -120,3 +121,35 @@ def test_moe_intermediate_next_to_the_end_of_fp32():
     y = I4.moe_int4(x, x, q13, s13, q2, s2, 1, 32)
     ref = torch.full((1, 1), 7.875 * 8.125 * 2.0 ** 102, dtype=torch.float64, device="cuda")
     close(y, ref, 2.0 ** -16 * ref)
+
+
+# ------------------------------------------------------------------ gradients
+def test_no_gradient_is_dropped():
+    """Scales are numbers too: whoever wants their gradient, or a tangent, is told that there is none."""
+    q, s, _ = weight(40, 256, 64)
+    q13, s13, _ = weight(128, 256, 64, lead=(6,))
+    q2, s2, _ = weight(256, 64, 64, lead=(6,))
+    x, router, b = randn(3, 256, dtype=BF), randn(6, 256, dtype=BF), randn(40, dtype=BF)
+    grad = lambda t: t.clone().requires_grad_()  # noqa: E731
+
+    def calls(f):
+        """Each call with f of one of its arguments."""
+        return [lambda: I4.int4_linear(f(x), q, s, 64, b), lambda: I4.int4_linear(x, q, f(s), 64, b),
+                lambda: I4.int4_linear(x, q, s, 64, f(b)), lambda: I4.weight_dequant_int4(q, f(s), 256, 64, BF),
+                lambda: I4.moe_int4(f(x), router, q13, s13, q2, s2, 2, 64),
+                lambda: I4.moe_int4(x, f(router), q13, s13, q2, s2, 2, 64),
+                lambda: I4.moe_int4(x, router, q13, f(s13), q2, s2, 2, 64),
+                lambda: I4.moe_int4(x, router, q13, s13, q2, f(s2), 2, 64)]
+
+    for call in calls(grad):
+        with pytest.raises(RuntimeError, match="backward"):
+            call()
+        with torch.no_grad():
+            call()
+    with fwAD.dual_level():
+        for call in calls(lambda t: fwAD.make_dual(t, torch.ones_like(t))):
+            for no_grad in (False, True):  # forward mode goes on under no_grad
+                with torch.set_grad_enabled(not no_grad), pytest.raises(RuntimeError, match="backward"):
+                    call()
+        for call in calls(lambda t: t):
+            call()

@@ -1,0 +1,38 @@
+"""CPU tests of the 4-bit operators' host side: what they refuse before a kernel runs, the layout tensor, the build."""
+
+import pytest
+import torch
+import torch.autograd.forward_ad as fwAD
+
+from convert_to_quant_quip_int8_b200 import ops
+
+
+def _weight(n=16, k=256, group=128):
+    return (torch.zeros(n, k // 2, dtype=torch.uint8), torch.ones(n, k // group, dtype=torch.bfloat16))
+
+
+def test_no_gradient_of_a_scale_is_dropped(monkeypatch):
+    monkeypatch.setattr(ops, "_one_device", lambda x, *t: x.device)
+    q, s = _weight()
+    x = torch.zeros(2, 256, dtype=torch.bfloat16)
+    q13, s13, q2, s2 = q.expand(4, 16, 128), s.expand(4, 16, 2), *(t.expand(4, -1, -1) for t in _weight(256, 128))
+
+    def calls(f):
+        return (lambda: ops.gemm_w4(x, q, f(s)), lambda: ops.dequant_i4(q, f(s), 256),
+                lambda: ops.moe_w4(x, torch.zeros(4, 256), q13, f(s13), q2, s2, 2),
+                lambda: ops.moe_w4(x, torch.zeros(4, 256), q13, s13, q2, f(s2), 2))
+
+    for call in calls(lambda t: t.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="backward"):
+            call()
+
+
+def test_tangents_are_refused():
+    x = torch.zeros(2, 2)
+    with fwAD.dual_level():
+        d = fwAD.make_dual(x, torch.ones(2, 2))
+        for no_grad in (False, True):
+            with torch.set_grad_enabled(not no_grad), pytest.raises(RuntimeError, match="backward"):
+                ops._no_grad(None, x, d)
+        ops._no_grad(x, None)
+    ops._no_grad(d, x)
