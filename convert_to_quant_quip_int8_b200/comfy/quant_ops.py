@@ -81,13 +81,19 @@ class QuantizedLayout:
     def get_plain_tensors(cls, qtensor):
         raise NotImplementedError(f"{cls.__name__} must implement get_plain_tensors()")
 
+    @staticmethod
+    def shape(qdata, layout_params) -> torch.Size:
+        """The shape that the tensor shows: the one that ``dequantize`` returns, where a layout packs its data."""
+        return qdata.shape
+
 
 class QuantizedTensor(torch.Tensor):
-    """Wrapper subclass holding int8 ``_qdata`` plus layout parameters."""
+    """Wrapper subclass holding quantized ``_qdata`` plus layout parameters."""
 
     @staticmethod
     def __new__(cls, qdata, layout_type, layout_params):
-        return torch.Tensor._make_wrapper_subclass(cls, qdata.shape, device=qdata.device,
+        layout = LAYOUTS.get(layout_type, QuantizedLayout)
+        return torch.Tensor._make_wrapper_subclass(cls, layout.shape(qdata, layout_params), device=qdata.device,
                                                    dtype=qdata.dtype, requires_grad=False)
 
     def __init__(self, qdata, layout_type, layout_params):
@@ -377,7 +383,7 @@ class QuIPHadamardINT8Layout(QuantizedLayout):
 class GroupWiseINT4Layout(QuantizedLayout):
     """Weight [..., N, K] of 4-bit codes with one bf16 scale per (row, group of
     ``group_size`` input features); no counterpart in the reference.  ``_qdata``
-    is the packed uint8 [..., N, Kp/2].  ``linear`` keeps the activations in
+    is the packed uint8 [..., N, Kp/2]; the tensor's shape is the weight's.  ``linear`` keeps the activations in
     bf16 / fp16 and is meant for single tokens (see int4_kernels)."""
 
     @classmethod
@@ -391,6 +397,10 @@ class GroupWiseINT4Layout(QuantizedLayout):
     @staticmethod
     def dequantize(qdata, scale, group_size, in_features, orig_dtype, **kwargs):
         return ops.dequant_i4(qdata, scale, in_features, group_size, orig_dtype)
+
+    @staticmethod
+    def shape(qdata, layout_params):
+        return torch.Size((*qdata.shape[:-1], layout_params["in_features"]))
 
     @classmethod
     def get_plain_tensors(cls, qtensor):

@@ -13,10 +13,12 @@ import numpy as np
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
+import torch.nn.functional as F
 
 import oracle as O
 from convert_to_quant_quip_int8_b200 import ops
 from convert_to_quant_quip_int8_b200.comfy import int4_kernels as I4
+from convert_to_quant_quip_int8_b200.comfy.quant_ops import QuantizedTensor
 from test_gpu_int4 import close, moe_reference, randn
 
 pytestmark = pytest.mark.gpu
@@ -153,3 +155,25 @@ def test_no_gradient_is_dropped():
                     call()
         for call in calls(lambda t: t):
             call()
+
+
+# ----------------------------------------------------------- the layout's shape
+def test_layout_has_the_weights_shape():
+    w = randn(40, 300, scale=0.02, dtype=BF)
+    wq = QuantizedTensor.from_float(w, "GroupWiseINT4Layout", group_size=32)
+    d = wq.dequantize()
+    assert wq.shape == w.shape == d.shape and wq.numel() == w.numel() and wq.size(1) == 300
+    # what torch works out from the shape before it reaches the tensor
+    assert torch.equal(wq.reshape(-1), d.reshape(-1)) and torch.equal(wq.flatten(), d.flatten())
+    for a, b in zip(wq.split(100, 1), d.split(100, 1)):
+        assert torch.equal(a, b)
+    for a, b in zip(wq.chunk(2, 1), d.chunk(2, 1)):
+        assert torch.equal(a, b)
+    assert torch.equal(wq[:, -7:], d[:, -7:]) and torch.equal(wq.t(), d.t())
+    for v in (wq.detach(), wq.clone(), wq.to("cuda"), torch.empty_like(wq)):
+        assert isinstance(v, QuantizedTensor) and v.shape == w.shape
+    x = randn(3, 300, seed=1, dtype=BF)
+    assert torch.equal(F.linear(x, torch.nn.Parameter(wq, requires_grad=False)), F.linear(x, wq))
+    w3 = randn(4, 10, 200, scale=0.02, dtype=BF)
+    q3 = QuantizedTensor.from_float(w3, "GroupWiseINT4Layout", group_size=64)
+    assert q3.shape == w3.shape and torch.equal(q3.flatten(), q3.dequantize().flatten())

@@ -5,6 +5,7 @@ import torch
 import torch.autograd.forward_ad as fwAD
 
 from convert_to_quant_quip_int8_b200 import ops
+from convert_to_quant_quip_int8_b200.comfy import quant_ops as Q
 
 
 def _weight(n=16, k=256, group=128):
@@ -36,3 +37,24 @@ def test_tangents_are_refused():
                 ops._no_grad(None, x, d)
         ops._no_grad(x, None)
     ops._no_grad(d, x)
+
+
+def _layout(n=16, k=250, group=64, lead=()):
+    q, s = _weight(n, -(-k // 128) * 128, group)
+    return Q.QuantizedTensor(q.expand(*lead, *q.shape), "GroupWiseINT4Layout",
+                             {"scale": s.expand(*lead, *s.shape), "group_size": group, "in_features": k,
+                              "orig_dtype": torch.bfloat16})
+
+
+def test_layout_shows_the_weights_shape():
+    wq = _layout()
+    assert wq.shape == (16, 250) and wq.numel() == 4000 and wq._qdata.shape == (16, 128)
+    for v in (wq.detach(), wq.clone(), torch.empty_like(wq), torch.nn.Parameter(wq, requires_grad=False), wq.to("cpu")):
+        assert isinstance(v, Q.QuantizedTensor) and v.shape == (16, 250)
+    assert _layout(lead=(3,)).shape == (3, 16, 250)
+    inner, ctx = wq.__tensor_flatten__()
+    again = Q.QuantizedTensor.__tensor_unflatten__({k: getattr(wq, k) for k in inner}, ctx, None, None)
+    assert again.shape == (16, 250)
+    w8 = Q.QuantizedTensor(torch.zeros(16, 128, dtype=torch.int8), "TensorWiseINT8Layout",
+                           {"scale": torch.ones(()), "orig_dtype": torch.bfloat16})
+    assert w8.shape == (16, 128)
