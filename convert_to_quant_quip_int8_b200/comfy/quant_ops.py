@@ -419,7 +419,7 @@ QUANT_ALGOS = {
     },
     "int4_groupwise": {
         "storage_t": torch.uint8,
-        "required_parameters": {"weight_scale"},
+        "required_parameters": {"weight_scale", "in_features"},  # rows are padded to whole 128s
         "optional_parameters": set(),
         "comfy_tensor_layout": "GroupWiseINT4Layout",
         "group_size": 128,

@@ -58,3 +58,10 @@ def test_layout_shows_the_weights_shape():
     w8 = Q.QuantizedTensor(torch.zeros(16, 128, dtype=torch.int8), "TensorWiseINT8Layout",
                            {"scale": torch.ones(()), "orig_dtype": torch.bfloat16})
     assert w8.shape == (16, 128)
+
+
+def test_a_checkpoint_entry_needs_what_rebuilds_the_weight():
+    wq = _layout(k=250)
+    needs = Q.QUANT_ALGOS["int4_groupwise"]["required_parameters"]
+    assert needs == {"weight_scale", "in_features"}
+    assert {k for k in wq._layout_params if k not in ("scale", "orig_dtype", "group_size")} <= needs
