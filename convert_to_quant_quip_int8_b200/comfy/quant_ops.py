@@ -260,6 +260,14 @@ def generic_copy_(func, args, kwargs):
     return func(*args, **kwargs)
 
 
+@register_generic_util(torch.ops.aten.record_stream.default)
+def generic_record_stream(func, args, kwargs):
+    qt = args[0]
+    for t in (qt._qdata, *qt._layout_params.values()):
+        if isinstance(t, torch.Tensor):
+            t.record_stream(args[1])
+
+
 @register_generic_util(torch.ops.aten._has_compatible_shallow_copy_type.default)
 def generic_has_compatible_shallow_copy_type(func, args, kwargs):
     return True

@@ -177,3 +177,20 @@ def test_layout_has_the_weights_shape():
     w3 = randn(4, 10, 200, scale=0.02, dtype=BF)
     q3 = QuantizedTensor.from_float(w3, "GroupWiseINT4Layout", group_size=64)
     assert q3.shape == w3.shape and torch.equal(q3.flatten(), q3.dequantize().flatten())
+
+
+@pytest.mark.parametrize("layout", ["GroupWiseINT4Layout", "TensorWiseINT8Layout"])
+def test_layout_records_a_stream_for_its_memory(layout):
+    """The memory of a tensor that another stream still uses is not handed out again."""
+    wq = QuantizedTensor.from_float(randn(2048, 8192, scale=0.02, dtype=BF), layout)
+    torch.cuda.synchronize()
+    at, n = wq._qdata.data_ptr(), wq._qdata.numel()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(200_000_000)  # about 0.1 s
+    wq.record_stream(side)
+    del wq
+    new = [torch.empty(n, dtype=torch.uint8, device="cuda").data_ptr() for _ in range(3)]
+    busy = not side.query()
+    torch.cuda.synchronize()
+    assert busy and at not in new
