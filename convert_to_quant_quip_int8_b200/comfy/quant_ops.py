@@ -69,6 +69,8 @@ def _map_tensors(params, fn):
 
 
 class QuantizedLayout:
+    packed = False  # _qdata is no number per element: a write goes through the layout or is refused
+
     @classmethod
     def quantize(cls, tensor, **kwargs) -> Tuple[torch.Tensor, Dict]:
         raise NotImplementedError(f"{cls.__name__} must implement quantize()")
@@ -161,6 +163,8 @@ class QuantizedTensor(torch.Tensor):
 
     @classmethod
     def _dequant_and_fallback(cls, func, args, kwargs):
+        _refuse_write(func, args, kwargs)
+
         def deq(a):
             if isinstance(a, QuantizedTensor):
                 return a.dequantize()
@@ -180,6 +184,35 @@ class QuantizedTensor(torch.Tensor):
 
     def storage(self):
         return self._qdata.storage()
+
+
+def _is_packed(t):
+    return isinstance(t, QuantizedTensor) and LAYOUTS[t._layout_type].packed
+
+
+def _refuse_write(func, args, kwargs):
+    """An operation in place would change a dequantized copy of a packed tensor, and the result would be lost."""
+    if not func._schema.is_mutable:
+        return
+    for i, a in enumerate(func._schema.arguments):
+        if a.alias_info is not None and a.alias_info.is_write:
+            v = args[i] if i < len(args) else kwargs.get(a.name)
+            if any(_is_packed(t) for t in (v if isinstance(v, (list, tuple)) else (v,))):
+                raise RuntimeError(f"{func} cannot write to a packed tensor: dequantize it, change that and quantize")
+
+
+def _check_copy(dst, src):
+    """Into a packed tensor go raw codes of its shape or a tensor of the same format."""
+    if not isinstance(src, QuantizedTensor):
+        ok = src.dtype == dst._qdata.dtype and src.shape == dst._qdata.shape
+    else:
+        def form(t):
+            return t._layout_type, t.shape, {k: v.shape if isinstance(v, torch.Tensor) else v
+                                             for k, v in t._layout_params.items() if k != "orig_dtype"}
+        ok = form(dst) == form(src)
+    if not ok:
+        raise TypeError(f"{dst!r} takes its raw codes or a tensor of the same format, got {src.dtype} "
+                        f"{tuple(src.shape)}" + (f" {src._layout_type}" if isinstance(src, QuantizedTensor) else ""))
 
 
 def _new_like(qt, qdata, params=None):
@@ -244,6 +277,8 @@ def generic_copy_(func, args, kwargs):
     dst, src = args[0], args[1]
     non_blocking = args[2] if len(args) > 2 else False
     if isinstance(dst, QuantizedTensor):
+        if _is_packed(dst) or _is_packed(src):
+            _check_copy(dst, src)
         if isinstance(src, QuantizedTensor):
             dst._qdata.copy_(src._qdata, non_blocking=non_blocking)
             dst._layout_type = src._layout_type
@@ -393,6 +428,8 @@ class GroupWiseINT4Layout(QuantizedLayout):
     ``group_size`` input features); no counterpart in the reference.  ``_qdata``
     is the packed uint8 [..., N, Kp/2]; the tensor's shape is the weight's.  ``linear`` keeps the activations in
     bf16 / fp16 and is meant for single tokens (see int4_kernels)."""
+
+    packed = True
 
     @classmethod
     def quantize(cls, tensor, scale=None, group_size=128, **kwargs):

@@ -194,3 +194,26 @@ def test_layout_records_a_stream_for_its_memory(layout):
     busy = not side.query()
     torch.cuda.synchronize()
     assert busy and at not in new
+
+
+def test_layout_is_not_changed_behind_its_back():
+    """Writing to a 4-bit tensor: raw codes or a tensor of the same format, or an error; never nothing or half of
+    it."""
+    w, w2 = randn(40, 300, scale=0.02, dtype=BF), randn(40, 300, seed=1, scale=0.02, dtype=BF)
+    wq, other = (QuantizedTensor.from_float(v, "GroupWiseINT4Layout", group_size=32) for v in (w, w2))
+    before = wq.dequantize()
+    for bad in (lambda: wq.add_(1), lambda: wq.mul_(2), lambda: wq.zero_(), lambda: torch.add(w, w, out=wq),
+                lambda: wq.copy_(w2), lambda: wq.copy_(w2[:, :192].to(torch.uint8).t().contiguous()),
+                lambda: wq.copy_(QuantizedTensor.from_float(w2, "GroupWiseINT4Layout", group_size=64)),
+                lambda: wq.copy_(QuantizedTensor.from_float(w2[:, :290], "GroupWiseINT4Layout", group_size=32)),
+                lambda: wq.copy_(QuantizedTensor.from_float(w2, "TensorWiseINT8Layout")),
+                lambda: QuantizedTensor.from_float(w2, "TensorWiseINT8Layout").copy_(wq)):
+        with pytest.raises((RuntimeError, TypeError)):
+            bad()
+        assert torch.equal(wq.dequantize(), before)
+    assert torch.equal(wq + 1, before + 1)
+    x = before.clone()
+    assert torch.equal(x.add_(wq), before + before)  # reading it is no writing
+    assert torch.equal(wq.copy_(other).dequantize(), other.dequantize())
+    same = QuantizedTensor.from_float(w, "GroupWiseINT4Layout", group_size=32)
+    assert torch.equal(same.copy_(other._qdata)._qdata, other._qdata)

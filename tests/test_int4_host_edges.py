@@ -65,3 +65,25 @@ def test_a_checkpoint_entry_needs_what_rebuilds_the_weight():
     needs = Q.QUANT_ALGOS["int4_groupwise"]["required_parameters"]
     assert needs == {"weight_scale", "in_features"}
     assert {k for k in wq._layout_params if k not in ("scale", "orig_dtype", "group_size")} <= needs
+
+
+def test_writes_to_a_packed_tensor_are_refused():
+    wq, before = _layout(), _layout()._qdata.clone()
+    plain = torch.ones(16, 250, dtype=torch.bfloat16)
+    w8 = Q.QuantizedTensor(torch.zeros(16, 250, dtype=torch.int8), "TensorWiseINT8Layout",
+                           {"scale": torch.ones(()), "orig_dtype": torch.bfloat16})
+    for bad in (lambda: wq.add_(1), lambda: wq.zero_(), lambda: wq.fill_(3), lambda: torch.mul(plain, 2, out=wq),
+                lambda: torch._foreach_add_([wq], 1.0), lambda: wq.copy_(plain), lambda: wq.copy_(plain.byte()),
+                lambda: wq.copy_(before.to(torch.int16)), lambda: wq.copy_(before[:1]), lambda: wq.copy_(w8),
+                lambda: w8.copy_(wq), lambda: wq.copy_(_layout(k=249)), lambda: wq.copy_(_layout(group=32))):
+        with pytest.raises((RuntimeError, TypeError)) as e:
+            bad()
+        assert not isinstance(e.value, RecursionError)
+        assert torch.equal(wq._qdata, before) and wq._layout_params["group_size"] == 64
+    other = _layout()
+    other._qdata.fill_(0x9A)
+    other._layout_params["scale"].fill_(0.5)
+    assert wq.copy_(other) is wq
+    assert torch.equal(wq._qdata, other._qdata) and (wq._layout_params["scale"] == 0.5).all()
+    wq.copy_(before)
+    assert torch.equal(wq._qdata, before)
