@@ -292,7 +292,7 @@ def generic_copy_(func, args, kwargs):
         else:
             dst._qdata.copy_(src)
         return dst
-    return func(*args, **kwargs)
+    return func(dst, src.dequantize(), *args[2:], **kwargs)
 
 
 @register_generic_util(torch.ops.aten.record_stream.default)

@@ -87,3 +87,11 @@ def test_writes_to_a_packed_tensor_are_refused():
     assert torch.equal(wq._qdata, other._qdata) and (wq._layout_params["scale"] == 0.5).all()
     wq.copy_(before)
     assert torch.equal(wq._qdata, before)
+
+
+def test_copy_into_a_plain_tensor_dequantizes(monkeypatch):
+    wq = _layout()
+    value = torch.arange(4000.0).view(16, 250)
+    monkeypatch.setattr(Q.GroupWiseINT4Layout, "dequantize", staticmethod(lambda *a, **k: value))
+    buf = torch.zeros(16, 250)
+    assert buf.copy_(wq) is buf and torch.equal(buf, value)
