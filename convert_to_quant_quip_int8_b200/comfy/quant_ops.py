@@ -143,10 +143,21 @@ class QuantizedTensor(torch.Tensor):
         # sees it, so F.linear is routed to the registered linear handlers here.
         kwargs = kwargs or {}
         if func is torch.nn.functional.linear:
-            layout = _get_layout_from_args(args)
+            layout, out = _get_layout_from_args(args), None
+            if kwargs:  # the handlers take positions
+                given = dict(zip(("input", "weight", "bias"), args), **kwargs)
+                if layout is None and _is_packed(given["weight"]):
+                    layout = given["weight"]._layout_type
             handler = _LAYOUT_REGISTRY.get(torch.ops.aten.linear.default, {}).get(layout)
             if handler is not None:
-                return handler(torch.ops.aten.linear.default, args, kwargs)
+                if kwargs:
+                    args, out = (given["input"], given["weight"], given.get("bias")), given.get("out")
+                y = handler(torch.ops.aten.linear.default, args, {})
+                if out is None:
+                    return y
+                if out.shape != y.shape:
+                    raise RuntimeError(f"out of shape {tuple(out.shape)} for a result of {tuple(y.shape)}")
+                return out.copy_(y)
         return torch._C._disabled_torch_function_impl(func, types, args, kwargs)
 
     @classmethod
@@ -658,7 +669,7 @@ def quip_hadamard_linear(func, args, kwargs):
 def int4_linear(func, args, kwargs):
     """4-bit weight, 16-bit activations: ``x W^T + bias`` with fp32 sums."""
     x, weight = args[0], args[1]
-    bias = args[2] if len(args) > 2 else kwargs.get("bias")
+    bias = args[2] if len(args) > 2 else None
     if not isinstance(weight, QuantizedTensor) or isinstance(x, QuantizedTensor):
         return QuantizedTensor._dequant_and_fallback(func, args, kwargs)
     q, scale, group_size, in_features = GroupWiseINT4Layout.get_plain_tensors(weight)

@@ -217,3 +217,16 @@ def test_layout_is_not_changed_behind_its_back():
     assert torch.equal(wq.copy_(other).dequantize(), other.dequantize())
     same = QuantizedTensor.from_float(w, "GroupWiseINT4Layout", group_size=32)
     assert torch.equal(same.copy_(other._qdata)._qdata, other._qdata)
+
+
+def test_linear_takes_keywords():
+    w = randn(48, 256, scale=0.02, dtype=BF)  # int8 layers have outputs in sixteens
+    x, b = randn(3, 256, seed=1, dtype=BF), randn(48, seed=2, dtype=BF)
+    for layout in ("GroupWiseINT4Layout", "TensorWiseINT8Layout", "AxisWiseINT8Layout"):
+        wq = QuantizedTensor.from_float(w, layout)
+        y = F.linear(x, wq, b)
+        assert not torch.equal(y, F.linear(x, wq))
+        assert torch.equal(F.linear(x, wq, bias=b), y)
+    wq = QuantizedTensor.from_float(w, "GroupWiseINT4Layout", group_size=64)
+    assert torch.equal(F.linear(x.half(), weight=wq, bias=b), F.linear(x.half(), wq, b))
+    assert torch.equal(F.linear(input=x, weight=wq), F.linear(x, wq))

@@ -95,3 +95,29 @@ def test_copy_into_a_plain_tensor_dequantizes(monkeypatch):
     monkeypatch.setattr(Q.GroupWiseINT4Layout, "dequantize", staticmethod(lambda *a, **k: value))
     buf = torch.zeros(16, 250)
     assert buf.copy_(wq) is buf and torch.equal(buf, value)
+
+
+def test_linear_passes_keywords_on(monkeypatch):
+    seen = []
+    linear = torch.nn.functional.linear
+    for layout in ("GroupWiseINT4Layout", "TensorWiseINT8Layout"):
+        monkeypatch.setitem(Q._LAYOUT_REGISTRY[torch.ops.aten.linear.default], layout,
+                            lambda func, args, kwargs: seen.append((*args, None)[:3]) or torch.zeros(()))
+    wq, x, b = _layout(), torch.zeros(2, 250), torch.zeros(16)
+    w8 = Q.QuantizedTensor(torch.zeros(16, 250, dtype=torch.int8), "TensorWiseINT8Layout",
+                           {"scale": torch.ones(()), "orig_dtype": torch.bfloat16})
+    for w in (wq, w8):
+        linear(x, w, bias=b)
+        assert seen[-1][0] is x and seen[-1][1] is w and seen[-1][2] is b
+        linear(x, w)
+        assert seen[-1][1] is w and seen[-1][2] is None
+    linear(x, weight=wq, bias=b)
+    assert seen[-1][0] is x and seen[-1][1] is wq and seen[-1][2] is b
+    linear(input=x, weight=wq)
+    assert seen[-1][0] is x and seen[-1][1] is wq and seen[-1][2] is None
+    out = torch.ones(())
+    assert linear(x, wq, out=out) is out and out == 0
+    with pytest.raises(RuntimeError, match="shape"):
+        linear(x, w8, b, out=torch.ones(3))
+    with pytest.raises(TypeError):
+        linear(x, wq, b, bias=b)
