@@ -15,6 +15,8 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <vector>
+
 #include "../../include/qi8.h"
 
 namespace {
@@ -31,6 +33,14 @@ int code(at::ScalarType t) {
 int64_t padded(int64_t k) { return (k + 127) / 128 * 128; }
 
 const at::Tensor* tensor(PyObject* o) { return THPVariable_CheckExact(o) ? &THPVariable_Unpack(o) : nullptr; }
+
+// A Python integer of 64 bits; -1, which no argument here may be, for all others.
+int64_t integer(PyObject* o) {
+  if (!PyLong_CheckExact(o)) return -1;
+  int overflow = 0;
+  const int64_t v = PyLong_AsLongLongAndOverflow(o, &overflow);  // raises nothing
+  return overflow ? -1 : v;
+}
 
 // On the current device, and nobody waits for its gradient or has given it a tangent.
 bool plain(const at::Tensor& t, int device) {
@@ -73,8 +83,8 @@ PyObject* gemm_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (n_args != 5 || !gemm_fn) Py_RETURN_NONE;
     const at::Tensor *x = tensor(args[0]), *q = tensor(args[1]), *s = tensor(args[2]);
     const at::Tensor* b = args[4] == Py_None ? nullptr : tensor(args[4]);
-    if (!x || !q || !s || (!b && args[4] != Py_None) || !PyLong_CheckExact(args[3])) Py_RETURN_NONE;
-    const int64_t group = PyLong_AsLongLong(args[3]);
+    if (!x || !q || !s || (!b && args[4] != Py_None)) Py_RETURN_NONE;
+    const int64_t group = integer(args[3]);
     const int device = c10::cuda::current_device();
     if (!activations(*x, device)) Py_RETURN_NONE;
     const int64_t k = x->size(-1), m = x->numel() / k, n = q->dim() == 2 ? q->size(0) : 0;
@@ -105,8 +115,8 @@ PyObject* quant_weight_i4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
     if (n_args != 2 || !quant_fn) Py_RETURN_NONE;
     const at::Tensor* w = tensor(args[0]);
-    if (!w || !PyLong_CheckExact(args[1])) Py_RETURN_NONE;
-    const int64_t group = PyLong_AsLongLong(args[1]);
+    if (!w) Py_RETURN_NONE;
+    const int64_t group = integer(args[1]);
     const int device = c10::cuda::current_device();
     if (!plain(*w, device) || w->dim() < 2 || !w->is_contiguous() || w->numel() == 0 || code(w->scalar_type()) < 0 ||
         (group != 32 && group != 64 && group != 128))
@@ -133,9 +143,8 @@ PyObject* dequant_i4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   return guarded([&]() -> PyObject* {
     if (n_args != 5 || !dequant_fn) Py_RETURN_NONE;
     const at::Tensor *q = tensor(args[0]), *s = tensor(args[1]);
-    if (!q || !s || !PyLong_CheckExact(args[2]) || !PyLong_CheckExact(args[3]) || !THPDtype_Check(args[4]))
-      Py_RETURN_NONE;
-    const int64_t k = PyLong_AsLongLong(args[2]), group = PyLong_AsLongLong(args[3]);
+    if (!q || !s || !THPDtype_Check(args[4])) Py_RETURN_NONE;
+    const int64_t k = integer(args[2]), group = integer(args[3]);
     const at::ScalarType t = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
     const int device = c10::cuda::current_device();
     if (code(t) < 0 || q->dim() < 2 || q->numel() == 0 || !weight(*q, *s, k, group, q->dim(), device)) Py_RETURN_NONE;
@@ -156,10 +165,8 @@ PyObject* moe_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const at::Tensor* t[6];
     for (int i = 0; i < 6; ++i)
       if (!(t[i] = tensor(args[i]))) Py_RETURN_NONE;
-    if (!PyLong_CheckExact(args[6]) || !PyLong_CheckExact(args[7]) || !PyBool_Check(args[8]) ||
-        !PyLong_CheckExact(args[9]))
-      Py_RETURN_NONE;
-    const int64_t top_k = PyLong_AsLongLong(args[6]), group = PyLong_AsLongLong(args[7]);
+    if (!PyBool_Check(args[8])) Py_RETURN_NONE;
+    const int64_t top_k = integer(args[6]), group = integer(args[7]), act = integer(args[9]);
     const int device = c10::cuda::current_device();
     const at::Tensor &x = *t[0], &router = *t[1], &q13 = *t[2], &q2 = *t[4];
     if (!activations(x, device) || !plain(router, device) || router.dim() != 2 || !router.is_contiguous())
@@ -168,7 +175,7 @@ PyObject* moe_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (q13.dim() != 3 || !weight(q13, *t[3], h, group, 3, device) || q13.size(1) % 2) Py_RETURN_NONE;
     const int64_t e = q13.size(0), i = q13.size(1) / 2;
     if (q2.dim() != 3 || !weight(q2, *t[5], i, group, 3, device) || q2.size(0) != e || q2.size(1) != h ||
-        router.size(0) != e || router.size(1) != h || top_k <= 0 || top_k > e)
+        router.size(0) != e || router.size(1) != h || top_k <= 0 || top_k > e || act < 0 || act > QI8_ACT_SILU)
       Py_RETURN_NONE;
     const int64_t bytes = moe_bytes_fn(tokens, h, e, i, (int)top_k);
     if (bytes <= 0) Py_RETURN_NONE;
@@ -177,7 +184,7 @@ PyObject* moe_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (moe_fn(x.data_ptr(), code(x.scalar_type()), tokens, h, h, router.data_ptr(), code(router.scalar_type()), e,
                static_cast<const uint8_t*>(q13.data_ptr()), t[3]->data_ptr(), i,
                static_cast<const uint8_t*>(q2.data_ptr()), t[5]->data_ptr(), (int)group, (int)top_k,
-               args[8] == Py_True, (int)PyLong_AsLong(args[9]), out.data_ptr(), h, ws.data_ptr(), bytes,
+               args[8] == Py_True, (int)act, out.data_ptr(), h, ws.data_ptr(), bytes,
                stream(device)))
       Py_RETURN_NONE;
     return THPVariable_Wrap(std::move(out));

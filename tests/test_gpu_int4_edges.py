@@ -230,3 +230,19 @@ def test_linear_takes_keywords():
     wq = QuantizedTensor.from_float(w, "GroupWiseINT4Layout", group_size=64)
     assert torch.equal(F.linear(x.half(), weight=wq, bias=b), F.linear(x.half(), wq, b))
     assert torch.equal(F.linear(input=x, weight=wq), F.linear(x, wq))
+
+
+# ------------------------------------------------------------------- refusals
+def test_integers_beyond_the_c_types_are_refused():
+    q, s, _ = weight(40, 256, 64)
+    q13, s13, _ = weight(128, 256, 64, lead=(6,))
+    q2, s2, _ = weight(256, 64, 64, lead=(6,))
+    x, router = randn(3, 256, dtype=BF), randn(6, 256, dtype=BF)
+    for big in (1 << 70, -(1 << 70), (1 << 32) + 64, -1):
+        for bad in (lambda: I4.int4_linear(x, q, s, big), lambda: I4.weight_quant_int4(x, big),
+                    lambda: I4.weight_dequant_int4(q, s, 256, big, BF),
+                    lambda: I4.weight_dequant_int4(q, s, big, 64, BF),
+                    lambda: I4.moe_int4(x, router, q13, s13, q2, s2, big, 64),
+                    lambda: I4.moe_int4(x, router, q13, s13, q2, s2, 2, big)):
+            with pytest.raises(AssertionError):
+                bad()
