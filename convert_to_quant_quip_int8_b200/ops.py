@@ -640,6 +640,9 @@ def moe_w4(x: torch.Tensor, router: torch.Tensor, q13: torch.Tensor, s13: torch.
     assert tuple(q2.shape[:2]) == (e, h), f"down weights of shape {tuple(q2.shape)}: expected [{e}, {h}, ...]"
     assert tuple(router.shape) == (e, h), f"router of shape {tuple(router.shape)}: expected [{e}, {h}]"
     assert router.is_contiguous(), "router must be contiguous"
+    # before they become C integers, which would take their lowest bits
+    assert 0 < top_k <= e, f"top_k {top_k}: 1 to the {e} experts"
+    assert act in (L.QI8_ACT_SILU, L.QI8_ACT_GELU), f"activation must be SiLU or GELU, got code {act}"
     x2 = x if x.dim() == 2 else x.reshape(-1, h)
     if x2.stride(1) != 1 or x2.stride(0) < h:
         x2 = x2.contiguous()

@@ -246,3 +246,6 @@ def test_integers_beyond_the_c_types_are_refused():
                     lambda: I4.moe_int4(x, router, q13, s13, q2, s2, 2, big)):
             with pytest.raises(AssertionError):
                 bad()
+    for top_k in ((1 << 32) + 2, 2 - (1 << 32)):  # 2 in their lowest 32 bits
+        with pytest.raises(AssertionError):
+            I4.moe_int4(x, router, q13, s13, q2, s2, top_k, 64)

@@ -121,3 +121,14 @@ def test_linear_passes_keywords_on(monkeypatch):
         linear(x, w8, b, out=torch.ones(3))
     with pytest.raises(TypeError):
         linear(x, wq, b, bias=b)
+
+
+def test_integers_are_not_cut_to_c_integers(monkeypatch):
+    monkeypatch.setattr(ops, "_one_device", lambda x, *t: x.device)
+    q13, s13, q2, s2 = (t.expand(6, -1, -1).contiguous() for t in (*_weight(128, 256, 64), *_weight(256, 64, 64)))
+    x, router = torch.zeros(3, 256, dtype=torch.bfloat16), torch.zeros(6, 256, dtype=torch.bfloat16)
+    for top_k in ((1 << 32) + 2, 2 - (1 << 32), 1 << 70, 0, 7, -1):
+        with pytest.raises(AssertionError, match="top_k"):
+            ops.moe_w4(x, router, q13, s13, q2, s2, top_k, 64)
+    with pytest.raises(AssertionError, match="activation"):
+        ops.moe_w4(x, router, q13, s13, q2, s2, 2, 64, True, (1 << 32) + 1)
