@@ -521,6 +521,7 @@ def _check_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int, dims: in
     if q.dtype != torch.uint8 or scale.dtype != torch.bfloat16:
         raise TypeError(f"4-bit weights are uint8 codes and bfloat16 scales, got {q.dtype} and {scale.dtype}")
     assert group in _I4_GROUPS, f"group_size must be 32, 64 or 128, got {group}"
+    assert k > 0, f"a weight of {k} features"
     kp = _i4_padded(k)
     shape = q.shape
     assert len(shape) == dims and shape[-1] * 2 == kp, \

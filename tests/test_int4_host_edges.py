@@ -132,3 +132,13 @@ def test_integers_are_not_cut_to_c_integers(monkeypatch):
             ops.moe_w4(x, router, q13, s13, q2, s2, top_k, 64)
     with pytest.raises(AssertionError, match="activation"):
         ops.moe_w4(x, router, q13, s13, q2, s2, 2, 64, True, (1 << 32) + 1)
+
+
+@pytest.mark.parametrize("k", [0, -5])
+def test_weights_without_features_are_refused(monkeypatch, k):
+    monkeypatch.setattr(ops, "_one_device", lambda x, *t: x.device)
+    q, s = torch.empty(4, 0, dtype=torch.uint8), torch.empty(4, 0, dtype=torch.bfloat16)
+    with pytest.raises(AssertionError, match="features"):
+        ops.dequant_i4(q, s, k)
+    with pytest.raises(AssertionError, match="features"):
+        ops._check_i4(q, s, k, 128, 2)
