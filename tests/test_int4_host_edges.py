@@ -125,7 +125,7 @@ def test_linear_passes_keywords_on(monkeypatch):
 
 def test_integers_are_not_cut_to_c_integers(monkeypatch):
     monkeypatch.setattr(ops, "_one_device", lambda x, *t: x.device)
-    q13, s13, q2, s2 = (t.expand(6, -1, -1).contiguous() for t in (*_weight(128, 256, 64), *_weight(256, 64, 64)))
+    q13, s13, q2, s2 = (t.expand(6, -1, -1).contiguous() for t in (*_weight(128, 256, 64), *_weight(256, 128, 64)))
     x, router = torch.zeros(3, 256, dtype=torch.bfloat16), torch.zeros(6, 256, dtype=torch.bfloat16)
     for top_k in ((1 << 32) + 2, 2 - (1 << 32), 1 << 70, 0, 7, -1):
         with pytest.raises(AssertionError, match="top_k"):
