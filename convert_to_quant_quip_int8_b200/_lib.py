@@ -8,6 +8,7 @@ an sm_100 part, every kernel call raises.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 
@@ -129,10 +130,13 @@ def fast_call():
     libqi8; ``None`` where it was not built for this interpreter and torch."""
     global _call
     if _call is None:
+        from .build import call_path
         lib = load()
         try:
-            from . import _call as mod
-        except ImportError:
+            spec = importlib.util.spec_from_file_location(__package__ + "._call", call_path())
+            mod = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(mod)
+        except ImportError:  # not there, or does not load
             _call = False
         else:
             mod.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (

@@ -16,7 +16,6 @@ import sys
 PKG = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(PKG, "csrc")
 LIB = os.path.join(PKG, "libqi8.so")
-CALL = os.path.join(PKG, "_call.so")
 BUILD_DIR = os.path.join(PKG, "_build")
 
 NVCC_FLAGS = [
@@ -82,12 +81,22 @@ def build(force: bool = False, verbose: bool = False, ptxas_verbose: bool = Fals
     return LIB
 
 
+def call_path() -> str:
+    """The host-side shortcut's file.  It is compiled against the layouts in torch's and Python's headers, so its name
+    says for which of both: another torch or interpreter does not find it and builds its own."""
+    import sysconfig
+
+    import torch
+    return os.path.join(PKG, f"_call.torch-{torch.__version__}{sysconfig.get_config_var('EXT_SUFFIX')}")
+
+
 def build_call(force: bool = False, verbose: bool = False) -> str:
-    """Compile ``_call.so`` (csrc/call.cpp, host code against torch's C++ headers) if it is out of date."""
+    """Compile the host-side shortcut (csrc/call.cpp) if it is out of date; returns its path."""
+    out = call_path()
     src = os.path.join(CSRC, "call.cpp")
     deps = [src, os.path.join(os.path.dirname(PKG), "include", "qi8.h")]
-    if not force and os.path.exists(CALL) and os.path.getmtime(CALL) > max(os.path.getmtime(d) for d in deps):
-        return CALL
+    if not force and os.path.exists(out) and os.path.getmtime(out) > max(os.path.getmtime(d) for d in deps):
+        return out
     import sysconfig
 
     import torch
@@ -97,15 +106,22 @@ def build_call(force: bool = False, verbose: bool = False) -> str:
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-fPIC", "-shared", "-std=c++17", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", "-I" + inc,
            "-I" + os.path.join(inc, "torch", "csrc", "api", "include"), "-I" + cuda,
-           "-I" + sysconfig.get_paths()["include"], src, "-o", CALL + ".tmp", "-L" + lib, "-lc10", "-lc10_cuda",
+           "-I" + sysconfig.get_paths()["include"], src, "-o", out + ".tmp", "-L" + lib, "-lc10", "-lc10_cuda",
            "-ltorch_cpu", "-ltorch_python"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
-    os.replace(CALL + ".tmp", CALL)
-    return CALL
+    os.replace(out + ".tmp", out)
+    return out
+
+
+def main(argv) -> None:
+    print(build(force="--force" in argv, verbose=True, ptxas_verbose="-v" in argv))
+    try:
+        print(build_call(force="--force" in argv, verbose=True))
+    except (OSError, ImportError, subprocess.CalledProcessError) as e:
+        print(f"warning: the host-side shortcut was not built, the 4-bit operators do without it: {e}", file=sys.stderr)
 
 
 if __name__ == "__main__":
-    build_call(force="--force" in sys.argv, verbose=True)
-    print(build(force="--force" in sys.argv, verbose=True, ptxas_verbose="-v" in sys.argv))
+    main(sys.argv)

@@ -1,9 +1,15 @@
 """CPU tests of the 4-bit operators' host side: what they refuse before a kernel runs, the layout tensor, the build."""
 
+import os
+import subprocess
+import sysconfig
+
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
+from convert_to_quant_quip_int8_b200 import _lib as L
+from convert_to_quant_quip_int8_b200 import build as B
 from convert_to_quant_quip_int8_b200 import ops
 from convert_to_quant_quip_int8_b200.comfy import quant_ops as Q
 
@@ -142,3 +148,28 @@ def test_weights_without_features_are_refused(monkeypatch, k):
         ops.dequant_i4(q, s, k)
     with pytest.raises(AssertionError, match="features"):
         ops._check_i4(q, s, k, 128, 2)
+
+
+def test_shortcut_belongs_to_one_torch_and_one_python(monkeypatch):
+    """csrc/call.cpp holds layouts of torch's and Python's objects: the file for another of either is not loaded."""
+    here = B.call_path()
+    assert torch.__version__ in here and here.endswith(sysconfig.get_config_var("EXT_SUFFIX"))
+    assert os.path.exists(B.build_call())
+    monkeypatch.setattr(L, "_call", None)
+    assert L.fast_call() is not None
+    monkeypatch.setattr(L, "_call", None)
+    monkeypatch.setattr(torch, "__version__", "0.0.1+other")
+    assert B.call_path() != here and not os.path.exists(B.call_path())
+    assert L.fast_call() is None
+
+
+def test_build_without_a_host_compiler_still_builds_the_library(monkeypatch, capsys):
+    done = []
+    monkeypatch.setattr(B, "build", lambda **k: done.append("lib"))
+
+    def no_compiler(**k):
+        raise subprocess.CalledProcessError(1, "g++")
+
+    monkeypatch.setattr(B, "build_call", no_compiler)
+    B.main(["build"])
+    assert done == ["lib"] and "warning" in capsys.readouterr().err
