@@ -249,3 +249,18 @@ def test_integers_beyond_the_c_types_are_refused():
     for top_k in ((1 << 32) + 2, 2 - (1 << 32)):  # 2 in their lowest 32 bits
         with pytest.raises(AssertionError):
             I4.moe_int4(x, router, q13, s13, q2, s2, top_k, 64)
+
+
+# ------------------------------------- variants for large layers, many tiles
+def sms():
+    return torch.cuda.get_device_properties(0).multi_processor_count
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,over,k,group,bias", [
+    (1, 1, 264, 32, False), (7, 267, 2989, 32, True), (8, 16, 1000, 64, False), (2, 17, 9000, 128, True),
+    (9, 9, 264, 128, False), (12, 267, 1000, 64, True), (16, 1, 2989, 32, False), (10, 17, 640, 64, False),
+    (13, 31, 1100, 128, True), (16, 32, 9000, 32, False)])
+def test_linear_of_few_tokens_and_many_rows(m, over, k, group, bias, dtype):
+    """More than 32 rows per SM: one block of codes ahead and, from 9 tokens on, two tiles of rows per warp."""
+    check_linear(m, 32 * sms() + over, k, group, dtype, 8, seed=m, bias=bias)
