@@ -264,3 +264,30 @@ def sms():
 def test_linear_of_few_tokens_and_many_rows(m, over, k, group, bias, dtype):
     """More than 32 rows per SM: one block of codes ahead and, from 9 tokens on, two tiles of rows per warp."""
     check_linear(m, 32 * sms() + over, k, group, dtype, 8, seed=m, bias=bias)
+
+
+def experts_variant(t, e, top_k, h, i):
+    """(pairs per chunk, rows over the warps in gate/up, in down), by the launch's rules."""
+    pairs = t * top_k
+    cap = 4 if t <= 4 or pairs <= 3 * e else 8 if t <= 8 or pairs <= 10 * e else 16
+    used = min(pairs, e)
+    return (cap, *(used * (-(-rows // tile) // 8) >= 2 * sms() for rows, tile in ((O.i4_padded(i), 16), (h, 32))))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("t,e,top_k,h,i,group,cap", [
+    (16, 64, 8, 1349, 601, 32, 4), (16, 64, 8, 1352, 600, 128, 4), (10, 300, 30, 250, 100, 64, 4),
+    (40, 64, 8, 1352, 513, 64, 8), (40, 64, 8, 1281, 640, 32, 8), (64, 150, 24, 550, 250, 128, 16),
+    (64, 150, 24, 552, 129, 32, 16), (64, 150, 24, 512, 256, 64, 16)])
+def test_moe_of_wide_layers(t, e, top_k, h, i, group, cap, dtype):
+    """Eight warps side by side over an expert's rows, in gate/up and in down."""
+    assert experts_variant(t, e, top_k, h, i) == (cap, True, True)
+    q13, s13, v13 = weight(2 * i, h, group, seed=1, lead=(e,))
+    q2, s2, v2 = weight(h, i, group, seed=2, lead=(e,))
+    x, router = randn(t, h, seed=3, dtype=dtype), randn(e, h, seed=4, scale=h ** -0.5, dtype=dtype)
+    s13, v13 = s13 * 0.25, v13 * 0.25  # g and u of a few units
+    s2, v2 = s2 * 0.25, v2 * 0.25
+    for act, renorm in (("silu", True), ("gelu", False)):
+        y = I4.moe_int4(x, router, q13, s13, q2, s2, top_k, group, renorm, act)
+        close(y, *moe_reference(x, router, v13, v2, top_k, renorm, act))
+        assert torch.equal(y, I4.moe_int4(x, router, q13, s13, q2, s2, top_k, group, renorm, act))
