@@ -291,3 +291,18 @@ def test_moe_of_wide_layers(t, e, top_k, h, i, group, cap, dtype):
         y = I4.moe_int4(x, router, q13, s13, q2, s2, top_k, group, renorm, act)
         close(y, *moe_reference(x, router, v13, v2, top_k, renorm, act))
         assert torch.equal(y, I4.moe_int4(x, router, q13, s13, q2, s2, top_k, group, renorm, act))
+
+
+@pytest.mark.parametrize("dtype", [BF, HF])
+@pytest.mark.parametrize("m,n,k,group", [
+    (32, 140000, 128, 64), (24, 60000, 384, 32), (24, 60001, 1150, 128),
+    (64, 90000, 100, 32), (48, 60000, 384, 128), (40, 57001, 1152, 64),
+    (128, 60000, 104, 128), (100, 60000, 384, 64), (100, 60000, 1147, 32),
+    (1100, 12000, 100, 32), (1100, 12000, 384, 128), (700, 30001, 1152, 64)])
+def test_linear_of_several_tiles_per_block(m, n, k, group, dtype):
+    """At least three tiles on some block for every width of the tensor-core tile, an odd number of 128-feature blocks
+    each: rings, accumulators and their phases carry over from tile to tile."""
+    width = next(b for b in (32, 64, 128, 256) if m <= b or b == 256)
+    blocks = O.i4_padded(k) // 128
+    assert blocks % 2 and -(-n // 128) * -(-m // width) > 2 * sms() and m * n * k > 1 << 29
+    check_linear(m, n, k, group, dtype, 8 * blocks, seed=m + k, bias=bool(k & 128))
