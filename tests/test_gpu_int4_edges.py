@@ -306,3 +306,12 @@ def test_linear_of_several_tiles_per_block(m, n, k, group, dtype):
     blocks = O.i4_padded(k) // 128
     assert blocks % 2 and -(-n // 128) * -(-m // width) > 2 * sms() and m * n * k > 1 << 29
     check_linear(m, n, k, group, dtype, 8 * blocks, seed=m + k, bias=bool(k & 128))
+
+
+@pytest.mark.parametrize("m", [4, 30, 300])
+def test_small_products_keep_scales_of_eight_bits(m):
+    """Up to 2^29 multiply-adds and 8192 features the scale multiplies the fp32 sum: nothing is rounded but the
+    result."""
+    for dtype in (BF, HF):
+        for group in (32, 64, 128):
+            check_linear(m, 70, 200, group, dtype, 8, seed=m, bits=8)
