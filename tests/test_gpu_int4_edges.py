@@ -315,3 +315,18 @@ def test_small_products_keep_scales_of_eight_bits(m):
     for dtype in (BF, HF):
         for group in (32, 64, 128):
             check_linear(m, 70, 200, group, dtype, 8, seed=m, bits=8)
+
+
+def test_linear_weight_of_more_than_4_gb():
+    """Row offsets in bytes pass 32 bits, in the rows kernel and in the tensor-core tiles."""
+    n, k = 66000, 131072
+    q = torch.full((n, k // 2), 0x88, dtype=torch.uint8, device="cuda")
+    s = torch.ones(n, k // 128, dtype=BF, device="cuda")
+    q[1], q[65537], q[-1] = 0x77, 0xAA, 0x99  # codes -1, 2 (4 GB behind row 1) and 1
+    for m in (2, 20):
+        x = torch.ones(m, k, dtype=BF, device="cuda")
+        x[1] = 2
+        y = I4.int4_linear(x, q, s)
+        for col, code in ((1, -1), (65537, 2), (-1, 1)):
+            assert y[:2, col].tolist() == [code * k, 2 * code * k]
+        assert int((y != 0).sum()) == 3 * m
