@@ -538,7 +538,7 @@ int launch(const LinArgs& l, cudaStream_t st) {
   if (p.code_stages > CODE_BARS) p.code_stages = CODE_BARS;
   CUtensorMap map, codes;
   if (int rc = activation_map(&map, l, std::is_same<T, __half>::value, BN)) return rc;
-  if (int rc = code_map(&codes, l.q, l.N, l.KB, SEG, p.rows, CU_TENSOR_MAP_SWIZZLE_128B)) return rc;
+  if (int rc = code_map(&codes, l.q, l.N, l.KB, SEG, p.rows)) return rc;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(p.split > 1 ? tiles * p.split : tiles < sms ? tiles : sms));
   cfg.blockDim = dim3(THREADS);

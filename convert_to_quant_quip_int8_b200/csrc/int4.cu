@@ -53,29 +53,17 @@ struct Walk {
   __device__ __forceinline__ int feature(int b) const { return (piece >> 2) * 128 + 32 * b + 8 * (piece & 3); }
 };
 
-template <typename T, bool VEC>
-__device__ __forceinline__ void load8(const T* row, int k, int K, float (&v)[8]) {
-  if constexpr (sizeof(T) == 4) {
-    if (VEC && k + 8 <= K) {
-      const float4 a = __ldg(reinterpret_cast<const float4*>(row + k));
-      const float4 b = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
-      v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
-      v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      return;
-    }
-  } else if (VEC && k + 8 <= K) {
-    const uint4 u = __ldg(reinterpret_cast<const uint4*>(row + k));
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const T lo = reinterpret_cast<const T*>(&w[i])[0], hi = reinterpret_cast<const T*>(&w[i])[1];
-      v[2 * i] = Elem<T>::to_f32(lo);
-      v[2 * i + 1] = Elem<T>::to_f32(hi);
-    }
+template <bool VEC>
+__device__ __forceinline__ void load8(const float* row, int k, int K, float (&v)[8]) {
+  if (VEC && k + 8 <= K) {
+    const float4 a = __ldg(reinterpret_cast<const float4*>(row + k));
+    const float4 b = __ldg(reinterpret_cast<const float4*>(row + k) + 1);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+    v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? Elem<T>::to_f32(row[k + i]) : 0.0f;
+  for (int i = 0; i < 8; ++i) v[i] = k + i < K ? row[k + i] : 0.0f;
 }
 
 // Positive finite fp32 to five significant bits, ties to even.
@@ -156,7 +144,7 @@ struct Piece32 {
   float v[4][8];
   template <bool VEC>
   __device__ __forceinline__ void load(const float* row, int b, int k, int K) {
-    load8<float, VEC>(row, k, K, v[b]);
+    load8<VEC>(row, k, K, v[b]);
   }
   __device__ __forceinline__ void clear(int b) {
 #pragma unroll

@@ -159,16 +159,15 @@ inline EncodeTiledFn encode_fn() {
 }
 
 // 4-bit codes, rows of `blocks` x 64 bytes -> boxes of box_blocks x 64 bytes of
-// box_rows rows, as 32-bit elements (a box may then be 1 KB wide).
-inline int code_map(CUtensorMap* map, const uint8_t* q, int64_t rows, int64_t blocks, int box_blocks, int box_rows,
-                    CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_NONE) {
+// box_rows rows, as 32-bit elements, 128-byte swizzle.
+inline int code_map(CUtensorMap* map, const uint8_t* q, int64_t rows, int64_t blocks, int box_blocks, int box_rows) {
   EncodeTiledFn fn = encode_fn();
   QI8_REQUIRE(fn, QI8_ECUDA, "cuTensorMapEncodeTiled unavailable");
   cuuint64_t dims[2] = {(cuuint64_t)blocks * 16, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)blocks * 64};
   cuuint32_t box[2] = {(cuuint32_t)box_blocks * 16, (cuuint32_t)box_rows}, one[2] = {1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_INT32, 2, const_cast<uint8_t*>(q), dims, strides, box, one,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   QI8_REQUIRE(r == CUDA_SUCCESS, QI8_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
   return QI8_OK;
