@@ -15,8 +15,10 @@
 // async proxy took 800 to 1900 cycles a block (counted with clock64), here 140.
 // What bounds the kernel is the MMAs, about 64 cycles for each M = 128, K = 16
 // step up to 128 tokens, and as many more cycles a block of the issuing lane's
-// waits and commits (slots of 64 features were slower for that).  4096 x 10240 x
-// 4096 takes 248 us (1.39 PFLOP/s, 0.84 of measured), 100 x 10240 x 4096 26 us.
+// waits and commits (slots of 64 features were slower for that); with 256 tokens a
+// tile also the epilogues, which the one accumulator does not let overlap.  4096 x
+// 10240 x 4096 takes 248 us (1.39 PFLOP/s, 0.84 of measured), fp16 300, with
+// groups of 32 363 (row_shift, for every tile), 100 x 10240 x 4096 26 us.
 // Rings: codes (stages of two blocks), activations, operand slots of 128
 // features.  A group fills about every
 // other slot of the sequence and had waited for slot n - 3 - SLOTS or a later one

@@ -260,7 +260,7 @@ dequant_i4_kernel(const uint32_t* __restrict__ q, const __nv_bfloat16* __restric
 // columns) keep the arithmetic per weight at the unpacking alone.  fp32 sums
 // per warp, joined in shared memory in the order of the warps.
 // Measured for 1 x 65536 x 8192: 63 us, 4.4 TB/s (0.67 of the copy rate); issue
-// slots 59 %, ALU (the unpacking) 49 %, half of the stalls wait for memory.  64
+// slots 66 %, ALU (the unpacking) 55 %, nearly half of the stalls wait for memory.  64
 // registers, four blocks per SM: three blocks take 72 us, five with spills 78; two
 // and four blocks of codes ahead 76 and 83.  With few blocks per SM a deep
 // lookahead helps instead: 1 x 4096 x 4096 6.5 -> 5.4 us.  9 to 16 tokens pair two
