@@ -94,8 +94,8 @@ class QuantizedTensor(torch.Tensor):
 
     @staticmethod
     def __new__(cls, qdata, layout_type, layout_params):
-        layout = LAYOUTS.get(layout_type, QuantizedLayout)
-        return torch.Tensor._make_wrapper_subclass(cls, layout.shape(qdata, layout_params), device=qdata.device,
+        shape = getattr(LAYOUTS.get(layout_type), "shape", QuantizedLayout.shape)
+        return torch.Tensor._make_wrapper_subclass(cls, shape(qdata, layout_params), device=qdata.device,
                                                    dtype=qdata.dtype, requires_grad=False)
 
     def __init__(self, qdata, layout_type, layout_params):
@@ -198,7 +198,7 @@ class QuantizedTensor(torch.Tensor):
 
 
 def _is_packed(t):
-    return isinstance(t, QuantizedTensor) and LAYOUTS[t._layout_type].packed
+    return isinstance(t, QuantizedTensor) and getattr(LAYOUTS.get(t._layout_type), "packed", False)
 
 
 def _refuse_write(func, args, kwargs):

@@ -173,3 +173,20 @@ def test_build_without_a_host_compiler_still_builds_the_library(monkeypatch, cap
     monkeypatch.setattr(B, "build_call", no_compiler)
     B.main(["build"])
     assert done == ["lib"] and "warning" in capsys.readouterr().err
+
+
+def test_layouts_of_others_work_as_before(monkeypatch):
+    """A registered class without the base class, and a type that nobody registered: shape and copies are the data's."""
+    class Bare:
+        pass
+
+    monkeypatch.setitem(Q.LAYOUTS, "Bare", Bare)
+    for name in ("Bare", "Unknown"):
+        def make(v):
+            return Q.QuantizedTensor(torch.full((4, 6), v, dtype=torch.int8), name,
+                                     {"scale": torch.ones(()) * v, "orig_dtype": torch.float32})
+        a, b = make(1), make(2)
+        assert a.shape == (4, 6) and a.clone().shape == (4, 6)
+        assert a.copy_(b) is a and (a._qdata == 2).all() and a._layout_params["scale"] == 2
+        a.copy_(torch.full((4, 6), 3.0))
+        assert (a._qdata == 3).all()
