@@ -95,7 +95,7 @@ def draw(rng):
 # ------------------------------------------------------ the formats, plainly
 def _exponents(amax):
     m, x = torch.frexp(amax)  # amax = m 2^x, 0.5 <= m < 1; 448 = 0.875 * 2^9
-    return (x - 9 + (m > 0.875).int()).clamp_min(_E_MIN)
+    return torch.where(m > 0, (x - 9 + (m > 0.875).int()).clamp_min(_E_MIN), _E_MIN)
 
 
 def _scales(e):
