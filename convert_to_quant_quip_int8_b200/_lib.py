@@ -30,12 +30,12 @@ QI8_EUNSUPPORTED = -7
 # element types
 QI8_BF16, QI8_F16, QI8_F32, QI8_I8, QI8_I32 = 0, 1, 2, 3, 4
 # row quantization modes
-QI8_Q_TOKEN, QI8_Q_BLOCK, QI8_Q_GELU = 0, 1, 0x100
+QI8_Q_TOKEN, QI8_Q_BLOCK, QI8_Q_FP8, QI8_Q_GELU = 0, 1, 2, 0x100
 # scale kinds
 QI8_S_NONE, QI8_S_SCALAR, QI8_S_ROW, QI8_S_ROW_KBLOCK, QI8_S_TILE128 = 0, 1, 2, 3, 4
 QI8_MAX_PEERS = 8
 # epilogue activation
-QI8_ACT_NONE, QI8_ACT_GELU, QI8_ACT_SILU = 0, 1, 2
+QI8_ACT_NONE, QI8_ACT_GELU, QI8_ACT_SILU, QI8_ACT_GELU_TANH = 0, 1, 2, 3
 # weight requant schemes
 QI8_REQ_ROW, QI8_REQ_GLOBAL, QI8_REQ_BLOCK = 0, 1, 2
 
@@ -93,6 +93,16 @@ SIGNATURES = {
     "qi8_moe_w4_workspace_bytes": (_I64, [_I64, _I64, _I64, _I64, _I]),
     "qi8_moe_w4": (_I, [_P, _I, _I64, _I64, _I64, _P, _I, _I64, _P, _P, _I64, _P, _P, _I, _I, _I, _I, _P, _I64,
                         _P, _I64, _P]),
+    "qi8_quant_rows_f8": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P]),
+    "qi8_quant_weight_f8": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _P]),
+    "qi8_dequant_f8": (_I, [_P, _I64, _I64, _I64, _P, _I, _P, _I, _I64, _P]),
+    "qi8_gemm_f8_workspace_bytes": (_I64, [_P, _I64, _I64, _I64, _P, _I64, _I64]),
+    "qi8_gemm_f8": (_I, [_P, _P, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _I, _I64, _P, _I64, _P]),
+    "qi8_linear_f8_workspace_bytes": (_I64, [_I64, _I64, _P, _I64, _I64]),
+    "qi8_linear_f8": (_I, [_P, _I, _I64, _I64, _I64, _P, _P, _I64, _I64, _P, _I, _P, _I, _I64, _P, _I64, _P]),
+    "qi8_rms_norm_quant": (_I, [_P, _I, _I64, _I64, _I64, _P, _I64, _P, _I, ctypes.c_double, _I, _P, _I64, _P, _P,
+                                _I64, _P]),
+    "qi8_gated_quant": (_I, [_P, _I64, _P, _I64, _I, _I64, _I64, _I, _I, _P, _I64, _P, _P]),
 }
 
 _lib = None

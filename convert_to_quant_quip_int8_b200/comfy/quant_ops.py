@@ -18,6 +18,7 @@ dispatch order.  Differences, all on the hot path:
 * ``QuIPHadamardINT8Layout`` (new) consumes transformed-space checkpoints
   (``sign_row`` / ``sign_col`` / ``hadamard_size_*``) as a W8A8 linear;
 * ``GroupWiseINT4Layout`` (new) holds weights of 4 bits with group scales;
+* ``BlockWiseFP8Layout`` (new) holds fp8 weights and activations with block scales;
 * ``F.linear`` reaches the linear handlers through ``__torch_function__``
   (in the reference it decomposes into ``t`` + ``mm`` before dispatch).
 """
@@ -464,6 +465,33 @@ class GroupWiseINT4Layout(QuantizedLayout):
         return qtensor._qdata, p["scale"], p["group_size"], p["in_features"]
 
 
+class BlockWiseFP8Layout(QuantizedLayout):
+    """fp8 (e4m3) with power-of-two scales: 128 x 128-tile weights, activations
+    with a scale per row and 128 columns; no counterpart in the reference (see
+    fp8_kernels).  ``linear`` takes such activations or plain ones, which it
+    quantizes so.  Codes mean nothing without their scales, so writes other
+    than copies of whole tensors are refused (``packed``)."""
+
+    packed = True
+
+    @classmethod
+    def quantize(cls, tensor, scale=None, block_size=128, is_weight=False, **kwargs):
+        from .fp8_kernels import act_quant_fp8, weight_quant_fp8
+        if scale is not None:
+            raise NotImplementedError("static (pre-computed) block scales are not supported")
+        qdata, scale = (weight_quant_fp8 if is_weight else act_quant_fp8)(tensor, block_size)
+        return qdata, {"scale": scale, "block_size": block_size, "is_weight": is_weight, "orig_dtype": tensor.dtype}
+
+    @staticmethod
+    def dequantize(qdata, scale, block_size, is_weight=False, orig_dtype=None, output_dtype=None, **kwargs):
+        return ops.dequant_f8(qdata, scale, 128 if is_weight else 1, output_dtype or orig_dtype)
+
+    @classmethod
+    def get_plain_tensors(cls, qtensor):
+        p = qtensor._layout_params
+        return qtensor._qdata, p["scale"], p["block_size"], p["is_weight"]
+
+
 QUANT_ALGOS = {
     "int8_blockwise": {
         "storage_t": torch.int8,
@@ -481,6 +509,14 @@ QUANT_ALGOS = {
         "group_size": 128,
         "asymmetric_layout": False,
     },
+    "float8_blockwise": {
+        "storage_t": torch.float8_e4m3fn,
+        "required_parameters": {"weight_scale"},
+        "optional_parameters": set(),
+        "comfy_tensor_layout": "BlockWiseFP8Layout",
+        "group_size": 128,
+        "asymmetric_layout": True,
+    },
 }
 
 LAYOUTS = {
@@ -489,6 +525,7 @@ LAYOUTS = {
     "AxisWiseINT8Layout": AxisWiseINT8Layout,
     "QuIPHadamardINT8Layout": QuIPHadamardINT8Layout,
     "GroupWiseINT4Layout": GroupWiseINT4Layout,
+    "BlockWiseFP8Layout": BlockWiseFP8Layout,
 }
 
 
@@ -675,6 +712,24 @@ def int4_linear(func, args, kwargs):
     q, scale, group_size, in_features = GroupWiseINT4Layout.get_plain_tensors(weight)
     assert x.shape[-1] == in_features, f"input has {x.shape[-1]} features, weight expects {in_features}"
     return ops.gemm_w4(x, q, scale, group_size, bias)
+
+
+@register_layout_op(torch.ops.aten.linear.default, "BlockWiseFP8Layout")
+def fp8_linear(func, args, kwargs):
+    """fp8 weight: quantized activations as they are, plain ones quantized first."""
+    x, weight = args[0], args[1]
+    bias = args[2] if len(args) > 2 else None
+
+    def fp8(t, is_weight):
+        return isinstance(t, QuantizedTensor) and t._layout_type == "BlockWiseFP8Layout" and \
+            t._layout_params["is_weight"] == is_weight
+    if not fp8(weight, True) or (isinstance(x, QuantizedTensor) and not fp8(x, False)):
+        return QuantizedTensor._dequant_and_fallback(func, args, kwargs)
+    w, w_s, _, _ = BlockWiseFP8Layout.get_plain_tensors(weight)
+    if isinstance(x, QuantizedTensor):
+        a, a_s, _, _ = BlockWiseFP8Layout.get_plain_tensors(x)
+        return ops.gemm_f8(a, a_s, w, w_s, bias, x._layout_params["orig_dtype"])
+    return ops.linear_f8(x, w, w_s, bias)
 
 
 def quip_hadamard_weight(q_rot: torch.Tensor, scale: torch.Tensor, sign_row: torch.Tensor, sign_col: torch.Tensor,

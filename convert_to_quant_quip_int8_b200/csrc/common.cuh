@@ -49,6 +49,10 @@ enum : unsigned int {
   ST_W4_UNPACK = 1u << 6,
   ST_W4_MMA = 1u << 7,
   ST_W4_EPILOGUE = 1u << 8,
+  ST_F8_PRODUCER = 1u << 9,
+  ST_F8_SCALES = 1u << 10,
+  ST_F8_MMA = 1u << 11,
+  ST_F8_EPILOGUE = 1u << 12,
 };
 
 // ---------------------------------------------------------- conversions

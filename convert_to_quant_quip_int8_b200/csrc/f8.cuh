@@ -1,0 +1,137 @@
+// The fp8 format with block scales and the pieces that its producers share.
+//
+//   value = code * 2^e,  code e4m3 (largest value 448),  e >= -100
+//
+// e is the smallest whole number with amax <= 448 * 2^e.  448 = 1.75 * 2^8, so
+// with the fp32 bits of amax, e is the exponent less 8, and one more when the
+// mantissa is above 0.75: adding 2^21 - 1 to the bits carries into the exponent
+// in just those cases.  A scale is one byte, e + 127, which is the exponent
+// field of the fp32 number 2^e; 255 is NaN.  value / 2^e is exact, so a code is
+// off by one rounding of e4m3, with a power of two as with any other scale.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace qi8 {
+
+constexpr int F8_BLOCK = 128;  // columns (of a weight: rows too) that share a scale
+constexpr int F8_E_MIN = -100;
+
+inline int64_t f8_blocks(int64_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }
+
+namespace {
+
+// The scale byte of a block whose largest |value| has these fp32 bits (an
+// infinity or a NaN, which compare above all numbers: 255).
+__device__ __forceinline__ uint32_t f8_scale_code(uint32_t amax_bits) {
+  if (amax_bits >= 0x7f800000u) return 255u;
+  const int c = (int)((amax_bits + 0x1fffffu) >> 23) - 8;
+  return (uint32_t)(c > F8_E_MIN + 127 ? c : F8_E_MIN + 127);
+}
+// 2^-e and 2^e of a scale byte, NaN for 255.
+__device__ __forceinline__ float f8_inverse(uint32_t code) {
+  return __uint_as_float(code == 255u ? 0x7fffffffu : (254u - code) << 23);
+}
+// Bytes of other origin reach down to 2^-127, a subnormal.
+__device__ __forceinline__ float f8_scale(uint32_t code) {
+  return __uint_as_float(code == 255u ? 0x7fffffffu : code == 0 ? 0x00400000u : code << 23);
+}
+__device__ __forceinline__ uint32_t f8_pack4(float a, float b, float c, float d) {
+  const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+  return lo | (hi << 16);
+}
+__device__ __forceinline__ float2 f8_unpack2(uint32_t two) {
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)two, __NV_E4M3);
+  return __half22float2(*reinterpret_cast<const __half2*>(&h));
+}
+
+// Eight consecutive elements of a row from column `col` on, zero from n on.
+// vec: the row starts on a 16-byte boundary (col is a multiple of 8).
+template <typename T>
+struct Eight {
+  uint4 v[sizeof(T) / 2];
+
+  __device__ __forceinline__ void load(const T* row, int64_t col, int64_t n, bool vec) {
+    if (vec && col + 8 <= n) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(row + col) + i);
+    } else {
+      T* e = reinterpret_cast<T*>(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) e[i] = col + i < n ? row[col + i] : T(0.0f);
+    }
+  }
+  __device__ __forceinline__ void store(T* row, int64_t col, int64_t n, bool vec) const {
+    if (vec && col + 8 <= n) {
+#pragma unroll
+      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + col)[i] = v[i];
+    } else {
+      const T* e = reinterpret_cast<const T*>(v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (col + i < n) row[col + i] = e[i];
+    }
+  }
+  __device__ __forceinline__ void get(float (&f)[8]) const {
+    const T* e = reinterpret_cast<const T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f32(e[i]);
+  }
+  __device__ __forceinline__ void set(const float (&f)[8]) {
+    T* e = reinterpret_cast<T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f32(f[i]);
+  }
+};
+
+// |values| as fp32 bits: whole-number comparisons keep infinities and NaN on top.
+__device__ __forceinline__ uint32_t amax_bits(const float (&f)[8]) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
+  return m;
+}
+// The largest over 16 neighbouring lanes: one block of 128 columns, eight per lane.
+__device__ __forceinline__ uint32_t max16(uint32_t m) {
+#pragma unroll
+  for (int o = 8; o > 0; o >>= 1) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
+  return m;
+}
+
+__device__ __forceinline__ uint2 f8_codes(const float (&f)[8], float inv) {
+  return make_uint2(f8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
+                    f8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+}
+// int8 scale of a block: amax / 127, at least `least` (an infinity or a NaN stays).
+__device__ __forceinline__ float i8_scale(uint32_t amax, float least) {
+  const float s = __fdiv_rn(__uint_as_float(amax), 127.0f);
+  return s < least ? least : s;
+}
+// rint(f * inv), |f * inv| < 127.5 or NaN (code 0)
+__device__ __forceinline__ uint2 i8_codes(const float (&f)[8], float inv) {
+  uint32_t w[2] = {0, 0};
+#pragma unroll
+  for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(__float2int_rn(f[i] * inv) & 0xff) << (8 * (i & 3));
+  return make_uint2(w[0], w[1]);
+}
+// Eight codes of a row.  vec: rows start on 8-byte boundaries.
+__device__ __forceinline__ void store_codes(uint8_t* row, int64_t col, int64_t n, uint2 c, bool vec) {
+  if (vec && col + 8 <= n) {
+    *reinterpret_cast<uint2*>(row + col) = c;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (col + i < n) row[col + i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
+  }
+}
+
+// Rows of elements of `size` bytes start on boundaries of `to` bytes.
+inline bool rows_aligned(const void* p, int64_t ld, int size, int to) {
+  return reinterpret_cast<uintptr_t>(p) % to == 0 && (ld * size) % to == 0;
+}
+
+}  // namespace
+}  // namespace qi8

@@ -531,13 +531,13 @@ def _check_i4(q: torch.Tensor, scale: torch.Tensor, k: int, group: int, dims: in
     assert q.is_contiguous() and scale.is_contiguous(), "4-bit codes and scales must be contiguous"
 
 
-def _no_grad(*tensors: Optional[torch.Tensor]) -> None:
+def _no_grad(*tensors: Optional[torch.Tensor], what: str = "4-bit operators") -> None:
     """Inference only: a result without a gradient (or a tangent of forward mode, which no_grad does not turn off) must
     not pass for one with it."""
     grad = torch.is_grad_enabled()
     for t in tensors:
         if t is not None and ((grad and t.requires_grad) or forward_ad.unpack_dual(t).tangent is not None):
-            raise RuntimeError("4-bit operators have no backward pass and no forward mode: call them on detached "
+            raise RuntimeError(f"{what} have no backward pass and no forward mode: call them on detached "
                                "tensors, or under torch.no_grad() if no input has a tangent")
 
 
@@ -658,6 +658,248 @@ def moe_w4(x: torch.Tensor, router: torch.Tensor, q13: torch.Tensor, s13: torch.
             router.data_ptr(), L.dtype_code(router.dtype), e, q13.data_ptr(), s13.data_ptr(), i, q2.data_ptr(),
             s2.data_ptr(), group, top_k, int(bool(renormalize)), act, out.data_ptr(), h, ws.data_ptr(), nbytes)
     return out if x.dim() == 2 else out.view(x.shape)
+
+
+# ---------------------------------------------------------------------------
+# fp8 with block scales, and the producers of quantized activations (formats:
+# include/qi8.h)
+# ---------------------------------------------------------------------------
+
+_F8, _E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+_FLOATS = (L.QI8_BF16, L.QI8_F16, L.QI8_F32)
+
+
+def _f8_blocks(n: int) -> int:
+    """Blocks of 128 columns (or rows) that ``n`` of them make."""
+    return -(-n // 128)
+
+
+def _refuse_grad(*tensors: Optional[torch.Tensor]) -> None:
+    _no_grad(*tensors, what="fp8 and fused quantization operators")
+
+
+def _float_code(dt: torch.dtype, what: str) -> int:
+    code = L._DTYPE.get(dt)
+    if code not in _FLOATS:
+        raise TypeError(f"{what} must be bfloat16, float16 or float32, got {dt}")
+    return code
+
+
+def _strided_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """``x`` as rows with unit column stride, and their stride."""
+    n = x.shape[-1]
+    x2 = x if x.dim() == 2 else x.reshape(-1, n)
+    if x2.shape[0] == 1 and (n <= 1 or x2.stride(1) == 1):
+        return x2, max(n, 1)
+    if (x2.stride(1) != 1 and n > 1) or x2.stride(0) < n:
+        x2 = x2.contiguous()
+    return x2, max(x2.stride(0), n, 1)
+
+
+def _new_codes(shape: tuple, dtype: torch.dtype, device) -> torch.Tensor:
+    """Room for codes of one byte whose rows start on 16-byte boundaries: the last dimension's rows are padded in
+    memory where they are no multiple of 16 long (a view, then)."""
+    n = shape[-1]
+    pitch = -(-n // 16) * 16
+    if pitch == n:
+        return torch.empty(shape, dtype=dtype, device=device)
+    return torch.empty((*shape[:-1], pitch), dtype=dtype, device=device)[..., :n]
+
+
+def _code_rows(q: torch.Tensor) -> Tuple[torch.Tensor, int]:
+    """Codes as rows [-1, n] and their stride; a layout that has no single row stride is copied."""
+    if q.dim() != 2:
+        q = q.reshape(-1, q.shape[-1])
+    return _strided_rows(q)
+
+
+def _check_f8(q: torch.Tensor, scale: torch.Tensor, tile: int) -> None:
+    """``q`` e4m3 [..., n] with a scale per row and 128 columns, or [N, K] with 128 x 128 tiles."""
+    if q.dtype != _F8 or scale.dtype != _E8:
+        raise TypeError(f"fp8 operands are float8_e4m3fn codes and float8_e8m0fnu scales, got {q.dtype} and {scale.dtype}")
+    assert q.dim() >= 1 and (tile == 1 or q.dim() == 2), f"fp8 codes of shape {tuple(q.shape)}"
+    lead = q.shape[:-1] if tile == 1 else (_f8_blocks(q.shape[0]),)
+    want = (*lead, _f8_blocks(q.shape[-1]))
+    assert tuple(scale.shape) == want, f"scales of shape {tuple(scale.shape)} for codes of shape {tuple(q.shape)}: " \
+                                       f"expected {want}"
+    assert scale.is_contiguous(), "fp8 scales must be contiguous"
+
+
+def quant_rows_f8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp8 codes ``[..., n]`` of ``x`` and one scale for each row and 128 columns ``[..., ceil(n / 128)]``."""
+    dev = _one_device(x)
+    dt = _float_code(x.dtype, "activations")
+    _refuse_grad(x)
+    assert x.dim() >= 1, "activations need a last dimension"
+    n = x.shape[-1]
+    q = _new_codes(x.shape, _F8, dev)
+    s = torch.empty(*x.shape[:-1], _f8_blocks(n), dtype=_E8, device=dev)
+    if q.numel():
+        x2, ld = _strided_rows(x)
+        _launch(dev, "qi8_quant_rows_f8", L.load().qi8_quant_rows_f8, x2.data_ptr(), dt, x2.shape[0], n, ld,
+                q.data_ptr(), -(-n // 16) * 16, s.data_ptr())
+    return q, s
+
+
+def quant_weight_f8(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp8 codes of ``w`` [N, K] (a parameter is read as it is) and one scale for each 128 x 128 tile."""
+    dev = _one_device(w)
+    dt = _float_code(w.dtype, "weights")
+    assert w.dim() == 2, f"weight of shape {tuple(w.shape)}: expected [N, K]"
+    n, k = w.shape
+    q = _new_codes(w.shape, _F8, dev)
+    s = torch.empty(_f8_blocks(n), _f8_blocks(k), dtype=_E8, device=dev)
+    if q.numel():
+        w2, ld = _strided_rows(w.detach())
+        _launch(dev, "qi8_quant_weight_f8", L.load().qi8_quant_weight_f8, w2.data_ptr(), dt, n, k, ld, q.data_ptr(),
+                -(-k // 16) * 16, s.data_ptr())
+    return q, s
+
+
+def dequant_f8(q: torch.Tensor, scale: torch.Tensor, tile: int, out_dtype: torch.dtype) -> torch.Tensor:
+    """The values that fp8 codes stand for: ``tile`` 1 for activations' scales, 128 for a weight's."""
+    dev = _one_device(q, scale)
+    _refuse_grad(q, scale)
+    _check_f8(q, scale, tile)
+    dt = _float_code(out_dtype, "output dtype")
+    out = torch.empty(q.shape, dtype=out_dtype, device=dev)
+    if out.numel():
+        q2, ld = _code_rows(q)
+        n = q.shape[-1]
+        _launch(dev, "qi8_dequant_f8", L.load().qi8_dequant_f8, q2.data_ptr(), q2.shape[0], n, ld, scale.data_ptr(), tile,
+                out.data_ptr(), dt, n)
+    return out
+
+
+def _f8_bias(bias: Optional[torch.Tensor], n: int) -> Tuple[Optional[torch.Tensor], Optional[int], int]:
+    if bias is None:
+        return None, None, 0
+    assert bias.dim() == 1 and bias.shape[0] == n, f"Bias must be 1D with length {n}, got shape {tuple(bias.shape)}"
+    bias = bias.contiguous()
+    return bias, bias.data_ptr(), _float_code(bias.dtype, "bias")
+
+
+def _no_columns(shape: tuple, n: int, bias: Optional[torch.Tensor], dtype: torch.dtype, dev) -> torch.Tensor:
+    """The product over no columns at all: the bias."""
+    out = torch.zeros(*shape, n, dtype=dtype, device=dev)
+    return out if bias is None else out.copy_(bias)
+
+
+def gemm_f8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+            bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+    """``a [..., K] b [N, K]^T + bias`` of fp8 operands."""
+    dev = _one_device(a, a_scale, b, b_scale, bias)
+    _refuse_grad(a, a_scale, b, b_scale, bias)
+    _check_f8(a, a_scale, 1)
+    _check_f8(b, b_scale, 128)
+    n, k = b.shape
+    assert a.shape[-1] == k, f"Shape mismatch: b.shape={tuple(b.shape)}, expected [N, {a.shape[-1]}]"
+    dt = _float_code(out_dtype, "output dtype")
+    bias, bias_ptr, bias_dt = _f8_bias(bias, n)
+    if k == 0:
+        return _no_columns(a.shape[:-1], n, bias, out_dtype, dev)
+    out = torch.empty(*a.shape[:-1], n, dtype=out_dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    a2, ld_a = _code_rows(a)
+    b2, ld_b = _strided_rows(b)
+    m = a2.shape[0]
+    lib = L.load()
+    nbytes = lib.qi8_gemm_f8_workspace_bytes(a2.data_ptr(), m, k, ld_a, b2.data_ptr(), n, ld_b)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(dev, "qi8_gemm_f8", lib.qi8_gemm_f8, a2.data_ptr(), a_scale.data_ptr(), m, k, ld_a, b2.data_ptr(),
+            b_scale.data_ptr(), n, ld_b, bias_ptr, bias_dt, out.data_ptr(), dt, n, ws.data_ptr() if nbytes else None, nbytes)
+    return out
+
+
+def linear_f8(x: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
+              bias: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """``quantized(x) b^T + bias`` in x's dtype: ``quant_rows_f8`` and ``gemm_f8``."""
+    dev = _one_device(x, b, b_scale, bias)
+    _refuse_grad(x, b, b_scale, bias)
+    _check_f8(b, b_scale, 128)
+    n, k = b.shape
+    dt = _float_code(x.dtype, "activations")
+    assert x.dim() >= 1 and x.shape[-1] == k, f"input of shape {tuple(x.shape)}, weight expects {k} features"
+    bias, bias_ptr, bias_dt = _f8_bias(bias, n)
+    if k == 0:
+        return _no_columns(x.shape[:-1], n, bias, x.dtype, dev)
+    out = torch.empty(*x.shape[:-1], n, dtype=x.dtype, device=dev)
+    if out.numel() == 0:
+        return out
+    x2, ld = _strided_rows(x)
+    b2, ld_b = _strided_rows(b)
+    m = x2.shape[0]
+    lib = L.load()
+    nbytes = lib.qi8_linear_f8_workspace_bytes(m, k, b2.data_ptr(), n, ld_b)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=dev) if nbytes else None
+    _launch(dev, "qi8_linear_f8", lib.qi8_linear_f8, x2.data_ptr(), dt, m, k, ld, b2.data_ptr(), b_scale.data_ptr(), n,
+            ld_b, bias_ptr, bias_dt, out.data_ptr(), dt, n, ws.data_ptr() if nbytes else None, nbytes)
+    return out
+
+
+def _quantized_out(shape: tuple, mode: int, dev) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales that a producer fills."""
+    n = shape[-1]
+    if mode == L.QI8_Q_FP8:
+        return _new_codes(shape, _F8, dev), torch.empty(*shape[:-1], _f8_blocks(n), dtype=_E8, device=dev)
+    # int8 rows are contiguous: the int8 products take them so
+    assert mode == L.QI8_Q_TOKEN or n % 128 == 0, \
+        f"Last dimension size must be divisible by block_size (block_size=128), got {n}"
+    s = torch.empty(*shape[:-1], 1 if mode == L.QI8_Q_TOKEN else n // 128, dtype=torch.float32, device=dev)
+    return torch.empty(shape, dtype=torch.int8, device=dev), s
+
+
+def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                   residual: Optional[torch.Tensor] = None, mode: int = L.QI8_Q_FP8):
+    """The root-mean-square norm of ``h = x + residual`` over the last dimension, times ``weight``, quantized:
+    ``(q, scale)``, and ``h`` in x's dtype as a third result where there is a residual."""
+    dev = _one_device(x, weight, residual)
+    _refuse_grad(x, weight, residual)
+    dt = _float_code(x.dtype, "activations")
+    assert x.dim() >= 1, "activations need a last dimension"
+    n = x.shape[-1]
+    w_ptr, w_dt = None, 0
+    if weight is not None:
+        assert weight.dim() == 1 and weight.shape[0] == n, f"weight of shape {tuple(weight.shape)}: expected [{n}]"
+        weight = weight.contiguous()
+        w_ptr, w_dt = weight.data_ptr(), _float_code(weight.dtype, "weight")
+    if residual is not None:
+        assert residual.shape == x.shape, f"residual of shape {tuple(residual.shape)} for {tuple(x.shape)}"
+        if residual.dtype != x.dtype:
+            raise TypeError(f"residual of {residual.dtype} for activations of {x.dtype}")
+    assert eps >= 0.0, f"eps {eps}"
+    q, s = _quantized_out(x.shape, mode, dev)
+    h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
+    if q.numel():
+        x2, ld = _strided_rows(x)
+        r_ptr, ld_r, h_ptr = None, 0, None
+        if residual is not None:
+            r2, ld_r = _strided_rows(residual)
+            r_ptr, h_ptr = r2.data_ptr(), h.data_ptr()
+        _launch(dev, "qi8_rms_norm_quant", L.load().qi8_rms_norm_quant, x2.data_ptr(), dt, x2.shape[0], n, ld, r_ptr,
+                ld_r, w_ptr, w_dt, eps, mode, q.data_ptr(), -(-n // 16) * 16 if mode == L.QI8_Q_FP8 else n, s.data_ptr(),
+                h_ptr, n)
+    return (q, s) if residual is None else (q, s, h)
+
+
+def gated_quant(gate: torch.Tensor, up: torch.Tensor, act: int = L.QI8_ACT_SILU,
+                mode: int = L.QI8_Q_FP8) -> Tuple[torch.Tensor, torch.Tensor]:
+    """``act(gate) * up``, quantized: ``(q, scale)``."""
+    dev = _one_device(gate, up)
+    _refuse_grad(gate, up)
+    dt = _float_code(gate.dtype, "activations")
+    if up.dtype != gate.dtype:
+        raise TypeError(f"gate of {gate.dtype} and up of {up.dtype}")
+    assert gate.dim() >= 1 and gate.shape == up.shape, f"gate of shape {tuple(gate.shape)}, up of {tuple(up.shape)}"
+    n = gate.shape[-1]
+    q, s = _quantized_out(gate.shape, mode, dev)
+    if q.numel():
+        g2, ld_g = _strided_rows(gate)
+        u2, ld_u = _strided_rows(up)
+        _launch(dev, "qi8_gated_quant", L.load().qi8_gated_quant, g2.data_ptr(), ld_g, u2.data_ptr(), ld_u, dt,
+                g2.shape[0], n, act, mode, q.data_ptr(), -(-n // 16) * 16 if mode == L.QI8_Q_FP8 else n, s.data_ptr())
+    return q, s
 
 
 def device_status(reset: bool = True) -> None:

@@ -59,6 +59,9 @@ enum {
   /* per (row, 128-block): s = amax/127; q = trunc(x / s)
      -- Triton act_quant, comfy/int8_kernels.py:72-123 */
   QI8_Q_BLOCK = 1,
+  /* qi8_rms_norm_quant, qi8_gated_quant: e4m3 codes, one power-of-two scale per
+     128 columns (the fp8 format below) */
+  QI8_Q_FP8 = 2,
   /* flag for qi8_quant_rows: apply exact-erf GELU to every element first
      (rounded to the input dtype, as torch's gelu on that tensor), then
      quantize -- the GELU between the two projections of a DiT MLP */
@@ -75,8 +78,9 @@ enum {
   QI8_S_TILE128 = 4    /* [rows/128, K/128]: per 128x128 weight tile (comfy block weight) */
 };
 
-/* GEMM epilogue activation (SILU: the expert layer's gate only) */
-enum { QI8_ACT_NONE = 0, QI8_ACT_GELU = 1, QI8_ACT_SILU = 2 };
+/* GEMM epilogue activation (SILU: the gates of the expert layer and of
+   qi8_gated_quant; GELU_TANH, the tanh form: the latter's only) */
+enum { QI8_ACT_NONE = 0, QI8_ACT_GELU = 1, QI8_ACT_SILU = 2, QI8_ACT_GELU_TANH = 3 };
 
 /* weight requantization schemes (converters/quip_int8.py:1614-1669) */
 enum { QI8_REQ_ROW = 0, QI8_REQ_GLOBAL = 1, QI8_REQ_BLOCK = 2 };
@@ -453,6 +457,75 @@ QI8_API int qi8_moe_w4(const void* x, int x_dtype, int64_t T, int64_t H, int64_t
                        int router_dtype, int64_t E, const uint8_t* q13, const void* s13, int64_t I,
                        const uint8_t* q2, const void* s2, int group, int top_k, int renormalize, int act, void* out,
                        int64_t ld_out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- fp8 with block scales (no counterpart in the reference).
+   value = code * 2^e.  Codes are e4m3 (one byte, largest value 448).  Scales
+   are powers of two held as one byte e + 127 (255: NaN): e is the smallest
+   whole number >= -100 with amax <= 448 * 2^e, so that value / 2^e is exact
+   and a code is one rounding (to nearest, ties to even) away from the value.
+   Activations have a scale for each row and 128 columns, [rows, ceil(n / 128)],
+   weights one for each 128 x 128 tile, [ceil(N / 128), ceil(K / 128)]; the last
+   blocks may be smaller.  A block that holds an infinity or a NaN reads back as
+   NaN as a whole. */
+
+/* x [rows, n] bf16 / f16 / f32 (row stride ld_x) -> q_out [rows, n] (row
+   stride ld_q bytes), scale_out [rows, ceil(n / 128)]. */
+QI8_API int qi8_quant_rows_f8(const void* x, int x_dtype, int64_t rows, int64_t n, int64_t ld_x, uint8_t* q_out,
+                              int64_t ld_q, uint8_t* scale_out, void* stream);
+
+/* The same in 128 x 128 tiles: scale_out [ceil(N / 128), ceil(K / 128)]. */
+QI8_API int qi8_quant_weight_f8(const void* w, int w_dtype, int64_t N, int64_t K, int64_t ld_w, uint8_t* q_out,
+                                int64_t ld_q, uint8_t* scale_out, void* stream);
+
+/* out [rows, n] (row stride ld_out) = code * scale as bf16 / f16 / f32.  tile:
+   1 for a scale per row and 128 columns, 128 for 128 x 128 tiles. */
+QI8_API int qi8_dequant_f8(const uint8_t* q, int64_t rows, int64_t n, int64_t ld_q, const uint8_t* scale, int tile,
+                           void* out, int out_dtype, int64_t ld_out, void* stream);
+
+/* out [M, N] = A B^T + bias, fp32 sums: A [M, K] codes (row stride ld_a) with
+   a scale per row and 128 columns, B [N, K] codes (row stride ld_b) with 128 x
+   128 tiles; bias (or null) [N] bf16 / f16 / f32; out bf16 / f16 / f32 (row
+   stride ld_out).  Operands whose rows do not start on 16-byte boundaries are
+   copied to such rows in the workspace: qi8_gemm_f8_workspace_bytes bytes (0
+   when none is needed), 16-byte aligned, its contents do not matter; calls that
+   overlap need one each. */
+QI8_API int64_t qi8_gemm_f8_workspace_bytes(const uint8_t* a, int64_t M, int64_t K, int64_t ld_a, const uint8_t* b,
+                                            int64_t N, int64_t ld_b);
+QI8_API int qi8_gemm_f8(const uint8_t* a, const uint8_t* a_scale, int64_t M, int64_t K, int64_t ld_a,
+                        const uint8_t* b, const uint8_t* b_scale, int64_t N, int64_t ld_b, const void* bias,
+                        int bias_dtype, void* out, int out_dtype, int64_t ld_out, void* workspace,
+                        int64_t workspace_bytes, void* stream);
+
+/* out [M, N] = quantized(x) B^T + bias: x [M, K] bf16 / f16 / f32 (row stride
+   ld_x) quantized as by qi8_quant_rows_f8, then as qi8_gemm_f8.  Workspace as
+   there, qi8_linear_f8_workspace_bytes bytes. */
+QI8_API int64_t qi8_linear_f8_workspace_bytes(int64_t M, int64_t K, const uint8_t* b, int64_t N, int64_t ld_b);
+QI8_API int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* b,
+                          const uint8_t* b_scale, int64_t N, int64_t ld_b, const void* bias, int bias_dtype, void* out,
+                          int out_dtype, int64_t ld_out, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- producers of quantized activations (no counterpart in the reference).
+   mode QI8_Q_TOKEN: q_out int8, scale_out fp32 [rows] = max(amax / 127, 1e-30);
+   QI8_Q_BLOCK: q_out int8, scale_out fp32 [rows, n / 128] = max(amax / 127,
+   1e-8), n % 128 == 0; both q = rint(y * (1 / scale)) in [-127, 127] (act_quant
+   and qi8_quant_rows' block mode truncate: twice the error).  QI8_Q_FP8: q_out
+   e4m3, scale_out bytes [rows, ceil(n / 128)].  A scale whose block holds an
+   infinity or a NaN is no finite number, and the block reads back as NaN.
+   Strides in elements of their tensor; q_out has row stride ld_q. */
+
+/* y = h * (mean(h^2) + eps)^-1/2 * weight with h = x + residual (residual or
+   null), rounded to x's type and stored to sum_out (when not null); y is not
+   rounded before it is quantized.  x, residual, sum_out of x_dtype (bf16 / f16
+   / f32), weight (or null: ones) [n] bf16 / f16 / f32. */
+QI8_API int qi8_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int64_t n, int64_t ld_x,
+                               const void* residual, int64_t ld_residual, const void* weight, int weight_dtype,
+                               double eps, int mode, void* q_out, int64_t ld_q, void* scale_out, void* sum_out,
+                               int64_t ld_sum, void* stream);
+
+/* y = act(gate) * up in fp32; act QI8_ACT_SILU, QI8_ACT_GELU (erf) or
+   QI8_ACT_GELU_TANH; gate and up [rows, n] of the same type (bf16 / f16 / f32). */
+QI8_API int qi8_gated_quant(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, int64_t rows,
+                            int64_t n, int act, int mode, void* q_out, int64_t ld_q, void* scale_out, void* stream);
 
 #ifdef __cplusplus
 }

@@ -821,3 +821,46 @@ def moe_route(logits: np.ndarray, top_k: int, renormalize: bool) -> np.ndarray:
         p = np.exp(row - row.max())
         out[t, best] = p[best] / (p[best].sum() if renormalize else p.sum())
     return out
+
+
+# ---------------------------------------------------------------------------
+# fp8 with block scales (no counterpart in the reference)
+# ---------------------------------------------------------------------------
+
+def f8_scale(amax: np.ndarray) -> np.ndarray:
+    """2^e with the smallest whole e >= -100 for which amax <= 448 * 2^e; NaN
+    where amax is not finite."""
+    amax = np.asarray(amax, np.float64)
+    finite = np.isfinite(amax)
+    mant, exp = np.frexp(np.where(finite, amax, 0.0))  # mant in [0.5, 1), 448 = 0.875 * 2^9
+    e = np.where(mant > 0, np.maximum(exp - 9 + (mant > 0.875), -100), -100)
+    return np.where(finite, np.ldexp(1.0, e), np.nan)
+
+
+def f8_round(v: np.ndarray) -> np.ndarray:
+    """The nearest e4m3 number of each |v| <= 448, ties to the even code."""
+    v = np.asarray(v, np.float64)
+    _, exp = np.frexp(v)
+    step = np.ldexp(1.0, np.maximum(exp - 1, -6) - 3)
+    return np.rint(v / step) * step
+
+
+def f8_quantize(v: np.ndarray, tile: int) -> Tuple[np.ndarray, np.ndarray]:
+    """``(codes, scales)`` as fp64 numbers of a matrix, blocks of ``tile`` rows (1 or
+    128) by 128 columns; a block that is not finite gets NaN."""
+    v = np.asarray(v, np.float64)
+    rows, n = v.shape
+    s = np.empty((-(-rows // tile), -(-n // 128)))
+    q = np.empty_like(v)
+    for i in range(s.shape[0]):
+        for j in range(s.shape[1]):
+            at = np.s_[i * tile:(i + 1) * tile, j * 128:(j + 1) * 128]
+            s[i, j] = f8_scale(np.abs(v[at]).max())
+            q[at] = f8_round(v[at] / s[i, j]) if np.isfinite(s[i, j]) else np.nan
+    return q, s
+
+
+def f8_values(q: np.ndarray, s: np.ndarray, tile: int) -> np.ndarray:
+    """What codes and scales stand for, in fp64."""
+    full = np.repeat(np.repeat(np.asarray(s, np.float64), tile, 0)[:q.shape[0]], 128, 1)[:, :q.shape[1]]
+    return np.asarray(q, np.float64) * full
