@@ -19,6 +19,19 @@ namespace qi8 {
 constexpr int F8_BLOCK = 128;  // columns (of a weight: rows too) that share a scale
 constexpr int F8_E_MIN = -100;
 
+// A product of fp8 operands: out [M, N] = a [M, K] b [N, K]^T + bias.
+struct F8Gemm {
+  const uint8_t *a, *b, *sa, *sb;  // codes; scales [M, KB] and [ceil(N / 128), KB]
+  const void* bias;
+  void* out;
+  int64_t ld_a, ld_b, ld_out;
+  int M, N, K, KB;  // KB = ceil(K / 128)
+  int bias_dtype, out_dtype;
+};
+
+// The tcgen05 kernels (gemm_f8_tc.cu): rows of both operands start on 16-byte boundaries.
+int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st);
+
 inline int64_t f8_blocks(int64_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }
 
 namespace {

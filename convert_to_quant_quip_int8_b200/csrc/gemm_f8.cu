@@ -13,14 +13,7 @@ int quant_rows_f8(const void* x, int x_dtype, int64_t rows, int64_t n, int64_t l
 namespace {
 namespace f8g {
 
-struct Args {
-  const uint8_t *a, *b, *sa, *sb;
-  const void* bias;
-  void* out;
-  int64_t ld_a, ld_b, ld_out;
-  int M, N, K, KB;
-  int bias_dtype, out_dtype;
-};
+using Args = F8Gemm;
 
 // 32 x 32 outputs per thread block, 32 columns of K at a time.
 __global__ void __launch_bounds__(256) tile_kernel(const Args p) {
@@ -53,6 +46,7 @@ __global__ void __launch_bounds__(256) tile_kernel(const Args p) {
 bool is_float(int dtype) { return dtype == QI8_BF16 || dtype == QI8_F16 || dtype == QI8_F32; }
 
 int gemm(const Args& p, cudaStream_t st) {
+  if (rows_aligned(p.a, p.ld_a, 1, 16) && rows_aligned(p.b, p.ld_b, 1, 16)) return gemm_f8_tiles(p, st);
   const dim3 grid((unsigned)((p.N + 31) / 32), (unsigned)((p.M + 31) / 32));
   tile_kernel<<<grid, 256, 0, st>>>(p);
   return check_cuda(cudaGetLastError(), "tile_kernel launch");
@@ -91,7 +85,7 @@ extern "C" int qi8_gemm_f8(const uint8_t* a, const uint8_t* a_scale, int64_t M, 
   QI8_REQUIRE(ld_a >= K, QI8_ESHAPE, "row stride %lld for %lld columns", (long long)ld_a, (long long)K);
   if (M == 0 || N == 0) return QI8_OK;
   QI8_REQUIRE(a && a_scale && b && b_scale && out, QI8_EINVAL, "null pointer");
-  const f8g::Args p{a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
+  const F8Gemm p{a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
                     bias_dtype, out_dtype};
   return f8g::gemm(p, static_cast<cudaStream_t>(stream));
 }
@@ -114,7 +108,7 @@ extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, i
   uint8_t* q = static_cast<uint8_t*>(workspace);
   uint8_t* s = q + M * f8g::pitch(K);
   if (int rc = quant_rows_f8(x, x_dtype, M, K, ld_x, q, f8g::pitch(K), s, st)) return rc;
-  const f8g::Args p{q, b, s, b_scale, bias, out, f8g::pitch(K), ld_b, ld_out, (int)M, (int)N, (int)K,
+  const F8Gemm p{q, b, s, b_scale, bias, out, f8g::pitch(K), ld_b, ld_out, (int)M, (int)N, (int)K,
                     (int)f8_blocks(K), bias_dtype, out_dtype};
   return f8g::gemm(p, st);
 }

@@ -1,0 +1,400 @@
+// Products of fp8 operands with block scales on the tcgen05 tensor cores
+// (format: f8.cuh):
+//
+//   out[t, n] = sum_kb 2^(ea[t, kb] + eb[n / 128, kb]) sum_{k in kb} a[t, k] b[n, k] + bias[n]
+//
+// Scales that are powers of two are what tcgen05.mma.kind::mxf8f6f4 applies by
+// itself: it takes one byte e + 127 per row and 32 columns of K from tensor
+// memory, so the four steps of a 128-block read the same byte.  The sums stay in
+// the accumulator over all of K.
+#include <cstdint>
+
+#include "f8.cuh"
+#include "tc05.cuh"
+
+namespace qi8 {
+namespace {
+namespace f8tc {
+
+constexpr int BK = 128;  // columns of K per stage: one swizzled row of codes, one scale
+constexpr uint32_t TMEM_COLS = 512;
+
+// e4m3 operands, K-major, fp32 sums, scale bytes (UE8M0); sf: which of the four
+// bytes of a scale word this step reads, for both operands
+__host__ __device__ constexpr uint32_t idesc(int m, int n, uint32_t sf = 0) {
+  return (sf << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) | (sf << 29);
+}
+
+// Four scale bytes of a row, K blocks kb .. kb + 3 (whatever stands there past the end).
+__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int kb, int KB, bool words) {
+  if (words) return __ldg(reinterpret_cast<const uint32_t*>(row + kb));
+  uint32_t w = 0;
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (kb + i < KB) w |= (uint32_t)__ldg(row + kb + i) << (8 * i);
+  return w;
+}
+
+__device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&r)[4]) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3])
+               : "memory");
+}
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// 32 results of one row from column n on.  vec: rows start on 16-byte boundaries.
+__device__ __forceinline__ void store32(const F8Gemm& g, int64_t m, int n, const float (&y)[32], bool vec) {
+  const int64_t at = m * g.ld_out + n;
+  if (vec && n + 32 <= g.N) {
+    if (g.out_dtype == QI8_F32) {
+      float4* o = reinterpret_cast<float4*>(static_cast<float*>(g.out) + at);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) o[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
+    } else {
+      uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + at);
+      const bool half = g.out_dtype == QI8_F16;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t w[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float a = y[8 * i + 2 * j], b = y[8 * i + 2 * j + 1];
+          if (half) {
+            const __half2 h = __floats2half2_rn(a, b);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          } else {
+            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+            w[j] = *reinterpret_cast<const uint32_t*>(&h);
+          }
+        }
+        o[i] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j)
+      if (n + j < g.N) store_from_f32(g.out, g.out_dtype, at + j, y[j]);
+  }
+}
+
+// ------------------------------------------------- large: pairs of blocks
+// A cluster of two blocks computes 256 tokens x 256 features: each block holds
+// 128 tokens (TMEM lanes) and loads half of both operands' rows, so that a
+// 128-column stage costs 32 KB of L2 reads per block.  Roles of a block:
+//   warps 0..7    epilogue (warp w: lanes 32 (w % 4), every other half)
+//   warps 8..11   scales: global memory -> tensor memory, four K blocks at a time
+//   warp 12       TMA producer
+//   warp 13       TMEM allocation; MMA issue (one thread of the even block)
+// Two accumulators of 256 columns and the scales do not fit 512 columns, so the
+// accumulators share 32: the epilogue reads those first, and the next tile's
+// MMAs wait for just that.
+namespace pair {
+
+constexpr int EPI_WARPS = 8, SCALE_WARP0 = 8, SCALE_WARPS = 4, PRODUCER = 12, ISSUER = 13;
+constexpr int THREADS = 14 * 32;
+constexpr int STAGES = 6, OPERAND = 128 * BK, STAGE = 2 * OPERAND;
+constexpr int ACC1 = 224, SHARED_CHUNK0 = 7, SHARED_CHUNK1 = 0;  // accumulator 1's columns; the shared 32 of each
+constexpr int SCALES = 480, SLOT = 16;                           // two slots: 8 columns of b, 4 of a
+constexpr int BARS = 2 * STAGES + 4 + 4 + 2;
+constexpr int SMEM = 1024 + STAGES * STAGE + EPI_WARPS * 32 * 4 + BARS * 8 + 16;
+static_assert(SMEM <= 232448 && SCALES + 2 * SLOT <= (int)TMEM_COLS && ACC1 + 256 <= SCALES, "memories");
+
+struct Args {
+  F8Gemm g;
+  int m_tiles, n_tiles;
+  bool words_a, words_b, vec_out;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                    uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accum)
+      : "memory");
+}
+// arrives on the barrier at this offset in both blocks once all earlier MMAs are done
+__device__ __forceinline__ void commit(uint32_t bar, uint16_t mask) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+               "h"(mask)
+               : "memory");
+}
+__device__ __forceinline__ void arrive_release(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                    const __grid_constant__ Args p) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* sm = smem_raw + (base - raw);
+  const uint32_t sA = base, sB = base + STAGES * OPERAND;
+  float* sbias = reinterpret_cast<float*>(sm + STAGES * STAGE);
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sbias + EPI_WARPS * 32);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto full_bar = [&](int s) { return smem_u32(bars + s); };
+  auto empty_bar = [&](int s) { return smem_u32(bars + STAGES + s); };
+  auto tfull_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + b); };
+  auto tempty_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + 2 + b); };
+  auto sfull_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + 4 + b); };
+  auto sempty_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + 6 + b); };
+  const uint32_t tshared_bar = smem_u32(bars + 2 * STAGES + 8), drain_bar = smem_u32(bars + 2 * STAGES + 9);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cta_rank();
+  const bool leader = rank == 0;
+  const int pair0 = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {  // warps of both blocks
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), 2 * EPI_WARPS);
+      mbar_init(sfull_bar(b), 2 * SCALE_WARPS);
+      mbar_init(sempty_bar(b), 1);
+    }
+    mbar_init(tshared_bar, 2 * EPI_WARPS / 2);
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == ISSUER) {
+    asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+  }
+  if (warp == PRODUCER && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  tc_fence_before();
+  cluster_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int KB = p.g.KB, tiles = p.m_tiles * p.n_tiles;
+
+  if (warp == PRODUCER) {
+    if (lane == 0) {
+      const uint32_t full0 = mapa(full_bar(0), 0);
+      int s = 0;
+      uint32_t ph = 0, issued = 0, issued_ph = 0;
+      bool ok = true;
+      for (int tile = pair0; ok && tile < tiles; tile += pairs) {
+        const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128, n0 = (tile / p.m_tiles) * 256 + (int)rank * 128;
+        for (int kb = 0; kb < KB; ++kb) {
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, ST_F8_PRODUCER, WAIT_LIMIT_NS)) {
+            ok = false;
+            break;
+          }
+          if (leader) mbar_arrive_expect_tx(full_bar(s), 2 * STAGE);
+          tma_load(sA + s * OPERAND, &tmA, kb * BK, m0, full0 + 8 * s);
+          tma_load(sB + s * OPERAND, &tmB, kb * BK, n0, full0 + 8 * s);
+          issued |= 1u << s;
+          issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
+          if (++s == STAGES) s = 0, ph ^= 1u;
+        }
+      }
+      // copies that no MMA waits for any more land before the blocks exit
+      if (!ok && leader)
+        for (int t = 0; t < STAGES; ++t)
+          if (issued & (1u << t)) drain_wait(full_bar(t), (issued_ph >> t) & 1u);
+    }
+  } else if (warp == ISSUER) {
+    if (leader && lane == 0) {
+      int s = 0, unit = 0;
+      uint32_t ph = 0;
+      unsigned slot = 0;  // scale slots used so far
+      bool ok = true;
+      for (int tile = pair0; ok && tile < tiles; tile += pairs, ++unit) {
+        const int buf = unit & 1;
+        if (!mbar_wait(tempty_bar(buf), ((unit >> 1) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+        if (unit > 0 && !mbar_wait(tshared_bar, (unit - 1) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + (buf ? ACC1 : 0);
+        for (int kb = 0; kb < KB; ++kb) {
+          const uint32_t sb = tmem + SCALES + (slot & 1) * SLOT;
+          if (((kb & 3) == 0 && !mbar_wait(sfull_bar(slot & 1), (slot >> 1) & 1, abort_flag, p.status, ST_F8_MMA,
+                                           WAIT_LIMIT_NS)) ||
+              !mbar_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const uint64_t da = sw128_desc(sA + s * OPERAND), db = sw128_desc(sB + s * OPERAND);
+#pragma unroll
+          for (int k = 0; k < BK / 32; ++k)
+            mma(d, da + 2 * k, db + 2 * k, idesc(256, 256, kb & 3), sb + 8, sb, kb > 0 || k > 0);
+          commit(empty_bar(s), 3);
+          if ((kb & 3) == 3 || kb + 1 == KB) {
+            commit(sempty_bar(slot & 1), 3);
+            ++slot;
+          }
+          if (++s == STAGES) s = 0, ph ^= 1u;
+        }
+        if (ok) commit(tfull_bar(buf), 3);
+      }
+      commit(drain_bar, 1);
+      drain_wait(drain_bar, 0);
+    }
+  } else if (warp >= SCALE_WARP0) {
+    // ---------------------------------------------------------- scales
+    // word i of a: token 32 i + lane, in the same lane of all four quarters of
+    // tensor memory; the features' words are the same for 128 of them
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + SCALES;
+    const uint32_t sfull0 = mapa(sfull_bar(0), 0);
+    auto load = [&](int tile, int kb, uint32_t (&a)[4], uint32_t (&b)[2]) {
+      const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128, t0 = (tile / p.m_tiles) * 2;
+      const int last = (p.g.N - 1) / F8_BLOCK;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        a[i] = scale_word(p.g.sa + (int64_t)min(m0 + 32 * i + lane, p.g.M - 1) * KB, kb, KB, p.words_a);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) b[i] = scale_word(p.g.sb + (int64_t)min(t0 + i, last) * KB, kb, KB, p.words_b);
+    };
+    unsigned slot = 0;
+    bool ok = true;
+    uint32_t a[4], b[2];
+    if (pair0 < tiles) load(pair0, 0, a, b);
+    for (int tile = pair0; ok && tile < tiles; tile += pairs) {
+      for (int kb = 0; kb < KB; kb += 4, ++slot) {
+        uint32_t a_next[4] = {0, 0, 0, 0}, b_next[2] = {0, 0};
+        if (kb + 4 < KB) load(tile, kb + 4, a_next, b_next);
+        else if (tile + pairs < tiles) load(tile + pairs, 0, a_next, b_next);
+        if (!warp_wait(sempty_bar(slot & 1), ((slot >> 1) & 1) ^ 1u, abort_flag, p.status, ST_F8_SCALES, WAIT_LIMIT_NS)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at = lanes + (slot & 1) * SLOT;
+        const uint32_t lo[4] = {b[0], b[0], b[0], b[0]}, hi[4] = {b[1], b[1], b[1], b[1]};
+        tmem_st4(at, lo);
+        tmem_st4(at + 4, hi);
+        tmem_st4(at + 8, a);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_release(sfull0 + 8 * (slot & 1));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) a[i] = a_next[i];
+        b[0] = b_next[0];
+        b[1] = b_next[1];
+      }
+    }
+  } else {
+    // -------------------------------------------------------- epilogue
+    const int quarter = warp & 3, half = warp >> 2;
+    const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t tempty0 = mapa(tempty_bar(0), 0), tshared0 = mapa(tshared_bar, 0);
+    float* my_bias = sbias + warp * 32;
+    int unit = 0;
+    for (int tile = pair0; tile < tiles; tile += pairs, ++unit) {
+      const int buf = unit & 1;
+      const int64_t m = (int64_t)(tile % p.m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane;
+      const int n0 = (tile / p.m_tiles) * 256;
+      // the shared 32 columns first: the lower half of the warps has them in both accumulators
+      auto chunk = [&](int i) {
+        if (buf) return 4 * half + i;
+        return half ? 3 + i : (i == 0 ? SHARED_CHUNK0 : i - 1);
+      };
+      if (!warp_wait(tfull_bar(buf), (unit >> 1) & 1, abort_flag, p.status, ST_F8_EPILOGUE, WAIT_LIMIT_NS)) break;
+      tc_fence_after();
+      const uint32_t acc = lanes + (buf ? ACC1 : 0);
+      uint32_t r[2][32];
+      tmem_ld32(acc + 32 * chunk(0), r[0]);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        tmem_wait_ld();
+        if (i < 3) tmem_ld32(acc + 32 * chunk(i + 1), r[(i + 1) & 1]);
+        if (i == 0 && half == 0) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_release(tshared0);
+        }
+        if (i == 3) {
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) arrive_release(tempty0 + 8 * buf);
+        }
+        const int n = n0 + 32 * chunk(i);
+        float y[32];
+#pragma unroll
+        for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(r[i & 1][j]);
+        if (p.g.bias) {
+          __syncwarp();
+          my_bias[lane] = n + lane < p.g.N ? load_as_f32(p.g.bias, p.g.bias_dtype, n + lane) : 0.0f;
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 32; ++j) y[j] += my_bias[j];
+        }
+        if (m < p.g.M && n < p.g.N) store32(p.g, m, n, y, p.vec_out);
+      }
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  cluster_sync();
+  if (warp == ISSUER) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+}  // namespace pair
+
+// Codes [rows, K] -> boxes of `box` rows x 128 columns, 128-byte swizzle, zeros outside.
+int code_map8(CUtensorMap* map, const uint8_t* q, int64_t rows, int64_t K, int64_t ld, int box) {
+  EncodeTiledFn fn = encode_fn();
+  QI8_REQUIRE(fn, QI8_ECUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t dims[2] = {(cuuint64_t)K, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)ld};
+  cuuint32_t boxes[2] = {(cuuint32_t)BK, (cuuint32_t)box}, one[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<uint8_t*>(q), dims, strides, boxes, one,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  QI8_REQUIRE(r == CUDA_SUCCESS, QI8_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return QI8_OK;
+}
+
+// Scale rows that can be read a word at a time.
+bool word_rows(const uint8_t* s, int KB) { return KB % 4 == 0 && reinterpret_cast<uintptr_t>(s) % 4 == 0; }
+
+int launch_pair(const F8Gemm& g, cudaStream_t st) {
+  static bool done[64];
+  int dev = 0;
+  QI8_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !done[dev]) {
+    QI8_CUDA(cudaFuncSetAttribute(pair::gemm_f8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM));
+    if (dev < 64) done[dev] = true;
+  }
+  CUtensorMap ma, mb;
+  if (int rc = code_map8(&ma, g.a, g.M, g.K, g.ld_a, 128)) return rc;
+  if (int rc = code_map8(&mb, g.b, g.N, g.K, g.ld_b, 128)) return rc;
+  pair::Args p{g, (g.M + 255) / 256, (g.N + 255) / 256, word_rows(g.sa, g.KB), word_rows(g.sb, g.KB),
+               rows_aligned(g.out, g.ld_out, elem_size(g.out_dtype), 16), device_status_ptr()};
+  const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+  QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
+  const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
+  pair::gemm_f8_pair_kernel<<<(unsigned)(2 * pairs), pair::THREADS, pair::SMEM, st>>>(ma, mb, p);
+  return check_cuda(cudaGetLastError(), "gemm_f8_pair_kernel launch");
+}
+
+}  // namespace f8tc
+}  // namespace
+
+int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) { return f8tc::launch_pair(g, st); }
+
+}  // namespace qi8
