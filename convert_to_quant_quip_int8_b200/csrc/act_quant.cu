@@ -24,33 +24,48 @@ struct Args {
   void *q, *scale, *sum;
   int64_t ld_x, ld_second, ld_q, ld_sum;
   int64_t rows, n, blocks;
-  double eps;
-  int weight_dtype, act, mode;
+  float eps;
+  int weight_dtype, mode;
   bool vec, vec_weight, vec_q, vec_sum;
 };
 
-// g / (1 + exp(-t)).  An exp beyond fp32 makes it 0, as it should be.
-__device__ __forceinline__ float swish(float g, float t) { return __fdividef(g, 1.0f + expf(-t)); }
+// x 2^t / (1 + 2^t) ... as x / (1 + 2^-t): 0 where 2^-t passes fp32, as it should be
+// (MUFU's exp2 and reciprocal: 2 and 1 units in the last place)
+__device__ __forceinline__ float2 swish(float2 x, float2 minus_t) {
+  float2 e;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(minus_t.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(minus_t.y));
+  e = __fadd2_rn(e, make_float2(1.0f, 1.0f));
+  return make_float2(__fdividef(x.x, e.x), __fdividef(x.y, e.y));
+}
 
-// One activation for eight columns: y = act(y) * up
-__device__ __forceinline__ void gate(float (&y)[8], const float (&up)[8], int act) {
-  if (act == QI8_ACT_SILU) {
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+// y = act(g) * up
+template <int ACT>
+__device__ __forceinline__ F8x gate(const F8x& g, const F8x& up) {
+  F8x y;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = swish(y[i], y[i]) * up[i];
-  } else if (act == QI8_ACT_GELU) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = gelu_erf(y[i]) * up[i];
-  } else {
-    // 0.5 g (1 + tanh(u)) = g / (1 + exp(-2 u)), u = sqrt(2 / pi) (g + 0.044715 g^3)
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      y[i] = swish(y[i], 1.5957691216057308f * fmaf(0.044715f * y[i] * y[i], y[i], y[i])) * up[i];
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = g.v[i];
+    float2 a;
+    if constexpr (ACT == QI8_ACT_SILU) {
+      a = swish(x, __fmul2_rn(x, both(-1.4426950408889634f)));  // -log2(e)
+    } else if constexpr (ACT == QI8_ACT_GELU) {
+      a = make_float2(gelu_erf(x.x), gelu_erf(x.y));
+    } else {
+      // 0.5 x (1 + tanh(u)) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
+      const float2 c = __ffma2_rn(__fmul2_rn(x, x), both(-0.10294324f), both(-2.3022082f));
+      a = swish(x, __fmul2_rn(x, c));
+    }
+    y.v[i] = __fmul2_rn(a, up.v[i]);
   }
+  return y;
 }
 
 // A block of columns to codes and a scale; m: the maximum of what shares the
 // scale, as bits.  `first`: this lane writes the scale at index s.
-__device__ __forceinline__ void emit(const Args& p, const float (&y)[8], uint32_t m, int64_t row, int64_t col, bool first,
+__device__ __forceinline__ void emit(const Args& p, const F8x& y, uint32_t m, int64_t row, int64_t col, bool first,
                                      int64_t s) {
   uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.ld_q;
   if (p.mode == QI8_Q_FP8) {
@@ -64,46 +79,89 @@ __device__ __forceinline__ void emit(const Args& p, const float (&y)[8], uint32_
   }
 }
 
-__device__ __forceinline__ void load_weight(const Args& p, int64_t col, float (&w)[8]) {
-  if (p.weight_dtype == QI8_F32) {
-    Eight<float> e;
-    e.load(static_cast<const float*>(p.weight), col, p.n, p.vec_weight);
-    e.get(w);
-  } else if (p.weight_dtype == QI8_BF16) {
-    Eight<__nv_bfloat16> e;
-    e.load(static_cast<const __nv_bfloat16*>(p.weight), col, p.n, p.vec_weight);
-    e.get(w);
-  } else {
-    Eight<__half> e;
-    e.load(static_cast<const __half*>(p.weight), col, p.n, p.vec_weight);
-    e.get(w);
-  }
+template <typename W>
+__device__ __forceinline__ F8x weight_as(const Args& p, int64_t col) {
+  Eight<W> e;
+  const W* w = static_cast<const W*>(p.weight);
+  if (p.vec_weight && col + 8 <= p.n) e.load(w + col);
+  else e.load_some(w, col, p.n);
+  return e.get();
+}
+__device__ __forceinline__ F8x load_weight(const Args& p, int64_t col) {
+  if (p.weight_dtype == QI8_BF16) return weight_as<__nv_bfloat16>(p, col);
+  return p.weight_dtype == QI8_F16 ? weight_as<__half>(p, col) : weight_as<float>(p, col);
 }
 
-// Eight columns' worth of y before the norm's factor (norm: h), zero past the end.
-template <typename T, bool NORM>
-__device__ __forceinline__ void row_values(const Args& p, int64_t row, int64_t col, float (&y)[8]) {
-  Eight<T> e, f;
-  e.load(static_cast<const T*>(p.x) + row * p.ld_x, col, p.n, p.vec);
-  if (p.second) f.load(static_cast<const T*>(p.second) + row * p.ld_second, col, p.n, p.vec);
-  e.get(y);
-  if (p.second) {
-    float b[8];
-    f.get(b);
-    if constexpr (NORM) {
+// What is done to the two inputs of a column before any step over the row.
+enum { PLAIN, NORM, GATED_SILU, GATED_GELU, GATED_TANH };
+
+template <typename T, int OP>
+__device__ __forceinline__ F8x combine(const Args& p, const Eight<T>& a, const Eight<T>& b) {
+  F8x y = a.get();
+  if constexpr (OP == NORM) {
+    if (p.second) {
+      const F8x r = b.get();
 #pragma unroll
-      for (int i = 0; i < 8; ++i) y[i] = Elem<T>::to_f32(Elem<T>::from_f32(y[i] + b[i]));
-    } else {
-      gate(y, b, p.act);
+      for (int i = 0; i < 4; ++i) y.v[i] = __fadd2_rn(y.v[i], r.v[i]);
+      if constexpr (sizeof(T) == 2) {
+        Eight<T> e;
+        e.set(y);
+        y = e.get();
+      }
+    }
+  } else if constexpr (OP != PLAIN) {
+    y = gate<OP == GATED_SILU ? QI8_ACT_SILU : OP == GATED_GELU ? QI8_ACT_GELU : QI8_ACT_GELU_TANH>(y, b.get());
+  }
+  return y;
+}
+
+// `N` pieces of a row, `step` columns apart, zero past the end: all loads are
+// issued before the first is used.
+template <typename T, int OP, int N>
+__device__ __forceinline__ void row_values(const Args& p, int64_t row, int64_t col, int step, F8x (&y)[N]) {
+  const T* a = static_cast<const T*>(p.x) + row * p.ld_x;
+  const T* b = static_cast<const T*>(p.second) + row * p.ld_second;
+  const bool two = OP != PLAIN && p.second;
+  Eight<T> u[N], v[N];
+  if (p.vec && col + (N - 1) * step + 8 <= p.n) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) u[i].load(a + col + i * step);
+    if (two)
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i].load(b + col + i * step);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      u[i].load_some(a, col + i * step, p.n);
+      if (two) v[i].load_some(b, col + i * step, p.n);
     }
   }
+#pragma unroll
+  for (int i = 0; i < N; ++i) y[i] = combine<T, OP>(p, u[i], v[i]);
 }
 
 template <typename T>
-__device__ __forceinline__ void store_sum(const Args& p, int64_t row, int64_t col, const float (&h)[8]) {
+__device__ __forceinline__ void store_sum(const Args& p, int64_t row, int64_t col, const F8x& h) {
   Eight<T> e;
   e.set(h);
   e.store(static_cast<T*>(p.sum) + row * p.ld_sum, col, p.n, p.vec_sum);
+}
+
+__device__ __forceinline__ float squares(const F8x& h, float ss, float by) {
+  float2 s = make_float2(ss, 0.0f);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __fmul2_rn(h.v[i], both(by));
+    s = __ffma2_rn(t, t, s);
+  }
+  return s.x + s.y;
+}
+__device__ __forceinline__ F8x normed(const Args& p, F8x h, float rstd, const F8x& w) {
+  h = scaled(h, rstd);
+  if (p.weight)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h.v[i] = __fmul2_rn(h.v[i], w.v[i]);
+  return h;
 }
 
 // Sums (or maxima) over the `warps` warps of a row.  Each call takes shared words
@@ -129,56 +187,51 @@ __device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return max(a
 // theirs: the largest becomes 2^48.
 constexpr float SMALLER = 8.271806125530277e-25f;  // 2^-80
 
-__device__ __forceinline__ float root(float ss, bool smaller, const Args& p) {
-  const double sum = smaller ? (double)ss * 0x1p160 : (double)ss;
-  return (float)(1.0 / sqrt(sum / (double)p.n + p.eps));
+__device__ __forceinline__ float root(const Args& p, float ss, bool smaller) {
+  if (smaller) return __frsqrt_rn(__fdiv_rn(ss, (float)p.n)) * SMALLER;  // eps would vanish beside it
+  return __frsqrt_rn(__fdiv_rn(ss, (float)p.n) + p.eps);
 }
 
 // Whole rows in registers: `warps` warps hold one, eight columns per lane and
 // chunk, and a thread block holds as many rows as fit.
-template <typename T, bool NORM, int CHUNKS>
-__global__ void __launch_bounds__(1024) row_kernel(const __grid_constant__ Args p, const int warps) {
+constexpr int ROW_THREADS = 512;
+
+template <typename T, int OP, int CHUNKS>
+__global__ void __launch_bounds__(ROW_THREADS) row_kernel(const __grid_constant__ Args p, const int warps) {
   __shared__ float sums[2][32];
   __shared__ uint32_t tops[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int mine = warp / warps, first_warp = mine * warps, threads = warps * 32;
+  const int mine = warp / warps, first_warp = mine * warps, step = warps * 256;
   const int t = threadIdx.x - first_warp * 32;
-  const int64_t per = (blockDim.x >> 5) / warps;
+  const int64_t col0 = t * 8, per = (blockDim.x >> 5) / warps;
   int64_t row = blockIdx.x * per + mine;
   const bool live = row < p.rows;
   if (!live) row = p.rows - 1;  // takes part in the barriers
-  float y[CHUNKS][8], w[8];
+  F8x y[CHUNKS];
+  row_values<T, OP>(p, row, col0, step, y);
+  if constexpr (OP == NORM) {
+    F8x w[CHUNKS];  // loads that wait behind the reduction's barrier
+    if (p.weight)
 #pragma unroll
-  for (int c = 0; c < CHUNKS; ++c) row_values<T, NORM>(p, row, (int64_t)(c * threads + t) * 8, y[c]);
-  // the weight's latency behind the reduction's, where registers allow
-  if (NORM && CHUNKS == 1 && p.weight) load_weight(p, (int64_t)t * 8, w);
-  if constexpr (NORM) {
+      for (int c = 0; c < CHUNKS; ++c) w[c] = load_weight(p, col0 + c * step);
     float ss = 0.0f;
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(y[c][j], y[c][j], ss);
+    for (int c = 0; c < CHUNKS; ++c) ss = squares(y[c], ss, 1.0f);
     if (p.sum && live)
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c) store_sum<T>(p, row, (int64_t)(c * threads + t) * 8, y[c]);
+      for (int c = 0; c < CHUNKS; ++c) store_sum<T>(p, row, col0 + c * step, y[c]);
     ss = over_row(ss, sums[0], first_warp, warps, add_f);
-    bool smaller = isinf(ss);
+    const bool smaller = isinf(ss);
     if (__syncthreads_or(smaller)) {
       float s2 = 0.0f;
 #pragma unroll
-      for (int c = 0; c < CHUNKS; ++c)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) s2 = fmaf(y[c][j] * SMALLER, y[c][j] * SMALLER, s2);
+      for (int c = 0; c < CHUNKS; ++c) s2 = squares(y[c], s2, SMALLER);
       s2 = over_row(s2, sums[1], first_warp, warps, add_f);
       if (smaller) ss = s2;
     }
-    const float rstd = root(ss, smaller, p);
+    const float rstd = root(p, ss, smaller);
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) {
-      if (CHUNKS > 1 && p.weight) load_weight(p, (int64_t)(c * threads + t) * 8, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[c][j] = p.weight ? y[c][j] * rstd * w[j] : y[c][j] * rstd;
-    }
+    for (int c = 0; c < CHUNKS; ++c) y[c] = normed(p, y[c], rstd, w[c]);
   }
   uint32_t m = 0;
   if (p.mode == QI8_Q_TOKEN) {
@@ -188,7 +241,7 @@ __global__ void __launch_bounds__(1024) row_kernel(const __grid_constant__ Args 
   }
 #pragma unroll
   for (int c = 0; c < CHUNKS; ++c) {
-    const int64_t col = (int64_t)(c * threads + t) * 8;
+    const int64_t col = col0 + c * step;
     const uint32_t top = p.mode == QI8_Q_TOKEN ? m : max16(amax_bits(y[c]));
     if (!live || col >= p.n) continue;
     if (p.mode == QI8_Q_TOKEN) emit(p, y[c], top, row, col, c == 0 && t == 0, row);
@@ -199,80 +252,72 @@ __global__ void __launch_bounds__(1024) row_kernel(const __grid_constant__ Args 
 // Rows too long for that are read again for each step (from L2, mostly).
 constexpr int LONG_THREADS = 1024;
 
-template <typename T, bool NORM>
+template <typename T, int OP>
 __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_constant__ Args p) {
   __shared__ float sums[2][32];
   __shared__ uint32_t tops[32];
-  const int64_t row = blockIdx.x, end = (p.n + 127) / 128 * 128;  // whole half warps
-  const int64_t col0 = threadIdx.x * 8, step = LONG_THREADS * 8;
+  constexpr int STEP = LONG_THREADS * 8;
+  const int64_t row = blockIdx.x, col0 = threadIdx.x * 8;
   float rstd = 1.0f;
-  if constexpr (NORM) {
-    bool smaller = false;
+  F8x y[1];
+  if constexpr (OP == NORM) {
     float ss = 0.0f;
-    for (int64_t col = col0; col < end; col += step) {
-      float y[8];
-      row_values<T, NORM>(p, row, col, y);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) ss = fmaf(y[j], y[j], ss);
-      if (p.sum && col < p.n) store_sum<T>(p, row, col, y);
+    for (int64_t col = col0; col < p.n; col += STEP) {
+      row_values<T, OP>(p, row, col, STEP, y);
+      ss = squares(y[0], ss, 1.0f);
+      if (p.sum) store_sum<T>(p, row, col, y[0]);
     }
     ss = over_row(ss, sums[0], 0, LONG_THREADS / 32, add_f);
-    if (isinf(ss)) {
-      smaller = true;
+    const bool smaller = isinf(ss);  // the same for all threads
+    if (smaller) {
       ss = 0.0f;
-      for (int64_t col = col0; col < end; col += step) {
-        float y[8];
-        row_values<T, NORM>(p, row, col, y);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) ss = fmaf(y[j] * SMALLER, y[j] * SMALLER, ss);
+      for (int64_t col = col0; col < p.n; col += STEP) {
+        row_values<T, OP>(p, row, col, STEP, y);
+        ss = squares(y[0], ss, SMALLER);
       }
       ss = over_row(ss, sums[1], 0, LONG_THREADS / 32, add_f);
     }
-    rstd = root(ss, smaller, p);
+    rstd = root(p, ss, smaller);
   }
-  auto final_values = [&](int64_t col, float (&y)[8]) {
-    row_values<T, NORM>(p, row, col, y);
-    if constexpr (NORM) {
-      float w[8];
-      if (p.weight) load_weight(p, col, w);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) y[j] = p.weight ? y[j] * rstd * w[j] : y[j] * rstd;
+  auto final_values = [&](int64_t col) {
+    row_values<T, OP>(p, row, col, STEP, y);
+    if constexpr (OP == NORM) {
+      F8x w;
+      if (p.weight) w = load_weight(p, col);
+      y[0] = normed(p, y[0], rstd, w);
     }
   };
   uint32_t m = 0;
   if (p.mode == QI8_Q_TOKEN) {
-    for (int64_t col = col0; col < end; col += step) {
-      float y[8];
-      final_values(col, y);
-      m = max(m, amax_bits(y));
+    for (int64_t col = col0; col < p.n; col += STEP) {
+      final_values(col);
+      m = max(m, amax_bits(y[0]));
     }
     m = over_row(m, tops, 0, LONG_THREADS / 32, max_u);
   }
-  for (int64_t first = 0; first < end; first += step) {  // the warp's lanes together
+  for (int64_t first = 0; first < p.n; first += STEP) {  // the warp's lanes together
     const int64_t col = first + col0;
-    float y[8] = {0, 0, 0, 0, 0, 0, 0, 0};
-    if (col < p.n) final_values(col, y);
-    const uint32_t top = p.mode == QI8_Q_TOKEN ? m : max16(amax_bits(y));
+    if (col < p.n) final_values(col);
+    const uint32_t top = p.mode == QI8_Q_TOKEN ? m : max16(col < p.n ? amax_bits(y[0]) : 0);
     if (col >= p.n) continue;
-    if (p.mode == QI8_Q_TOKEN) emit(p, y, top, row, col, col == 0, row);
-    else emit(p, y, top, row, col, (threadIdx.x & 15) == 0, row * p.blocks + col / F8_BLOCK);
+    if (p.mode == QI8_Q_TOKEN) emit(p, y[0], top, row, col, col == 0, row);
+    else emit(p, y[0], top, row, col, (threadIdx.x & 15) == 0, row * p.blocks + col / F8_BLOCK);
   }
 }
 
 // No step over whole rows: 16 lanes per block of 128 columns.  A warp takes 2 *
-// STEPS neighbouring blocks of one row, all loads before the first use.
+// STEPS neighbouring blocks of one row.
 constexpr int THREADS = 256;
 
-template <typename T, int STEPS>
+template <typename T, int OP, int STEPS>
 __global__ void __launch_bounds__(THREADS) block_kernel(const __grid_constant__ Args p, const unsigned groups) {
   const int lane = threadIdx.x & 31;
-  const int64_t unit = (int64_t)blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
-  const int64_t row = unit / groups;
+  const unsigned unit = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
+  const unsigned row = unit / groups;
   if (row >= p.rows) return;
-  const int64_t col0 = (unit - row * groups) * (STEPS * 256) + lane * 8;
-  float y[STEPS][8];
-#pragma unroll
-  for (int i = 0; i < STEPS; ++i) row_values<T, false>(p, row, col0 + i * 256, y[i]);
+  const int64_t col0 = (int64_t)(unit - row * groups) * (STEPS * 256) + lane * 8;
+  F8x y[STEPS];
+  row_values<T, OP>(p, row, col0, 256, y);
 #pragma unroll
   for (int i = 0; i < STEPS; ++i) {
     const int64_t col = col0 + i * 256;
@@ -281,45 +326,50 @@ __global__ void __launch_bounds__(THREADS) block_kernel(const __grid_constant__ 
   }
 }
 
-template <typename T, int STEPS>
+template <typename T, int OP, int STEPS>
 int launch_blocks(const Args& p, cudaStream_t st) {
-  const int64_t groups = (p.blocks + 2 * STEPS - 1) / (2 * STEPS);
-  const int64_t grid = (p.rows * groups + THREADS / 32 - 1) / (THREADS / 32);
-  QI8_REQUIRE(grid < (1ll << 31), QI8_ESHAPE, "%lld rows of %lld", (long long)p.rows, (long long)p.n);
-  block_kernel<T, STEPS><<<(unsigned)grid, THREADS, 0, st>>>(p, (unsigned)groups);
+  const int64_t groups = (p.blocks + 2 * STEPS - 1) / (2 * STEPS), units = p.rows * groups;
+  QI8_REQUIRE(units < (1ll << 32) - THREADS, QI8_ESHAPE, "%lld rows of %lld", (long long)p.rows, (long long)p.n);
+  block_kernel<T, OP, STEPS><<<(unsigned)((units + THREADS / 32 - 1) / (THREADS / 32)), THREADS, 0, st>>>(
+      p, (unsigned)groups);
   return check_cuda(cudaGetLastError(), "block_kernel launch");
 }
 
-template <typename T, bool NORM, int CHUNKS>
+template <typename T, int OP, int CHUNKS>
 int launch_rows(const Args& p, cudaStream_t st) {
   const int warps = (int)((p.n + 256 * CHUNKS - 1) / (256 * CHUNKS));
   const int per = warps >= 8 ? 1 : 8 / warps;  // rows per thread block
-  row_kernel<T, NORM, CHUNKS><<<(unsigned)((p.rows + per - 1) / per), warps * per * 32, 0, st>>>(p, warps);
+  row_kernel<T, OP, CHUNKS><<<(unsigned)((p.rows + per - 1) / per), warps * per * 32, 0, st>>>(p, warps);
   return check_cuda(cudaGetLastError(), "row_kernel launch");
 }
 
-template <typename T, bool NORM>
+template <typename T, int OP>
 int launch_type(const Args& p, cudaStream_t st) {
-  if constexpr (!NORM) {
+  if constexpr (OP != NORM) {
     // few units: one step each spreads them over more SMs
     if (p.mode != QI8_Q_TOKEN)
-      return p.blocks < 8 || p.rows * p.blocks < 8 * 8 * 148 ? launch_blocks<T, 1>(p, st) : launch_blocks<T, 4>(p, st);
+      return p.blocks < 4 || p.rows * p.blocks < 4 * 8 * 148 * 4 ? launch_blocks<T, OP, 1>(p, st)
+                                                                 : launch_blocks<T, OP, 2>(p, st);
   }
-  if (p.n <= 8192) return launch_rows<T, NORM, 1>(p, st);
-  if (p.n <= 16384) return launch_rows<T, NORM, 2>(p, st);
-  if (p.n <= 32768) return launch_rows<T, NORM, 4>(p, st);
-  long_row_kernel<T, NORM><<<(unsigned)p.rows, LONG_THREADS, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), "long_row_kernel launch");
+  if constexpr (OP != PLAIN) {
+    if (p.n <= 1024) return launch_rows<T, OP, 1>(p, st);
+    if (p.n <= 8192) return launch_rows<T, OP, 2>(p, st);
+    if (p.n <= 16384) return launch_rows<T, OP, 4>(p, st);
+    long_row_kernel<T, OP><<<(unsigned)p.rows, LONG_THREADS, 0, st>>>(p);
+    return check_cuda(cudaGetLastError(), "long_row_kernel launch");
+  }
+  return QI8_OK;
 }
 
-template <bool NORM>
+template <int OP>
 int launch(const Args& p, int dtype, cudaStream_t st) {
   if (p.rows == 0 || p.n == 0) return QI8_OK;
-  QI8_REQUIRE(p.rows < (1ll << 31), QI8_ESHAPE, "%lld rows", (long long)p.rows);
+  QI8_REQUIRE(p.rows < (1ll << 31) && p.n < (1ll << 31), QI8_ESHAPE, "%lld rows of %lld", (long long)p.rows,
+              (long long)p.n);
   switch (dtype) {
-    case QI8_BF16: return launch_type<__nv_bfloat16, NORM>(p, st);
-    case QI8_F16: return launch_type<__half, NORM>(p, st);
-    default: return launch_type<float, NORM>(p, st);
+    case QI8_BF16: return launch_type<__nv_bfloat16, OP>(p, st);
+    case QI8_F16: return launch_type<__half, OP>(p, st);
+    default: return launch_type<float, OP>(p, st);
   }
 }
 
@@ -344,7 +394,7 @@ int quant_rows_f8(const void* x, int x_dtype, int64_t rows, int64_t n, int64_t l
   p.mode = QI8_Q_FP8;
   p.vec = rows_aligned(x, ld_x, elem_size(x_dtype), 16);
   p.vec_q = rows_aligned(q, ld_q, 1, 8);
-  return launch<false>(p, x_dtype, st);
+  return launch<PLAIN>(p, x_dtype, st);
 }
 
 }  // namespace qi8
@@ -382,7 +432,7 @@ extern "C" int qi8_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int6
   QI8_REQUIRE(ld_x >= n && (!residual || ld_residual >= n) && (!sum_out || ld_sum >= n), QI8_ESHAPE,
               "row strides %lld, %lld and %lld for rows of %lld", (long long)ld_x, (long long)ld_residual,
               (long long)ld_sum, (long long)n);
-  QI8_REQUIRE(eps >= 0.0 && eps < 1e300, QI8_EINVAL, "eps %g", eps);
+  QI8_REQUIRE(eps >= 0.0 && eps < 1e30, QI8_EINVAL, "eps %g", eps);
   QI8_REQUIRE(!weight || aq::is_float(weight_dtype), QI8_EDTYPE, "weight dtype %d: bf16, f16 or f32", weight_dtype);
   if (rows == 0 || n == 0) return QI8_OK;
   QI8_REQUIRE(x && q_out && scale_out, QI8_EINVAL, "null pointer");
@@ -402,13 +452,13 @@ extern "C" int qi8_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int6
   p.rows = rows;
   p.n = n;
   p.blocks = f8_blocks(n);
-  p.eps = eps;
+  p.eps = (float)eps;
   p.mode = mode;
   p.vec = rows_aligned(x, ld_x, size, 16) && (!residual || rows_aligned(residual, ld_residual, size, 16));
   p.vec_weight = aligned16(weight);
   p.vec_q = rows_aligned(q_out, ld_q, 1, 8);
   p.vec_sum = sum_out && rows_aligned(sum_out, ld_sum, size, 16);
-  return aq::launch<true>(p, x_dtype, static_cast<cudaStream_t>(stream));
+  return aq::launch<aq::NORM>(p, x_dtype, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" int qi8_gated_quant(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, int dtype, int64_t rows,
@@ -431,9 +481,10 @@ extern "C" int qi8_gated_quant(const void* gate, int64_t ld_gate, const void* up
   p.rows = rows;
   p.n = n;
   p.blocks = f8_blocks(n);
-  p.act = act;
   p.mode = mode;
   p.vec = rows_aligned(gate, ld_gate, size, 16) && rows_aligned(up, ld_up, size, 16);
   p.vec_q = rows_aligned(q_out, ld_q, 1, 8);
-  return aq::launch<false>(p, dtype, static_cast<cudaStream_t>(stream));
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return act == QI8_ACT_SILU ? aq::launch<aq::GATED_SILU>(p, dtype, st)
+         : act == QI8_ACT_GELU ? aq::launch<aq::GATED_GELU>(p, dtype, st) : aq::launch<aq::GATED_TANH>(p, dtype, st);
 }

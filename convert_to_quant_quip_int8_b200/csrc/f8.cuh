@@ -12,6 +12,8 @@
 
 #include <cuda_fp8.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 
 namespace qi8 {
@@ -61,22 +63,29 @@ __device__ __forceinline__ float2 f8_unpack2(uint32_t two) {
   return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
 
-// Eight consecutive elements of a row from column `col` on, zero from n on.
-// vec: the row starts on a 16-byte boundary (col is a multiple of 8).
+// Eight consecutive elements of a row as fp32, in pairs: the packed fp32
+// instructions take two at a time.
+struct F8x {
+  float2 v[4];
+};
+
+// The same as they lie in memory.
 template <typename T>
 struct Eight {
   uint4 v[sizeof(T) / 2];
 
-  __device__ __forceinline__ void load(const T* row, int64_t col, int64_t n, bool vec) {
-    if (vec && col + 8 <= n) {
+  // A whole piece on a 16-byte boundary.
+  __device__ __forceinline__ void load(const T* at) {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(row + col) + i);
-    } else {
-      T* e = reinterpret_cast<T*>(v);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) e[i] = col + i < n ? row[col + i] : T(0.0f);
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
   }
+  // From column `col` on, zero from n on.
+  __device__ __forceinline__ void load_some(const T* row, int64_t col, int64_t n) {
+    T* e = reinterpret_cast<T*>(v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = col + i < n ? row[col + i] : T(0.0f);
+  }
+  // vec: the row starts on a 16-byte boundary (col is a multiple of 8)
   __device__ __forceinline__ void store(T* row, int64_t col, int64_t n, bool vec) const {
     if (vec && col + 8 <= n) {
 #pragma unroll
@@ -88,24 +97,37 @@ struct Eight {
         if (col + i < n) row[col + i] = e[i];
     }
   }
-  __device__ __forceinline__ void get(float (&f)[8]) const {
+  __device__ __forceinline__ F8x get() const {
+    F8x f;
     const T* e = reinterpret_cast<const T*>(v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = Elem<T>::to_f32(e[i]);
+    for (int i = 0; i < 4; ++i) f.v[i] = make_float2(Elem<T>::to_f32(e[2 * i]), Elem<T>::to_f32(e[2 * i + 1]));
+    return f;
   }
-  __device__ __forceinline__ void set(const float (&f)[8]) {
+  __device__ __forceinline__ void set(const F8x& f) {
     T* e = reinterpret_cast<T*>(v);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i] = Elem<T>::from_f32(f[i]);
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (sizeof(T) == 4) {
+        e[2 * i] = f.v[i].x;
+        e[2 * i + 1] = f.v[i].y;
+      } else if constexpr (std::is_same<T, __half>::value) {
+        reinterpret_cast<__half2*>(e)[i] = __float22half2_rn(f.v[i]);
+      } else {
+        reinterpret_cast<__nv_bfloat162*>(e)[i] = __float22bfloat162_rn(f.v[i]);
+      }
+    }
   }
 };
 
-// |values| as fp32 bits: whole-number comparisons keep infinities and NaN on top.
-__device__ __forceinline__ uint32_t amax_bits(const float (&f)[8]) {
-  uint32_t m = 0;
+// The largest |value| as fp32 bits; NaN is above infinity.  One instruction for
+// two values.
+__device__ __forceinline__ uint32_t amax_bits(const F8x& f) {
+  float m = 0.0f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, __float_as_uint(f[i]) & 0x7fffffffu);
-  return m;
+  for (int i = 0; i < 4; ++i)
+    asm("max.NaN.abs.f32 %0, %0, %1, %2;" : "+f"(m) : "f"(f.v[i].x), "f"(f.v[i].y));
+  return __float_as_uint(m);
 }
 // The largest over 16 neighbouring lanes: one block of 128 columns, eight per lane.
 __device__ __forceinline__ uint32_t max16(uint32_t m) {
@@ -114,9 +136,15 @@ __device__ __forceinline__ uint32_t max16(uint32_t m) {
   return m;
 }
 
-__device__ __forceinline__ uint2 f8_codes(const float (&f)[8], float inv) {
-  return make_uint2(f8_pack4(f[0] * inv, f[1] * inv, f[2] * inv, f[3] * inv),
-                    f8_pack4(f[4] * inv, f[5] * inv, f[6] * inv, f[7] * inv));
+__device__ __forceinline__ F8x scaled(const F8x& f, float by) {
+  F8x r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) r.v[i] = __fmul2_rn(f.v[i], make_float2(by, by));
+  return r;
+}
+__device__ __forceinline__ uint2 f8_codes(const F8x& f, float inv) {
+  const F8x s = scaled(f, inv);
+  return make_uint2(f8_pack4(s.v[0].x, s.v[0].y, s.v[1].x, s.v[1].y), f8_pack4(s.v[2].x, s.v[2].y, s.v[3].x, s.v[3].y));
 }
 // int8 scale of a block: amax / 127, at least `least` (an infinity or a NaN stays).
 __device__ __forceinline__ float i8_scale(uint32_t amax, float least) {
@@ -124,10 +152,13 @@ __device__ __forceinline__ float i8_scale(uint32_t amax, float least) {
   return s < least ? least : s;
 }
 // rint(f * inv), |f * inv| < 127.5 or NaN (code 0)
-__device__ __forceinline__ uint2 i8_codes(const float (&f)[8], float inv) {
+__device__ __forceinline__ uint2 i8_codes(const F8x& f, float inv) {
   uint32_t w[2] = {0, 0};
 #pragma unroll
-  for (int i = 0; i < 8; ++i) w[i >> 2] |= (uint32_t)(__float2int_rn(f[i] * inv) & 0xff) << (8 * (i & 3));
+  for (int i = 0; i < 4; ++i) {
+    const uint32_t a = __float2int_rn(f.v[i].x * inv) & 0xff, b = __float2int_rn(f.v[i].y * inv) & 0xff;
+    w[i >> 1] |= (a | (b << 8)) << (16 * (i & 1));
+  }
   return make_uint2(w[0], w[1]);
 }
 // Eight codes of a row.  vec: rows start on 8-byte boundaries.

@@ -13,46 +13,50 @@ int quant_rows_f8(const void* x, int x_dtype, int64_t rows, int64_t n, int64_t l
 namespace {
 namespace f8g {
 
-using Args = F8Gemm;
-
-// 32 x 32 outputs per thread block, 32 columns of K at a time.
-__global__ void __launch_bounds__(256) tile_kernel(const Args p) {
-  __shared__ float sa[32][33], sb[32][33];
-  const int n0 = blockIdx.x * 32, m0 = blockIdx.y * 32;
-  const int c = threadIdx.x & 31, r = threadIdx.x >> 5;
-  float acc[4] = {0, 0, 0, 0};
-  for (int k0 = 0; k0 < p.K; k0 += 32) {
-    for (int i = r; i < 32; i += 8) {
-      const int m = m0 + i, n = n0 + i, k = k0 + c;
-      sa[i][c] = m < p.M && k < p.K
-                     ? f8_unpack2(p.a[m * p.ld_a + k]).x * f8_scale(p.sa[(int64_t)m * p.KB + k / F8_BLOCK]) : 0.0f;
-      sb[i][c] = n < p.N && k < p.K
-                     ? f8_unpack2(p.b[n * p.ld_b + k]).x * f8_scale(p.sb[(int64_t)(n / F8_BLOCK) * p.KB + k / F8_BLOCK])
-                     : 0.0f;
-    }
-    __syncthreads();
-    for (int k = 0; k < 32; ++k)
+// Codes whose rows do not start on 16-byte boundaries -> such rows, zeros behind
+// the end.  16 bytes per thread.
+__global__ void __launch_bounds__(256)
+repitch_kernel(const uint8_t* __restrict__ src, int64_t rows, int64_t K, int64_t ld, uint4* __restrict__ dst) {
+  const int64_t per = (K + 15) / 16;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
+    const int64_t row = i / per, col = (i - row * per) * 16;
+    uint32_t w[4] = {0, 0, 0, 0};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[i] = fmaf(sa[r + 8 * i][k], sb[c][k], acc[i]);
-    __syncthreads();
+    for (int j = 0; j < 16; ++j)
+      if (col + j < K) w[j >> 2] |= (uint32_t)src[row * ld + col + j] << (8 * (j & 3));
+    dst[i] = make_uint4(w[0], w[1], w[2], w[3]);
   }
-  if (n0 + c >= p.N) return;
-  const float bias = p.bias ? load_as_f32(p.bias, p.bias_dtype, n0 + c) : 0.0f;
-  for (int i = 0; i < 4; ++i)
-    if (m0 + r + 8 * i < p.M)
-      store_from_f32(p.out, p.out_dtype, (int64_t)(m0 + r + 8 * i) * p.ld_out + n0 + c, acc[i] + bias);
 }
 
 bool is_float(int dtype) { return dtype == QI8_BF16 || dtype == QI8_F16 || dtype == QI8_F32; }
 
-int gemm(const Args& p, cudaStream_t st) {
-  if (rows_aligned(p.a, p.ld_a, 1, 16) && rows_aligned(p.b, p.ld_b, 1, 16)) return gemm_f8_tiles(p, st);
-  const dim3 grid((unsigned)((p.N + 31) / 32), (unsigned)((p.M + 31) / 32));
-  tile_kernel<<<grid, 256, 0, st>>>(p);
-  return check_cuda(cudaGetLastError(), "tile_kernel launch");
+int64_t pitch(int64_t k) { return (k + 15) / 16 * 16; }
+
+// Workspace of one operand: nothing where its rows are aligned already.
+int64_t copy_bytes(const uint8_t* q, int64_t rows, int64_t K, int64_t ld) {
+  return rows_aligned(q, ld, 1, 16) ? 0 : rows * pitch(K);
 }
 
-int64_t pitch(int64_t k) { return (k + 15) / 16 * 16; }
+// Brings an operand into the workspace where it has to be.
+int align_rows(const uint8_t*& q, int64_t rows, int64_t K, int64_t& ld, uint8_t*& workspace, cudaStream_t st) {
+  const int64_t bytes = copy_bytes(q, rows, K, ld);
+  if (bytes == 0) return QI8_OK;
+  const int64_t blocks = (bytes / 16 + 255) / 256, most = (int64_t)sm_count() * 32;
+  repitch_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(q, rows, K, ld,
+                                                                             reinterpret_cast<uint4*>(workspace));
+  if (int rc = check_cuda(cudaGetLastError(), "repitch_kernel launch")) return rc;
+  q = workspace;
+  ld = pitch(K);
+  workspace += bytes;
+  return QI8_OK;
+}
+
+int check_workspace(const void* workspace, int64_t have, int64_t need) {
+  QI8_REQUIRE(need == 0 || (workspace && have >= need), QI8_ESHAPE, "workspace of %lld bytes: %lld are needed",
+              (long long)have, (long long)need);
+  QI8_REQUIRE(need == 0 || aligned16(workspace), QI8_EALIGN, "workspace must be 16-byte aligned");
+  return QI8_OK;
+}
 
 int check(int64_t M, int64_t K, int64_t N, int64_t ld_b, int64_t ld_out, int out_dtype, const void* bias,
           int bias_dtype) {
@@ -74,7 +78,8 @@ using namespace qi8;
 
 extern "C" int64_t qi8_gemm_f8_workspace_bytes(const uint8_t* a, int64_t M, int64_t K, int64_t ld_a, const uint8_t* b,
                                                int64_t N, int64_t ld_b) {
-  return 0;
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return f8g::copy_bytes(a, M, K, ld_a) + f8g::copy_bytes(b, N, K, ld_b);
 }
 
 extern "C" int qi8_gemm_f8(const uint8_t* a, const uint8_t* a_scale, int64_t M, int64_t K, int64_t ld_a,
@@ -85,13 +90,19 @@ extern "C" int qi8_gemm_f8(const uint8_t* a, const uint8_t* a_scale, int64_t M, 
   QI8_REQUIRE(ld_a >= K, QI8_ESHAPE, "row stride %lld for %lld columns", (long long)ld_a, (long long)K);
   if (M == 0 || N == 0) return QI8_OK;
   QI8_REQUIRE(a && a_scale && b && b_scale && out, QI8_EINVAL, "null pointer");
-  const F8Gemm p{a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
-                    bias_dtype, out_dtype};
-  return f8g::gemm(p, static_cast<cudaStream_t>(stream));
+  if (int rc = f8g::check_workspace(workspace, workspace_bytes, qi8_gemm_f8_workspace_bytes(a, M, K, ld_a, b, N, ld_b)))
+    return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  if (int rc = f8g::align_rows(a, M, K, ld_a, ws, st)) return rc;
+  if (int rc = f8g::align_rows(b, N, K, ld_b, ws, st)) return rc;
+  return gemm_f8_tiles({a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K,
+                        (int)f8_blocks(K), bias_dtype, out_dtype}, st);
 }
 
 extern "C" int64_t qi8_linear_f8_workspace_bytes(int64_t M, int64_t K, const uint8_t* b, int64_t N, int64_t ld_b) {
-  return M * (f8g::pitch(K) + f8_blocks(K));
+  if (M <= 0 || N <= 0 || K <= 0) return 0;
+  return M * f8g::pitch(K) + f8g::pitch(M * f8_blocks(K)) + f8g::copy_bytes(b, N, K, ld_b);
 }
 
 extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, int64_t ld_x, const uint8_t* b,
@@ -101,14 +112,15 @@ extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, i
   QI8_REQUIRE(f8g::is_float(x_dtype), QI8_EDTYPE, "input dtype %d: bf16, f16 or f32", x_dtype);
   QI8_REQUIRE(ld_x >= K, QI8_ESHAPE, "row stride %lld for %lld columns", (long long)ld_x, (long long)K);
   if (M == 0 || N == 0) return QI8_OK;
-  QI8_REQUIRE(x && b && b_scale && out && workspace, QI8_EINVAL, "null pointer");
-  QI8_REQUIRE(workspace_bytes >= qi8_linear_f8_workspace_bytes(M, K, b, N, ld_b), QI8_ESHAPE, "workspace of %lld bytes",
-              (long long)workspace_bytes);
+  QI8_REQUIRE(x && b && b_scale && out, QI8_EINVAL, "null pointer");
+  if (int rc = f8g::check_workspace(workspace, workspace_bytes, qi8_linear_f8_workspace_bytes(M, K, b, N, ld_b)))
+    return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* q = static_cast<uint8_t*>(workspace);
   uint8_t* s = q + M * f8g::pitch(K);
+  uint8_t* ws = s + f8g::pitch(M * f8_blocks(K));
+  if (int rc = f8g::align_rows(b, N, K, ld_b, ws, st)) return rc;
   if (int rc = quant_rows_f8(x, x_dtype, M, K, ld_x, q, f8g::pitch(K), s, st)) return rc;
-  const F8Gemm p{q, b, s, b_scale, bias, out, f8g::pitch(K), ld_b, ld_out, (int)M, (int)N, (int)K,
-                    (int)f8_blocks(K), bias_dtype, out_dtype};
-  return f8g::gemm(p, st);
+  return gemm_f8_tiles({q, b, s, b_scale, bias, out, f8g::pitch(K), ld_b, ld_out, (int)M, (int)N, (int)K,
+                        (int)f8_blocks(K), bias_dtype, out_dtype}, st);
 }

@@ -21,17 +21,17 @@ weight_kernel(const T* __restrict__ w, int64_t N, int64_t K, int64_t ld_w, bool 
   const int64_t col = (int64_t)blockIdx.x * F8_BLOCK + (threadIdx.x & 15) * 8;
   const int64_t row = (int64_t)blockIdx.y * F8_BLOCK + (threadIdx.x >> 4);
   Eight<T> e[8];
+  const bool whole = vec && (int64_t)(blockIdx.x + 1) * F8_BLOCK <= K && (int64_t)(blockIdx.y + 1) * F8_BLOCK <= N;
+  if (whole) {  // all loads before the first use
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (row + 16 * i < N) e[i].load(w + (row + 16 * i) * ld_w, col, K, vec);
+    for (int i = 0; i < 8; ++i) e[i].load(w + (row + 16 * i) * ld_w + col);
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i].load_some(w + (row + 16 * i) * ld_w, col, row + 16 * i < N ? K : 0);
+  }
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (row + 16 * i < N) {
-      float f[8];
-      e[i].get(f);
-      m = max(m, amax_bits(f));
-    }
+  for (int i = 0; i < 8; ++i) m = max(m, amax_bits(e[i].get()));
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
   __syncthreads();
@@ -41,11 +41,7 @@ weight_kernel(const T* __restrict__ w, int64_t N, int64_t K, int64_t ld_w, bool 
   const float inv = f8_inverse(code);
 #pragma unroll
   for (int i = 0; i < 8; ++i)
-    if (row + 16 * i < N) {
-      float f[8];
-      e[i].get(f);
-      store_codes(q + (row + 16 * i) * ld_q, col, K, f8_codes(f, inv), vec_q);
-    }
+    if (row + 16 * i < N) store_codes(q + (row + 16 * i) * ld_q, col, K, f8_codes(e[i].get(), inv), vec_q);
   if (threadIdx.x == 0) scale[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = (uint8_t)code;
 }
 
@@ -69,15 +65,11 @@ dequant_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t n, int64_t l
         if (col + j < n) w[j >> 2] |= (uint32_t)src[col + j] << (8 * (j & 3));
     }
     const float s = f8_scale(scale[(row >> tile_shift) * blocks + col / F8_BLOCK]);
-    float f[8];
+    F8x f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float2 v = f8_unpack2((w[j >> 1] >> (16 * (j & 1))) & 0xffffu);
-      f[2 * j] = v.x * s;
-      f[2 * j + 1] = v.y * s;
-    }
+    for (int j = 0; j < 4; ++j) f.v[j] = f8_unpack2((w[j >> 1] >> (16 * (j & 1))) & 0xffffu);
     Eight<T> e;
-    e.set(f);
+    e.set(scaled(f, s));
     e.store(out + row * ld_out, col, n, vec);
   }
 }
