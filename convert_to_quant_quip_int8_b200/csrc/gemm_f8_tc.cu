@@ -8,6 +8,8 @@
 // memory, so the four steps of a 128-block read the same byte.  The sums stay in
 // the accumulator over all of K.
 #include <cstdint>
+#include <cstdio>
+#include <cstdlib>
 
 #include "f8.cuh"
 #include "tc05.cuh"
@@ -86,18 +88,22 @@ __device__ __forceinline__ void store32(const F8Gemm& g, int64_t m, int n, const
 //   warp 12       TMA producer
 //   warp 13       TMEM allocation; MMA issue (one thread of the even block)
 // Two accumulators of 256 columns and the scales do not fit 512 columns, so the
-// accumulators share 32: the epilogue reads those first, and the next tile's
+// accumulators share 64: the epilogue reads those first, and the next tile's
 // MMAs wait for just that.
+// The issuing warp sets the pace: an MMA takes it 72 cycles, a wait 110, a commit
+// 60 to 100 (clock64), and the tensor cores, which queue about 14 MMAs, 128 cycles
+// for each.  A stage of one K block cost it 700 cycles per block, two blocks a stage
+// keep it below the 512 of the MMAs.
 namespace pair {
 
 constexpr int EPI_WARPS = 8, SCALE_WARP0 = 8, SCALE_WARPS = 4, PRODUCER = 12, ISSUER = 13;
 constexpr int THREADS = 14 * 32;
-constexpr int STAGES = 6, OPERAND = 128 * BK, STAGE = 2 * OPERAND;
-constexpr int ACC1 = 224, SHARED_CHUNK0 = 7, SHARED_CHUNK1 = 0;  // accumulator 1's columns; the shared 32 of each
-constexpr int SCALES = 480, SLOT = 16;                           // two slots: 8 columns of b, 4 of a
-constexpr int BARS = 2 * STAGES + 4 + 4 + 2;
+constexpr int STAGES = 3, OPERAND = 128 * BK, STAGE = 4 * OPERAND;  // two K blocks of both operands
+constexpr int ACC1 = 192;                           // columns of accumulator 1; 64 are both accumulators'
+constexpr int SCALES = 448, SLOT = 16, SLOTS = 4;   // 8 columns of b, 4 of a
+constexpr int BARS = 2 * STAGES + 4 + 2 * SLOTS + 2;
 constexpr int SMEM = 1024 + STAGES * STAGE + EPI_WARPS * 32 * 4 + BARS * 8 + 16;
-static_assert(SMEM <= 232448 && SCALES + 2 * SLOT <= (int)TMEM_COLS && ACC1 + 256 <= SCALES, "memories");
+static_assert(SMEM <= 232448 && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && ACC1 + 256 <= SCALES, "memories");
 
 struct Args {
   F8Gemm g;
@@ -112,32 +118,32 @@ __device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap* map, i
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
-__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+__device__ __forceinline__ void mma(int one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                     uint32_t accum) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, q;\n\t"
       "setp.ne.b32 p, %6, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accum)
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q tcgen05.mma.cta_group::2.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accum), "r"(one)
       : "memory");
 }
 // arrives on the barrier at this offset in both blocks once all earlier MMAs are done
-__device__ __forceinline__ void commit(uint32_t bar, uint16_t mask) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
-               "h"(mask)
-               : "memory");
+__device__ __forceinline__ void commit(int one, uint32_t bar, uint16_t mask) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %2, 0;\n\t"
+      "@q tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;\n\t}" ::"r"(bar),
+      "h"(mask), "r"(one)
+      : "memory");
 }
-__device__ __forceinline__ void arrive_release(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
 gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                     const __grid_constant__ Args p) {
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* sm = smem_raw + (base - raw);
-  const uint32_t sA = base, sB = base + STAGES * OPERAND;
+  const uint32_t sA = base, sB = base + STAGES * 2 * OPERAND;
   float* sbias = reinterpret_cast<float*>(sm + STAGES * STAGE);
   uint64_t* bars = reinterpret_cast<uint64_t*>(sbias + EPI_WARPS * 32);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
@@ -147,8 +153,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   auto tfull_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + b); };
   auto tempty_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + 2 + b); };
   auto sfull_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + 4 + b); };
-  auto sempty_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + 6 + b); };
-  const uint32_t tshared_bar = smem_u32(bars + 2 * STAGES + 8), drain_bar = smem_u32(bars + 2 * STAGES + 9);
+  auto sempty_bar = [&](int b) { return smem_u32(bars + 2 * STAGES + 4 + SLOTS + b); };
+  const uint32_t tshared_bar = smem_u32(bars + BARS - 2), drain_bar = smem_u32(bars + BARS - 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cta_rank();
@@ -162,10 +168,12 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     for (int b = 0; b < 2; ++b) {  // warps of both blocks
       mbar_init(tfull_bar(b), 1);
       mbar_init(tempty_bar(b), 2 * EPI_WARPS);
+    }
+    for (int b = 0; b < SLOTS; ++b) {
       mbar_init(sfull_bar(b), 2 * SCALE_WARPS);
       mbar_init(sempty_bar(b), 1);
     }
-    mbar_init(tshared_bar, 2 * EPI_WARPS / 2);
+    mbar_init(tshared_bar, 2 * EPI_WARPS);
     mbar_init(drain_bar, 1);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -194,14 +202,17 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       bool ok = true;
       for (int tile = pair0; ok && tile < tiles; tile += pairs) {
         const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128, n0 = (tile / p.m_tiles) * 256 + (int)rank * 128;
-        for (int kb = 0; kb < KB; ++kb) {
+        for (int kb = 0; kb < KB; kb += 2) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, ST_F8_PRODUCER, WAIT_LIMIT_NS)) {
             ok = false;
             break;
           }
           if (leader) mbar_arrive_expect_tx(full_bar(s), 2 * STAGE);
-          tma_load(sA + s * OPERAND, &tmA, kb * BK, m0, full0 + 8 * s);
-          tma_load(sB + s * OPERAND, &tmB, kb * BK, n0, full0 + 8 * s);
+#pragma unroll
+          for (int i = 0; i < 2; ++i) {  // past the last K block: zeros
+            tma_load(sA + (2 * s + i) * OPERAND, &tmA, (kb + i) * BK, m0, full0 + 8 * s);
+            tma_load(sB + (2 * s + i) * OPERAND, &tmB, (kb + i) * BK, n0, full0 + 8 * s);
+          }
           issued |= 1u << s;
           issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
           if (++s == STAGES) s = 0, ph ^= 1u;
@@ -213,41 +224,51 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           if (issued & (1u << t)) drain_wait(full_bar(t), (issued_ph >> t) & 1u);
     }
   } else if (warp == ISSUER) {
-    if (leader && lane == 0) {
+    // the whole warp, so that addresses and descriptors stay in uniform registers; one lane issues
+    if (leader) {
+      const int one = lane == 0;
       int s = 0, unit = 0;
       uint32_t ph = 0;
       unsigned slot = 0;  // scale slots used so far
       bool ok = true;
       for (int tile = pair0; ok && tile < tiles; tile += pairs, ++unit) {
         const int buf = unit & 1;
-        if (!mbar_wait(tempty_bar(buf), ((unit >> 1) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
-        if (unit > 0 && !mbar_wait(tshared_bar, (unit - 1) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+        if (!warp_wait(tempty_bar(buf), ((unit >> 1) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+        if (unit > 0 && !warp_wait(tshared_bar, (unit - 1) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
         tc_fence_after();
         const uint32_t d = tmem + (buf ? ACC1 : 0);
-        for (int kb = 0; kb < KB; ++kb) {
-          const uint32_t sb = tmem + SCALES + (slot & 1) * SLOT;
-          if (((kb & 3) == 0 && !mbar_wait(sfull_bar(slot & 1), (slot >> 1) & 1, abort_flag, p.status, ST_F8_MMA,
-                                           WAIT_LIMIT_NS)) ||
-              !mbar_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
+        for (int kb = 0; ok && kb < KB; kb += 4, ++slot) {  // one slot of scales
+          const uint32_t sb = tmem + SCALES + (slot % SLOTS) * SLOT;
+          if (!warp_wait(sfull_bar(slot % SLOTS), (slot / SLOTS) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
             ok = false;
             break;
           }
-          tc_fence_after();
-          const uint64_t da = sw128_desc(sA + s * OPERAND), db = sw128_desc(sB + s * OPERAND);
 #pragma unroll
-          for (int k = 0; k < BK / 32; ++k)
-            mma(d, da + 2 * k, db + 2 * k, idesc(256, 256, kb & 3), sb + 8, sb, kb > 0 || k > 0);
-          commit(empty_bar(s), 3);
-          if ((kb & 3) == 3 || kb + 1 == KB) {
-            commit(sempty_bar(slot & 1), 3);
-            ++slot;
+          for (int h = 0; h < 4; h += 2) {  // one stage
+            if (kb + h >= KB) break;
+            if (!warp_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t da = sw128_desc(sA + 2 * s * OPERAND), db = sw128_desc(sB + 2 * s * OPERAND);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+              if (kb + h + i >= KB) break;
+#pragma unroll
+              for (int k = 0; k < BK / 32; ++k)
+                mma(one, d, da + (i * OPERAND / 16 + 2 * k), db + (i * OPERAND / 16 + 2 * k), idesc(256, 256, h + i),
+                    sb + 8, sb, h + i + k > 0 || kb > 0);
+            }
+            commit(one, empty_bar(s), 3);
+            if (++s == STAGES) s = 0, ph ^= 1u;
           }
-          if (++s == STAGES) s = 0, ph ^= 1u;
+          if (ok) commit(one, sempty_bar(slot % SLOTS), 3);
         }
-        if (ok) commit(tfull_bar(buf), 3);
+        if (ok) commit(one, tfull_bar(buf), 3);
       }
-      commit(drain_bar, 1);
-      drain_wait(drain_bar, 0);
+      commit(one, drain_bar, 1);
+      if (one) drain_wait(drain_bar, 0);
     }
   } else if (warp >= SCALE_WARP0) {
     // ---------------------------------------------------------- scales
@@ -273,12 +294,13 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         uint32_t a_next[4] = {0, 0, 0, 0}, b_next[2] = {0, 0};
         if (kb + 4 < KB) load(tile, kb + 4, a_next, b_next);
         else if (tile + pairs < tiles) load(tile + pairs, 0, a_next, b_next);
-        if (!warp_wait(sempty_bar(slot & 1), ((slot >> 1) & 1) ^ 1u, abort_flag, p.status, ST_F8_SCALES, WAIT_LIMIT_NS)) {
+        if (!warp_wait(sempty_bar(slot % SLOTS), ((slot / SLOTS) & 1) ^ 1u, abort_flag, p.status, ST_F8_SCALES,
+                       WAIT_LIMIT_NS)) {
           ok = false;
           break;
         }
         tc_fence_after();
-        const uint32_t at = lanes + (slot & 1) * SLOT;
+        const uint32_t at = lanes + (slot % SLOTS) * SLOT;
         const uint32_t lo[4] = {b[0], b[0], b[0], b[0]}, hi[4] = {b[1], b[1], b[1], b[1]};
         tmem_st4(at, lo);
         tmem_st4(at + 4, hi);
@@ -286,7 +308,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         tmem_wait_st();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) arrive_release(sfull0 + 8 * (slot & 1));
+        if (lane == 0) arrive_cluster(sfull0 + 8 * (slot % SLOTS));
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = a_next[i];
         b[0] = b_next[0];
@@ -304,11 +326,9 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       const int buf = unit & 1;
       const int64_t m = (int64_t)(tile % p.m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane;
       const int n0 = (tile / p.m_tiles) * 256;
-      // the shared 32 columns first: the lower half of the warps has them in both accumulators
-      auto chunk = [&](int i) {
-        if (buf) return 4 * half + i;
-        return half ? 3 + i : (i == 0 ? SHARED_CHUNK0 : i - 1);
-      };
+      // every other 32 columns, those first that the accumulators share: the lowest
+      // 64 of accumulator 1, the highest 64 of accumulator 0
+      auto chunk = [&](int i) { return (buf ? 2 * i : 6 - 2 * i) + half; };
       if (!warp_wait(tfull_bar(buf), (unit >> 1) & 1, abort_flag, p.status, ST_F8_EPILOGUE, WAIT_LIMIT_NS)) break;
       tc_fence_after();
       const uint32_t acc = lanes + (buf ? ACC1 : 0);
@@ -318,15 +338,15 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       for (int i = 0; i < 4; ++i) {
         tmem_wait_ld();
         if (i < 3) tmem_ld32(acc + 32 * chunk(i + 1), r[(i + 1) & 1]);
-        if (i == 0 && half == 0) {
+        if (i == 0) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_release(tshared0);
+          if (lane == 0) arrive_cluster(tshared0);
         }
         if (i == 3) {
           tc_fence_before();
           __syncwarp();
-          if (lane == 0) arrive_release(tempty0 + 8 * buf);
+          if (lane == 0) arrive_cluster(tempty0 + 8 * buf);
         }
         const int n = n0 + 32 * chunk(i);
         float y[32];
@@ -354,6 +374,325 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 }
 
 }  // namespace pair
+
+// ------------------------------------------ few tokens: weights on the lanes
+// The weight rows are the MMA's M (128 TMEM lanes, of which a tile may use
+// fewer), the tokens its N.  A tile has `rows` weight rows, so that the tiles of a
+// weight that is read once fill the SMs; a cluster of `split` blocks may share a
+// tile's K and joins its fp32 sums through distributed shared memory in the order of
+// the ranks.  Roles of a block:
+//   warps 0..3  epilogue: TMEM -> registers -> out (thread = weight row)
+//   warps 4..7  scales: global memory -> tensor memory, four K blocks at a time
+//   warp 8      TMA producer: weight rows and tokens of one K block per stage
+//   warp 9      TMEM allocation, MMA issue (one thread)
+namespace few {
+
+constexpr int BM = 128;
+constexpr int EPI_WARPS = 4, SCALE_WARP0 = 4, SCALE_WARPS = 4, PRODUCER = 8, ISSUER = 9;
+constexpr int THREADS = 10 * 32;
+constexpr int RING = 216 * 1024, MAX_STAGES = 8;
+constexpr int SCALES = 448, SLOT = 16, SLOTS = 4;  // 8 columns of the tokens, 4 of the weight rows
+constexpr int BARS = 2 * MAX_STAGES + 4 + 2 * SLOTS + 1;
+constexpr int SMEM = 1024 + RING + BARS * 8 + 16;
+
+struct Args {
+  F8Gemm g;
+  int rows, n_tiles, t_tiles, split, stages;
+  bool words_a, words_b;
+  unsigned int* status;
+};
+
+__device__ __forceinline__ void mma(int one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
+                                    uint32_t accum) {
+  asm volatile(
+      "{\n\t.reg .pred p, q;\n\t"
+      "setp.ne.b32 p, %6, 0;\n\t"
+      "setp.ne.b32 q, %7, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::mxf8f6f4.block_scale.scale_vec::1X [%0], %1, %2, %3, [%4], [%5], p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(sa), "r"(sb), "r"(accum), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void commit(int one, uint32_t bar) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\t"
+      "setp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(bar), "r"(one)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st1(uint32_t addr, uint32_t r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "r"(r) : "memory");
+}
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+               : "memory");
+}
+
+template <int BN>
+__global__ void __launch_bounds__(THREADS, 1)
+gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
+                   const __grid_constant__ Args p) {
+  constexpr int ACCS = BN == 256 ? 1 : 2;
+  constexpr int KPS = BN == 256 ? 1 : 2;  // K blocks per stage
+  static_assert(ACCS * BN <= SCALES && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && (BN + 64) * 512 <= RING &&
+                    SMEM <= 232448, "memories");
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
+  uint8_t* sm = smem_raw + (base - raw);
+  const int w_bytes = p.rows * BK, stage_bytes = KPS * (w_bytes + BN * BK);
+  // an MMA reads 128 rows from a stage's weights on, past a smaller tile's into what follows
+  const uint32_t sW = base, sX = base + p.stages * KPS * w_bytes;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(sm + RING);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  auto full_bar = [&](int s) { return smem_u32(bars + s); };
+  auto empty_bar = [&](int s) { return smem_u32(bars + MAX_STAGES + s); };
+  auto tfull_bar = [&](int b) { return smem_u32(bars + 2 * MAX_STAGES + b); };
+  auto tempty_bar = [&](int b) { return smem_u32(bars + 2 * MAX_STAGES + 2 + b); };
+  auto sfull_bar = [&](int b) { return smem_u32(bars + 2 * MAX_STAGES + 4 + b); };
+  auto sempty_bar = [&](int b) { return smem_u32(bars + 2 * MAX_STAGES + 4 + SLOTS + b); };
+  const uint32_t drain_bar = smem_u32(bars + BARS - 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int split = p.split, rank = split > 1 ? (int)cta_rank() : 0;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(tfull_bar(b), 1);
+      mbar_init(tempty_bar(b), EPI_WARPS);
+    }
+    for (int b = 0; b < SLOTS; ++b) {
+      mbar_init(sfull_bar(b), SCALE_WARPS);
+      mbar_init(sempty_bar(b), 1);
+    }
+    mbar_init(drain_bar, 1);
+    *abort_flag = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == ISSUER) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(TMEM_COLS)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  if (warp == PRODUCER && lane == 0) {
+    tma_prefetch_desc(&tmA);
+    tma_prefetch_desc(&tmB);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  const int tiles = p.n_tiles * p.t_tiles;
+  const int tile0 = blockIdx.x / split, tile_step = gridDim.x / split;
+  const int KB = p.g.KB;
+  const int kb0 = (int)((int64_t)KB * rank / split), kb1 = (int)((int64_t)KB * (rank + 1) / split), kn = kb1 - kb0;
+
+  if (warp == PRODUCER) {
+    if (lane == 0) {
+      int s = 0;
+      uint32_t ph = 0, issued = 0, issued_ph = 0;
+      bool ok = true;
+      for (int tile = tile0; ok && tile < tiles; tile += tile_step) {
+        const int n0 = (tile % p.n_tiles) * p.rows, t0 = (tile / p.n_tiles) * BN;
+        for (int kb = kb0; kb < kb1; kb += KPS) {
+          if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, ST_F8_PRODUCER, WAIT_LIMIT_NS)) {
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(full_bar(s), (uint32_t)stage_bytes);
+#pragma unroll
+          for (int i = 0; i < KPS; ++i) {  // past the split's last K block too: the stage is whole
+            tma_load_2d(sW + (s * KPS + i) * w_bytes, &tmB, (kb + i) * BK, n0, full_bar(s));
+            tma_load_2d(sX + (s * KPS + i) * BN * BK, &tmA, (kb + i) * BK, t0, full_bar(s));
+          }
+          issued |= 1u << s;
+          issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
+          if (++s == p.stages) s = 0, ph ^= 1u;
+        }
+      }
+      // copies that no MMA waits for any more land before the block exits
+      if (!ok)
+        for (int t = 0; t < p.stages; ++t)
+          if (issued & (1u << t)) drain_wait(full_bar(t), (issued_ph >> t) & 1u);
+    }
+  } else if (warp == ISSUER) {
+    {  // the whole warp, so that addresses and descriptors stay in uniform registers; one lane issues
+      const int one = lane == 0;
+      int s = 0, unit = 0;
+      uint32_t ph = 0;
+      unsigned slot = 0;
+      bool ok = true;
+      for (int tile = tile0; ok && tile < tiles; tile += tile_step, ++unit) {
+        const int buf = unit % ACCS;
+        if (!warp_wait(tempty_bar(buf), ((unit / ACCS) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+        tc_fence_after();
+        const uint32_t d = tmem + buf * BN;
+        for (int kb = 0; ok && kb < kn; kb += 4, ++slot) {  // one slot of scales
+          const uint32_t sb = tmem + SCALES + (slot % SLOTS) * SLOT;
+          if (!warp_wait(sfull_bar(slot % SLOTS), (slot / SLOTS) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
+            ok = false;
+            break;
+          }
+#pragma unroll
+          for (int h = 0; h < 4; h += KPS) {  // one stage
+            if (kb + h >= kn) break;
+            if (!warp_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            const uint64_t dw = sw128_desc(sW + s * KPS * w_bytes), dx = sw128_desc(sX + s * KPS * BN * BK);
+#pragma unroll
+            for (int i = 0; i < KPS; ++i) {
+              if (kb + h + i >= kn) break;
+#pragma unroll
+              for (int k = 0; k < BK / 32; ++k)
+                mma(one, d, dw + (uint64_t)(i * (w_bytes >> 4) + 2 * k), dx + (i * BN * BK / 16 + 2 * k),
+                    idesc(BM, BN, h + i), sb + 8, sb, h + i + k > 0 || kb > 0);
+            }
+            commit(one, empty_bar(s));
+            if (++s == p.stages) s = 0, ph ^= 1u;
+          }
+          if (ok) commit(one, sempty_bar(slot % SLOTS));
+        }
+        if (ok) commit(one, tfull_bar(buf));
+      }
+      commit(one, drain_bar);
+      if (one) drain_wait(drain_bar, 0);
+    }
+  } else if (warp >= SCALE_WARP0) {
+    const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + SCALES;
+    const int last = (p.g.N - 1) / F8_BLOCK;
+    auto load = [&](int tile, int kb, uint32_t (&w)[4], uint32_t (&x)[BN / 32]) {
+      const int n0 = (tile % p.n_tiles) * p.rows, t0 = (tile / p.n_tiles) * BN;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = scale_word(p.g.sb + (int64_t)min((n0 + 32 * i + lane) / F8_BLOCK, last) * KB, kb, KB,
+                          p.words_b && (kb & 3) == 0);
+#pragma unroll
+      for (int i = 0; i < BN / 32; ++i)
+        x[i] = scale_word(p.g.sa + (int64_t)min(t0 + 32 * i + lane, p.g.M - 1) * KB, kb, KB, p.words_a && (kb & 3) == 0);
+    };
+    unsigned slot = 0;
+    bool ok = true;
+    uint32_t w[4], x[BN / 32];
+    load(tile0, kb0, w, x);
+    for (int tile = tile0; ok && tile < tiles; tile += tile_step) {
+      for (int kb = kb0; kb < kb1; kb += 4, ++slot) {
+        uint32_t w_next[4], x_next[BN / 32];
+        const bool more = kb + 4 < kb1;
+        load(more || tile + tile_step >= tiles ? tile : tile + tile_step, more ? kb + 4 : kb0, w_next, x_next);
+        if (!warp_wait(sempty_bar(slot % SLOTS), ((slot / SLOTS) & 1) ^ 1u, abort_flag, p.status, ST_F8_SCALES,
+                       WAIT_LIMIT_NS)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t at = lanes + (slot % SLOTS) * SLOT;
+        tmem_st4(at + 8, w);
+#pragma unroll
+        for (int i = 0; i < BN / 32; ++i) tmem_st1(at + i, x[i]);
+        tmem_wait_st();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(sfull_bar(slot % SLOTS));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[i] = w_next[i];
+#pragma unroll
+        for (int i = 0; i < BN / 32; ++i) x[i] = x_next[i];
+      }
+    }
+  } else {
+    int unit = 0;
+    const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+    const int r = warp * 32 + lane;
+    for (int tile = tile0; tile < tiles; tile += tile_step, ++unit) {
+      const int n = (tile % p.n_tiles) * p.rows + r, t0 = (tile / p.n_tiles) * BN;
+      const int buf = unit % ACCS;
+      const float bias = p.g.bias && n < p.g.N ? load_as_f32(p.g.bias, p.g.bias_dtype, n) : 0.0f;
+      if (!warp_wait(tfull_bar(buf), (unit / ACCS) & 1, abort_flag, p.status, ST_F8_EPILOGUE, WAIT_LIMIT_NS)) break;
+      tc_fence_after();
+      if (split == 1) {
+        const int t1 = min(BN, p.g.M - t0);
+        if (warp * 32 < p.rows)
+#pragma unroll 1
+          for (int c = 0; c < t1; c += 32) {
+            uint32_t v[32];
+            tmem_ld32(lanes + (uint32_t)(buf * BN + c), v);
+            tmem_wait_ld();
+            if (r < p.rows && n < p.g.N) {
+              const int64_t at = (int64_t)(t0 + c) * p.g.ld_out + n;
+#pragma unroll
+              for (int j = 0; j < 32; ++j) {
+                if (c + j >= t1) break;
+                store_from_f32(p.g.out, p.g.out_dtype, at + j * p.g.ld_out, __uint_as_float(v[j]) + bias);
+              }
+            }
+          }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(tempty_bar(buf));
+      }
+    }
+  }
+
+  if (split > 1) {
+    // one tile per cluster; every block's MMAs are done with its ring: the sums go there
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const int n0 = (tile0 % p.n_tiles) * p.rows, t0 = (tile0 / p.n_tiles) * BN, t1 = min(BN, p.g.M - t0);
+    const int per = ((BN + split - 1) / split + 3) & ~3, pitch = per + 4;  // tokens per rank; padded against conflicts
+    if (warp < EPI_WARPS && __all_sync(0xffffffffu, !*abort_flag)) {
+      const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
+      const int r = warp * 32 + lane;
+      // rank d finishes tokens [d per, (d + 1) per): sums as [source][row][pitch]
+#pragma unroll 1
+      for (int c = 0; c < t1; c += 32) {
+        uint32_t v[32];
+        tmem_ld32(lanes + (uint32_t)c, v);
+        tmem_wait_ld();
+        if (r < p.rows) {
+          int d = c / per, at = c - d * per;
+#pragma unroll
+          for (int j = 0; j < 32; j += 4) {
+            st_cluster_f32x4(mapa(base + (uint32_t)(((rank * BM + r) * pitch + at) * 4), (uint32_t)d), v[j], v[j + 1],
+                             v[j + 2], v[j + 3]);
+            if ((at += 4) >= per) at -= per, ++d;
+          }
+        }
+      }
+    }
+    __syncwarp();
+    tc_fence_before();
+    cluster_sync();
+    tc_fence_after();
+    const float* part = reinterpret_cast<const float*>(sm);
+    for (int i = threadIdx.x; i < per * BM; i += THREADS) {
+      const int r = i & (BM - 1), c = i / BM;
+      const int t = rank * per + c, n = n0 + r;
+      if (t >= t1 || r >= p.rows || n >= p.g.N) continue;
+      float y = 0.0f;
+      for (int s = 0; s < split; ++s) y += part[(s * BM + r) * pitch + c];
+      if (p.g.bias) y += load_as_f32(p.g.bias, p.g.bias_dtype, n);
+      store_from_f32(p.g.out, p.g.out_dtype, (int64_t)(t0 + t) * p.g.ld_out + n, y);
+    }
+  }
+
+  __syncwarp();
+  tc_fence_before();
+  __syncthreads();
+  if (warp == ISSUER) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+}
+
+}  // namespace few
 
 // Codes [rows, K] -> boxes of `box` rows x 128 columns, 128-byte swizzle, zeros outside.
 int code_map8(CUtensorMap* map, const uint8_t* q, int64_t rows, int64_t K, int64_t ld, int box) {
@@ -392,9 +731,60 @@ int launch_pair(const F8Gemm& g, cudaStream_t st) {
   return check_cuda(cudaGetLastError(), "gemm_f8_pair_kernel launch");
 }
 
+template <int BN>
+int launch_few(const F8Gemm& g, int rows, int split, cudaStream_t st) {
+  static bool done[64];
+  int dev = 0;
+  QI8_CUDA(cudaGetDevice(&dev));
+  auto kern = few::gemm_f8_few_kernel<BN>;
+  if (split > g.KB) split = g.KB;
+  if (dev >= 64 || !done[dev]) {
+    QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few::SMEM));
+    if (dev < 64) done[dev] = true;
+  }
+  CUtensorMap ma, mb;
+  if (int rc = code_map8(&ma, g.a, g.M, g.K, g.ld_a, BN)) return rc;
+  if (int rc = code_map8(&mb, g.b, g.N, g.K, g.ld_b, rows)) return rc;
+  int stages = few::RING / ((BN == 256 ? 1 : 2) * (rows + BN) * BK);
+  if (stages > few::MAX_STAGES) stages = few::MAX_STAGES;
+  few::Args p{g, rows, (g.N + rows - 1) / rows, (g.M + BN - 1) / BN, split, stages, word_rows(g.sa, g.KB),
+              word_rows(g.sb, g.KB), device_status_ptr()};
+  const int64_t tiles = (int64_t)p.n_tiles * p.t_tiles;
+  QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < sm_count() ? tiles : sm_count()));
+  cfg.blockDim = dim3(few::THREADS);
+  cfg.dynamicSmemBytes = few::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)split;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, ma, mb, p), "gemm_f8_few_kernel launch");
+}
+
 }  // namespace f8tc
 }  // namespace
 
-int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) { return f8tc::launch_pair(g, st); }
+int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) {
+  const char* e = getenv("F8_TUNE");
+  if (e) {
+    int bn, rows, split;
+    if (sscanf(e, "%d,%d,%d", &bn, &rows, &split) == 3 && bn > 0) {
+      if (bn == 32) return f8tc::launch_few<32>(g, rows, split, st);
+      if (bn == 64) return f8tc::launch_few<64>(g, rows, split, st);
+      if (bn == 128) return f8tc::launch_few<128>(g, rows, split, st);
+      return f8tc::launch_few<256>(g, rows, split, st);
+    }
+    return f8tc::launch_pair(g, st);
+  }
+  if (g.M <= 32) return f8tc::launch_few<32>(g, 128, 2, st);
+  if (g.M <= 64) return f8tc::launch_few<64>(g, 64, 1, st);
+  if (g.M <= 128) return f8tc::launch_few<128>(g, 128, 3, st);
+  if (g.M <= 256) return f8tc::launch_few<256>(g, 72, 1, st);
+  return f8tc::launch_pair(g, st);
+}
 
 }  // namespace qi8
