@@ -311,6 +311,7 @@ constexpr int THREADS = 256;
 
 template <typename T, int OP, int STEPS>
 __global__ void __launch_bounds__(THREADS) block_kernel(const __grid_constant__ Args p, const unsigned groups) {
+  pdl_launch_dependents();  // the product behind it prepares itself
   const int lane = threadIdx.x & 31;
   const unsigned unit = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
   const unsigned row = unit / groups;

@@ -31,8 +31,16 @@ struct F8Gemm {
   int bias_dtype, out_dtype;
 };
 
-// The tcgen05 kernels (gemm_f8_tc.cu): rows of both operands start on 16-byte boundaries.
-int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st);
+// The tcgen05 kernels (gemm_f8_tc.cu): rows of both operands start on 16-byte
+// boundaries.  after_quant: the stream's last kernel writes a and sa and lets the
+// next one start early.
+int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st);
+
+// The kernel for single tokens (gemm_f8_rows.cu), where the tokens fit beside its
+// ring: rows of codes start on 16-byte boundaries.  x (not null): the tokens as
+// numbers of x_dtype, quantized on the way, in place of g.a and g.sa.
+bool gemm_f8_rows_fits(int M, int K);
+int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st);
 
 inline int64_t f8_blocks(int64_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }
 

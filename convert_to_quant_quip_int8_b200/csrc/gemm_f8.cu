@@ -2,6 +2,7 @@
 //
 //   out[t, n] = sum_kb 2^(ea[t, kb] + eb[n / 128, kb]) sum_{k in kb} a[t, k] b[n, k] + bias[n]
 #include <cstdint>
+#include <cstdlib>
 
 #include "f8.cuh"
 
@@ -96,8 +97,10 @@ extern "C" int qi8_gemm_f8(const uint8_t* a, const uint8_t* a_scale, int64_t M, 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   if (int rc = f8g::align_rows(a, M, K, ld_a, ws, st)) return rc;
   if (int rc = f8g::align_rows(b, N, K, ld_b, ws, st)) return rc;
-  return gemm_f8_tiles({a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K,
-                        (int)f8_blocks(K), bias_dtype, out_dtype}, st);
+  const F8Gemm g{a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
+                 bias_dtype, out_dtype};
+  if (gemm_f8_rows_fits((int)M, (int)K) && !getenv("F8_TUNE")) return gemm_f8_rows(g, nullptr, 0, 0, false, st);
+  return gemm_f8_tiles(g, false, st);
 }
 
 extern "C" int64_t qi8_linear_f8_workspace_bytes(int64_t M, int64_t K, const uint8_t* b, int64_t N, int64_t ld_b) {
@@ -120,7 +123,10 @@ extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, i
   uint8_t* s = q + M * f8g::pitch(K);
   uint8_t* ws = s + f8g::pitch(M * f8_blocks(K));
   if (int rc = f8g::align_rows(b, N, K, ld_b, ws, st)) return rc;
+  F8Gemm g{q, b, s, b_scale, bias, out, f8g::pitch(K), ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
+           bias_dtype, out_dtype};
+  if (gemm_f8_rows_fits((int)M, (int)K) && !getenv("F8_PRE")) return gemm_f8_rows(g, x, x_dtype, ld_x, false, st);
   if (int rc = quant_rows_f8(x, x_dtype, M, K, ld_x, q, f8g::pitch(K), s, st)) return rc;
-  return gemm_f8_tiles({q, b, s, b_scale, bias, out, f8g::pitch(K), ld_b, ld_out, (int)M, (int)N, (int)K,
-                        (int)f8_blocks(K), bias_dtype, out_dtype}, st);
+  if (gemm_f8_rows_fits((int)M, (int)K) && !getenv("F8_TUNE")) return gemm_f8_rows(g, nullptr, 0, 0, true, st);
+  return gemm_f8_tiles(g, true, st);
 }

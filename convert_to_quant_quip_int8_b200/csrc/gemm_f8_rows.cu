@@ -1,0 +1,279 @@
+// Products of fp8 operands with block scales for single tokens (format: f8.cuh),
+// on m16n8k32 steps fed from shared memory.
+//
+// A thread block computes 16 features.  One warp copies the weight rows, 1024
+// columns at a time, into a ring that holds a row of 4096 columns as a whole; eight
+// warps take one block of 128 columns of each such piece and add up in the order of
+// the warps.  The tokens' codes lie in shared memory as a whole, copied or, for few
+// of them, quantized here while the weight is on its way.  Rows are 16 bytes longer
+// than whole 128s, so that eight of them read as one ldmatrix row block touch all
+// banks once.
+//
+// Against the tcgen05 kernel this one starts sooner (no tensor memory, maps or
+// scales to set up) and keeps every SM at work at any number of rows, but its steps
+// take 8.3 cycles for 16 rows and 8 tokens, too long for more than 16 of them.
+#include <cstdint>
+#include <cstdlib>
+
+#include "f8.cuh"
+#include "tc05.cuh"
+
+namespace qi8 {
+namespace {
+namespace f8r {
+
+constexpr int ROWS = 16, WARPS = 8, COPIER = WARPS, THREADS = (WARPS + 1) * 32;
+constexpr int PIECE = WARPS * F8_BLOCK;           // columns of K per stage
+constexpr int PIECE_PITCH = PIECE + 16, STAGE = ROWS * PIECE_PITCH;
+constexpr int MAX_STAGES = 4, SMEM_MOST = 110 * 1024;  // two blocks per SM at least
+
+struct Args {
+  F8Gemm g;
+  const void* x;  // tokens to quantize, in place of codes
+  int64_t ld_x;
+  bool vec_x;
+  int stages, x_pitch;
+  unsigned int* status;
+};
+
+// D[16, 8] += A[16, 32] B[32, 8], e4m3, fp32 sums
+__device__ __forceinline__ void mma(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four blocks of eight rows x 16 bytes; lane l gives the address of row l % 8 of block l / 8.
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+// Contiguous bytes, whole 16s, global to shared memory.
+__device__ __forceinline__ void bulk_copy(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+               "l"(src), "r"(bytes), "r"(bar)
+               : "memory");
+}
+// Of the four codes in a word, those at columns below K.
+__device__ __forceinline__ uint32_t below(uint32_t w, int k, int K) {
+  const int left = K - k;
+  return left >= 4 ? w : left <= 0 ? 0u : w & ((1u << (8 * left)) - 1u);
+}
+
+// 2^(ea + eb) for two scale bytes as two factors, the second of which is 1 but for
+// sums that fp32's exponent does not hold: multiplied one after the other they
+// overflow only where the result does.
+__device__ __forceinline__ float2 both_scales(uint32_t a, uint32_t b) {
+  if (a == 255u || b == 255u) return make_float2(__uint_as_float(0x7fffffffu), 1.0f);
+  const int e = (int)(a + b) - 254, in = e < -126 ? -126 : e > 127 ? 127 : e;
+  return make_float2(__uint_as_float((uint32_t)(in + 127) << 23), __uint_as_float((uint32_t)(e - in + 127) << 23));
+}
+
+template <typename X, int NT>  // X uint8_t: codes; NT groups of eight tokens
+__global__ void __launch_bounds__(THREADS) gemm_f8_rows_kernel(const __grid_constant__ Args p) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float part[WARPS][ROWS][8 * NT + 1];
+  __shared__ __align__(16) uint8_t zeros[F8_BLOCK];
+  __shared__ uint64_t bars[2 * MAX_STAGES];
+  __shared__ int abort_word;
+  volatile int* abort_flag = &abort_word;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int n0 = blockIdx.x * ROWS, M = p.g.M, K = p.g.K, KB = p.g.KB;
+  const int pieces = (K + PIECE - 1) / PIECE;
+  const uint32_t ring = smem_u32(smem);
+  uint8_t* codes = smem + p.stages * STAGE;
+  uint8_t* scales = codes + M * p.x_pitch;  // [KB][M]
+  auto full_bar = [&](int s) { return smem_u32(bars + s); };
+  auto empty_bar = [&](int s) { return smem_u32(bars + MAX_STAGES + s); };
+  if (threadIdx.x == COPIER * 32) {
+    for (int s = 0; s < p.stages; ++s) {
+      mbar_init(full_bar(s), 1);
+      mbar_init(empty_bar(s), WARPS);
+    }
+    abort_word = 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (threadIdx.x < F8_BLOCK / 4) reinterpret_cast<uint32_t*>(zeros)[threadIdx.x] = 0;
+  __syncthreads();
+
+  // one piece of the block's rows into a stage; lane = row
+  const uint8_t* my_row = p.g.b + (int64_t)min(n0 + lane, p.g.N - 1) * p.g.ld_b;
+  auto copy_piece = [&](int i, int s) {
+    const int k = i * PIECE, bytes = min(PIECE, (K - k + 15) & ~15);
+    if (lane == 0) mbar_arrive_expect_tx(full_bar(s), ROWS * bytes);
+    __syncwarp();
+    if (lane < ROWS) bulk_copy(ring + s * STAGE + lane * PIECE_PITCH, my_row + k, bytes, full_bar(s));
+  };
+  if (warp == COPIER)
+    for (int i = 0; i < pieces && i < p.stages; ++i) copy_piece(i, i);
+
+  // the tokens, by all warps but that one
+  if (warp < WARPS) {
+    if constexpr (std::is_same<X, uint8_t>::value) {
+      pdl_wait();  // the kernel before may write them
+      const int per = KB * (F8_BLOCK / 16);
+      for (int i = threadIdx.x; i < M * per; i += WARPS * 32) {
+        const int t = i / per, k = (i - t * per) * 16;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (k < K) v = __ldg(reinterpret_cast<const uint4*>(p.g.a + t * p.g.ld_a + k));
+        if (k + 16 > K) v = make_uint4(below(v.x, k, K), below(v.y, k + 4, K), below(v.z, k + 8, K), below(v.w, k + 12, K));
+        *reinterpret_cast<uint4*>(codes + t * p.x_pitch + k) = v;
+      }
+      for (int i = threadIdx.x; i < M * KB; i += WARPS * 32) {
+        const int t = i / KB, kb = i - t * KB;
+        scales[kb * M + t] = __ldg(p.g.sa + i);
+      }
+    } else {
+      // eight columns per lane, 16 lanes per block of 128
+      const int per = KB * 16;
+      for (int i0 = 0; i0 < M * per; i0 += WARPS * 32) {
+        const int i = i0 + threadIdx.x, t = i / per, k = (i - t * per) * 8;
+        const bool live = t < M;
+        Eight<X> e;
+        const X* row = static_cast<const X*>(p.x) + (live ? t : 0) * p.ld_x;
+        if (live && p.vec_x && k + 8 <= K) e.load(row + k);
+        else e.load_some(row, k, live ? K : 0);
+        const F8x f = e.get();
+        const uint32_t code = f8_scale_code(max16(amax_bits(f)));
+        if (!live) continue;
+        *reinterpret_cast<uint2*>(codes + t * p.x_pitch + k) = f8_codes(f, f8_inverse(code));
+        if ((lane & 15) == 0) scales[k / F8_BLOCK * M + t] = (uint8_t)code;
+      }
+    }
+    asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory");
+  }
+
+  if (warp == COPIER) {
+    int s = 0, sent = p.stages;
+    uint32_t ph = 0;
+    for (; sent < pieces; ++sent) {
+      if (!warp_wait(empty_bar(s), ph, abort_flag, p.status, ST_F8_PRODUCER, WAIT_LIMIT_NS)) break;
+      copy_piece(sent, s);
+      if (++s == p.stages) s = 0, ph ^= 1u;
+    }
+    // nobody may be waiting any more, but what is on its way lands before the block exits
+    for (int j = sent - p.stages; j < sent; ++j) drain_wait(full_bar(j % p.stages), (j / p.stages) & 1u);
+  } else {
+    float acc[NT][4] = {};
+    // rows and 16-byte halves of an A block: (0..7, 0), (8..15, 0), (0..7, 1), (8..15, 1)
+    const uint32_t a_at = (uint32_t)((lane & 15) * PIECE_PITCH + warp * F8_BLOCK + (lane >> 4) * 16);
+    const uint8_t* sw = p.g.sb + (int64_t)(n0 / F8_BLOCK) * KB;
+    int s = 0;
+    uint32_t ph = 0;
+    for (int i = 0; i < pieces; ++i) {
+      const int kb = i * WARPS + warp;
+      const bool mine = kb < KB;
+      const uint32_t w_scale = mine ? __ldg(sw + kb) : 127u;
+      if (!warp_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+      if (mine) {
+        uint32_t a[4][4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) ldmatrix4(a[j], ring + s * STAGE + a_at + 32 * j);
+        if ((kb + 1) * F8_BLOCK > K) {  // nothing was copied past K's 16 bytes, and those may hold anything
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int h = 0; h < 4; ++h)
+              a[j][h] = below(a[j][h], kb * F8_BLOCK + 32 * j + 16 * (h >> 1) + 4 * (lane & 3), K);
+        }
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+          // lane l: token l % 8, 16 bytes l / 8 of 64
+          const int tok = 8 * t + (lane & 7);
+          const uint32_t b_at = (tok < M ? smem_u32(codes + tok * p.x_pitch + kb * F8_BLOCK) : smem_u32(zeros)) + (lane >> 3) * 16;
+          uint32_t b[2][4];
+          ldmatrix4(b[0], b_at);
+          ldmatrix4(b[1], b_at + 64);
+          float d[4] = {0, 0, 0, 0};
+#pragma unroll
+          for (int j = 0; j < 4; ++j) mma(d, a[j], b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const int mine_t = 8 * t + 2 * (lane & 3) + u;
+            const float2 f = both_scales(mine_t < M ? scales[kb * M + mine_t] : 127u, w_scale);
+            acc[t][u] = fmaf(d[u] * f.y, f.x, acc[t][u]);
+            acc[t][u + 2] = fmaf(d[u + 2] * f.y, f.x, acc[t][u + 2]);
+          }
+        }
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(empty_bar(s));
+      if (++s == p.stages) s = 0, ph ^= 1u;
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) part[warp][(lane >> 2) + 8 * (j >> 1)][8 * t + 2 * (lane & 3) + (j & 1)] = acc[t][j];
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < ROWS * M; i += THREADS) {
+    const int t = i / ROWS, r = i % ROWS, n = n0 + r;
+    if (n >= p.g.N) continue;
+    float y = 0.0f;
+#pragma unroll
+    for (int k = 0; k < WARPS; ++k) y += part[k][r][t];
+    if (p.g.bias) y += load_as_f32(p.g.bias, p.g.bias_dtype, n);
+    store_from_f32(p.g.out, p.g.out_dtype, t * p.g.ld_out + n, y);
+  }
+}
+
+// Stages beside the tokens in half of an SM's shared memory; under two: none.
+int stages_for(int M, int K, int KB, int* x_pitch, int* smem) {
+  *x_pitch = KB * F8_BLOCK + 16;
+  const int64_t tokens = (int64_t)M * (*x_pitch + KB);
+  const int64_t left = (SMEM_MOST - tokens) / STAGE;
+  const int pieces = (K + PIECE - 1) / PIECE;
+  int stages = left > MAX_STAGES ? MAX_STAGES : (int)left;
+  if (stages > pieces) stages = pieces;
+  *smem = (int)(stages * STAGE + tokens);
+  return tokens > SMEM_MOST || (stages < 2 && stages < pieces) ? 0 : stages;
+}
+
+template <typename X, int NT>
+int launch(const Args& p, int smem, bool after_quant, cudaStream_t st) {
+  static bool done[64];
+  int dev = 0;
+  QI8_CUDA(cudaGetDevice(&dev));
+  auto kern = gemm_f8_rows_kernel<X, NT>;
+  if (dev >= 64 || !done[dev]) {
+    QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST));
+    if (dev < 64) done[dev] = true;
+  }
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((p.g.N + ROWS - 1) / ROWS));
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_quant ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "gemm_f8_rows_kernel launch");
+}
+
+template <typename X>
+int launch_tokens(const Args& p, int smem, bool after_quant, cudaStream_t st) {
+  return p.g.M <= 8 ? launch<X, 1>(p, smem, after_quant, st) : launch<X, 2>(p, smem, after_quant, st);
+}
+
+}  // namespace f8r
+}  // namespace
+
+bool gemm_f8_rows_fits(int M, int K) {
+  int pitch, smem;
+  return M <= 16 && f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) > 0;
+}
+
+int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st) {
+  f8r::Args p{g, x, ld_x, x && rows_aligned(x, ld_x, elem_size(x_dtype), 16), 0, 0, device_status_ptr()};
+  int smem = 0;
+  p.stages = f8r::stages_for(g.M, g.K, g.KB, &p.x_pitch, &smem);
+  if (!x) return f8r::launch_tokens<uint8_t>(p, smem, after_quant, st);
+  switch (x_dtype) {
+    case QI8_BF16: return f8r::launch_tokens<__nv_bfloat16>(p, smem, false, st);
+    case QI8_F16: return f8r::launch_tokens<__half>(p, smem, false, st);
+    default: return f8r::launch_tokens<float>(p, smem, false, st);
+  }
+}
+
+}  // namespace qi8

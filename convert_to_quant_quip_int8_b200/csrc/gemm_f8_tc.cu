@@ -191,6 +191,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
+  pdl_wait();
   const uint32_t tmem = *tmem_slot;
   const int KB = p.g.KB, tiles = p.m_tiles * p.n_tiles;
 
@@ -484,6 +485,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_wait();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.n_tiles * p.t_tiles;
   const int tile0 = blockIdx.x / split, tile_step = gridDim.x / split;
@@ -711,7 +713,7 @@ int code_map8(CUtensorMap* map, const uint8_t* q, int64_t rows, int64_t K, int64
 // Scale rows that can be read a word at a time.
 bool word_rows(const uint8_t* s, int KB) { return KB % 4 == 0 && reinterpret_cast<uintptr_t>(s) % 4 == 0; }
 
-int launch_pair(const F8Gemm& g, cudaStream_t st) {
+int launch_pair(const F8Gemm& g, bool after_quant, cudaStream_t st) {
   static bool done[64];
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
@@ -727,12 +729,21 @@ int launch_pair(const F8Gemm& g, cudaStream_t st) {
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
   const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
-  pair::gemm_f8_pair_kernel<<<(unsigned)(2 * pairs), pair::THREADS, pair::SMEM, st>>>(ma, mb, p);
-  return check_cuda(cudaGetLastError(), "gemm_f8_pair_kernel launch");
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(pair::THREADS);
+  cfg.dynamicSmemBytes = pair::SMEM;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = after_quant ? 1 : 0;
+  return check_cuda(cudaLaunchKernelEx(&cfg, pair::gemm_f8_pair_kernel, ma, mb, p), "gemm_f8_pair_kernel launch");
 }
 
 template <int BN>
-int launch_few(const F8Gemm& g, int rows, int split, cudaStream_t st) {
+int launch_few(const F8Gemm& g, int rows, int split, bool after_quant, cudaStream_t st) {
   static bool done[64];
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
@@ -756,35 +767,37 @@ int launch_few(const F8Gemm& g, int rows, int split, cudaStream_t st) {
   cfg.blockDim = dim3(few::THREADS);
   cfg.dynamicSmemBytes = few::SMEM;
   cfg.stream = st;
-  cudaLaunchAttribute attr[1];
+  cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)split;
   attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
   cfg.attrs = attr;
-  cfg.numAttrs = 1;
+  cfg.numAttrs = after_quant ? 2 : 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, kern, ma, mb, p), "gemm_f8_few_kernel launch");
 }
 
 }  // namespace f8tc
 }  // namespace
 
-int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) {
+int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st) {
   const char* e = getenv("F8_TUNE");
   if (e) {
     int bn, rows, split;
     if (sscanf(e, "%d,%d,%d", &bn, &rows, &split) == 3 && bn > 0) {
-      if (bn == 32) return f8tc::launch_few<32>(g, rows, split, st);
-      if (bn == 64) return f8tc::launch_few<64>(g, rows, split, st);
-      if (bn == 128) return f8tc::launch_few<128>(g, rows, split, st);
-      return f8tc::launch_few<256>(g, rows, split, st);
+      if (bn == 32) return f8tc::launch_few<32>(g, rows, split, after_quant, st);
+      if (bn == 64) return f8tc::launch_few<64>(g, rows, split, after_quant, st);
+      if (bn == 128) return f8tc::launch_few<128>(g, rows, split, after_quant, st);
+      return f8tc::launch_few<256>(g, rows, split, after_quant, st);
     }
-    return f8tc::launch_pair(g, st);
+    return f8tc::launch_pair(g, after_quant, st);
   }
-  if (g.M <= 32) return f8tc::launch_few<32>(g, 128, 2, st);
-  if (g.M <= 64) return f8tc::launch_few<64>(g, 64, 1, st);
-  if (g.M <= 128) return f8tc::launch_few<128>(g, 128, 3, st);
-  if (g.M <= 256) return f8tc::launch_few<256>(g, 72, 1, st);
-  return f8tc::launch_pair(g, st);
+  if (g.M <= 32) return f8tc::launch_few<32>(g, 128, 2, after_quant, st);
+  if (g.M <= 64) return f8tc::launch_few<64>(g, 64, 1, after_quant, st);
+  if (g.M <= 128) return f8tc::launch_few<128>(g, 128, 3, after_quant, st);
+  if (g.M <= 256) return f8tc::launch_few<256>(g, 72, 1, after_quant, st);
+  return f8tc::launch_pair(g, after_quant, st);
 }
 
 }  // namespace qi8
