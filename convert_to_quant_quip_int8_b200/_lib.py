@@ -136,7 +136,7 @@ _call = None
 
 
 def fast_call():
-    """The host-side shortcut of the 4-bit operators (csrc/call.cpp), bound to
+    """The host-side shortcut of the 4-bit and fp8 operators (csrc/call.cpp), bound to
     libqi8; ``None`` where it was not built for this interpreter and torch."""
     global _call
     if _call is None:
@@ -151,7 +151,9 @@ def fast_call():
         else:
             mod.bind(*(ctypes.cast(f, ctypes.c_void_p).value for f in (
                 lib.qi8_quant_weight_i4, lib.qi8_dequant_i4, lib.qi8_gemm_w4, lib.qi8_moe_w4,
-                lib.qi8_moe_w4_workspace_bytes)))
+                lib.qi8_moe_w4_workspace_bytes, lib.qi8_quant_rows_f8, lib.qi8_quant_weight_f8,
+                lib.qi8_gemm_f8_workspace_bytes, lib.qi8_gemm_f8, lib.qi8_linear_f8_workspace_bytes, lib.qi8_linear_f8,
+                lib.qi8_rms_norm_quant, lib.qi8_gated_quant)))
             _call = mod
     return _call or None
 

@@ -1,6 +1,6 @@
-// The common case of the 4-bit operators' wrappers, without the interpreter: a
-// product for one token takes the GPU about 5 us and its Python wrapper took the
-// host 11.  Each function checks that its arguments are what the kernels take as
+// The common case of the 4-bit and fp8 operators' wrappers, without the
+// interpreter: a product for one token takes the GPU about 5 us and its Python
+// wrapper took the host 11 (4 bits) or 20 (fp8).  Each function checks that its arguments are what the kernels take as
 // they are (plain tensors on the current device, right types and shapes,
 // contiguous where that is needed, no gradient wanted), allocates the result and
 // calls the C ABI of libqi8.  For anything else, and for any error, it returns
@@ -15,6 +15,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <type_traits>
 #include <vector>
 
 #include "../../include/qi8.h"
@@ -26,6 +27,14 @@ decltype(&qi8_dequant_i4) dequant_fn;
 decltype(&qi8_gemm_w4) gemm_fn;
 decltype(&qi8_moe_w4) moe_fn;
 decltype(&qi8_moe_w4_workspace_bytes) moe_bytes_fn;
+decltype(&qi8_quant_rows_f8) quant_rows_f8_fn;
+decltype(&qi8_quant_weight_f8) quant_weight_f8_fn;
+decltype(&qi8_gemm_f8_workspace_bytes) gemm_f8_bytes_fn;
+decltype(&qi8_gemm_f8) gemm_f8_fn;
+decltype(&qi8_linear_f8_workspace_bytes) linear_f8_bytes_fn;
+decltype(&qi8_linear_f8) linear_f8_fn;
+decltype(&qi8_rms_norm_quant) norm_fn;
+decltype(&qi8_gated_quant) gated_fn;
 
 int code(at::ScalarType t) {
   return t == at::kBFloat16 ? QI8_BF16 : t == at::kHalf ? QI8_F16 : t == at::kFloat ? QI8_F32 : -1;
@@ -191,28 +200,267 @@ PyObject* moe_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   });
 }
 
-// addresses of qi8_quant_weight_i4, qi8_dequant_i4, qi8_gemm_w4, qi8_moe_w4, qi8_moe_w4_workspace_bytes
+// ---------------------------------------------------------------- fp8
+
+constexpr int64_t F8_BLOCK = 128;
+int64_t blocks(int64_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }
+
+// A float type on the current device with at least one element.
+bool numbers(const at::Tensor& t, int device) {
+  return plain(t, device) && code(t.scalar_type()) >= 0 && t.dim() >= 1 && t.numel() > 0;
+}
+
+// Whether `t` [..., n] is rows with unit column stride a fixed stride apart, which is
+// what the kernels take: that stride, or -1.
+int64_t row_stride(const at::Tensor& t) {
+  const int64_t d = t.dim(), n = t.size(d - 1);
+  if (t.stride(d - 1) != 1 && n > 1) return -1;
+  if (d == 1 || t.numel() == n) return n;
+  int64_t step = 0, ld = 0;  // of the next outer dimension with more than one row
+  for (int64_t i = d - 2; i >= 0; --i) {
+    if (t.size(i) == 1) continue;
+    if (step == 0) ld = t.stride(i);
+    else if (t.stride(i) != step) return -1;
+    step = t.stride(i) * t.size(i);
+  }
+  return ld >= n ? ld : -1;
+}
+
+// e4m3 codes [..., n] and contiguous e8m0 scales [lead..., blocks(n)].
+bool codes(const at::Tensor& q, const at::Tensor& s, bool weight, int device) {
+  if (!plain(q, device) || !plain(s, device) || q.scalar_type() != at::kFloat8_e4m3fn ||
+      s.scalar_type() != at::kFloat8_e8m0fnu || q.dim() != s.dim() || q.dim() < (weight ? 2 : 1) || q.numel() == 0 ||
+      !s.is_contiguous())
+    return false;
+  const int64_t d = q.dim();
+  if (weight) return d == 2 && s.size(0) == blocks(q.size(0)) && s.size(1) == blocks(q.size(1));
+  for (int64_t i = 0; i + 1 < d; ++i)
+    if (q.size(i) != s.size(i)) return false;
+  return s.size(d - 1) == blocks(q.size(d - 1));
+}
+
+std::vector<int64_t> with_last(const at::Tensor& t, int64_t last) {
+  std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
+  shape.back() = last;
+  return shape;
+}
+
+// Room for codes whose rows start on 16-byte boundaries.
+at::Tensor new_codes(const at::Tensor& like) {
+  const int64_t n = like.size(-1), pitch = (n + 15) / 16 * 16;
+  const auto options = like.options().dtype(at::kFloat8_e4m3fn);
+  if (pitch == n) return at::empty(like.sizes(), options);
+  return at::empty(with_last(like, pitch), options).narrow(-1, 0, n);
+}
+int64_t code_pitch(const at::Tensor& q) { return (q.size(-1) + 15) / 16 * 16; }
+
+PyObject* tuple_of(at::Tensor&& a, at::Tensor&& b) {
+  PyObject* t = PyTuple_New(2);
+  if (!t) return nullptr;
+  PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(a)));
+  PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(b)));
+  return t;
+}
+
+// x
+PyObject* quant_rows_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* x = n_args == 1 && quant_rows_f8_fn ? tensor(args[0]) : nullptr;
+    const int device = c10::cuda::current_device();
+    if (!x || !numbers(*x, device)) Py_RETURN_NONE;
+    const int64_t n = x->size(-1), ld = row_stride(*x);
+    if (ld < 0) Py_RETURN_NONE;
+    at::Tensor q = new_codes(*x), s = at::empty(with_last(*x, blocks(n)), x->options().dtype(at::kFloat8_e8m0fnu));
+    if (quant_rows_f8_fn(x->data_ptr(), code(x->scalar_type()), x->numel() / n, n, ld,
+                         static_cast<uint8_t*>(q.data_ptr()), code_pitch(q), static_cast<uint8_t*>(s.data_ptr()),
+                         stream(device)))
+      Py_RETURN_NONE;
+    return tuple_of(std::move(q), std::move(s));
+  });
+}
+
+// w
+PyObject* quant_weight_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor* w = n_args == 1 && quant_weight_f8_fn ? tensor(args[0]) : nullptr;
+    const int device = c10::cuda::current_device();
+    if (!w || !numbers(*w, device) || w->dim() != 2) Py_RETURN_NONE;
+    const int64_t n = w->size(0), k = w->size(1), ld = row_stride(*w);
+    if (ld < 0) Py_RETURN_NONE;
+    at::Tensor q = new_codes(*w), s = at::empty({blocks(n), blocks(k)}, w->options().dtype(at::kFloat8_e8m0fnu));
+    if (quant_weight_f8_fn(w->data_ptr(), code(w->scalar_type()), n, k, ld, static_cast<uint8_t*>(q.data_ptr()),
+                           code_pitch(q), static_cast<uint8_t*>(s.data_ptr()), stream(device)))
+      Py_RETURN_NONE;
+    return tuple_of(std::move(q), std::move(s));
+  });
+}
+
+// The weight and bias of a product over k columns: checked, the weight's row stride and the bias's pointer.
+bool f8_weight(PyObject* qo, PyObject* so, PyObject* bo, int64_t k, int device, const at::Tensor*& q,
+               const at::Tensor*& s, const at::Tensor*& bias, int64_t& ld) {
+  q = tensor(qo);
+  s = tensor(so);
+  bias = bo == Py_None ? nullptr : tensor(bo);
+  if (!q || !s || (!bias && bo != Py_None) || !codes(*q, *s, true, device) || q->size(1) != k) return false;
+  if (bias && (!plain(*bias, device) || bias->dim() != 1 || bias->size(0) != q->size(0) || !bias->is_contiguous() ||
+               code(bias->scalar_type()) < 0))
+    return false;
+  ld = row_stride(*q);
+  return ld > 0;
+}
+at::Tensor workspace(const at::Tensor& like, int64_t bytes) {
+  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+}
+
+// a, a_scale, b, b_scale, bias or None, output dtype
+PyObject* gemm_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 6 || !gemm_f8_fn || !THPDtype_Check(args[5])) Py_RETURN_NONE;
+    const at::Tensor *a = tensor(args[0]), *a_s = tensor(args[1]), *b, *b_s, *bias;
+    const at::ScalarType t = reinterpret_cast<THPDtype*>(args[5])->scalar_type;
+    const int device = c10::cuda::current_device();
+    int64_t ld_b;
+    if (!a || !a_s || code(t) < 0 || !codes(*a, *a_s, false, device)) Py_RETURN_NONE;
+    const int64_t k = a->size(-1), m = a->numel() / k, ld_a = row_stride(*a);
+    if (ld_a < 0 || !f8_weight(args[2], args[3], args[4], k, device, b, b_s, bias, ld_b)) Py_RETURN_NONE;
+    const int64_t n = b->size(0);
+    const auto *ap = static_cast<const uint8_t*>(a->data_ptr()), *bp = static_cast<const uint8_t*>(b->data_ptr());
+    at::Tensor out = at::empty(with_last(*a, n), a->options().dtype(t));
+    const int64_t bytes = gemm_f8_bytes_fn(ap, m, k, ld_a, bp, n, ld_b);
+    at::Tensor ws = workspace(*a, bytes);
+    if (gemm_f8_fn(ap, static_cast<const uint8_t*>(a_s->data_ptr()), m, k, ld_a, bp,
+                   static_cast<const uint8_t*>(b_s->data_ptr()), n, ld_b, bias ? bias->data_ptr() : nullptr,
+                   bias ? code(bias->scalar_type()) : 0, out.data_ptr(), code(t), n, bytes ? ws.data_ptr() : nullptr,
+                   bytes, stream(device)))
+      Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// x, b, b_scale, bias or None
+PyObject* linear_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    const at::Tensor *x = n_args == 4 && linear_f8_fn ? tensor(args[0]) : nullptr, *b, *b_s, *bias;
+    const int device = c10::cuda::current_device();
+    if (!x || !numbers(*x, device)) Py_RETURN_NONE;
+    const int64_t k = x->size(-1), m = x->numel() / k, ld = row_stride(*x);
+    int64_t ld_b;
+    if (ld < 0 || !f8_weight(args[1], args[2], args[3], k, device, b, b_s, bias, ld_b)) Py_RETURN_NONE;
+    const int64_t n = b->size(0);
+    const auto* bp = static_cast<const uint8_t*>(b->data_ptr());
+    at::Tensor out = at::empty(with_last(*x, n), x->options());
+    const int64_t bytes = linear_f8_bytes_fn(m, k, bp, n, ld_b);
+    at::Tensor ws = workspace(*x, bytes);
+    const int dt = code(x->scalar_type());
+    if (linear_f8_fn(x->data_ptr(), dt, m, k, ld, bp, static_cast<const uint8_t*>(b_s->data_ptr()), n, ld_b,
+                     bias ? bias->data_ptr() : nullptr, bias ? code(bias->scalar_type()) : 0, out.data_ptr(), dt, n,
+                     bytes ? ws.data_ptr() : nullptr, bytes, stream(device)))
+      Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
+// The codes and scales of a producer's output mode.
+bool new_output(const at::Tensor& like, int64_t mode, at::Tensor& q, at::Tensor& s) {
+  const int64_t n = like.size(-1);
+  if (mode == QI8_Q_FP8) {
+    q = new_codes(like);
+    s = at::empty(with_last(like, blocks(n)), like.options().dtype(at::kFloat8_e8m0fnu));
+    return true;
+  }
+  if (mode != QI8_Q_TOKEN && (mode != QI8_Q_BLOCK || n % F8_BLOCK)) return false;
+  q = at::empty(like.sizes(), like.options().dtype(at::kChar));
+  s = at::empty(with_last(like, mode == QI8_Q_TOKEN ? 1 : n / F8_BLOCK), like.options().dtype(at::kFloat));
+  return true;
+}
+
+// x, weight or None, eps, residual or None, mode
+PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 5 || !norm_fn || !PyFloat_CheckExact(args[2])) Py_RETURN_NONE;
+    const at::Tensor* x = tensor(args[0]);
+    const at::Tensor* w = args[1] == Py_None ? nullptr : tensor(args[1]);
+    const at::Tensor* r = args[3] == Py_None ? nullptr : tensor(args[3]);
+    const int device = c10::cuda::current_device();
+    if (!x || (!w && args[1] != Py_None) || (!r && args[3] != Py_None) || !numbers(*x, device)) Py_RETURN_NONE;
+    const int64_t n = x->size(-1), ld = row_stride(*x), mode = integer(args[4]);
+    if (ld < 0 || (w && (!plain(*w, device) || w->dim() != 1 || w->size(0) != n || !w->is_contiguous() ||
+                         code(w->scalar_type()) < 0)))
+      Py_RETURN_NONE;
+    if (r && (!plain(*r, device) || r->scalar_type() != x->scalar_type() || r->sizes() != x->sizes())) Py_RETURN_NONE;
+    const int64_t ld_r = r ? row_stride(*r) : 0;
+    at::Tensor q, s, h;
+    if (ld_r < 0 || !new_output(*x, mode, q, s)) Py_RETURN_NONE;
+    if (r) h = at::empty(x->sizes(), x->options());
+    if (norm_fn(x->data_ptr(), code(x->scalar_type()), x->numel() / n, n, ld, r ? r->data_ptr() : nullptr, ld_r,
+                w ? w->data_ptr() : nullptr, w ? code(w->scalar_type()) : 0, PyFloat_AS_DOUBLE(args[2]), (int)mode,
+                q.data_ptr(), mode == QI8_Q_FP8 ? code_pitch(q) : n, s.data_ptr(), r ? h.data_ptr() : nullptr, n,
+                stream(device)))
+      Py_RETURN_NONE;
+    if (!r) return tuple_of(std::move(q), std::move(s));
+    PyObject* t = PyTuple_New(3);
+    if (!t) return nullptr;
+    PyTuple_SET_ITEM(t, 0, THPVariable_Wrap(std::move(q)));
+    PyTuple_SET_ITEM(t, 1, THPVariable_Wrap(std::move(s)));
+    PyTuple_SET_ITEM(t, 2, THPVariable_Wrap(std::move(h)));
+    return t;
+  });
+}
+
+// gate, up, activation code, mode
+PyObject* gated_quant(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 4 || !gated_fn) Py_RETURN_NONE;
+    const at::Tensor *g = tensor(args[0]), *u = tensor(args[1]);
+    const int device = c10::cuda::current_device();
+    if (!g || !u || !numbers(*g, device) || !plain(*u, device) || u->scalar_type() != g->scalar_type() ||
+        u->sizes() != g->sizes())
+      Py_RETURN_NONE;
+    const int64_t n = g->size(-1), ld_g = row_stride(*g), ld_u = row_stride(*u);
+    const int64_t act = integer(args[2]), mode = integer(args[3]);
+    at::Tensor q, s;
+    if (ld_g < 0 || ld_u < 0 || act < 0 || act > QI8_ACT_GELU_TANH || !new_output(*g, mode, q, s)) Py_RETURN_NONE;
+    if (gated_fn(g->data_ptr(), ld_g, u->data_ptr(), ld_u, code(g->scalar_type()), g->numel() / n, n, (int)act, (int)mode,
+                 q.data_ptr(), mode == QI8_Q_FP8 ? code_pitch(q) : n, s.data_ptr(), stream(device)))
+      Py_RETURN_NONE;
+    return tuple_of(std::move(q), std::move(s));
+  });
+}
+
+// addresses of the entry points, in the order of the assignments below
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
-  void* p[5];
-  if (n_args != 5) {
-    PyErr_SetString(PyExc_TypeError, "bind takes five addresses");
+  constexpr int N = 13;
+  void* p[N];
+  if (n_args != N) {
+    PyErr_SetString(PyExc_TypeError, "bind takes thirteen addresses");
     return nullptr;
   }
-  for (int i = 0; i < 5; ++i) {
+  for (int i = 0; i < N; ++i) {
     p[i] = PyLong_AsVoidPtr(args[i]);
     if (PyErr_Occurred()) return nullptr;
   }
-  quant_fn = reinterpret_cast<decltype(quant_fn)>(p[0]);
-  dequant_fn = reinterpret_cast<decltype(dequant_fn)>(p[1]);
-  gemm_fn = reinterpret_cast<decltype(gemm_fn)>(p[2]);
-  moe_fn = reinterpret_cast<decltype(moe_fn)>(p[3]);
-  moe_bytes_fn = reinterpret_cast<decltype(moe_bytes_fn)>(p[4]);
+  int i = 0;
+  auto set = [&](auto& fn) { fn = reinterpret_cast<std::remove_reference_t<decltype(fn)>>(p[i++]); };
+  set(quant_fn);
+  set(dequant_fn);
+  set(gemm_fn);
+  set(moe_fn);
+  set(moe_bytes_fn);
+  set(quant_rows_f8_fn);
+  set(quant_weight_f8_fn);
+  set(gemm_f8_bytes_fn);
+  set(gemm_f8_fn);
+  set(linear_f8_bytes_fn);
+  set(linear_f8_fn);
+  set(norm_fn);
+  set(gated_fn);
   Py_RETURN_NONE;
 }
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
-PyMethodDef methods[] = {FAST(gemm_w4), FAST(quant_weight_i4), FAST(dequant_i4), FAST(moe_w4), FAST(bind),
-                         {nullptr, nullptr, 0, nullptr}};
+PyMethodDef methods[] = {FAST(gemm_w4), FAST(quant_weight_i4), FAST(dequant_i4), FAST(moe_w4), FAST(quant_rows_f8),
+                         FAST(quant_weight_f8), FAST(gemm_f8), FAST(linear_f8), FAST(rms_norm_quant), FAST(gated_quant),
+                         FAST(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

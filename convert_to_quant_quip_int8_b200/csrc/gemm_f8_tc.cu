@@ -389,8 +389,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 namespace few {
 
 constexpr int BM = 128;
-constexpr int EPI_WARPS = 4, SCALE_WARP0 = 4, SCALE_WARPS = 4, PRODUCER = 8, ISSUER = 9;
-constexpr int THREADS = 10 * 32;
+constexpr int EPI_WARPS = 4, SCALE_WARP0 = 4, SCALE_WARPS = 4, PRODUCER = 8, ISSUER0 = 9;
+constexpr int THREADS = 11 * 32;
 constexpr int RING = 216 * 1024, MAX_STAGES = 8;
 constexpr int SCALES = 448, SLOT = 16, SLOTS = 4;  // 8 columns of the tokens, 4 of the weight rows
 constexpr int BARS = 2 * MAX_STAGES + 4 + 2 * SLOTS + 1;
@@ -423,18 +423,29 @@ __device__ __forceinline__ void commit(int one, uint32_t bar) {
 __device__ __forceinline__ void tmem_st1(uint32_t addr, uint32_t r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x1.b32 [%0], {%1};" ::"r"(addr), "r"(r) : "memory");
 }
-__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-  asm volatile("st.shared::cluster.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d)
+__device__ __forceinline__ void st_cluster_f32x4(uint32_t addr, float a, float b, float c, float d) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "f"(a), "f"(b), "f"(c), "f"(d)
                : "memory");
+}
+// 32 columns of an accumulator, or of the two issuers' accumulators
+template <int BN>
+__device__ __forceinline__ void sums(uint32_t at, bool two, float (&y)[32]) {
+  uint32_t v[32], u[32];
+  tmem_ld32(at, v);
+  if (two) tmem_ld32(at + BN, u);
+  tmem_wait_ld();
+#pragma unroll
+  for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(v[j]) + (two ? __uint_as_float(u[j]) : 0.0f);
 }
 
 template <int BN>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ Args p) {
-  constexpr int ACCS = BN == 256 ? 1 : 2;
-  constexpr int KPS = BN == 256 ? 1 : 2;  // K blocks per stage
-  static_assert(ACCS * BN <= SCALES && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && (BN + 64) * 512 <= RING &&
+  constexpr int ISSUERS = BN == 256 ? 1 : 2;  // each with an accumulator of its own
+  constexpr int ACCS = BN >= 128 ? 1 : 2;     // tiles that may be under way
+  constexpr int KPS = BN == 256 ? 1 : 2;      // K blocks per stage
+  static_assert(ACCS * ISSUERS * BN <= SCALES && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && (BN + 64) * 512 <= RING &&
                     SMEM <= 232448, "memories");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
@@ -461,18 +472,18 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       mbar_init(empty_bar(s), 1);
     }
     for (int b = 0; b < 2; ++b) {
-      mbar_init(tfull_bar(b), 1);
+      mbar_init(tfull_bar(b), ISSUERS);
       mbar_init(tempty_bar(b), EPI_WARPS);
     }
     for (int b = 0; b < SLOTS; ++b) {
       mbar_init(sfull_bar(b), SCALE_WARPS);
-      mbar_init(sempty_bar(b), 1);
+      mbar_init(sempty_bar(b), ISSUERS);
     }
-    mbar_init(drain_bar, 1);
+    mbar_init(drain_bar, ISSUERS);
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
-  if (warp == ISSUER) {
+  if (warp == ISSUER0) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
                  "r"(TMEM_COLS)
                  : "memory");
@@ -520,18 +531,28 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         for (int t = 0; t < p.stages; ++t)
           if (issued & (1u << t)) drain_wait(full_bar(t), (issued_ph >> t) & 1u);
     }
-  } else if (warp == ISSUER) {
-    {  // the whole warp, so that addresses and descriptors stay in uniform registers; one lane issues
+  } else if (warp >= ISSUER0) {
+    // the whole warp, so that addresses and descriptors stay in uniform registers; one
+    // lane issues.  Every other stage of a tile is the other warp's
+    const int which = warp - ISSUER0;
+    if (which < ISSUERS) {
       const int one = lane == 0;
       int s = 0, unit = 0;
       uint32_t ph = 0;
+      auto advance = [&](int by) {  // -1 to 2 stages
+        s += by;
+        if (s < 0) s += p.stages, ph ^= 1u;
+        else if (s >= p.stages) s -= p.stages, ph ^= 1u;
+      };
+      advance(which);
       unsigned slot = 0;
       bool ok = true;
       for (int tile = tile0; ok && tile < tiles; tile += tile_step, ++unit) {
         const int buf = unit % ACCS;
         if (!warp_wait(tempty_bar(buf), ((unit / ACCS) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
         tc_fence_after();
-        const uint32_t d = tmem + buf * BN;
+        const uint32_t d = tmem + (buf * ISSUERS + which) * BN;
+        int left = (kn + KPS - 1) / KPS + which;  // stages up to this warp's first of the next tile
         for (int kb = 0; ok && kb < kn; kb += 4, ++slot) {  // one slot of scales
           const uint32_t sb = tmem + SCALES + (slot % SLOTS) * SLOT;
           if (!warp_wait(sfull_bar(slot % SLOTS), (slot / SLOTS) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
@@ -539,7 +560,8 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
             break;
           }
 #pragma unroll
-          for (int h = 0; h < 4; h += KPS) {  // one stage
+          for (int h0 = 0; h0 < 4; h0 += KPS * ISSUERS) {  // one stage
+            const int h = h0 + which * KPS;
             if (kb + h >= kn) break;
             if (!warp_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
               ok = false;
@@ -553,14 +575,16 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
               for (int k = 0; k < BK / 32; ++k)
                 mma(one, d, dw + (uint64_t)(i * (w_bytes >> 4) + 2 * k), dx + (i * BN * BK / 16 + 2 * k),
-                    idesc(BM, BN, h + i), sb + 8, sb, h + i + k > 0 || kb > 0);
+                    idesc(BM, BN, h + i), sb + 8, sb, h0 + i + k > 0 || kb > 0);
             }
             commit(one, empty_bar(s));
-            if (++s == p.stages) s = 0, ph ^= 1u;
+            advance(ISSUERS);
+            left -= ISSUERS;
           }
           if (ok) commit(one, sempty_bar(slot % SLOTS));
         }
         if (ok) commit(one, tfull_bar(buf));
+        if (ISSUERS == 2) advance(left - which);
       }
       commit(one, drain_bar);
       if (one) drain_wait(drain_bar, 0);
@@ -622,15 +646,14 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
         if (warp * 32 < p.rows)
 #pragma unroll 1
           for (int c = 0; c < t1; c += 32) {
-            uint32_t v[32];
-            tmem_ld32(lanes + (uint32_t)(buf * BN + c), v);
-            tmem_wait_ld();
+            float v[32];
+            sums<BN>(lanes + (uint32_t)(buf * ISSUERS * BN + c), kn > KPS && ISSUERS == 2, v);
             if (r < p.rows && n < p.g.N) {
               const int64_t at = (int64_t)(t0 + c) * p.g.ld_out + n;
 #pragma unroll
               for (int j = 0; j < 32; ++j) {
                 if (c + j >= t1) break;
-                store_from_f32(p.g.out, p.g.out_dtype, at + j * p.g.ld_out, __uint_as_float(v[j]) + bias);
+                store_from_f32(p.g.out, p.g.out_dtype, at + j * p.g.ld_out, v[j] + bias);
               }
             }
           }
@@ -655,9 +678,8 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       // rank d finishes tokens [d per, (d + 1) per): sums as [source][row][pitch]
 #pragma unroll 1
       for (int c = 0; c < t1; c += 32) {
-        uint32_t v[32];
-        tmem_ld32(lanes + (uint32_t)c, v);
-        tmem_wait_ld();
+        float v[32];
+        sums<BN>(lanes + (uint32_t)c, kn > KPS && ISSUERS == 2, v);
         if (r < p.rows) {
           int d = c / per, at = c - d * per;
 #pragma unroll
@@ -688,7 +710,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   __syncwarp();
   tc_fence_before();
   __syncthreads();
-  if (warp == ISSUER) {
+  if (warp == ISSUER0) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }

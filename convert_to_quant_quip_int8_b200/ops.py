@@ -727,6 +727,9 @@ def _check_f8(q: torch.Tensor, scale: torch.Tensor, tile: int) -> None:
 
 def quant_rows_f8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """fp8 codes ``[..., n]`` of ``x`` and one scale for each row and 128 columns ``[..., ceil(n / 128)]``."""
+    pair = _fast("quant_rows_f8", x)
+    if pair is not None:
+        return pair
     dev = _one_device(x)
     dt = _float_code(x.dtype, "activations")
     _refuse_grad(x)
@@ -743,6 +746,9 @@ def quant_rows_f8(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
 
 def quant_weight_f8(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """fp8 codes of ``w`` [N, K] (a parameter is read as it is) and one scale for each 128 x 128 tile."""
+    pair = _fast("quant_weight_f8", w)
+    if pair is not None:
+        return pair
     dev = _one_device(w)
     dt = _float_code(w.dtype, "weights")
     assert w.dim() == 2, f"weight of shape {tuple(w.shape)}: expected [N, K]"
@@ -788,6 +794,9 @@ def _no_columns(shape: tuple, n: int, bias: Optional[torch.Tensor], dtype: torch
 def gemm_f8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
             bias: Optional[torch.Tensor] = None, out_dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
     """``a [..., K] b [N, K]^T + bias`` of fp8 operands."""
+    out = _fast("gemm_f8", a, a_scale, b, b_scale, bias, out_dtype)
+    if out is not None:
+        return out
     dev = _one_device(a, a_scale, b, b_scale, bias)
     _refuse_grad(a, a_scale, b, b_scale, bias)
     _check_f8(a, a_scale, 1)
@@ -815,6 +824,9 @@ def gemm_f8(a: torch.Tensor, a_scale: torch.Tensor, b: torch.Tensor, b_scale: to
 def linear_f8(x: torch.Tensor, b: torch.Tensor, b_scale: torch.Tensor,
               bias: Optional[torch.Tensor] = None) -> torch.Tensor:
     """``quantized(x) b^T + bias`` in x's dtype: ``quant_rows_f8`` and ``gemm_f8``."""
+    out = _fast("linear_f8", x, b, b_scale, bias)
+    if out is not None:
+        return out
     dev = _one_device(x, b, b_scale, bias)
     _refuse_grad(x, b, b_scale, bias)
     _check_f8(b, b_scale, 128)
@@ -854,6 +866,9 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: 
                    residual: Optional[torch.Tensor] = None, mode: int = L.QI8_Q_FP8):
     """The root-mean-square norm of ``h = x + residual`` over the last dimension, times ``weight``, quantized:
     ``(q, scale)``, and ``h`` in x's dtype as a third result where there is a residual."""
+    got = _fast("rms_norm_quant", x, weight, eps, residual, mode)
+    if got is not None:
+        return got
     dev = _one_device(x, weight, residual)
     _refuse_grad(x, weight, residual)
     dt = _float_code(x.dtype, "activations")
@@ -886,6 +901,9 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: 
 def gated_quant(gate: torch.Tensor, up: torch.Tensor, act: int = L.QI8_ACT_SILU,
                 mode: int = L.QI8_Q_FP8) -> Tuple[torch.Tensor, torch.Tensor]:
     """``act(gate) * up``, quantized: ``(q, scale)``."""
+    pair = _fast("gated_quant", gate, up, act, mode)
+    if pair is not None:
+        return pair
     dev = _one_device(gate, up)
     _refuse_grad(gate, up)
     dt = _float_code(gate.dtype, "activations")
