@@ -39,7 +39,7 @@ int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st);
 // The kernel for single tokens (gemm_f8_rows.cu), where the tokens fit beside its
 // ring: rows of codes start on 16-byte boundaries.  x (not null): the tokens as
 // numbers of x_dtype, quantized on the way, in place of g.a and g.sa.
-bool gemm_f8_rows_fits(int M, int K);
+bool gemm_f8_rows_fits(int M, int N, int K);
 int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st);
 
 inline int64_t f8_blocks(int64_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }

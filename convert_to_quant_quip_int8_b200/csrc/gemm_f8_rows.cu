@@ -13,7 +13,6 @@
 // scales to set up) and keeps every SM at work at any number of rows, but its steps
 // take 8.3 cycles for 16 rows and 8 tokens, too long for more than 16 of them.
 #include <cstdint>
-#include <cstdlib>
 
 #include "f8.cuh"
 #include "tc05.cuh"
@@ -259,9 +258,14 @@ int launch_tokens(const Args& p, int smem, bool after_quant, cudaStream_t st) {
 }  // namespace f8r
 }  // namespace
 
-bool gemm_f8_rows_fits(int M, int K) {
+// Up to where this kernel is the faster one (1 x 4096 x 4096: 6.1 us, on tcgen05 7.4;
+// 8 x 4096 x 4096 7.1 and 7.5, 16 x 4096 x 4096 10.3 and 7.7, 1 x 10240 x 4096 13.5 and
+// 11.3): every block reads the tokens beside its 16 weight rows, and from 9 tokens on
+// the steps take as long as the loads.
+bool gemm_f8_rows_fits(int M, int N, int K) {
+  if (M > 16 || (int64_t)N * K / 16 * (16 + M) > (M > 8 ? 16000000 : 25500000)) return false;
   int pitch, smem;
-  return M <= 16 && f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) > 0;
+  return f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) > 0;
 }
 
 int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st) {

@@ -392,16 +392,27 @@ constexpr int BM = 128;
 constexpr int EPI_WARPS = 4, SCALE_WARP0 = 4, SCALE_WARPS = 4, PRODUCER = 8, ISSUER0 = 9;
 constexpr int THREADS = 11 * 32;
 constexpr int RING = 216 * 1024, MAX_STAGES = 8;
+constexpr int ISSUERS = 2;                         // each with an accumulator of its own
 constexpr int SCALES = 448, SLOT = 16, SLOTS = 4;  // 8 columns of the tokens, 4 of the weight rows
 constexpr int BARS = 2 * MAX_STAGES + 4 + 2 * SLOTS + 1;
-constexpr int SMEM = 1024 + RING + BARS * 8 + 16;
+constexpr int SMEM = 1024 + RING + BARS * 8 + 16;  // the ring, behind it a split tile's sums
 
 struct Args {
   F8Gemm g;
   int rows, n_tiles, t_tiles, split, stages;
+  int bn;    // tokens of a tile, a multiple of 16
+  int join;  // where the sums of a split tile's blocks meet, from the ring's start
   bool words_a, words_b;
   unsigned int* status;
 };
+
+// K blocks per stage of the ring
+__host__ __device__ constexpr int kps(int bn) { return bn == 128 ? 1 : 2; }
+// The issuer of a tile's first stage: they take turns over all stages.
+template <int KPS>
+__device__ __forceinline__ int first_issuer(int unit, int kn) { return (unit * ((kn + KPS - 1) / KPS)) & 1; }
+// tokens that each block of a split tile finishes
+__host__ __device__ constexpr int join_per(int bn, int split) { return ((bn + split - 1) / split + 3) & ~3; }
 
 __device__ __forceinline__ void mma(int one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                     uint32_t accum) {
@@ -442,15 +453,13 @@ template <int BN>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ Args p) {
-  constexpr int ISSUERS = BN == 256 ? 1 : 2;  // each with an accumulator of its own
-  constexpr int ACCS = BN >= 128 ? 1 : 2;     // tiles that may be under way
-  constexpr int KPS = BN == 256 ? 1 : 2;      // K blocks per stage
-  static_assert(ACCS * ISSUERS * BN <= SCALES && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && (BN + 64) * 512 <= RING &&
-                    SMEM <= 232448, "memories");
+  constexpr int KPS = kps(BN);             // K blocks per stage
+  constexpr int ACCS = BN == 128 ? 1 : 2;  // tiles that may be under way
+  static_assert(ACCS * ISSUERS * BN <= SCALES && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && SMEM <= 232448, "memories");
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* sm = smem_raw + (base - raw);
-  const int w_bytes = p.rows * BK, stage_bytes = KPS * (w_bytes + BN * BK);
+  const int w_bytes = p.rows * BK, x_bytes = p.bn * BK, stage_bytes = KPS * (w_bytes + x_bytes);
   // an MMA reads 128 rows from a stage's weights on, past a smaller tile's into what follows
   const uint32_t sW = base, sX = base + p.stages * KPS * w_bytes;
   uint64_t* bars = reinterpret_cast<uint64_t*>(sm + RING);
@@ -496,6 +505,8 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // waited for where blocks first reach into one another's memory
+  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   pdl_wait();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.n_tiles * p.t_tiles;
@@ -509,7 +520,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       uint32_t ph = 0, issued = 0, issued_ph = 0;
       bool ok = true;
       for (int tile = tile0; ok && tile < tiles; tile += tile_step) {
-        const int n0 = (tile % p.n_tiles) * p.rows, t0 = (tile / p.n_tiles) * BN;
+        const int n0 = (tile % p.n_tiles) * p.rows, t0 = (tile / p.n_tiles) * p.bn;
         for (int kb = kb0; kb < kb1; kb += KPS) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, ST_F8_PRODUCER, WAIT_LIMIT_NS)) {
             ok = false;
@@ -519,7 +530,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
           for (int i = 0; i < KPS; ++i) {  // past the split's last K block too: the stage is whole
             tma_load_2d(sW + (s * KPS + i) * w_bytes, &tmB, (kb + i) * BK, n0, full_bar(s));
-            tma_load_2d(sX + (s * KPS + i) * BN * BK, &tmA, (kb + i) * BK, t0, full_bar(s));
+            tma_load_2d(sX + (s * KPS + i) * x_bytes, &tmA, (kb + i) * BK, t0, full_bar(s));
           }
           issued |= 1u << s;
           issued_ph = (issued_ph & ~(1u << s)) | (ph << s);
@@ -532,68 +543,61 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           if (issued & (1u << t)) drain_wait(full_bar(t), (issued_ph >> t) & 1u);
     }
   } else if (warp >= ISSUER0) {
-    // the whole warp, so that addresses and descriptors stay in uniform registers; one
-    // lane issues.  Every other stage of a tile is the other warp's
+    // The whole warp, so that addresses and descriptors stay in uniform registers; one
+    // lane issues.  Each issuer has every other stage of the ring, and so sees every
+    // phase of its stages' barriers.
     const int which = warp - ISSUER0;
-    if (which < ISSUERS) {
-      const int one = lane == 0;
-      int s = 0, unit = 0;
-      uint32_t ph = 0;
-      auto advance = [&](int by) {  // -1 to 2 stages
-        s += by;
-        if (s < 0) s += p.stages, ph ^= 1u;
-        else if (s >= p.stages) s -= p.stages, ph ^= 1u;
-      };
-      advance(which);
-      unsigned slot = 0;
-      bool ok = true;
-      for (int tile = tile0; ok && tile < tiles; tile += tile_step, ++unit) {
-        const int buf = unit % ACCS;
-        if (!warp_wait(tempty_bar(buf), ((unit / ACCS) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
-        tc_fence_after();
-        const uint32_t d = tmem + (buf * ISSUERS + which) * BN;
-        int left = (kn + KPS - 1) / KPS + which;  // stages up to this warp's first of the next tile
-        for (int kb = 0; ok && kb < kn; kb += 4, ++slot) {  // one slot of scales
-          const uint32_t sb = tmem + SCALES + (slot % SLOTS) * SLOT;
-          if (!warp_wait(sfull_bar(slot % SLOTS), (slot / SLOTS) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
+    const int one = lane == 0;
+    int s = which, unit = 0;
+    uint32_t ph = 0;
+    unsigned slot = 0;
+    bool ok = true;
+    for (int tile = tile0; ok && tile < tiles; tile += tile_step, ++unit) {
+      const int buf = unit % ACCS;
+      if (!warp_wait(tempty_bar(buf), ((unit / ACCS) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+      tc_fence_after();
+      const uint32_t d = tmem + (buf * ISSUERS + which) * BN;
+      const int first = (which ^ first_issuer<KPS>(unit, kn)) * KPS;  // K block of this issuer's first stage
+      uint32_t sums_there = 0;
+      for (int kb = 0; ok && kb < kn; kb += 4, ++slot) {  // one slot of scales
+        const uint32_t sb = tmem + SCALES + (slot % SLOTS) * SLOT;
+        if (!warp_wait(sfull_bar(slot % SLOTS), (slot / SLOTS) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
+          ok = false;
+          break;
+        }
+#pragma unroll
+        for (int h0 = 0; h0 < 4; h0 += KPS * ISSUERS) {  // one stage
+          const int h = h0 + first;
+          if (kb + h >= kn) break;
+          if (!warp_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
             ok = false;
             break;
           }
+          tc_fence_after();
+          const uint64_t dw = sw128_desc(sW + s * KPS * w_bytes), dx = sw128_desc(sX + s * KPS * x_bytes);
 #pragma unroll
-          for (int h0 = 0; h0 < 4; h0 += KPS * ISSUERS) {  // one stage
-            const int h = h0 + which * KPS;
-            if (kb + h >= kn) break;
-            if (!warp_wait(full_bar(s), ph, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            const uint64_t dw = sw128_desc(sW + s * KPS * w_bytes), dx = sw128_desc(sX + s * KPS * BN * BK);
+          for (int i = 0; i < KPS; ++i) {
+            if (kb + h + i >= kn) break;
 #pragma unroll
-            for (int i = 0; i < KPS; ++i) {
-              if (kb + h + i >= kn) break;
-#pragma unroll
-              for (int k = 0; k < BK / 32; ++k)
-                mma(one, d, dw + (uint64_t)(i * (w_bytes >> 4) + 2 * k), dx + (i * BN * BK / 16 + 2 * k),
-                    idesc(BM, BN, h + i), sb + 8, sb, h0 + i + k > 0 || kb > 0);
-            }
-            commit(one, empty_bar(s));
-            advance(ISSUERS);
-            left -= ISSUERS;
+            for (int k = 0; k < BK / 32; ++k)
+              mma(one, d, dw + (uint64_t)(i * (w_bytes >> 4) + 2 * k), dx + (uint64_t)(i * (x_bytes >> 4) + 2 * k),
+                  idesc(BM, p.bn, h + i), sb + 8, sb, i + k > 0 ? 1u : sums_there);
           }
-          if (ok) commit(one, sempty_bar(slot % SLOTS));
+          sums_there = 1;
+          commit(one, empty_bar(s));
+          if ((s += ISSUERS) >= p.stages) s = which, ph ^= 1u;
         }
-        if (ok) commit(one, tfull_bar(buf));
-        if (ISSUERS == 2) advance(left - which);
+        if (ok) commit(one, sempty_bar(slot % SLOTS));
       }
-      commit(one, drain_bar);
-      if (one) drain_wait(drain_bar, 0);
+      if (ok) commit(one, tfull_bar(buf));
     }
+    commit(one, drain_bar);
+    if (one) drain_wait(drain_bar, 0);
   } else if (warp >= SCALE_WARP0) {
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + SCALES;
     const int last = (p.g.N - 1) / F8_BLOCK;
     auto load = [&](int tile, int kb, uint32_t (&w)[4], uint32_t (&x)[BN / 32]) {
-      const int n0 = (tile % p.n_tiles) * p.rows, t0 = (tile / p.n_tiles) * BN;
+      const int n0 = (tile % p.n_tiles) * p.rows, t0 = (tile / p.n_tiles) * p.bn;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         w[i] = scale_word(p.g.sb + (int64_t)min((n0 + 32 * i + lane) / F8_BLOCK, last) * KB, kb, KB,
@@ -636,18 +640,20 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
     const int r = warp * 32 + lane;
     for (int tile = tile0; tile < tiles; tile += tile_step, ++unit) {
-      const int n = (tile % p.n_tiles) * p.rows + r, t0 = (tile / p.n_tiles) * BN;
+      const int n = (tile % p.n_tiles) * p.rows + r, t0 = (tile / p.n_tiles) * p.bn;
       const int buf = unit % ACCS;
       const float bias = p.g.bias && n < p.g.N ? load_as_f32(p.g.bias, p.g.bias_dtype, n) : 0.0f;
       if (!warp_wait(tfull_bar(buf), (unit / ACCS) & 1, abort_flag, p.status, ST_F8_EPILOGUE, WAIT_LIMIT_NS)) break;
       tc_fence_after();
       if (split == 1) {
-        const int t1 = min(BN, p.g.M - t0);
+        const int t1 = min(p.bn, p.g.M - t0);
+        // of a tile of one stage one accumulator has sums
+        const int acc0 = (buf * ISSUERS + (kn > KPS ? 0 : first_issuer<KPS>(unit, kn))) * BN;
         if (warp * 32 < p.rows)
 #pragma unroll 1
           for (int c = 0; c < t1; c += 32) {
             float v[32];
-            sums<BN>(lanes + (uint32_t)(buf * ISSUERS * BN + c), kn > KPS && ISSUERS == 2, v);
+            sums<BN>(lanes + (uint32_t)(acc0 + c), kn > KPS, v);
             if (r < p.rows && n < p.g.N) {
               const int64_t at = (int64_t)(t0 + c) * p.g.ld_out + n;
 #pragma unroll
@@ -665,13 +671,12 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   }
 
   if (split > 1) {
-    // one tile per cluster; every block's MMAs are done with its ring: the sums go there
+    // one tile per cluster
     __syncwarp();
-    tc_fence_before();
-    cluster_sync();
+    asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     tc_fence_after();
-    const int n0 = (tile0 % p.n_tiles) * p.rows, t0 = (tile0 / p.n_tiles) * BN, t1 = min(BN, p.g.M - t0);
-    const int per = ((BN + split - 1) / split + 3) & ~3, pitch = per + 4;  // tokens per rank; padded against conflicts
+    const int n0 = (tile0 % p.n_tiles) * p.rows, t0 = (tile0 / p.n_tiles) * p.bn, t1 = min(p.bn, p.g.M - t0);
+    const int per = join_per(p.bn, split), pitch = per + 4;  // tokens per rank; padded against conflicts
     if (warp < EPI_WARPS && __all_sync(0xffffffffu, !*abort_flag)) {
       const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
       const int r = warp * 32 + lane;
@@ -679,12 +684,13 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll 1
       for (int c = 0; c < t1; c += 32) {
         float v[32];
-        sums<BN>(lanes + (uint32_t)c, kn > KPS && ISSUERS == 2, v);
+        sums<BN>(lanes + (uint32_t)c, kn > KPS, v);
         if (r < p.rows) {
           int d = c / per, at = c - d * per;
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
-            st_cluster_f32x4(mapa(base + (uint32_t)(((rank * BM + r) * pitch + at) * 4), (uint32_t)d), v[j], v[j + 1],
+            if (c + j >= p.bn) break;  // past the last rank's
+            st_cluster_f32x4(mapa(base + (uint32_t)(p.join + ((rank * BM + r) * pitch + at) * 4), (uint32_t)d), v[j], v[j + 1],
                              v[j + 2], v[j + 3]);
             if ((at += 4) >= per) at -= per, ++d;
           }
@@ -695,7 +701,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     tc_fence_before();
     cluster_sync();
     tc_fence_after();
-    const float* part = reinterpret_cast<const float*>(sm);
+    const float* part = reinterpret_cast<const float*>(sm + p.join);
     for (int i = threadIdx.x; i < per * BM; i += THREADS) {
       const int r = i & (BM - 1), c = i / BM;
       const int t = rank * per + c, n = n0 + r;
@@ -775,12 +781,15 @@ int launch_few(const F8Gemm& g, int rows, int split, bool after_quant, cudaStrea
     QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few::SMEM));
     if (dev < 64) done[dev] = true;
   }
+  const int t_tiles = (g.M + BN - 1) / BN, bn = ((g.M + t_tiles - 1) / t_tiles + 15) & ~15;
   CUtensorMap ma, mb;
-  if (int rc = code_map8(&ma, g.a, g.M, g.K, g.ld_a, BN)) return rc;
+  if (int rc = code_map8(&ma, g.a, g.M, g.K, g.ld_a, bn)) return rc;
   if (int rc = code_map8(&mb, g.b, g.N, g.K, g.ld_b, rows)) return rc;
-  int stages = few::RING / ((BN == 256 ? 1 : 2) * (rows + BN) * BK);
+  const int join = split > 1 ? split * few::BM * (few::join_per(bn, split) + 4) * 4 : 0;
+  int stages = (few::RING - join) / (few::kps(BN) * (rows + bn) * BK) / few::ISSUERS * few::ISSUERS;
   if (stages > few::MAX_STAGES) stages = few::MAX_STAGES;
-  few::Args p{g, rows, (g.N + rows - 1) / rows, (g.M + BN - 1) / BN, split, stages, word_rows(g.sa, g.KB),
+  QI8_REQUIRE(stages >= few::ISSUERS, QI8_ESHAPE, "no room for two stages");
+  few::Args p{g, rows, (g.N + rows - 1) / rows, t_tiles, split, stages, bn, few::RING - join, word_rows(g.sa, g.KB),
               word_rows(g.sb, g.KB), device_status_ptr()};
   const int64_t tiles = (int64_t)p.n_tiles * p.t_tiles;
   QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
@@ -804,22 +813,38 @@ int launch_few(const F8Gemm& g, int rows, int split, bool after_quant, cudaStrea
 }  // namespace
 
 int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st) {
-  const char* e = getenv("F8_TUNE");
-  if (e) {
-    int bn, rows, split;
-    if (sscanf(e, "%d,%d,%d", &bn, &rows, &split) == 3 && bn > 0) {
-      if (bn == 32) return f8tc::launch_few<32>(g, rows, split, after_quant, st);
-      if (bn == 64) return f8tc::launch_few<64>(g, rows, split, after_quant, st);
-      if (bn == 128) return f8tc::launch_few<128>(g, rows, split, after_quant, st);
-      return f8tc::launch_few<256>(g, rows, split, after_quant, st);
-    }
-    return f8tc::launch_pair(g, after_quant, st);
+  using namespace f8tc;
+  const int sms = sm_count();
+  // Tiles of 128 weight rows and up to 128 tokens, as far as one wave of blocks goes:
+  // 512 x 4096 x 4096 takes 15.1 us so and 16.3 in tiles of 256 x 256, 512 x 10240 x
+  // 4096 (320 tiles) 37 and 30.  Up to 128 tokens half of a 256-token tile would be empty.
+  const int64_t t_tiles = ((int64_t)g.M + 127) / 128, n_tiles = ((int64_t)g.N + 127) / 128;
+  if (g.M > 128 && n_tiles * t_tiles > sms) return launch_pair(g, after_quant, st);
+  // Blocks that share a tile's K: a K block takes about 0.19 us up to 64 tokens and 0.3
+  // with 128, the join 0.8 us and 0.05 for each token
+  const int bn = (int)((g.M + t_tiles - 1) / t_tiles + 15) & ~15;
+  const double block_us = bn <= 64 ? 0.19 : 0.19 + 0.0017 * (bn - 64), join_us = 0.8 + 0.05 * bn;
+  int split = 1;
+  double best = g.KB * block_us;
+  for (int s = 2; s <= 4 && s <= g.KB && n_tiles * t_tiles * s <= sms; ++s) {
+    const double us = (g.KB + s - 1) / s * block_us + join_us;
+    if (us < best) best = us, split = s;
   }
-  if (g.M <= 32) return f8tc::launch_few<32>(g, 128, 2, after_quant, st);
-  if (g.M <= 64) return f8tc::launch_few<64>(g, 64, 1, after_quant, st);
-  if (g.M <= 128) return f8tc::launch_few<128>(g, 128, 3, after_quant, st);
-  if (g.M <= 256) return f8tc::launch_few<256>(g, 72, 1, after_quant, st);
-  return f8tc::launch_pair(g, after_quant, st);
+  // as few rows per tile as spread them over the SMs in as many waves
+  const int64_t waves = (n_tiles * t_tiles * split + sms - 1) / sms, most = waves * sms / (t_tiles * split);
+  int rows = (int)(((int64_t)g.N + most - 1) / most + 15) & ~15;
+  if (rows < 32) rows = 32;
+  if (rows > 128) rows = 128;
+  if (const char* e = getenv("F8_TUNE")) {
+    int b;
+    if (sscanf(e, "%d,%d,%d", &b, &rows, &split) != 3) return launch_pair(g, after_quant, st);
+    if (b == 32) return launch_few<32>(g, rows, split, after_quant, st);
+    if (b == 64) return launch_few<64>(g, rows, split, after_quant, st);
+    return launch_few<128>(g, rows, split, after_quant, st);
+  }
+  if (g.M <= 32) return launch_few<32>(g, rows, split, after_quant, st);
+  if (g.M <= 64) return launch_few<64>(g, rows, split, after_quant, st);
+  return launch_few<128>(g, rows, split, after_quant, st);
 }
 
 }  // namespace qi8

@@ -158,6 +158,29 @@ def test_gemm(m, n, k, out):
     check_product(y, values(a, a_s, 1), values(b, b_s, 128), bias)
 
 
+# more tiles than blocks: the rings, scales and accumulators go round
+@pytest.mark.parametrize("m,n,k", [(17, 20000, 300), (32, 40000, 1100), (50, 20100, 640), (64, 30000, 129),
+                                   (100, 20000, 640), (100, 33000, 4096), (128, 24000, 130), (300, 20000, 384),
+                                   (2000, 5000, 640), (4100, 2600, 1300)])
+def test_gemm_with_many_tiles(m, n, k):
+    a, a_s = F8.act_quant_fp8(wide(m, k, seed=m))
+    b, b_s = F8.weight_quant_fp8(wide(n, k, seed=n))
+    va, vb = values(a, a_s, 1), values(b, b_s, 128)
+    for _ in range(3):
+        check_product(F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32), va, vb)
+
+
+# few tiles of many columns: blocks that share them
+@pytest.mark.parametrize("m", [1, 16, 17, 40, 65, 100, 128, 200])
+@pytest.mark.parametrize("n,k", [(100, 16384), (520, 8200), (2050, 4000), (4096, 4096), (4000, 10240)])
+def test_gemm_with_split_columns(m, n, k):
+    a, a_s = F8.act_quant_fp8(wide(m, k, seed=m))
+    b, b_s = F8.weight_quant_fp8(wide(n, k, seed=n))
+    y = F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)
+    check_product(y, values(a, a_s, 1), values(b, b_s, 128))
+    assert all(torch.equal(y, F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)) for _ in range(3))
+
+
 @pytest.mark.parametrize("m,n,k", SHAPES)
 @pytest.mark.parametrize("dtype", [BF, HF, F32])
 def test_linear(m, n, k, dtype):
