@@ -2,7 +2,6 @@
 //
 //   out[t, n] = sum_kb 2^(ea[t, kb] + eb[n / 128, kb]) sum_{k in kb} a[t, k] b[n, k] + bias[n]
 #include <cstdint>
-#include <cstdlib>
 
 #include "f8.cuh"
 
@@ -99,7 +98,7 @@ extern "C" int qi8_gemm_f8(const uint8_t* a, const uint8_t* a_scale, int64_t M, 
   if (int rc = f8g::align_rows(b, N, K, ld_b, ws, st)) return rc;
   const F8Gemm g{a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
                  bias_dtype, out_dtype};
-  if (gemm_f8_rows_fits((int)M, (int)N, (int)K) && !getenv("F8_TUNE")) return gemm_f8_rows(g, nullptr, 0, 0, false, st);
+  if (gemm_f8_rows_fits((int)M, (int)N, (int)K)) return gemm_f8_rows(g, nullptr, 0, 0, false, st);
   return gemm_f8_tiles(g, false, st);
 }
 
@@ -128,9 +127,9 @@ extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, i
   // Quantized by each block itself, the tokens cost a launch less, but every block the
   // work: 1 x 4096 x 4096 takes 6.1 us so and 6.7 with a kernel for it, two tokens 6.8 and
   // 6.7, four 8.4 and 7.0.
-  if (gemm_f8_rows_fits((int)M, (int)N, (int)K) && M * K <= 8192 && !getenv("F8_PRE"))
+  if (gemm_f8_rows_fits((int)M, (int)N, (int)K) && M * K <= 8192)
     return gemm_f8_rows(g, x, x_dtype, ld_x, false, st);
   if (int rc = quant_rows_f8(x, x_dtype, M, K, ld_x, q, f8g::pitch(K), s, st)) return rc;
-  if (gemm_f8_rows_fits((int)M, (int)N, (int)K) && !getenv("F8_TUNE")) return gemm_f8_rows(g, nullptr, 0, 0, true, st);
+  if (gemm_f8_rows_fits((int)M, (int)N, (int)K)) return gemm_f8_rows(g, nullptr, 0, 0, true, st);
   return gemm_f8_tiles(g, true, st);
 }

@@ -8,8 +8,6 @@
 // memory, so the four steps of a 128-block read the same byte.  The sums stay in
 // the accumulator over all of K.
 #include <cstdint>
-#include <cstdio>
-#include <cstdlib>
 
 #include "f8.cuh"
 #include "tc05.cuh"
@@ -413,6 +411,9 @@ template <int KPS>
 __device__ __forceinline__ int first_issuer(int unit, int kn) { return (unit * ((kn + KPS - 1) / KPS)) & 1; }
 // tokens that each block of a split tile finishes
 __host__ __device__ constexpr int join_per(int bn, int split) { return ((bn + split - 1) / split + 3) & ~3; }
+// Their row's length in memory: an odd number of 16-byte pieces, so that eight rows
+// touch all banks.  (With 32 words a row the join of four blocks took 16 us.)
+__host__ __device__ constexpr int join_pitch(int bn, int split) { return join_per(bn, split) | 4; }
 
 __device__ __forceinline__ void mma(int one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                     uint32_t accum) {
@@ -676,7 +677,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     tc_fence_after();
     const int n0 = (tile0 % p.n_tiles) * p.rows, t0 = (tile0 / p.n_tiles) * p.bn, t1 = min(p.bn, p.g.M - t0);
-    const int per = join_per(p.bn, split), pitch = per + 4;  // tokens per rank; padded against conflicts
+    const int per = join_per(p.bn, split), pitch = join_pitch(p.bn, split);
     if (warp < EPI_WARPS && __all_sync(0xffffffffu, !*abort_flag)) {
       const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
       const int r = warp * 32 + lane;
@@ -702,14 +703,22 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     cluster_sync();
     tc_fence_after();
     const float* part = reinterpret_cast<const float*>(sm + p.join);
-    for (int i = threadIdx.x; i < per * BM; i += THREADS) {
-      const int r = i & (BM - 1), c = i / BM;
+    for (int i = threadIdx.x; i < per / 4 * BM; i += THREADS) {  // four tokens of a row
+      const int r = i & (BM - 1), c = i / BM * 4;
       const int t = rank * per + c, n = n0 + r;
       if (t >= t1 || r >= p.rows || n >= p.g.N) continue;
-      float y = 0.0f;
-      for (int s = 0; s < split; ++s) y += part[(s * BM + r) * pitch + c];
-      if (p.g.bias) y += load_as_f32(p.g.bias, p.g.bias_dtype, n);
-      store_from_f32(p.g.out, p.g.out_dtype, (int64_t)(t0 + t) * p.g.ld_out + n, y);
+      float y[4] = {0, 0, 0, 0};
+      for (int s = 0; s < split; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(part + (s * BM + r) * pitch + c);
+        y[0] += v.x;
+        y[1] += v.y;
+        y[2] += v.z;
+        y[3] += v.w;
+      }
+      const float bias = p.g.bias ? load_as_f32(p.g.bias, p.g.bias_dtype, n) : 0.0f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (t + j < t1) store_from_f32(p.g.out, p.g.out_dtype, (int64_t)(t0 + t + j) * p.g.ld_out + n, y[j] + bias);
     }
   }
 
@@ -776,7 +785,6 @@ int launch_few(const F8Gemm& g, int rows, int split, bool after_quant, cudaStrea
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
   auto kern = few::gemm_f8_few_kernel<BN>;
-  if (split > g.KB) split = g.KB;
   if (dev >= 64 || !done[dev]) {
     QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few::SMEM));
     if (dev < 64) done[dev] = true;
@@ -785,7 +793,7 @@ int launch_few(const F8Gemm& g, int rows, int split, bool after_quant, cudaStrea
   CUtensorMap ma, mb;
   if (int rc = code_map8(&ma, g.a, g.M, g.K, g.ld_a, bn)) return rc;
   if (int rc = code_map8(&mb, g.b, g.N, g.K, g.ld_b, rows)) return rc;
-  const int join = split > 1 ? split * few::BM * (few::join_per(bn, split) + 4) * 4 : 0;
+  const int join = split > 1 ? split * few::BM * few::join_pitch(bn, split) * 4 : 0;
   int stages = (few::RING - join) / (few::kps(BN) * (rows + bn) * BK) / few::ISSUERS * few::ISSUERS;
   if (stages > few::MAX_STAGES) stages = few::MAX_STAGES;
   QI8_REQUIRE(stages >= few::ISSUERS, QI8_ESHAPE, "no room for two stages");
@@ -816,34 +824,32 @@ int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st) {
   using namespace f8tc;
   const int sms = sm_count();
   // Tiles of 128 weight rows and up to 128 tokens, as far as one wave of blocks goes:
-  // 512 x 4096 x 4096 takes 15.1 us so and 16.3 in tiles of 256 x 256, 512 x 10240 x
-  // 4096 (320 tiles) 37 and 30.  Up to 128 tokens half of a 256-token tile would be empty.
+  // 512 x 4096 x 4096 takes 14.5 us so and 16.2 in tiles of 256 x 256, 512 x 10240 x
+  // 4096 (320 tiles) 37 and 30.  Up to 128 tokens half of a 256-token tile would be
+  // empty: 100 x 32768 x 4096 takes 30.1 us so and 32.5 in those.
   const int64_t t_tiles = ((int64_t)g.M + 127) / 128, n_tiles = ((int64_t)g.N + 127) / 128;
   if (g.M > 128 && n_tiles * t_tiles > sms) return launch_pair(g, after_quant, st);
-  // Blocks that share a tile's K: a K block takes about 0.19 us up to 64 tokens and 0.3
-  // with 128, the join 0.8 us and 0.05 for each token
+  // Blocks that share a tile's K: a K block takes about 0.19 us up to 64 tokens and 0.24
+  // with 128, the join 0.5 us and 0.012 for each token and block (fitted to 17 shapes of
+  // 9 to 700 tokens; 100 x 4096 x 4096 takes 12.5 us with whole tiles, 11.5 with two blocks
+  // each, 16 x 4096 x 4096 9.2 and, with four, 7.3).  Of clusters of two 74 run at once, of
+  // three 45, of four 33, of eight 15.
   const int bn = (int)((g.M + t_tiles - 1) / t_tiles + 15) & ~15;
-  const double block_us = bn <= 64 ? 0.19 : 0.19 + 0.0017 * (bn - 64), join_us = 0.8 + 0.05 * bn;
-  int split = 1;
+  const double block_us = bn <= 64 ? 0.19 : 0.19 + 0.0008 * (bn - 64);
+  int split = 1, room = sms;
   double best = g.KB * block_us;
-  for (int s = 2; s <= 4 && s <= g.KB && n_tiles * t_tiles * s <= sms; ++s) {
-    const double us = (g.KB + s - 1) / s * block_us + join_us;
-    if (us < best) best = us, split = s;
+  for (int s : {2, 3, 4, 8}) {
+    const int there = s == 2 ? sms : s == 8 ? sms * 13 / 16 : sms * 57 / 64;
+    const double us = (g.KB + s - 1) / s * block_us + 0.5 + 0.012 * bn * s;
+    if (s <= g.KB && n_tiles * t_tiles * s <= there && us < best) best = us, split = s, room = there;
   }
   // as few rows per tile as spread them over the SMs in as many waves
-  const int64_t waves = (n_tiles * t_tiles * split + sms - 1) / sms, most = waves * sms / (t_tiles * split);
+  const int64_t waves = (n_tiles * t_tiles * split + room - 1) / room, most = waves * room / (t_tiles * split);
+  const int least = split > 1 ? 64 : 32;
   int rows = (int)(((int64_t)g.N + most - 1) / most + 15) & ~15;
-  if (rows < 32) rows = 32;
-  if (rows > 128) rows = 128;
-  if (const char* e = getenv("F8_TUNE")) {
-    int b;
-    if (sscanf(e, "%d,%d,%d", &b, &rows, &split) != 3) return launch_pair(g, after_quant, st);
-    if (b == 32) return launch_few<32>(g, rows, split, after_quant, st);
-    if (b == 64) return launch_few<64>(g, rows, split, after_quant, st);
-    return launch_few<128>(g, rows, split, after_quant, st);
-  }
-  if (g.M <= 32) return launch_few<32>(g, rows, split, after_quant, st);
-  if (g.M <= 64) return launch_few<64>(g, rows, split, after_quant, st);
+  rows = rows < least ? least : rows > 128 ? 128 : rows;
+  if (bn <= 32) return launch_few<32>(g, rows, split, after_quant, st);
+  if (bn <= 64) return launch_few<64>(g, rows, split, after_quant, st);
   return launch_few<128>(g, rows, split, after_quant, st);
 }
 
