@@ -153,7 +153,7 @@ def fast_call():
                 lib.qi8_quant_weight_i4, lib.qi8_dequant_i4, lib.qi8_gemm_w4, lib.qi8_moe_w4,
                 lib.qi8_moe_w4_workspace_bytes, lib.qi8_quant_rows_f8, lib.qi8_quant_weight_f8,
                 lib.qi8_gemm_f8_workspace_bytes, lib.qi8_gemm_f8, lib.qi8_linear_f8_workspace_bytes, lib.qi8_linear_f8,
-                lib.qi8_rms_norm_quant, lib.qi8_gated_quant)))
+                lib.qi8_rms_norm_quant, lib.qi8_gated_quant, lib.qi8_dequant)))
             _call = mod
     return _call or None
 

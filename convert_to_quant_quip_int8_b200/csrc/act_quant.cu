@@ -207,6 +207,7 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const __grid_constant_
   int64_t row = blockIdx.x * per + mine;
   const bool live = row < p.rows;
   if (!live) row = p.rows - 1;  // takes part in the barriers
+  wait_for_last_kernel();
   F8x y[CHUNKS];
   row_values<T, OP>(p, row, col0, step, y);
   if constexpr (OP == NORM) {
@@ -258,6 +259,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_con
   __shared__ uint32_t tops[32];
   constexpr int STEP = LONG_THREADS * 8;
   const int64_t row = blockIdx.x, col0 = threadIdx.x * 8;
+  wait_for_last_kernel();
   float rstd = 1.0f;
   F8x y[1];
   if constexpr (OP == NORM) {
@@ -311,12 +313,12 @@ constexpr int THREADS = 256;
 
 template <typename T, int OP, int STEPS>
 __global__ void __launch_bounds__(THREADS) block_kernel(const __grid_constant__ Args p, const unsigned groups) {
-  pdl_launch_dependents();  // the product behind it prepares itself
   const int lane = threadIdx.x & 31;
   const unsigned unit = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
   const unsigned row = unit / groups;
   if (row >= p.rows) return;
   const int64_t col0 = (int64_t)(unit - row * groups) * (STEPS * 256) + lane * 8;
+  wait_for_last_kernel();
   F8x y[STEPS];
   row_values<T, OP>(p, row, col0, 256, y);
 #pragma unroll
@@ -331,17 +333,17 @@ template <typename T, int OP, int STEPS>
 int launch_blocks(const Args& p, cudaStream_t st) {
   const int64_t groups = (p.blocks + 2 * STEPS - 1) / (2 * STEPS), units = p.rows * groups;
   QI8_REQUIRE(units < (1ll << 32) - THREADS, QI8_ESHAPE, "%lld rows of %lld", (long long)p.rows, (long long)p.n);
-  block_kernel<T, OP, STEPS><<<(unsigned)((units + THREADS / 32 - 1) / (THREADS / 32)), THREADS, 0, st>>>(
-      p, (unsigned)groups);
-  return check_cuda(cudaGetLastError(), "block_kernel launch");
+  return launch_early("block_kernel launch", block_kernel<T, OP, STEPS>,
+                      dim3((unsigned)((units + THREADS / 32 - 1) / (THREADS / 32))), THREADS, 0, 1, st, p,
+                      (unsigned)groups);
 }
 
 template <typename T, int OP, int CHUNKS>
 int launch_rows(const Args& p, cudaStream_t st) {
   const int warps = (int)((p.n + 256 * CHUNKS - 1) / (256 * CHUNKS));
   const int per = warps >= 8 ? 1 : 8 / warps;  // rows per thread block
-  row_kernel<T, OP, CHUNKS><<<(unsigned)((p.rows + per - 1) / per), warps * per * 32, 0, st>>>(p, warps);
-  return check_cuda(cudaGetLastError(), "row_kernel launch");
+  return launch_early("row_kernel launch", row_kernel<T, OP, CHUNKS>, dim3((unsigned)((p.rows + per - 1) / per)),
+                      warps * per * 32, 0, 1, st, p, warps);
 }
 
 template <typename T, int OP>
@@ -356,8 +358,8 @@ int launch_type(const Args& p, cudaStream_t st) {
     if (p.n <= 1024) return launch_rows<T, OP, 1>(p, st);
     if (p.n <= 8192) return launch_rows<T, OP, 2>(p, st);
     if (p.n <= 16384) return launch_rows<T, OP, 4>(p, st);
-    long_row_kernel<T, OP><<<(unsigned)p.rows, LONG_THREADS, 0, st>>>(p);
-    return check_cuda(cudaGetLastError(), "long_row_kernel launch");
+    return launch_early("long_row_kernel launch", long_row_kernel<T, OP>, dim3((unsigned)p.rows), LONG_THREADS, 0, 1, st,
+                        p);
   }
   return QI8_OK;
 }

@@ -35,6 +35,7 @@ decltype(&qi8_linear_f8_workspace_bytes) linear_f8_bytes_fn;
 decltype(&qi8_linear_f8) linear_f8_fn;
 decltype(&qi8_rms_norm_quant) norm_fn;
 decltype(&qi8_gated_quant) gated_fn;
+decltype(&qi8_dequant) dequant8_fn;
 
 int code(at::ScalarType t) {
   return t == at::kBFloat16 ? QI8_BF16 : t == at::kHalf ? QI8_F16 : t == at::kFloat ? QI8_F32 : -1;
@@ -427,12 +428,37 @@ PyObject* gated_quant(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   });
 }
 
+// q int8, scale, kind, block, output dtype: the int8 outputs of the two above, read back
+PyObject* dequant(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+  return guarded([&]() -> PyObject* {
+    if (n_args != 5 || !dequant8_fn || !THPDtype_Check(args[4])) Py_RETURN_NONE;
+    const at::Tensor *q = tensor(args[0]), *s = tensor(args[1]);
+    const at::ScalarType t = reinterpret_cast<THPDtype*>(args[4])->scalar_type;
+    const int device = c10::cuda::current_device();
+    const int64_t kind = integer(args[2]), block = integer(args[3]);
+    if (!q || !s || code(t) < 0 || !plain(*q, device) || !plain(*s, device) || q->scalar_type() != at::kChar ||
+        s->scalar_type() != at::kFloat || q->dim() < 1 || q->numel() == 0 || !q->is_contiguous() || !s->is_contiguous())
+      Py_RETURN_NONE;
+    const int64_t n = q->size(-1), rows = q->numel() / n;
+    // as many scales as the kernel reads
+    if (kind == QI8_S_SCALAR ? s->numel() < 1
+        : kind == QI8_S_ROW ? s->numel() != rows
+                            : kind != QI8_S_ROW_KBLOCK || block <= 0 || n % block || s->numel() != rows * (n / block))
+      Py_RETURN_NONE;
+    at::Tensor out = at::empty(q->sizes(), q->options().dtype(t));
+    if (dequant8_fn(static_cast<const int8_t*>(q->data_ptr()), rows, n, static_cast<const float*>(s->data_ptr()),
+                    (int)kind, (int)block, out.data_ptr(), code(t), stream(device)))
+      Py_RETURN_NONE;
+    return THPVariable_Wrap(std::move(out));
+  });
+}
+
 // addresses of the entry points, in the order of the assignments below
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
-  constexpr int N = 13;
+  constexpr int N = 14;
   void* p[N];
   if (n_args != N) {
-    PyErr_SetString(PyExc_TypeError, "bind takes thirteen addresses");
+    PyErr_SetString(PyExc_TypeError, "bind takes fourteen addresses");
     return nullptr;
   }
   for (int i = 0; i < N; ++i) {
@@ -454,12 +480,14 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
   set(linear_f8_fn);
   set(norm_fn);
   set(gated_fn);
+  set(dequant8_fn);
   Py_RETURN_NONE;
 }
 
 #define FAST(f) {#f, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(f)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FAST(gemm_w4), FAST(quant_weight_i4), FAST(dequant_i4), FAST(moe_w4), FAST(quant_rows_f8),
                          FAST(quant_weight_f8), FAST(gemm_f8), FAST(linear_f8), FAST(rms_norm_quant), FAST(gated_quant),
+                         FAST(dequant),
                          FAST(bind), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module_def = {PyModuleDef_HEAD_INIT, "_call", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -32,13 +32,14 @@ struct F8Gemm {
 };
 
 // The tcgen05 kernels (gemm_f8_tc.cu): rows of both operands start on 16-byte
-// boundaries.  after_quant: the stream's last kernel writes a and sa and lets the
-// next one start early.
-int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st);
+// boundaries.
+int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st);
 
 // The kernel for single tokens (gemm_f8_rows.cu), where the tokens fit beside its
 // ring: rows of codes start on 16-byte boundaries.  x (not null): the tokens as
-// numbers of x_dtype, quantized on the way, in place of g.a and g.sa.
+// numbers of x_dtype, quantized on the way, in place of g.a and g.sa.  after_quant:
+// the kernel before on the stream is the tokens' quantizer, so the weight may be read
+// before that is done.
 bool gemm_f8_rows_fits(int M, int N, int K);
 int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st);
 
@@ -178,6 +179,34 @@ __device__ __forceinline__ void store_codes(uint8_t* row, int64_t col, int64_t n
     for (int i = 0; i < 8; ++i)
       if (col + i < n) row[col + i] = (uint8_t)((i < 4 ? c.x : c.y) >> (8 * (i & 3)));
   }
+}
+
+// Launches a kernel that may start while the one before it on the stream ends: it
+// sets itself up, then waits in pdl_wait() before its first access to memory that
+// another kernel may write, and lets the next one start after that.  So where the
+// kernel before is one of these too, all kernels before that one are done when this
+// one starts.  Back to back and without a graph a call takes the GPU 2 us less so.
+template <typename... KArgs, typename... Args>
+int launch_early(const char* what, void (*kern)(KArgs...), dim3 grid, int block, int smem, int cluster, cudaStream_t st,
+                 Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)block);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = (unsigned)cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 2 : 1;
+  return check_cuda(cudaLaunchKernelEx(&cfg, kern, static_cast<KArgs>(args)...), what);
+}
+__device__ __forceinline__ void wait_for_last_kernel() {
+  pdl_wait();
+  pdl_launch_dependents();
 }
 
 // Rows of elements of `size` bytes start on boundaries of `to` bytes.

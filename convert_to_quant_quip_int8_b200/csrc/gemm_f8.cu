@@ -17,6 +17,7 @@ namespace f8g {
 // the end.  16 bytes per thread.
 __global__ void __launch_bounds__(256)
 repitch_kernel(const uint8_t* __restrict__ src, int64_t rows, int64_t K, int64_t ld, uint4* __restrict__ dst) {
+  wait_for_last_kernel();
   const int64_t per = (K + 15) / 16;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * 256) {
     const int64_t row = i / per, col = (i - row * per) * 16;
@@ -42,9 +43,9 @@ int align_rows(const uint8_t*& q, int64_t rows, int64_t K, int64_t& ld, uint8_t*
   const int64_t bytes = copy_bytes(q, rows, K, ld);
   if (bytes == 0) return QI8_OK;
   const int64_t blocks = (bytes / 16 + 255) / 256, most = (int64_t)sm_count() * 32;
-  repitch_kernel<<<(unsigned)(blocks < most ? blocks : most), 256, 0, st>>>(q, rows, K, ld,
-                                                                             reinterpret_cast<uint4*>(workspace));
-  if (int rc = check_cuda(cudaGetLastError(), "repitch_kernel launch")) return rc;
+  if (int rc = launch_early("repitch_kernel launch", repitch_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256,
+                            0, 1, st, q, rows, K, ld, reinterpret_cast<uint4*>(workspace)))
+    return rc;
   q = workspace;
   ld = pitch(K);
   workspace += bytes;
@@ -99,7 +100,7 @@ extern "C" int qi8_gemm_f8(const uint8_t* a, const uint8_t* a_scale, int64_t M, 
   const F8Gemm g{a, b, a_scale, b_scale, bias, out, ld_a, ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
                  bias_dtype, out_dtype};
   if (gemm_f8_rows_fits((int)M, (int)N, (int)K)) return gemm_f8_rows(g, nullptr, 0, 0, false, st);
-  return gemm_f8_tiles(g, false, st);
+  return gemm_f8_tiles(g, st);
 }
 
 extern "C" int64_t qi8_linear_f8_workspace_bytes(int64_t M, int64_t K, const uint8_t* b, int64_t N, int64_t ld_b) {
@@ -131,5 +132,5 @@ extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, i
     return gemm_f8_rows(g, x, x_dtype, ld_x, false, st);
   if (int rc = quant_rows_f8(x, x_dtype, M, K, ld_x, q, f8g::pitch(K), s, st)) return rc;
   if (gemm_f8_rows_fits((int)M, (int)N, (int)K)) return gemm_f8_rows(g, nullptr, 0, 0, true, st);
-  return gemm_f8_tiles(g, true, st);
+  return gemm_f8_tiles(g, st);
 }

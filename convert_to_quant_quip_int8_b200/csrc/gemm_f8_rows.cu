@@ -32,6 +32,7 @@ struct Args {
   int64_t ld_x;
   bool vec_x;
   int stages, x_pitch;
+  bool after_quant;
   unsigned int* status;
 };
 
@@ -102,13 +103,15 @@ __global__ void __launch_bounds__(THREADS) gemm_f8_rows_kernel(const __grid_cons
     __syncwarp();
     if (lane < ROWS) bulk_copy(ring + s * STAGE + lane * PIECE_PITCH, my_row + k, bytes, full_bar(s));
   };
-  if (warp == COPIER)
+  if (warp == COPIER) {
+    if (!p.after_quant) pdl_wait();
     for (int i = 0; i < pieces && i < p.stages; ++i) copy_piece(i, i);
+  }
 
   // the tokens, by all warps but that one
   if (warp < WARPS) {
+    wait_for_last_kernel();
     if constexpr (std::is_same<X, uint8_t>::value) {
-      pdl_wait();  // the kernel before may write them
       const int per = KB * (F8_BLOCK / 16);
       for (int i = threadIdx.x; i < M * per; i += WARPS * 32) {
         const int t = i / per, k = (i - t * per) * 16;
@@ -228,7 +231,7 @@ int stages_for(int M, int K, int KB, int* x_pitch, int* smem) {
 }
 
 template <typename X, int NT>
-int launch(const Args& p, int smem, bool after_quant, cudaStream_t st) {
+int launch(const Args& p, int smem, cudaStream_t st) {
   static bool done[64];
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
@@ -237,22 +240,13 @@ int launch(const Args& p, int smem, bool after_quant, cudaStream_t st) {
     QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST));
     if (dev < 64) done[dev] = true;
   }
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)((p.g.N + ROWS - 1) / ROWS));
-  cfg.blockDim = dim3(THREADS);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = after_quant ? 1 : 0;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, p), "gemm_f8_rows_kernel launch");
+  return launch_early("gemm_f8_rows_kernel launch", kern, dim3((unsigned)((p.g.N + ROWS - 1) / ROWS)), THREADS, smem, 1, st,
+                      p);
 }
 
 template <typename X>
-int launch_tokens(const Args& p, int smem, bool after_quant, cudaStream_t st) {
-  return p.g.M <= 8 ? launch<X, 1>(p, smem, after_quant, st) : launch<X, 2>(p, smem, after_quant, st);
+int launch_tokens(const Args& p, int smem, cudaStream_t st) {
+  return p.g.M <= 8 ? launch<X, 1>(p, smem, st) : launch<X, 2>(p, smem, st);
 }
 
 }  // namespace f8r
@@ -261,22 +255,24 @@ int launch_tokens(const Args& p, int smem, bool after_quant, cudaStream_t st) {
 // Up to where this kernel is the faster one (1 x 4096 x 4096: 6.1 us, on tcgen05 7.4;
 // 8 x 4096 x 4096 7.1 and 7.5, 16 x 4096 x 4096 10.3 and 7.7, 1 x 10240 x 4096 13.5 and
 // 11.3): every block reads the tokens beside its 16 weight rows, and from 9 tokens on
-// the steps take as long as the loads.
+// the steps take as long as the loads.  Nor does it split K, so that few rows of many
+// columns are left to the few SMs that their blocks fill (1 x 500 x 16384: 15 and 9 us).
 bool gemm_f8_rows_fits(int M, int N, int K) {
+  if (N < 148 * f8r::ROWS && K > 6 * f8r::PIECE) return false;
   if (M > 16 || (int64_t)N * K / 16 * (16 + M) > (M > 8 ? 16000000 : 25500000)) return false;
   int pitch, smem;
   return f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) > 0;
 }
 
 int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st) {
-  f8r::Args p{g, x, ld_x, x && rows_aligned(x, ld_x, elem_size(x_dtype), 16), 0, 0, device_status_ptr()};
+  f8r::Args p{g, x, ld_x, x && rows_aligned(x, ld_x, elem_size(x_dtype), 16), 0, 0, after_quant, device_status_ptr()};
   int smem = 0;
   p.stages = f8r::stages_for(g.M, g.K, g.KB, &p.x_pitch, &smem);
-  if (!x) return f8r::launch_tokens<uint8_t>(p, smem, after_quant, st);
+  if (!x) return f8r::launch_tokens<uint8_t>(p, smem, st);
   switch (x_dtype) {
-    case QI8_BF16: return f8r::launch_tokens<__nv_bfloat16>(p, smem, false, st);
-    case QI8_F16: return f8r::launch_tokens<__half>(p, smem, false, st);
-    default: return f8r::launch_tokens<float>(p, smem, false, st);
+    case QI8_BF16: return f8r::launch_tokens<__nv_bfloat16>(p, smem, st);
+    case QI8_F16: return f8r::launch_tokens<__half>(p, smem, st);
+    default: return f8r::launch_tokens<float>(p, smem, st);
   }
 }
 

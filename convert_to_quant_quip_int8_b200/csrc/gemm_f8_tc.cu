@@ -189,7 +189,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   tc_fence_before();
   cluster_sync();
   tc_fence_after();
-  pdl_wait();
+  wait_for_last_kernel();
   const uint32_t tmem = *tmem_slot;
   const int KB = p.g.KB, tiles = p.m_tiles * p.n_tiles;
 
@@ -508,7 +508,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   tc_fence_after();
   // waited for where blocks first reach into one another's memory
   if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
-  pdl_wait();
+  wait_for_last_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.n_tiles * p.t_tiles;
   const int tile0 = blockIdx.x / split, tile_step = gridDim.x / split;
@@ -750,7 +750,7 @@ int code_map8(CUtensorMap* map, const uint8_t* q, int64_t rows, int64_t K, int64
 // Scale rows that can be read a word at a time.
 bool word_rows(const uint8_t* s, int KB) { return KB % 4 == 0 && reinterpret_cast<uintptr_t>(s) % 4 == 0; }
 
-int launch_pair(const F8Gemm& g, bool after_quant, cudaStream_t st) {
+int launch_pair(const F8Gemm& g, cudaStream_t st) {
   static bool done[64];
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
@@ -766,21 +766,12 @@ int launch_pair(const F8Gemm& g, bool after_quant, cudaStream_t st) {
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
   const int64_t pairs = tiles < sm_count() / 2 ? tiles : sm_count() / 2;
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(2 * pairs));
-  cfg.blockDim = dim3(pair::THREADS);
-  cfg.dynamicSmemBytes = pair::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = after_quant ? 1 : 0;
-  return check_cuda(cudaLaunchKernelEx(&cfg, pair::gemm_f8_pair_kernel, ma, mb, p), "gemm_f8_pair_kernel launch");
+  return launch_early("gemm_f8_pair_kernel launch", pair::gemm_f8_pair_kernel, dim3((unsigned)(2 * pairs)), pair::THREADS,
+                      pair::SMEM, 1, st, ma, mb, p);  // its clusters are in its attributes
 }
 
 template <int BN>
-int launch_few(const F8Gemm& g, int rows, int split, bool after_quant, cudaStream_t st) {
+int launch_few(const F8Gemm& g, int rows, int split, cudaStream_t st) {
   static bool done[64];
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
@@ -801,26 +792,15 @@ int launch_few(const F8Gemm& g, int rows, int split, bool after_quant, cudaStrea
               word_rows(g.sb, g.KB), device_status_ptr()};
   const int64_t tiles = (int64_t)p.n_tiles * p.t_tiles;
   QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(split > 1 ? tiles * split : tiles < sm_count() ? tiles : sm_count()));
-  cfg.blockDim = dim3(few::THREADS);
-  cfg.dynamicSmemBytes = few::SMEM;
-  cfg.stream = st;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = (unsigned)split;
-  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = after_quant ? 2 : 1;
-  return check_cuda(cudaLaunchKernelEx(&cfg, kern, ma, mb, p), "gemm_f8_few_kernel launch");
+  const int64_t blocks = split > 1 ? tiles * split : tiles < sm_count() ? tiles : sm_count();
+  return launch_early("gemm_f8_few_kernel launch", kern, dim3((unsigned)blocks), few::THREADS, few::SMEM, split, st, ma, mb,
+                      p);
 }
 
 }  // namespace f8tc
 }  // namespace
 
-int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st) {
+int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) {
   using namespace f8tc;
   const int sms = sm_count();
   // Tiles of 128 weight rows and up to 128 tokens, as far as one wave of blocks goes:
@@ -828,17 +808,17 @@ int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st) {
   // 4096 (320 tiles) 37 and 30.  Up to 128 tokens half of a 256-token tile would be
   // empty: 100 x 32768 x 4096 takes 30.1 us so and 32.5 in those.
   const int64_t t_tiles = ((int64_t)g.M + 127) / 128, n_tiles = ((int64_t)g.N + 127) / 128;
-  if (g.M > 128 && n_tiles * t_tiles > sms) return launch_pair(g, after_quant, st);
+  if (g.M > 128 && n_tiles * t_tiles > sms) return launch_pair(g, st);
   // Blocks that share a tile's K: a K block takes about 0.19 us up to 64 tokens and 0.24
   // with 128, the join 0.5 us and 0.012 for each token and block (fitted to 17 shapes of
   // 9 to 700 tokens; 100 x 4096 x 4096 takes 12.5 us with whole tiles, 11.5 with two blocks
-  // each, 16 x 4096 x 4096 9.2 and, with four, 7.3).  Of clusters of two 74 run at once, of
-  // three 45, of four 33, of eight 15.
+  // each, 16 x 4096 x 4096 9.2 and, with four, 7.3).  Of clusters of two 74 run at once, of four
+  // 33, of eight 15; three blocks were never faster than two or four.
   const int bn = (int)((g.M + t_tiles - 1) / t_tiles + 15) & ~15;
   const double block_us = bn <= 64 ? 0.19 : 0.19 + 0.0008 * (bn - 64);
   int split = 1, room = sms;
   double best = g.KB * block_us;
-  for (int s : {2, 3, 4, 8}) {
+  for (int s : {2, 4, 8}) {
     const int there = s == 2 ? sms : s == 8 ? sms * 13 / 16 : sms * 57 / 64;
     const double us = (g.KB + s - 1) / s * block_us + 0.5 + 0.012 * bn * s;
     if (s <= g.KB && n_tiles * t_tiles * s <= there && us < best) best = us, split = s, room = there;
@@ -848,9 +828,9 @@ int gemm_f8_tiles(const F8Gemm& g, bool after_quant, cudaStream_t st) {
   const int least = split > 1 ? 64 : 32;
   int rows = (int)(((int64_t)g.N + most - 1) / most + 15) & ~15;
   rows = rows < least ? least : rows > 128 ? 128 : rows;
-  if (bn <= 32) return launch_few<32>(g, rows, split, after_quant, st);
-  if (bn <= 64) return launch_few<64>(g, rows, split, after_quant, st);
-  return launch_few<128>(g, rows, split, after_quant, st);
+  if (bn <= 32) return launch_few<32>(g, rows, split, st);
+  if (bn <= 64) return launch_few<64>(g, rows, split, st);
+  return launch_few<128>(g, rows, split, st);
 }
 
 }  // namespace qi8

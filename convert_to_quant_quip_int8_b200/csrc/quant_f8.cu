@@ -20,6 +20,7 @@ weight_kernel(const T* __restrict__ w, int64_t N, int64_t K, int64_t ld_w, bool 
   __shared__ uint32_t warp_max[THREADS / 32];
   const int64_t col = (int64_t)blockIdx.x * F8_BLOCK + (threadIdx.x & 15) * 8;
   const int64_t row = (int64_t)blockIdx.y * F8_BLOCK + (threadIdx.x >> 4);
+  wait_for_last_kernel();
   Eight<T> e[8];
   const bool whole = vec && (int64_t)(blockIdx.x + 1) * F8_BLOCK <= K && (int64_t)(blockIdx.y + 1) * F8_BLOCK <= N;
   if (whole) {  // all loads before the first use
@@ -50,6 +51,7 @@ template <typename T>
 __global__ void __launch_bounds__(THREADS)
 dequant_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t n, int64_t ld_q, bool vec_q,
                const uint8_t* __restrict__ scale, int tile_shift, T* __restrict__ out, int64_t ld_out, bool vec) {
+  wait_for_last_kernel();
   const int64_t per = (n + 7) / 8, blocks = (n + F8_BLOCK - 1) / F8_BLOCK;
   for (int64_t i = (int64_t)blockIdx.x * THREADS + threadIdx.x; i < rows * per; i += (int64_t)gridDim.x * THREADS) {
     const int64_t row = i / per, col = (i - row * per) * 8;
@@ -78,19 +80,17 @@ template <typename T>
 int quant_weight(const void* w, int64_t N, int64_t K, int64_t ld_w, uint8_t* q, int64_t ld_q, uint8_t* scale,
                  cudaStream_t st) {
   const dim3 grid((unsigned)f8_blocks(K), (unsigned)f8_blocks(N));
-  weight_kernel<T><<<grid, THREADS, 0, st>>>(static_cast<const T*>(w), N, K, ld_w, rows_aligned(w, ld_w, sizeof(T), 16),
-                                             q, ld_q, rows_aligned(q, ld_q, 1, 8), scale);
-  return check_cuda(cudaGetLastError(), "weight_kernel launch");
+  return launch_early("weight_kernel launch", weight_kernel<T>, grid, THREADS, 0, 1, st, static_cast<const T*>(w), N, K,
+                      ld_w, rows_aligned(w, ld_w, sizeof(T), 16), q, ld_q, rows_aligned(q, ld_q, 1, 8), scale);
 }
 
 template <typename T>
 int dequant(const uint8_t* q, int64_t rows, int64_t n, int64_t ld_q, const uint8_t* scale, int tile, void* out,
             int64_t ld_out, cudaStream_t st) {
   const int64_t blocks = (rows * ((n + 7) / 8) + THREADS - 1) / THREADS, most = (int64_t)sm_count() * 64;
-  dequant_kernel<T><<<(unsigned)(blocks < most ? blocks : most), THREADS, 0, st>>>(
-      q, rows, n, ld_q, rows_aligned(q, ld_q, 1, 8), scale, tile == 1 ? 0 : 7, static_cast<T*>(out), ld_out,
-      rows_aligned(out, ld_out, sizeof(T), 16));
-  return check_cuda(cudaGetLastError(), "dequant_kernel launch");
+  return launch_early("dequant_kernel launch", dequant_kernel<T>, dim3((unsigned)(blocks < most ? blocks : most)), THREADS,
+                      0, 1, st, q, rows, n, ld_q, rows_aligned(q, ld_q, 1, 8), scale, tile == 1 ? 0 : 7,
+                      static_cast<T*>(out), ld_out, rows_aligned(out, ld_out, sizeof(T), 16));
 }
 
 }  // namespace f8q

@@ -228,6 +228,9 @@ def _gemm_ws_bytes(M: int, N: int, K: int, a_kind: int, b_kind: int) -> int:
 
 def dequant(q: torch.Tensor, scale: torch.Tensor, kind: int, block: int = 128,
             out_dtype: torch.dtype = torch.float32) -> torch.Tensor:
+    out = _fast("dequant", q, scale, kind, block, out_dtype)
+    if out is not None:
+        return out
     L.require_cuda(q, scale)
     q2 = q.reshape(-1, q.shape[-1]).contiguous()
     rows, n = q2.shape
