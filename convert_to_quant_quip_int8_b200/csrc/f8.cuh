@@ -88,6 +88,29 @@ struct Eight {
 #pragma unroll
     for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = __ldg(reinterpret_cast<const uint4*>(at) + i);
   }
+  // A whole piece anywhere: the aligned 16 bytes that it begins and ends in, shifted.
+  // These lie in the row when eight columns do before the piece and after it.
+  __device__ __forceinline__ void load_shifted(const T* at) {
+    constexpr int WORDS = 2 * sizeof(T);
+    const uint32_t off = (uint32_t)(reinterpret_cast<uintptr_t>(at) & 15u);
+    const uint4* base = reinterpret_cast<const uint4*>(reinterpret_cast<uintptr_t>(at) - off);
+    uint32_t a[WORDS + 4];
+#pragma unroll
+    for (int i = 0; i <= WORDS / 4; ++i) {
+      const uint4 c = __ldg(base + i);
+      a[4 * i] = c.x;
+      a[4 * i + 1] = c.y;
+      a[4 * i + 2] = c.z;
+      a[4 * i + 3] = c.w;
+    }
+#pragma unroll
+    for (int i = 0; i < WORDS + 3; ++i) a[i] = off & 4u ? a[i + 1] : a[i];
+#pragma unroll
+    for (int i = 0; i < WORDS + 1; ++i) a[i] = off & 8u ? a[i + 2] : a[i];
+    uint32_t* w = reinterpret_cast<uint32_t*>(v);
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = __funnelshift_r(a[i], a[i + 1], 8 * (off & 3u));
+  }
   // From column `col` on, zero from n on.
   __device__ __forceinline__ void load_some(const T* row, int64_t col, int64_t n) {
     T* e = reinterpret_cast<T*>(v);

@@ -9,9 +9,9 @@ namespace qi8 {
 namespace {
 namespace f8q {
 
-constexpr int THREADS = 256;
+constexpr int THREADS = 512, PASSES = F8_BLOCK * 16 / THREADS;
 
-// One 128 x 128 tile per thread block: 16 lanes by eight columns, 16 rows at a
+// One 128 x 128 tile per thread block: 16 lanes by eight columns, 32 rows at a
 // time.  The tile stays in registers between its maximum and its codes.
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
@@ -21,18 +21,21 @@ weight_kernel(const T* __restrict__ w, int64_t N, int64_t K, int64_t ld_w, bool 
   const int64_t col = (int64_t)blockIdx.x * F8_BLOCK + (threadIdx.x & 15) * 8;
   const int64_t row = (int64_t)blockIdx.y * F8_BLOCK + (threadIdx.x >> 4);
   wait_for_last_kernel();
-  Eight<T> e[8];
-  const bool whole = vec && (int64_t)(blockIdx.x + 1) * F8_BLOCK <= K && (int64_t)(blockIdx.y + 1) * F8_BLOCK <= N;
-  if (whole) {  // all loads before the first use
+  Eight<T> e[PASSES];
+  const bool whole = (int64_t)(blockIdx.x + 1) * F8_BLOCK <= K && (int64_t)(blockIdx.y + 1) * F8_BLOCK <= N;
+  if (whole && vec) {  // all loads before the first use
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i].load(w + (row + 16 * i) * ld_w + col);
+    for (int i = 0; i < PASSES; ++i) e[i].load(w + (row + THREADS / 16 * i) * ld_w + col);
+  } else if (whole && col >= 8 && col + 16 <= K) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) e[i].load_shifted(w + (row + THREADS / 16 * i) * ld_w + col);
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) e[i].load_some(w + (row + 16 * i) * ld_w, col, row + 16 * i < N ? K : 0);
+    for (int i = 0; i < PASSES; ++i) e[i].load_some(w + (row + THREADS / 16 * i) * ld_w, col, row + THREADS / 16 * i < N ? K : 0);
   }
   uint32_t m = 0;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) m = max(m, amax_bits(e[i].get()));
+  for (int i = 0; i < PASSES; ++i) m = max(m, amax_bits(e[i].get()));
   m = __reduce_max_sync(0xffffffffu, m);
   if ((threadIdx.x & 31) == 0) warp_max[threadIdx.x >> 5] = m;
   __syncthreads();
@@ -41,8 +44,8 @@ weight_kernel(const T* __restrict__ w, int64_t N, int64_t K, int64_t ld_w, bool 
   const uint32_t code = f8_scale_code(m);
   const float inv = f8_inverse(code);
 #pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (row + 16 * i < N) store_codes(q + (row + 16 * i) * ld_q, col, K, f8_codes(e[i].get(), inv), vec_q);
+  for (int i = 0; i < PASSES; ++i)
+    if (row + THREADS / 16 * i < N) store_codes(q + (row + THREADS / 16 * i) * ld_q, col, K, f8_codes(e[i].get(), inv), vec_q);
   if (threadIdx.x == 0) scale[(int64_t)blockIdx.y * gridDim.x + blockIdx.x] = (uint8_t)code;
 }
 

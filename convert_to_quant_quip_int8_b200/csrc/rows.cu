@@ -731,33 +731,43 @@ __global__ void dequant_kernel(const int8_t* __restrict__ q, int64_t rows, int64
   }
 }
 
-// The same for scales that eight neighbouring columns share, eight values per
-// thread: 515 x 2731 fp16 took 9 us with a division per value.
+// The same for one scale, or one per row: a warp takes 256 columns of a row, eight
+// neighbouring ones per lane where rows are aligned and else every 32nd, so that a
+// warp's accesses are whole lines.  (With a division per value 515 x 2731 took 9 us.)
 template <typename T>
-__global__ void dequant8_kernel(const int8_t* __restrict__ q, int64_t rows, unsigned n, const float* __restrict__ scale,
-                                int kind, int block, bool vec, T* __restrict__ out) {
-  const unsigned per = (n + 7) / 8, nb = block > 0 ? n / block : 1;
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < rows * per;
-       i += (int64_t)gridDim.x * blockDim.x) {
+__global__ void __launch_bounds__(256)
+dequant_rows_kernel(const int8_t* __restrict__ q, int64_t rows, unsigned n, const float* __restrict__ scale, bool per_row,
+                    bool vec, T* __restrict__ out) {
+  constexpr int DT = sizeof(T) == 4 ? QI8_F32 : std::is_same<T, __half>::value ? QI8_F16 : QI8_BF16;
+  const unsigned per = (n + 255) / 256, lane = threadIdx.x & 31;
+  for (int64_t i = blockIdx.x * (int64_t)8 + (threadIdx.x >> 5); i < rows * per; i += (int64_t)gridDim.x * 8) {
     const int64_t r = i <= 0xffffffffll ? (unsigned)i / per : i / per;
-    const unsigned c = (unsigned)(i - r * per) * 8;
-    const int64_t at = r * n + c;
-    const float s = scale[kind == QI8_S_SCALAR ? 0 : kind == QI8_S_ROW ? r : r * nb + c / block];
+    const unsigned c0 = (unsigned)(i - r * per) * 256;
+    const float s = scale[per_row ? r : 0];
+    const int8_t* src = q + r * n;
+    T* dst = out + r * n;
     if (vec) {
-      const uint2 w = *reinterpret_cast<const uint2*>(q + at);
+      const unsigned c = c0 + lane * 8;
+      if (c >= n) continue;
+      const uint2 w = *reinterpret_cast<const uint2*>(src + c);
       __align__(16) T v[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        store_from_f32(v, sizeof(T) == 4 ? QI8_F32 : std::is_same<T, __half>::value ? QI8_F16 : QI8_BF16, j,
-                       __fmul_rn((float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))), s));
+        store_from_f32(v, DT, j, __fmul_rn((float)(int8_t)((j < 4 ? w.x : w.y) >> (8 * (j & 3))), s));
 #pragma unroll
-      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(out + at)[j] = reinterpret_cast<const uint4*>(v)[j];
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(dst + c)[j] = reinterpret_cast<const uint4*>(v)[j];
     } else {
+      int8_t v[8];
 #pragma unroll
-      for (int j = 0; j < 8; ++j)
-        if (c + j < n)
-          store_from_f32(out, sizeof(T) == 4 ? QI8_F32 : std::is_same<T, __half>::value ? QI8_F16 : QI8_BF16, at + j,
-                         __fmul_rn((float)q[at + j], s));
+      for (int j = 0; j < 8; ++j) {
+        const unsigned c = c0 + 32 * j + lane;
+        v[j] = c < n ? src[c] : 0;
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const unsigned c = c0 + 32 * j + lane;
+        if (c < n) store_from_f32(dst, DT, c, __fmul_rn((float)v[j], s));
+      }
     }
   }
 }
@@ -1217,17 +1227,18 @@ int qi8_dequant(const int8_t* q, int64_t rows, int64_t n, const float* scale, in
     QI8_REQUIRE(block > 0 && n % block == 0, QI8_ESHAPE, "n %% block != 0");
   if (rows == 0) return QI8_OK;
   const int64_t total = rows * n;
-  if (n < (1ll << 31) && (scale_kind <= QI8_S_ROW || (scale_kind == QI8_S_ROW_KBLOCK && block % 8 == 0))) {
+  if (n < (1ll << 31) && (scale_kind == QI8_S_SCALAR || scale_kind == QI8_S_ROW)) {
     cudaStream_t st = static_cast<cudaStream_t>(stream);
     const bool vec = n % 8 == 0 && reinterpret_cast<uintptr_t>(q) % 8 == 0 && aligned16(out);
-    const int grid = grid_for(rows * ((n + 7) / 8), 256), nb = scale_kind == QI8_S_ROW_KBLOCK ? block : 0;
+    const int grid = grid_for(rows * ((n + 255) / 256), 8);
+    const bool per_row = scale_kind == QI8_S_ROW;
     if (out_dtype == QI8_BF16)
-      dequant8_kernel<<<grid, 256, 0, st>>>(q, rows, (unsigned)n, scale, scale_kind, nb, vec, static_cast<__nv_bfloat16*>(out));
+      dequant_rows_kernel<<<grid, 256, 0, st>>>(q, rows, (unsigned)n, scale, per_row, vec, static_cast<__nv_bfloat16*>(out));
     else if (out_dtype == QI8_F16)
-      dequant8_kernel<<<grid, 256, 0, st>>>(q, rows, (unsigned)n, scale, scale_kind, nb, vec, static_cast<__half*>(out));
+      dequant_rows_kernel<<<grid, 256, 0, st>>>(q, rows, (unsigned)n, scale, per_row, vec, static_cast<__half*>(out));
     else
-      dequant8_kernel<<<grid, 256, 0, st>>>(q, rows, (unsigned)n, scale, scale_kind, nb, vec, static_cast<float*>(out));
-    return check_cuda(cudaGetLastError(), "dequant8_kernel launch");
+      dequant_rows_kernel<<<grid, 256, 0, st>>>(q, rows, (unsigned)n, scale, per_row, vec, static_cast<float*>(out));
+    return check_cuda(cudaGetLastError(), "dequant_rows_kernel launch");
   }
   dequant_kernel<<<grid_for(total, 256), 256, 0, static_cast<cudaStream_t>(stream)>>>(
       q, rows, n, scale, scale_kind, block, out, out_dtype);
