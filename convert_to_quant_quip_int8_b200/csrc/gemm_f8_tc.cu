@@ -25,14 +25,22 @@ __host__ __device__ constexpr uint32_t idesc(int m, int n, uint32_t sf = 0) {
   return (sf << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) | (sf << 29);
 }
 
-// Four scale bytes of a row, K blocks kb .. kb + 3 (whatever stands there past the end).
-__device__ __forceinline__ uint32_t scale_word(const uint8_t* row, int kb, int KB, bool words) {
-  if (words) return __ldg(reinterpret_cast<const uint32_t*>(row + kb));
-  uint32_t w = 0;
+// Four scale bytes, K blocks kb .. kb + 3, of N rows (`row` gives the start of row i):
+// words where rows lie on whole ones, else byte by byte, out of the way of the
+// instruction cache.  Past the end: 0.
+template <int N, typename F>
+__device__ __forceinline__ void scale_words(uint32_t (&w)[N], F&& row, int kb, int KB, bool words) {
+  if (words) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i)
-    if (kb + i < KB) w |= (uint32_t)__ldg(row + kb + i) << (8 * i);
-  return w;
+    for (int i = 0; i < N; ++i) w[i] = __ldg(reinterpret_cast<const uint32_t*>(row(i) + kb));
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = 0;
+#pragma unroll 1
+    for (int b = 0; b < 4 && kb + b < KB; ++b)
+#pragma unroll
+      for (int i = 0; i < N; ++i) w[i] |= (uint32_t)__ldg(row(i) + kb + b) << (8 * b);
+  }
 }
 
 __device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&r)[4]) {
@@ -42,38 +50,59 @@ __device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&r)[4]) 
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 results of one row from column n on.  vec: rows start on 16-byte boundaries.
-__device__ __forceinline__ void store32(const F8Gemm& g, int64_t m, int n, const float (&y)[32], bool vec) {
+// 32 results of one row from column n on, those before `end`.
+__device__ __forceinline__ void store32(const F8Gemm& g, int64_t m, int n, int end, const float (&y)[32]) {
   const int64_t at = m * g.ld_out + n;
-  if (vec && n + 32 <= g.N) {
-    if (g.out_dtype == QI8_F32) {
-      float4* o = reinterpret_cast<float4*>(static_cast<float*>(g.out) + at);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) o[i] = make_float4(y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]);
-    } else {
-      uint4* o = reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + at);
-      const bool half = g.out_dtype == QI8_F16;
+  for (int j = 0; j < 32; ++j)
+    if (n + j < end) store_from_f32(g.out, g.out_dtype, at + j, y[j]);
+}
+
+// A warp's 32 rows (m0 on, lane = row) x 32 columns, all of them there, rows of the
+// result on 16-byte boundaries.  Stored by rows each instruction touches 32 lines, and
+// a tile took 6000 cycles; through shared memory it is 8 (4 with fp32).  Pieces of 16
+// bytes are swapped so that eight lanes touch all banks, both ways.
+__device__ __forceinline__ void store_tile(const F8Gemm& g, uint4* buf, int m0, int n, const float (&y)[32]) {
+  const int lane = threadIdx.x & 31;
+  __syncwarp();
+  if (g.out_dtype == QI8_F32) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        uint32_t w[4];
+    for (int i = 0; i < 8; ++i)
+      buf[lane * 8 + (i ^ (lane & 7))] = make_uint4(__float_as_uint(y[4 * i]), __float_as_uint(y[4 * i + 1]),
+                                                    __float_as_uint(y[4 * i + 2]), __float_as_uint(y[4 * i + 3]));
+    __syncwarp();
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float a = y[8 * i + 2 * j], b = y[8 * i + 2 * j + 1];
-          if (half) {
-            const __half2 h = __floats2half2_rn(a, b);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-          } else {
-            const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-            w[j] = *reinterpret_cast<const uint32_t*>(&h);
-          }
-        }
-        o[i] = make_uint4(w[0], w[1], w[2], w[3]);
-      }
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 3), c = lane & 7;
+      if (m0 + r < g.M)
+        reinterpret_cast<uint4*>(static_cast<float*>(g.out) + (int64_t)(m0 + r) * g.ld_out + n)[c] = buf[r * 8 + (c ^ (r & 7))];
     }
   } else {
+    const bool half = g.out_dtype == QI8_F16;
 #pragma unroll
-    for (int j = 0; j < 32; ++j)
-      if (n + j < g.N) store_from_f32(g.out, g.out_dtype, at + j, y[j]);
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float2 v = make_float2(y[8 * i + 2 * j], y[8 * i + 2 * j + 1]);
+        if (half) {
+          const __half2 h = __float22half2_rn(v);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        } else {
+          const __nv_bfloat162 h = __float22bfloat162_rn(v);
+          w[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+      }
+      buf[lane * 4 + (i ^ ((lane >> 1) & 3))] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int r = 8 * i + (lane >> 2), c = lane & 3;
+      if (m0 + r < g.M)
+        reinterpret_cast<uint4*>(static_cast<uint16_t*>(g.out) + (int64_t)(m0 + r) * g.ld_out + n)[c] =
+            buf[r * 4 + (c ^ ((r >> 1) & 3))];
+    }
   }
 }
 
@@ -87,7 +116,8 @@ __device__ __forceinline__ void store32(const F8Gemm& g, int64_t m, int n, const
 //   warp 13       TMEM allocation; MMA issue (one thread of the even block)
 // Two accumulators of 256 columns and the scales do not fit 512 columns, so the
 // accumulators share 64: the epilogue reads those first, and the next tile's
-// MMAs wait for just that.
+// MMAs wait for just that.  Tiles may have fewer features, where that fills the last
+// wave of blocks better.
 // The issuing warp sets the pace: an MMA takes it 72 cycles, a wait 110, a commit
 // 60 to 100 (clock64), and the tensor cores, which queue about 14 MMAs, 128 cycles
 // for each.  A stage of one K block cost it 700 cycles per block, two blocks a stage
@@ -100,12 +130,14 @@ constexpr int STAGES = 3, OPERAND = 128 * BK, STAGE = 4 * OPERAND;  // two K blo
 constexpr int ACC1 = 192;                           // columns of accumulator 1; 64 are both accumulators'
 constexpr int SCALES = 448, SLOT = 16, SLOTS = 4;   // 8 columns of b, 4 of a
 constexpr int BARS = 2 * STAGES + 4 + 2 * SLOTS + 2;
-constexpr int SMEM = 1024 + STAGES * STAGE + EPI_WARPS * 32 * 4 + BARS * 8 + 16;
+constexpr int EPI_BYTES = 32 * 32 * 4 + 32 * 4;  // of an epilogue warp: a tile on its way out, the bias
+constexpr int SMEM = 1024 + STAGES * STAGE + EPI_WARPS * EPI_BYTES + BARS * 8 + 16;
 static_assert(SMEM <= 232448 && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && ACC1 + 256 <= SCALES, "memories");
 
 struct Args {
   F8Gemm g;
   int m_tiles, n_tiles;
+  int bn;  // features of a tile, a multiple of 16 up to 256
   bool words_a, words_b, vec_out;
   unsigned int* status;
 };
@@ -142,8 +174,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
   const uint32_t raw = smem_u32(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* sm = smem_raw + (base - raw);
   const uint32_t sA = base, sB = base + STAGES * 2 * OPERAND;
-  float* sbias = reinterpret_cast<float*>(sm + STAGES * STAGE);
-  uint64_t* bars = reinterpret_cast<uint64_t*>(sbias + EPI_WARPS * 32);
+  uint8_t* epi = sm + STAGES * STAGE;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(epi + EPI_WARPS * EPI_BYTES);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + BARS);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   auto full_bar = [&](int s) { return smem_u32(bars + s); };
@@ -200,13 +232,13 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       uint32_t ph = 0, issued = 0, issued_ph = 0;
       bool ok = true;
       for (int tile = pair0; ok && tile < tiles; tile += pairs) {
-        const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128, n0 = (tile / p.m_tiles) * 256 + (int)rank * 128;
+        const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128, n0 = (tile / p.m_tiles) * p.bn + (int)rank * (p.bn / 2);
         for (int kb = 0; kb < KB; kb += 2) {
           if (!mbar_wait(empty_bar(s), ph ^ 1u, abort_flag, p.status, ST_F8_PRODUCER, WAIT_LIMIT_NS)) {
             ok = false;
             break;
           }
-          if (leader) mbar_arrive_expect_tx(full_bar(s), 2 * STAGE);
+          if (leader) mbar_arrive_expect_tx(full_bar(s), 2 * 2 * (OPERAND + (uint32_t)p.bn / 2 * BK));
 #pragma unroll
           for (int i = 0; i < 2; ++i) {  // past the last K block: zeros
             tma_load(sA + (2 * s + i) * OPERAND, &tmA, (kb + i) * BK, m0, full0 + 8 * s);
@@ -233,7 +265,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       for (int tile = pair0; ok && tile < tiles; tile += pairs, ++unit) {
         const int buf = unit & 1;
         if (!warp_wait(tempty_bar(buf), ((unit >> 1) & 1) ^ 1u, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
-        if (unit > 0 && !warp_wait(tshared_bar, (unit - 1) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
+        if (unit > 0 && p.bn > ACC1 &&
+            !warp_wait(tshared_bar, (unit - 1) & 1, abort_flag, p.status, ST_F8_MMA, WAIT_LIMIT_NS)) break;
         tc_fence_after();
         const uint32_t d = tmem + (buf ? ACC1 : 0);
         for (int kb = 0; ok && kb < KB; kb += 4, ++slot) {  // one slot of scales
@@ -256,7 +289,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
               if (kb + h + i >= KB) break;
 #pragma unroll
               for (int k = 0; k < BK / 32; ++k)
-                mma(one, d, da + (i * OPERAND / 16 + 2 * k), db + (i * OPERAND / 16 + 2 * k), idesc(256, 256, h + i),
+                mma(one, d, da + (i * OPERAND / 16 + 2 * k), db + (i * OPERAND / 16 + 2 * k), idesc(256, p.bn, h + i),
                     sb + 8, sb, h + i + k > 0 || kb > 0);
             }
             commit(one, empty_bar(s), 3);
@@ -271,26 +304,24 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     }
   } else if (warp >= SCALE_WARP0) {
     // ---------------------------------------------------------- scales
-    // word i of a: token 32 i + lane, in the same lane of all four quarters of
-    // tensor memory; the features' words are the same for 128 of them
+    // word i: token (feature) 32 i + lane, in the same lane of all four quarters of
+    // tensor memory
     const uint32_t lanes = tmem + ((uint32_t)((warp & 3) * 32) << 16) + SCALES;
     const uint32_t sfull0 = mapa(sfull_bar(0), 0);
-    auto load = [&](int tile, int kb, uint32_t (&a)[4], uint32_t (&b)[2]) {
-      const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128, t0 = (tile / p.m_tiles) * 2;
+    auto load = [&](int tile, int kb, uint32_t (&a)[4], uint32_t (&b)[8]) {
+      const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128, n0 = (tile / p.m_tiles) * p.bn;
       const int last = (p.g.N - 1) / F8_BLOCK;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        a[i] = scale_word(p.g.sa + (int64_t)min(m0 + 32 * i + lane, p.g.M - 1) * KB, kb, KB, p.words_a);
-#pragma unroll
-      for (int i = 0; i < 2; ++i) b[i] = scale_word(p.g.sb + (int64_t)min(t0 + i, last) * KB, kb, KB, p.words_b);
+      scale_words(a, [&](int i) { return p.g.sa + (int64_t)min(m0 + 32 * i + lane, p.g.M - 1) * KB; }, kb, KB, p.words_a);
+      scale_words(b, [&](int i) { return p.g.sb + (int64_t)min((n0 + 32 * i + lane) / F8_BLOCK, last) * KB; }, kb, KB,
+                  p.words_b);
     };
     unsigned slot = 0;
     bool ok = true;
-    uint32_t a[4], b[2];
+    uint32_t a[4], b[8];
     if (pair0 < tiles) load(pair0, 0, a, b);
     for (int tile = pair0; ok && tile < tiles; tile += pairs) {
       for (int kb = 0; kb < KB; kb += 4, ++slot) {
-        uint32_t a_next[4] = {0, 0, 0, 0}, b_next[2] = {0, 0};
+        uint32_t a_next[4] = {0, 0, 0, 0}, b_next[8] = {0, 0, 0, 0, 0, 0, 0, 0};
         if (kb + 4 < KB) load(tile, kb + 4, a_next, b_next);
         else if (tile + pairs < tiles) load(tile + pairs, 0, a_next, b_next);
         if (!warp_wait(sempty_bar(slot % SLOTS), ((slot / SLOTS) & 1) ^ 1u, abort_flag, p.status, ST_F8_SCALES,
@@ -300,7 +331,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         }
         tc_fence_after();
         const uint32_t at = lanes + (slot % SLOTS) * SLOT;
-        const uint32_t lo[4] = {b[0], b[0], b[0], b[0]}, hi[4] = {b[1], b[1], b[1], b[1]};
+        const uint32_t lo[4] = {b[0], b[1], b[2], b[3]}, hi[4] = {b[4], b[5], b[6], b[7]};
         tmem_st4(at, lo);
         tmem_st4(at + 4, hi);
         tmem_st4(at + 8, a);
@@ -310,8 +341,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
         if (lane == 0) arrive_cluster(sfull0 + 8 * (slot % SLOTS));
 #pragma unroll
         for (int i = 0; i < 4; ++i) a[i] = a_next[i];
-        b[0] = b_next[0];
-        b[1] = b_next[1];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) b[i] = b_next[i];
       }
     }
   } else {
@@ -319,12 +350,13 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
     const int quarter = warp & 3, half = warp >> 2;
     const uint32_t lanes = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t tempty0 = mapa(tempty_bar(0), 0), tshared0 = mapa(tshared_bar, 0);
-    float* my_bias = sbias + warp * 32;
+    uint4* my_tile = reinterpret_cast<uint4*>(epi + warp * 32 * 32 * 4);
+    float* my_bias = reinterpret_cast<float*>(epi + EPI_WARPS * 32 * 32 * 4) + warp * 32;
     int unit = 0;
     for (int tile = pair0; tile < tiles; tile += pairs, ++unit) {
       const int buf = unit & 1;
-      const int64_t m = (int64_t)(tile % p.m_tiles) * 256 + (int)rank * 128 + quarter * 32 + lane;
-      const int n0 = (tile / p.m_tiles) * 256;
+      const int m0 = (tile % p.m_tiles) * 256 + (int)rank * 128 + quarter * 32;
+      const int n0 = (tile / p.m_tiles) * p.bn, end = min(n0 + p.bn, p.g.N);
       // every other 32 columns, those first that the accumulators share: the lowest
       // 64 of accumulator 1, the highest 64 of accumulator 0
       auto chunk = [&](int i) { return (buf ? 2 * i : 6 - 2 * i) + half; };
@@ -332,11 +364,11 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
       tc_fence_after();
       const uint32_t acc = lanes + (buf ? ACC1 : 0);
       uint32_t r[2][32];
-      tmem_ld32(acc + 32 * chunk(0), r[0]);
+      if (32 * chunk(0) < p.bn) tmem_ld32(acc + 32 * chunk(0), r[0]);
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         tmem_wait_ld();
-        if (i < 3) tmem_ld32(acc + 32 * chunk(i + 1), r[(i + 1) & 1]);
+        if (i < 3 && 32 * chunk(i + 1) < p.bn) tmem_ld32(acc + 32 * chunk(i + 1), r[(i + 1) & 1]);
         if (i == 0) {
           tc_fence_before();
           __syncwarp();
@@ -347,6 +379,7 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           __syncwarp();
           if (lane == 0) arrive_cluster(tempty0 + 8 * buf);
         }
+        if (32 * chunk(i) >= p.bn) continue;
         const int n = n0 + 32 * chunk(i);
         float y[32];
 #pragma unroll
@@ -358,7 +391,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 #pragma unroll
           for (int j = 0; j < 32; ++j) y[j] += my_bias[j];
         }
-        if (m < p.g.M && n < p.g.N) store32(p.g, m, n, y, p.vec_out);
+        if (p.vec_out && n + 32 <= end) store_tile(p.g, my_tile, m0, n, y);
+        else if (m0 + lane < p.g.M && n < end) store32(p.g, m0 + lane, n, end, y);
       }
     }
   }
@@ -599,13 +633,11 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     const int last = (p.g.N - 1) / F8_BLOCK;
     auto load = [&](int tile, int kb, uint32_t (&w)[4], uint32_t (&x)[BN / 32]) {
       const int n0 = (tile % p.n_tiles) * p.rows, t0 = (tile / p.n_tiles) * p.bn;
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        w[i] = scale_word(p.g.sb + (int64_t)min((n0 + 32 * i + lane) / F8_BLOCK, last) * KB, kb, KB,
-                          p.words_b && (kb & 3) == 0);
-#pragma unroll
-      for (int i = 0; i < BN / 32; ++i)
-        x[i] = scale_word(p.g.sa + (int64_t)min(t0 + 32 * i + lane, p.g.M - 1) * KB, kb, KB, p.words_a && (kb & 3) == 0);
+      const bool whole = (kb & 3) == 0;
+      scale_words(w, [&](int i) { return p.g.sb + (int64_t)min((n0 + 32 * i + lane) / F8_BLOCK, last) * KB; }, kb, KB,
+                  p.words_b && whole);
+      scale_words(x, [&](int i) { return p.g.sa + (int64_t)min(t0 + 32 * i + lane, p.g.M - 1) * KB; }, kb, KB,
+                  p.words_a && whole);
     };
     unsigned slot = 0;
     bool ok = true;
@@ -758,10 +790,22 @@ int launch_pair(const F8Gemm& g, cudaStream_t st) {
     QI8_CUDA(cudaFuncSetAttribute(pair::gemm_f8_pair_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, pair::SMEM));
     if (dev < 64) done[dev] = true;
   }
+  // Features per tile, by the last wave: a K block takes 2 cycles per feature, or what
+  // issuing its MMAs takes, a tile about 1500 more.  512 x 10240 x 4096 takes 25.4 us in
+  // tiles of 160, 27.7 in tiles of 256; 1024 x 4096 x 4096 17.2 with 256, 24 with 224 (a
+  // second wave).  Halves of a tile that are no whole 16s are slower than these.
+  int bn = 256;
+  double best = 1e300;
+  for (int n = 256; n >= 128; n -= 32) {
+    const int64_t tiles = (int64_t)((g.M + 255) / 256) * ((g.N + n - 1) / n);
+    const int64_t waves = (2 * tiles + sm_count() - 1) / sm_count();
+    const double cycles = (double)waves * ((n < 160 ? 320 : 2 * n) * (double)g.KB + 1500.0);
+    if (cycles < best) best = cycles, bn = n;
+  }
   CUtensorMap ma, mb;
   if (int rc = code_map8(&ma, g.a, g.M, g.K, g.ld_a, 128)) return rc;
-  if (int rc = code_map8(&mb, g.b, g.N, g.K, g.ld_b, 128)) return rc;
-  pair::Args p{g, (g.M + 255) / 256, (g.N + 255) / 256, word_rows(g.sa, g.KB), word_rows(g.sb, g.KB),
+  if (int rc = code_map8(&mb, g.b, g.N, g.K, g.ld_b, bn / 2)) return rc;
+  pair::Args p{g, (g.M + 255) / 256, (g.N + bn - 1) / bn, bn, word_rows(g.sa, g.KB), word_rows(g.sb, g.KB),
                rows_aligned(g.out, g.ld_out, elem_size(g.out_dtype), 16), device_status_ptr()};
   const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
   QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
