@@ -27,6 +27,7 @@ struct Args {
   float eps, inv_n;
   int weight_dtype, mode;
   bool vec, vec_weight, vec_q, vec_sum;
+  bool whole() const { return n % 8 == 0 && vec && vec_q && (!weight || vec_weight) && (!sum || vec_sum); }
 };
 
 // x 2^t / (1 + 2^t) ... as x / (1 + 2^-t): 0 where 2^-t passes fp32, as it should be
@@ -63,17 +64,19 @@ __device__ __forceinline__ F8x gate(const F8x& g, const F8x& up) {
   return y;
 }
 
-template <typename W>
+template <typename W, bool WHOLE>
 __device__ __forceinline__ F8x weight_as(const Args& p, int64_t col) {
   Eight<W> e;
   const W* w = static_cast<const W*>(p.weight);
-  if (p.vec_weight && col + 8 <= p.n) e.load(w + col);
+  if (WHOLE ? col < p.n : p.vec_weight && col + 8 <= p.n) e.load(w + col);
+  else if (WHOLE) e.clear();
   else e.load_some(w, col, p.n);
   return e.get();
 }
+template <bool WHOLE>
 __device__ __forceinline__ F8x load_weight(const Args& p, int64_t col) {
-  if (p.weight_dtype == QI8_BF16) return weight_as<__nv_bfloat16>(p, col);
-  return p.weight_dtype == QI8_F16 ? weight_as<__half>(p, col) : weight_as<float>(p, col);
+  if (p.weight_dtype == QI8_BF16) return weight_as<__nv_bfloat16, WHOLE>(p, col);
+  return p.weight_dtype == QI8_F16 ? weight_as<__half, WHOLE>(p, col) : weight_as<float, WHOLE>(p, col);
 }
 
 // What is done to the two inputs of a column before any step over the row.
@@ -101,31 +104,38 @@ __device__ __forceinline__ F8x combine(const Args& p, const Eight<T>& a, const E
 
 // `N` pieces of a row of each input, `step` columns apart, zero past the end: all
 // loads are issued before the first is used.
-template <typename T, int OP, int N>
+template <typename T, int OP, int N, bool WHOLE>
 struct Raw {
   Eight<T> u[N], v[N];
 
   __device__ __forceinline__ void load(const Args& p, int64_t row, int64_t col, int step) {
-    const T* a = static_cast<const T*>(p.x) + row * p.ld_x;
-    const T* b = static_cast<const T*>(p.second) + row * p.ld_second;
+    const T* a = static_cast<const T*>(p.x) + row * p.ld_x + col;
+    const T* b = static_cast<const T*>(p.second) + row * p.ld_second + col;
     const bool two = OP != PLAIN && p.second;
-    if (p.vec && col + (N - 1) * step + 8 <= p.n) {
+    const int64_t left = p.n - col;  // columns from the first piece on
+    if constexpr (WHOLE) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) u[i].load(a + col + i * step);
+      for (int i = 0; i < N; ++i) i * step < left ? u[i].load(a + i * step) : u[i].clear();
       if (two)
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i].load(b + col + i * step);
-    } else if (!p.vec && col >= 8 && col + (N - 1) * step + 16 <= p.n) {
+        for (int i = 0; i < N; ++i) i * step < left ? v[i].load(b + i * step) : v[i].clear();
+    } else if (p.vec && (N - 1) * step + 8 <= left) {
 #pragma unroll
-      for (int i = 0; i < N; ++i) u[i].load_shifted(a + col + i * step);
+      for (int i = 0; i < N; ++i) u[i].load(a + i * step);
       if (two)
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i].load_shifted(b + col + i * step);
+        for (int i = 0; i < N; ++i) v[i].load(b + i * step);
+    } else if (!p.vec && col >= 8 && (N - 1) * step + 16 <= left) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i].load_shifted(a + i * step);
+      if (two)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i].load_shifted(b + i * step);
     } else {
 #pragma unroll
       for (int i = 0; i < N; ++i) {
-        u[i].load_some(a, col + i * step, p.n);
-        if (two) v[i].load_some(b, col + i * step, p.n);
+        u[i].load_some(a + i * step, 0, left - i * step);
+        if (two) v[i].load_some(b + i * step, 0, left - i * step);
       }
     }
   }
@@ -134,18 +144,23 @@ struct Raw {
     for (int i = 0; i < N; ++i) y[i] = combine<T, OP>(p, u[i], v[i]);
   }
 };
-template <typename T, int OP, int N>
+template <typename T, int OP, bool WHOLE, int N>
 __device__ __forceinline__ void row_values(const Args& p, int64_t row, int64_t col, int step, F8x (&y)[N]) {
-  Raw<T, OP, N> raw;
+  Raw<T, OP, N, WHOLE> raw;
   raw.load(p, row, col, step);
   raw.get(p, y);
 }
 
-template <typename T>
+template <typename T, bool WHOLE>
 __device__ __forceinline__ void store_sum(const Args& p, int64_t row, int64_t col, const F8x& h) {
   Eight<T> e;
   e.set(h);
-  e.store(static_cast<T*>(p.sum) + row * p.ld_sum, col, p.n, p.vec_sum);
+  T* to = static_cast<T*>(p.sum) + row * p.ld_sum;
+  if constexpr (WHOLE) {
+    if (col < p.n) e.store(to + col);
+  } else {
+    e.store_some(to, col, p.n, p.vec_sum);
+  }
 }
 
 __device__ __forceinline__ float squares(const F8x& h, float ss) {
@@ -162,21 +177,21 @@ __device__ __forceinline__ F8x normed(const Args& p, F8x h, float rstd, const F8
   return h;
 }
 
-// Sums (or maxima) over the `warps` warps of a row.  Each call takes shared words
-// of its own, so that none waits for the reads of the one before.
+// Sums (or maxima) over the `warps` warps of a row, which meet at a barrier of their
+// own.  Calls take turns with two sets of words: a set is written again only behind
+// the barrier of the call in between.
 template <typename V, typename F>
-__device__ __forceinline__ V over_row(V v, V* shared, int first_warp, int warps, F&& f) {
+__device__ __forceinline__ V over_row(V v, V* shared, int row_in_block, int warps, F&& f) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
   if (warps == 1) return v;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  if (lane == 0) shared[warp] = v;
-  __syncthreads();
-  v = shared[first_warp + (lane < warps ? lane : 0)];
-  V rest = lane < warps ? v : V(0);
+  const int lane = threadIdx.x & 31;
+  if (lane == 0) shared[threadIdx.x >> 5] = v;
+  asm volatile("bar.sync %0, %1;" ::"r"(row_in_block + 1), "r"(warps * 32) : "memory");
+  v = lane < warps ? shared[row_in_block * warps + lane] : V(0);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) rest = f(rest, __shfl_xor_sync(0xffffffffu, rest, o));
-  return rest;
+  for (int o = 16; o > 0; o >>= 1) v = f(v, __shfl_xor_sync(0xffffffffu, v, o));
+  return v;
 }
 __device__ __forceinline__ float add_f(float a, float b) { return a + b; }
 __device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return max(a, b); }
@@ -211,9 +226,9 @@ __device__ __forceinline__ void block_codes(const uint32_t (&m)[N], uint32_t (&c
 
 // N pieces of a row, `step` columns apart, to codes and scales.  top: the row's
 // maximum (QI8_Q_TOKEN); t: the thread's place in the row.
-template <int N>
-__device__ __forceinline__ void emit_row(const Args& p, const F8x (&y)[N], int64_t row, int64_t col0, int step, uint32_t top,
-                                         bool live) {
+template <bool WHOLE, int N>
+__device__ __forceinline__ void emit_row(const Args& p, const F8x (&y)[N], int64_t row, int64_t col0, int step,
+                                         uint32_t top) {
   uint8_t* q = static_cast<uint8_t*>(p.q) + row * p.ld_q;
   if (p.mode == QI8_Q_FP8) {
     uint32_t m[N], code[N];
@@ -224,8 +239,8 @@ __device__ __forceinline__ void emit_row(const Args& p, const F8x (&y)[N], int64
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       const int64_t col = col0 + i * step;
-      if (!live || col >= p.n) continue;
-      store_codes(q, col, p.n, f8_codes(y[i], f8_inverse(code[i])), p.vec_q);
+      if (col >= p.n) continue;
+      store_codes<WHOLE>(q, col, p.n, f8_codes(y[i], f8_inverse(code[i])), p.vec_q);
       if ((threadIdx.x & 15) == 0) scale[col / F8_BLOCK] = (uint8_t)code[i];
     }
   } else {
@@ -242,8 +257,8 @@ __device__ __forceinline__ void emit_row(const Args& p, const F8x (&y)[N], int64
         s = i8_scale(max16(amax_bits(y[i])), 1e-8f);
         inv = __frcp_rn(s);
       }
-      if (!live || col >= p.n) continue;
-      store_codes(q, col, p.n, i8_codes(y[i], inv), p.vec_q);
+      if (col >= p.n) continue;
+      store_codes<WHOLE>(q, col, p.n, i8_codes(y[i], inv), p.vec_q);
       if (p.mode == QI8_Q_TOKEN ? col == 0 : (threadIdx.x & 15) == 0) scale[p.mode == QI8_Q_TOKEN ? 0 : col / F8_BLOCK] = s;
     }
   }
@@ -255,45 +270,40 @@ __device__ __forceinline__ void emit_row(const Args& p, const F8x (&y)[N], int64
 // 4096 bf16 with a residual takes 24.2 us so, 27 with a block for each row.
 constexpr int ROW_THREADS = 512;
 
-template <typename T, int OP, int CHUNKS>
+template <typename T, int OP, int CHUNKS, bool WHOLE>
 __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const __grid_constant__ Args p, const int warps) {
-  __shared__ float sums[2][32];
+  __shared__ float sums[2][32], again[2][32];
   __shared__ uint32_t tops[2][32];
-  const int warp = threadIdx.x >> 5;
-  const int mine = warp / warps, first_warp = mine * warps, step = warps * 256;
-  const int64_t col0 = (threadIdx.x - first_warp * 32) * 8, per = (blockDim.x >> 5) / warps;
+  const int mine = (threadIdx.x >> 5) / warps, step = warps * 256;
+  const int64_t col0 = (threadIdx.x - mine * warps * 32) * 8, per = (blockDim.x >> 5) / warps;
   const int64_t stride = gridDim.x * per;
-  // rows past the end take part in the barriers
-  auto in_range = [&](int64_t row) { return row < p.rows ? row : p.rows - 1; };
-  wait_for_last_kernel();
-  Raw<T, OP, CHUNKS> raw;
   int64_t row = blockIdx.x * per + mine;
-  raw.load(p, in_range(row), col0, step);
+  wait_for_last_kernel();
+  if (row >= p.rows) return;
+  Raw<T, OP, CHUNKS, WHOLE> raw;
+  raw.load(p, row, col0, step);
   F8x w[CHUNKS];
   if (OP == NORM && p.weight)
 #pragma unroll
-    for (int c = 0; c < CHUNKS; ++c) w[c] = load_weight(p, col0 + c * step);
-  int turn = 0;
-  for (int64_t first = blockIdx.x * per; first < p.rows; first += stride, row += stride, turn ^= 1) {
-    const bool live = row < p.rows;
+    for (int c = 0; c < CHUNKS; ++c) w[c] = load_weight<WHOLE>(p, col0 + c * step);
+  for (int turn = 0; row < p.rows; row += stride, turn ^= 1) {
     F8x y[CHUNKS];
     raw.get(p, y);
-    if (first + stride < p.rows) raw.load(p, in_range(row + stride), col0, step);
+    if (row + stride < p.rows) raw.load(p, row + stride, col0, step);
     if constexpr (OP == NORM) {
       float ss = 0.0f;
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) ss = squares(y[c], ss);
-      if (p.sum && live)
+      if (p.sum)
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) store_sum<T>(p, row, col0 + c * step, y[c]);
-      ss = over_row(ss, sums[0], first_warp, warps, add_f);
+        for (int c = 0; c < CHUNKS; ++c) store_sum<T, WHOLE>(p, row, col0 + c * step, y[c]);
+      ss = over_row(ss, sums[turn], mine, warps, add_f);
       const bool smaller = isinf(ss);
-      if (__syncthreads_or(smaller)) {  // a barrier before the next row's sums, too
-        float s2 = 0.0f;
+      if (smaller) {  // the whole row
+        ss = 0.0f;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) s2 = squares(scaled(y[c], SMALLER), s2);
-        s2 = over_row(s2, sums[1], first_warp, warps, add_f);
-        if (smaller) ss = s2;
+        for (int c = 0; c < CHUNKS; ++c) ss = squares(scaled(y[c], SMALLER), ss);
+        ss = over_row(ss, again[turn], mine, warps, add_f);
       }
       const float rstd = root(p, ss, smaller);
 #pragma unroll
@@ -303,9 +313,9 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const __grid_constant_
     if (p.mode == QI8_Q_TOKEN) {
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) top = max(top, amax_bits(y[c]));
-      top = over_row(top, tops[turn], first_warp, warps, max_u);
+      top = over_row(top, tops[turn], mine, warps, max_u);
     }
-    emit_row(p, y, row, col0, step, top, live);
+    emit_row<WHOLE>(p, y, row, col0, step, top);
   }
 }
 
@@ -314,7 +324,7 @@ constexpr int LONG_THREADS = 1024;
 
 template <typename T, int OP>
 __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_constant__ Args p) {
-  __shared__ float sums[2][32];
+  __shared__ float sums[32], again[32];
   __shared__ uint32_t tops[32];
   constexpr int STEP = LONG_THREADS * 8;
   const int64_t row = blockIdx.x, col0 = threadIdx.x * 8;
@@ -324,27 +334,27 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_con
   if constexpr (OP == NORM) {
     float ss = 0.0f;
     for (int64_t col = col0; col < p.n; col += STEP) {
-      row_values<T, OP>(p, row, col, STEP, y);
+      row_values<T, OP, false>(p, row, col, STEP, y);
       ss = squares(y[0], ss);
-      if (p.sum) store_sum<T>(p, row, col, y[0]);
+      if (p.sum) store_sum<T, false>(p, row, col, y[0]);
     }
-    ss = over_row(ss, sums[0], 0, LONG_THREADS / 32, add_f);
+    ss = over_row(ss, sums, 0, LONG_THREADS / 32, add_f);
     const bool smaller = isinf(ss);  // the same for all threads
     if (smaller) {
       ss = 0.0f;
       for (int64_t col = col0; col < p.n; col += STEP) {
-        row_values<T, OP>(p, row, col, STEP, y);
+        row_values<T, OP, false>(p, row, col, STEP, y);
         ss = squares(scaled(y[0], SMALLER), ss);
       }
-      ss = over_row(ss, sums[1], 0, LONG_THREADS / 32, add_f);
+      ss = over_row(ss, again, 0, LONG_THREADS / 32, add_f);
     }
     rstd = root(p, ss, smaller);
   }
   auto final_values = [&](int64_t col) {
-    row_values<T, OP>(p, row, col, STEP, y);
+    row_values<T, OP, false>(p, row, col, STEP, y);
     if constexpr (OP == NORM) {
       F8x w;
-      if (p.weight) w = load_weight(p, col);
+      if (p.weight) w = load_weight<false>(p, col);
       y[0] = normed(p, y[0], rstd, w);
     }
   };
@@ -362,7 +372,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_con
     else
 #pragma unroll
       for (int i = 0; i < 4; ++i) y[0].v[i] = make_float2(0.0f, 0.0f);
-    emit_row(p, y, row, col, 0, m, true);
+    emit_row<false>(p, y, row, col, 0, m);
   }
 }
 
@@ -370,7 +380,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_con
 // STEPS neighbouring blocks of one row.
 constexpr int THREADS = 256;
 
-template <typename T, int OP, int STEPS>
+template <typename T, int OP, int STEPS, bool WHOLE>
 __global__ void __launch_bounds__(THREADS) block_kernel(const __grid_constant__ Args p, const unsigned groups) {
   const int lane = threadIdx.x & 31;
   const unsigned unit = blockIdx.x * (THREADS / 32) + (threadIdx.x >> 5);
@@ -379,16 +389,16 @@ __global__ void __launch_bounds__(THREADS) block_kernel(const __grid_constant__ 
   const int64_t col0 = (int64_t)(unit - row * groups) * (STEPS * 256) + lane * 8;
   wait_for_last_kernel();
   F8x y[STEPS];
-  row_values<T, OP>(p, row, col0, 256, y);
-  emit_row(p, y, row, col0, 256, 0, true);
+  row_values<T, OP, WHOLE>(p, row, col0, 256, y);
+  emit_row<WHOLE>(p, y, row, col0, 256, 0);
 }
 
 template <typename T, int OP, int STEPS>
 int launch_blocks(const Args& p, cudaStream_t st) {
   const int64_t groups = (p.blocks + 2 * STEPS - 1) / (2 * STEPS), units = p.rows * groups;
   QI8_REQUIRE(units < (1ll << 32) - THREADS, QI8_ESHAPE, "%lld rows of %lld", (long long)p.rows, (long long)p.n);
-  return launch_early("block_kernel launch", block_kernel<T, OP, STEPS>,
-                      dim3((unsigned)((units + THREADS / 32 - 1) / (THREADS / 32))), THREADS, 0, 1, st, p,
+  return launch_early("block_kernel launch",
+                      p.whole() ? block_kernel<T, OP, STEPS, true> : block_kernel<T, OP, STEPS, false>, dim3((unsigned)((units + THREADS / 32 - 1) / (THREADS / 32))), THREADS, 0, 1, st, p,
                       (unsigned)groups);
 }
 
@@ -396,17 +406,19 @@ template <typename T, int OP, int CHUNKS>
 int launch_rows(const Args& p, cudaStream_t st) {
   const int warps = (int)((p.n + 256 * CHUNKS - 1) / (256 * CHUNKS));
   const int per = warps >= 8 ? 1 : 8 / warps;  // rows per thread block
-  static int resident[64][ROW_THREADS / 32 + 1];  // blocks per SM, by device and warps
+  const bool whole = p.whole();
+  auto kern = whole ? row_kernel<T, OP, CHUNKS, true> : row_kernel<T, OP, CHUNKS, false>;
+  static int resident[2][64][ROW_THREADS / 32 + 1];  // blocks per SM, by device and warps
   int dev = 0, blocks = 0;
   QI8_CUDA(cudaGetDevice(&dev));
-  if (dev < 64) blocks = resident[dev][warps * per];
+  if (dev < 64) blocks = resident[whole][dev][warps * per];
   if (blocks == 0) {
-    QI8_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, row_kernel<T, OP, CHUNKS>, warps * per * 32, 0));
-    if (dev < 64) resident[dev][warps * per] = blocks;
+    QI8_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&blocks, kern, warps * per * 32, 0));
+    if (dev < 64) resident[whole][dev][warps * per] = blocks;
   }
   const int64_t groups = (p.rows + per - 1) / per, most = (int64_t)blocks * sm_count();
-  return launch_early("row_kernel launch", row_kernel<T, OP, CHUNKS>, dim3((unsigned)(groups < most ? groups : most)),
-                      warps * per * 32, 0, 1, st, p, warps);
+  return launch_early("row_kernel launch", kern, dim3((unsigned)(groups < most ? groups : most)), warps * per * 32, 0, 1, st,
+                      p, warps);
 }
 
 template <typename T, int OP>

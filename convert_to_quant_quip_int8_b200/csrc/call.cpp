@@ -217,10 +217,10 @@ int64_t row_stride(const at::Tensor& t) {
   const int64_t d = t.dim(), n = t.size(d - 1);
   if (t.stride(d - 1) != 1 && n > 1) return -1;
   if (d == 1 || t.numel() == n) return n;
-  int64_t step = 0, ld = 0;  // of the next outer dimension with more than one row
+  int64_t step = -1, ld = 0;  // stride that the next outer dimension has to have
   for (int64_t i = d - 2; i >= 0; --i) {
     if (t.size(i) == 1) continue;
-    if (step == 0) ld = t.stride(i);
+    if (step < 0) ld = t.stride(i);
     else if (t.stride(i) != step) return -1;
     step = t.stride(i) * t.size(i);
   }

@@ -117,11 +117,18 @@ struct Eight {
 #pragma unroll
     for (int i = 0; i < 8; ++i) e[i] = col + i < n ? row[col + i] : T(0.0f);
   }
-  // vec: the row starts on a 16-byte boundary (col is a multiple of 8)
-  __device__ __forceinline__ void store(T* row, int64_t col, int64_t n, bool vec) const {
-    if (vec && col + 8 <= n) {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
-      for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(row + col)[i] = v[i];
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) v[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void store(T* at) const {
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) reinterpret_cast<uint4*>(at)[i] = v[i];
+  }
+  // vec: the row starts on a 16-byte boundary (col is a multiple of 8)
+  __device__ __forceinline__ void store_some(T* row, int64_t col, int64_t n, bool vec) const {
+    if (vec && col + 8 <= n) {
+      store(row + col);
     } else {
       const T* e = reinterpret_cast<const T*>(v);
 #pragma unroll
@@ -193,9 +200,11 @@ __device__ __forceinline__ uint2 i8_codes(const F8x& f, float inv) {
   }
   return make_uint2(w[0], w[1]);
 }
-// Eight codes of a row.  vec: rows start on 8-byte boundaries.
+// Eight codes of a row.  vec: rows start on 8-byte boundaries; WHOLE: and are whole
+// eights long.
+template <bool WHOLE = false>
 __device__ __forceinline__ void store_codes(uint8_t* row, int64_t col, int64_t n, uint2 c, bool vec) {
-  if (vec && col + 8 <= n) {
+  if (WHOLE || (vec && col + 8 <= n)) {
     *reinterpret_cast<uint2*>(row + col) = c;
   } else {
 #pragma unroll

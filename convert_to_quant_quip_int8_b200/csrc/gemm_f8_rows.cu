@@ -59,13 +59,12 @@ __device__ __forceinline__ uint32_t below(uint32_t w, int k, int K) {
   return left >= 4 ? w : left <= 0 ? 0u : w & ((1u << (8 * left)) - 1u);
 }
 
-// 2^(ea + eb) for two scale bytes as two factors, the second of which is 1 but for
-// sums that fp32's exponent does not hold: multiplied one after the other they
-// overflow only where the result does.
+// 2^(ea + eb) for two scale bytes as two factors of about half the exponent each:
+// multiplied one after the other they overflow, or vanish, only where the result does.
 __device__ __forceinline__ float2 both_scales(uint32_t a, uint32_t b) {
   if (a == 255u || b == 255u) return make_float2(__uint_as_float(0x7fffffffu), 1.0f);
-  const int e = (int)(a + b) - 254, in = e < -126 ? -126 : e > 127 ? 127 : e;
-  return make_float2(__uint_as_float((uint32_t)(in + 127) << 23), __uint_as_float((uint32_t)(e - in + 127) << 23));
+  const int e = (int)(a + b) - 254, h = e >> 1;
+  return make_float2(__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(e - h + 127) << 23));
 }
 
 template <typename X, int NT>  // X uint8_t: codes; NT groups of eight tokens

@@ -75,7 +75,7 @@ dequant_kernel(const uint8_t* __restrict__ q, int64_t rows, int64_t n, int64_t l
     for (int j = 0; j < 4; ++j) f.v[j] = f8_unpack2((w[j >> 1] >> (16 * (j & 1))) & 0xffffu);
     Eight<T> e;
     e.set(scaled(f, s));
-    e.store(out + row * ld_out, col, n, vec);
+    e.store_some(out + row * ld_out, col, n, vec);
   }
 }
 

@@ -127,7 +127,8 @@ def test_blocks_that_are_not_finite(bad):
 def test_quantizers_take_strides_and_leading_dimensions():
     big = wide(6, 10, 300, dtype=BF)
     for x in (big[:, 1:7, 3:260], big.transpose(0, 1), big[::2], big[:, :, ::3], big[0, 0], big[:, :0], big[..., :0],
-              big[:1, :1].expand(3, 4, 300), big.view(-1)[1:1 + 59 * 300].view(59, 300)):
+              big[:1, :1].expand(3, 4, 300), big[:, :1].expand(6, 4, 300), big[:1].expand(5, 10, 300), big[0, :3, None].expand(
+                  3, 4, 300), big[:, 0].unsqueeze(1), big[:, 2:3, 8:], big.view(-1)[1:1 + 59 * 300].view(59, 300)):
         q, s = F8.act_quant_fp8(x)
         assert q.shape == x.shape and s.shape == (*x.shape[:-1], -(-x.shape[-1] // 128))
         if x.numel():
@@ -220,6 +221,18 @@ def test_extreme_scales(m):
     b_s[1, 2] = 255
     y = F8.fp8_gemm(a, a_s.view(E8), b, b_s.view(E8), out_dtype=F32)
     assert torch.isnan(y[:, 128:]).all() and (y[:, :128] == k).all()
+
+
+@pytest.mark.parametrize("m", [1, 20, 300, 2000])
+@pytest.mark.parametrize("a_code,b_code", [(0, 254), (254, 0), (1, 253), (0, 0), (200, 200)])
+def test_scales_at_the_ends(m, a_code, b_code):
+    n, k = 2600, 130
+    a, b = torch.ones(m, k).to(E4).cuda(), torch.ones(n, k).to(E4).cuda()
+    a_s = torch.full((m, 2), a_code, dtype=torch.uint8).cuda().view(E8)
+    b_s = torch.full((21, 2), b_code, dtype=torch.uint8).cuda().view(E8)
+    y = F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)
+    # 2^(a + b - 254) k, or what fp32 makes of it
+    assert (y == torch.tensor(float(k) * 2.0 ** (a_code + b_code - 254), dtype=torch.float64).float().item()).all()
 
 
 @pytest.mark.parametrize("m", [1, 12, 40, 300])
@@ -334,6 +347,45 @@ def test_captured_graphs_replay_with_new_inputs(m):
         torch.cuda.synchronize()
         expected = F8.fp8_linear(x, *wq)
         assert all(torch.equal(expected, o) for o in outs)
+
+
+@pytest.mark.parametrize("m", [1, 5, 16, 40, 300])
+def test_two_streams_at_once(m):
+    x = [randn(m, 2100, seed=s, dtype=BF) for s in (1, 2)]
+    w = [F8.weight_quant_fp8(randn(1900, 2100, seed=s, scale=0.02, dtype=BF)) for s in (3, 4)]
+    expected = [F8.fp8_linear(*p) for p in ((x[0], *w[0]), (x[1], *w[1]))]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    outs = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                outs[i].append(F8.fp8_linear(x[i], *w[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(y, expected[i]) for y in outs[i])
+
+
+@pytest.mark.parametrize("m", [1, 9, 40, 600])
+def test_operands_written_just_before(m):
+    # kernels that start while the one before ends must not read what it still writes
+    n, k = 1500, 2048
+    xs, ws = [randn(m, k, seed=s, dtype=BF) for s in range(6)], [randn(n, k, seed=s, scale=0.05, dtype=BF) for s in range(6)]
+    expected = [F8.fp8_linear(x, *F8.weight_quant_fp8(w)) for x, w in zip(xs, ws)]
+    torch.cuda.synchronize()
+    x, w = torch.empty_like(xs[0]), torch.empty_like(ws[0])
+    q, s = F8.weight_quant_fp8(ws[0])
+    got = []
+    for i in list(range(6)) * 5:
+        x.copy_(xs[i])
+        w.copy_(ws[i])
+        q2, s2 = F8.weight_quant_fp8(w)
+        q.copy_(q2)
+        s.copy_(s2)
+        got.append(F8.fp8_linear(x, q, s))
+        got.append(F8.fp8_linear(x, *F8.weight_quant_fp8(w)))
+    for j, y in enumerate(got):
+        assert torch.equal(y, expected[j // 2 % 6])
 
 
 def test_rows_behind_the_result_are_left_alone():

@@ -125,6 +125,26 @@ def test_norm_takes_strides(dtype):
             assert torch.equal(got[2], (x.double() + r.double()).to(dtype))
 
 
+def test_norm_of_many_rows_and_broadcast_ones():
+    # more rows than resident blocks, several rows per block and one
+    for rows, n in ((5000, 256), (2777, 1536), (1500, 4096), (700, 12288), (900, 4099)):
+        x, r = randn(rows, n, seed=rows, dtype=BF), randn(rows, n, seed=n, scale=2.0, dtype=BF)
+        x[rows // 2] *= 2.0 ** 70
+        for output in ("fp8", "int8"):
+            q, s, h = FQ.rms_norm_quant(x, residual=r, output=output)
+            want, y = exact_norm(x, None, 1e-6, r)
+            assert torch.equal(h, want)
+            check_codes(q, s, y, DELTA * y.abs(), output)
+    x = randn(6, 256, dtype=BF)
+    for v in (x[:, None].expand(6, 3, 256), x[None].expand(4, 6, 256), x[:1].expand(5, 256)):
+        q, s, h = FQ.rms_norm_quant(v, residual=v)
+        e = FQ.rms_norm_quant(v.contiguous(), residual=v.contiguous())
+        assert all(torch.equal(a.double(), b.double()) for a, b in zip((q, s, h), e))
+        q, s = FQ.gated_act_quant(v, v)
+        e = FQ.gated_act_quant(v.contiguous(), v.contiguous())
+        assert torch.equal(q.double(), e[0].double()) and torch.equal(s.double(), e[1].double())
+
+
 @pytest.mark.parametrize("output", ["fp8", "int8", "int8_block"])
 @pytest.mark.parametrize("n", [256, 40064])
 def test_norm_of_rows_out_of_the_ordinary(output, n):
@@ -249,6 +269,16 @@ def test_int8_outputs_feed_the_int8_products():
     y = ops.gemm_i8(q, qr, s, L.QI8_S_ROW, sr, L.QI8_S_ROW, None, F32)
     ref = (q.double() @ qr.double().T) * s.double() * sr.double().view(1, -1)
     assert ((y.double() - ref).abs() <= 2.0 ** -22 * ref.abs()).all()
+
+
+@pytest.mark.parametrize("rows,n", [(3, 64), (5, 2731), (77, 300), (16, 4096)])
+@pytest.mark.parametrize("out", [BF, HF, F32])
+def test_int8_read_back(rows, n, out):
+    q = torch.randint(-127, 128, (rows, n), dtype=torch.int8, device="cuda")
+    s = randn(rows, 1).abs()
+    assert torch.equal(ops.dequant(q, s, L.QI8_S_ROW, out_dtype=out), (q.float() * s).to(out))
+    assert torch.equal(ops.dequant(q, s[:1, 0], L.QI8_S_SCALAR, out_dtype=out), (q.float() * s[0]).to(out))
+    assert torch.equal(ops.dequant(q[:, 1:], s, L.QI8_S_ROW, out_dtype=out), (q[:, 1:].float() * s).to(out))
 
 
 def test_refusals():
