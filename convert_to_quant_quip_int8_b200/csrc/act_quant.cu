@@ -30,17 +30,44 @@ struct Args {
   bool whole() const { return n % 8 == 0 && vec && vec_q && (!weight || vec_weight) && (!sum || vec_sum); }
 };
 
-// x 2^t / (1 + 2^t) ... as x / (1 + 2^-t): 0 where 2^-t passes fp32, as it should be
-// (MUFU's exp2 and reciprocal: 2 and 1 units in the last place)
-__device__ __forceinline__ float2 swish(float2 x, float2 minus_t) {
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// 2 units in the last place
+__device__ __forceinline__ float2 exp2_of(float2 x) {
   float2 e;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(minus_t.x));
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(minus_t.y));
-  e = __fadd2_rn(e, make_float2(1.0f, 1.0f));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.x) : "f"(x.x));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e.y) : "f"(x.y));
+  return e;
+}
+
+// x / (1 + 2^-t): 0 where 2^-t passes fp32, as it should be
+__device__ __forceinline__ float2 swish(float2 x, float2 minus_t) {
+  const float2 e = __fadd2_rn(exp2_of(minus_t), both(1.0f));
   return make_float2(__fdividef(x.x, e.x), __fdividef(x.y, e.y));
 }
 
-__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+// x Phi(x) = max(x, 0) - |x| h, h = Phi(-|x|) = exp(-x^2 / 2) R(|x|).  R, half the
+// scaled complementary error function of |x| / sqrt(2), falls like 1 / |x|: t times a
+// polynomial in t = 1 / (1 + 0.27 |x|), fitted here by least squares weighted
+// towards the largest relative error, which is 2.3e-8 (with fp32's roundings h is off
+// by under 4e-7 of itself up to |x| = 3 and x Phi(x) by 2e-7 of x everywhere).  erff
+// has two cases, of which a warp meets both: 4096 x 10240 took 58 us with it.
+__device__ __forceinline__ float2 gelu(float2 x) {
+  const float2 u = make_float2(fabsf(x.x), fabsf(x.y));
+  const float2 d = __ffma2_rn(u, both(0.27f), both(1.0f));
+  const float2 t = make_float2(__fdividef(1.0f, d.x), __fdividef(1.0f, d.y));
+  float2 r = both(0.0288554337f);
+  r = __ffma2_rn(r, t, both(-0.125953481f));
+  r = __ffma2_rn(r, t, both(0.168642223f));
+  r = __ffma2_rn(r, t, both(-0.0678447261f));
+  r = __ffma2_rn(r, t, both(0.106836453f));
+  r = __ffma2_rn(r, t, both(0.0724932477f));
+  r = __ffma2_rn(r, t, both(0.101690575f));
+  r = __ffma2_rn(r, t, both(0.107560746f));
+  r = __ffma2_rn(r, t, both(0.107719541f));
+  const float2 e = exp2_of(__fmul2_rn(__fmul2_rn(u, u), both(-0.72134752f)));  // -log2(e) / 2
+  const float2 h = __fmul2_rn(e, __fmul2_rn(r, t));
+  return __ffma2_rn(make_float2(-u.x, -u.y), h, make_float2(fmaxf(x.x, 0.0f), fmaxf(x.y, 0.0f)));
+}
 
 // y = act(g) * up
 template <int ACT>
@@ -53,7 +80,7 @@ __device__ __forceinline__ F8x gate(const F8x& g, const F8x& up) {
     if constexpr (ACT == QI8_ACT_SILU) {
       a = swish(x, __fmul2_rn(x, both(-1.4426950408889634f)));  // -log2(e)
     } else if constexpr (ACT == QI8_ACT_GELU) {
-      a = make_float2(gelu_erf(x.x), gelu_erf(x.y));
+      a = gelu(x);
     } else {
       // 0.5 x (1 + tanh(u)) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
       const float2 c = __ffma2_rn(__fmul2_rn(x, x), both(-0.10294324f), both(-2.3022082f));
@@ -225,7 +252,7 @@ __device__ __forceinline__ void block_codes(const uint32_t (&m)[N], uint32_t (&c
 }
 
 // N pieces of a row, `step` columns apart, to codes and scales.  top: the row's
-// maximum (QI8_Q_TOKEN); t: the thread's place in the row.
+// maximum (QI8_Q_TOKEN).
 template <bool WHOLE, int N>
 __device__ __forceinline__ void emit_row(const Args& p, const F8x (&y)[N], int64_t row, int64_t col0, int step,
                                          uint32_t top) {
@@ -267,7 +294,7 @@ __device__ __forceinline__ void emit_row(const Args& p, const F8x (&y)[N], int64
 // Whole rows in registers: `warps` warps hold one, eight columns per lane and
 // chunk, and a thread block holds as many rows as fit.  Blocks stay and go on to
 // other rows, whose loads are under way while these are reduced and stored: 4096 x
-// 4096 bf16 with a residual takes 24.2 us so, 27 with a block for each row.
+// 4096 bf16 with a residual takes 21.6 us so (5.4 TB/s), 27 with a block for each row.
 constexpr int ROW_THREADS = 512;
 
 template <typename T, int OP, int CHUNKS, bool WHOLE>
@@ -397,9 +424,10 @@ template <typename T, int OP, int STEPS>
 int launch_blocks(const Args& p, cudaStream_t st) {
   const int64_t groups = (p.blocks + 2 * STEPS - 1) / (2 * STEPS), units = p.rows * groups;
   QI8_REQUIRE(units < (1ll << 32) - THREADS, QI8_ESHAPE, "%lld rows of %lld", (long long)p.rows, (long long)p.n);
+  const dim3 grid((unsigned)((units + THREADS / 32 - 1) / (THREADS / 32)));
   return launch_early("block_kernel launch",
-                      p.whole() ? block_kernel<T, OP, STEPS, true> : block_kernel<T, OP, STEPS, false>, dim3((unsigned)((units + THREADS / 32 - 1) / (THREADS / 32))), THREADS, 0, 1, st, p,
-                      (unsigned)groups);
+                      p.whole() ? block_kernel<T, OP, STEPS, true> : block_kernel<T, OP, STEPS, false>, grid, THREADS, 0, 1,
+                      st, p, (unsigned)groups);
 }
 
 template <typename T, int OP, int CHUNKS>
@@ -424,15 +452,15 @@ int launch_rows(const Args& p, cudaStream_t st) {
 template <typename T, int OP>
 int launch_type(const Args& p, cudaStream_t st) {
   if constexpr (OP != NORM) {
-    // few units: one step each spreads them over more SMs
     if (p.mode != QI8_Q_TOKEN)
-      return p.blocks < 4 || p.rows * p.blocks < 4 * 8 * 148 * 4 ? launch_blocks<T, OP, 1>(p, st)
-                                                                 : launch_blocks<T, OP, 2>(p, st);
+      // Two steps per warp from 4096 blocks of 128 columns on: 4096 x 10240 gated takes
+      // 38.7 us so and 40.3 with one, 16 x 10240 1.54 and 1.47.
+      return p.rows * p.blocks < 4096 ? launch_blocks<T, OP, 1>(p, st) : launch_blocks<T, OP, 2>(p, st);
   }
   if constexpr (OP != PLAIN) {
     // Two chunks per lane from 2048 columns on (4096 x 2048 takes the same either way,
-    // 4096 x 4096 24.2 us in place of 25.1; 8192 x 256 would take 9.3 in place of 4.5);
-    // four need the registers of half as many blocks: only where two do not reach.
+    // 4096 x 4096 gains 4 %, 8192 x 256 would take twice as long); four need the registers
+    // of half as many blocks: only where two do not reach.
     if (p.n <= 2048) return launch_rows<T, OP, 1>(p, st);
     if (p.n <= 8192) return launch_rows<T, OP, 2>(p, st);
     if constexpr (sizeof(T) == 2)
@@ -534,7 +562,7 @@ extern "C" int qi8_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int6
   p.rows = rows;
   p.n = n;
   p.blocks = f8_blocks(n);
-  p.eps = (float)eps;
+  p.eps = eps > 0.0 && eps < 1.2e-38 ? 1.2e-38f : (float)eps;  // one above 0 stays so: zero rows are zeros then
   p.inv_n = (float)(1.0 / (double)n);
   p.mode = mode;
   p.vec = rows_aligned(x, ld_x, size, 16) && (!residual || rows_aligned(residual, ld_residual, size, 16));

@@ -137,7 +137,7 @@ static_assert(SMEM <= 232448 && SCALES + SLOTS * SLOT <= (int)TMEM_COLS && ACC1 
 struct Args {
   F8Gemm g;
   int m_tiles, n_tiles;
-  int bn;  // features of a tile, a multiple of 16 up to 256
+  int bn;  // features of a tile, a multiple of 32 up to 256
   bool words_a, words_b, vec_out;
   unsigned int* status;
 };
