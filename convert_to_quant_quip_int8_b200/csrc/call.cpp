@@ -9,12 +9,15 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <ATen/EmptyTensor.h>
 #include <c10/core/GradMode.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAFunctions.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <optional>
 #include <type_traits>
 #include <vector>
 
@@ -203,6 +206,12 @@ PyObject* moe_w4(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
 
 // ---------------------------------------------------------------- fp8
 
+// at::empty on the current device, past the dispatcher: three of them were half of a call.
+at::Tensor empty(at::IntArrayRef sizes, at::ScalarType type) {
+  return at::detail::empty_generic(sizes, c10::cuda::CUDACachingAllocator::get(),
+                                   c10::DispatchKeySet(c10::DispatchKey::CUDA), type, std::nullopt);
+}
+
 constexpr int64_t F8_BLOCK = 128;
 int64_t blocks(int64_t n) { return (n + F8_BLOCK - 1) / F8_BLOCK; }
 
@@ -240,8 +249,8 @@ bool codes(const at::Tensor& q, const at::Tensor& s, bool weight, int device) {
   return s.size(d - 1) == blocks(q.size(d - 1));
 }
 
-std::vector<int64_t> with_last(const at::Tensor& t, int64_t last) {
-  std::vector<int64_t> shape(t.sizes().begin(), t.sizes().end());
+c10::SmallVector<int64_t, 6> with_last(const at::Tensor& t, int64_t last) {
+  c10::SmallVector<int64_t, 6> shape(t.sizes().begin(), t.sizes().end());
   shape.back() = last;
   return shape;
 }
@@ -249,9 +258,8 @@ std::vector<int64_t> with_last(const at::Tensor& t, int64_t last) {
 // Room for codes whose rows start on 16-byte boundaries.
 at::Tensor new_codes(const at::Tensor& like) {
   const int64_t n = like.size(-1), pitch = (n + 15) / 16 * 16;
-  const auto options = like.options().dtype(at::kFloat8_e4m3fn);
-  if (pitch == n) return at::empty(like.sizes(), options);
-  return at::empty(with_last(like, pitch), options).narrow(-1, 0, n);
+  if (pitch == n) return empty(like.sizes(), at::kFloat8_e4m3fn);
+  return empty(with_last(like, pitch), at::kFloat8_e4m3fn).narrow(-1, 0, n);
 }
 int64_t code_pitch(const at::Tensor& q) { return (q.size(-1) + 15) / 16 * 16; }
 
@@ -271,7 +279,7 @@ PyObject* quant_rows_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (!x || !numbers(*x, device)) Py_RETURN_NONE;
     const int64_t n = x->size(-1), ld = row_stride(*x);
     if (ld < 0) Py_RETURN_NONE;
-    at::Tensor q = new_codes(*x), s = at::empty(with_last(*x, blocks(n)), x->options().dtype(at::kFloat8_e8m0fnu));
+    at::Tensor q = new_codes(*x), s = empty(with_last(*x, blocks(n)), at::kFloat8_e8m0fnu);
     if (quant_rows_f8_fn(x->data_ptr(), code(x->scalar_type()), x->numel() / n, n, ld,
                          static_cast<uint8_t*>(q.data_ptr()), code_pitch(q), static_cast<uint8_t*>(s.data_ptr()),
                          stream(device)))
@@ -288,7 +296,7 @@ PyObject* quant_weight_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (!w || !numbers(*w, device) || w->dim() != 2) Py_RETURN_NONE;
     const int64_t n = w->size(0), k = w->size(1), ld = row_stride(*w);
     if (ld < 0) Py_RETURN_NONE;
-    at::Tensor q = new_codes(*w), s = at::empty({blocks(n), blocks(k)}, w->options().dtype(at::kFloat8_e8m0fnu));
+    at::Tensor q = new_codes(*w), s = empty({blocks(n), blocks(k)}, at::kFloat8_e8m0fnu);
     if (quant_weight_f8_fn(w->data_ptr(), code(w->scalar_type()), n, k, ld, static_cast<uint8_t*>(q.data_ptr()),
                            code_pitch(q), static_cast<uint8_t*>(s.data_ptr()), stream(device)))
       Py_RETURN_NONE;
@@ -309,8 +317,8 @@ bool f8_weight(PyObject* qo, PyObject* so, PyObject* bo, int64_t k, int device, 
   ld = row_stride(*q);
   return ld > 0;
 }
-at::Tensor workspace(const at::Tensor& like, int64_t bytes) {
-  return bytes > 0 ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+at::Tensor workspace(int64_t bytes) {
+  return bytes > 0 ? empty({bytes}, at::kByte) : at::Tensor();
 }
 
 // a, a_scale, b, b_scale, bias or None, output dtype
@@ -326,9 +334,9 @@ PyObject* gemm_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (ld_a < 0 || !f8_weight(args[2], args[3], args[4], k, device, b, b_s, bias, ld_b)) Py_RETURN_NONE;
     const int64_t n = b->size(0);
     const auto *ap = static_cast<const uint8_t*>(a->data_ptr()), *bp = static_cast<const uint8_t*>(b->data_ptr());
-    at::Tensor out = at::empty(with_last(*a, n), a->options().dtype(t));
+    at::Tensor out = empty(with_last(*a, n), t);
     const int64_t bytes = gemm_f8_bytes_fn(ap, m, k, ld_a, bp, n, ld_b);
-    at::Tensor ws = workspace(*a, bytes);
+    at::Tensor ws = workspace(bytes);
     if (gemm_f8_fn(ap, static_cast<const uint8_t*>(a_s->data_ptr()), m, k, ld_a, bp,
                    static_cast<const uint8_t*>(b_s->data_ptr()), n, ld_b, bias ? bias->data_ptr() : nullptr,
                    bias ? code(bias->scalar_type()) : 0, out.data_ptr(), code(t), n, bytes ? ws.data_ptr() : nullptr,
@@ -349,9 +357,9 @@ PyObject* linear_f8(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     if (ld < 0 || !f8_weight(args[1], args[2], args[3], k, device, b, b_s, bias, ld_b)) Py_RETURN_NONE;
     const int64_t n = b->size(0);
     const auto* bp = static_cast<const uint8_t*>(b->data_ptr());
-    at::Tensor out = at::empty(with_last(*x, n), x->options());
+    at::Tensor out = empty(with_last(*x, n), x->scalar_type());
     const int64_t bytes = linear_f8_bytes_fn(m, k, bp, n, ld_b);
-    at::Tensor ws = workspace(*x, bytes);
+    at::Tensor ws = workspace(bytes);
     const int dt = code(x->scalar_type());
     if (linear_f8_fn(x->data_ptr(), dt, m, k, ld, bp, static_cast<const uint8_t*>(b_s->data_ptr()), n, ld_b,
                      bias ? bias->data_ptr() : nullptr, bias ? code(bias->scalar_type()) : 0, out.data_ptr(), dt, n,
@@ -366,12 +374,12 @@ bool new_output(const at::Tensor& like, int64_t mode, at::Tensor& q, at::Tensor&
   const int64_t n = like.size(-1);
   if (mode == QI8_Q_FP8) {
     q = new_codes(like);
-    s = at::empty(with_last(like, blocks(n)), like.options().dtype(at::kFloat8_e8m0fnu));
+    s = empty(with_last(like, blocks(n)), at::kFloat8_e8m0fnu);
     return true;
   }
   if (mode != QI8_Q_TOKEN && (mode != QI8_Q_BLOCK || n % F8_BLOCK)) return false;
-  q = at::empty(like.sizes(), like.options().dtype(at::kChar));
-  s = at::empty(with_last(like, mode == QI8_Q_TOKEN ? 1 : n / F8_BLOCK), like.options().dtype(at::kFloat));
+  q = empty(like.sizes(), at::kChar);
+  s = empty(with_last(like, mode == QI8_Q_TOKEN ? 1 : n / F8_BLOCK), at::kFloat);
   return true;
 }
 
@@ -392,7 +400,7 @@ PyObject* rms_norm_quant(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
     const int64_t ld_r = r ? row_stride(*r) : 0;
     at::Tensor q, s, h;
     if (ld_r < 0 || !new_output(*x, mode, q, s)) Py_RETURN_NONE;
-    if (r) h = at::empty(x->sizes(), x->options());
+    if (r) h = empty(x->sizes(), x->scalar_type());
     if (norm_fn(x->data_ptr(), code(x->scalar_type()), x->numel() / n, n, ld, r ? r->data_ptr() : nullptr, ld_r,
                 w ? w->data_ptr() : nullptr, w ? code(w->scalar_type()) : 0, PyFloat_AS_DOUBLE(args[2]), (int)mode,
                 q.data_ptr(), mode == QI8_Q_FP8 ? code_pitch(q) : n, s.data_ptr(), r ? h.data_ptr() : nullptr, n,
@@ -445,7 +453,7 @@ PyObject* dequant(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         : kind == QI8_S_ROW ? s->numel() != rows
                             : kind != QI8_S_ROW_KBLOCK || block <= 0 || n % block || s->numel() != rows * (n / block))
       Py_RETURN_NONE;
-    at::Tensor out = at::empty(q->sizes(), q->options().dtype(t));
+    at::Tensor out = empty(q->sizes(), t);
     if (dequant8_fn(static_cast<const int8_t*>(q->data_ptr()), rows, n, static_cast<const float*>(s->data_ptr()),
                     (int)kind, (int)block, out.data_ptr(), code(t), stream(device)))
       Py_RETURN_NONE;
