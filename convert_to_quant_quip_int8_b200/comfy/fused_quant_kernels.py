@@ -37,7 +37,8 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: 
                    residual: Optional[torch.Tensor] = None, output: str = "fp8"
                    ) -> Union[Tuple[torch.Tensor, torch.Tensor], Tuple[torch.Tensor, torch.Tensor, torch.Tensor]]:
     """``(q, scale)`` of ``h / sqrt(mean(h^2) + eps) * weight`` over the last dimension; with ``residual``
-    ``h = x + residual``, rounded to x's dtype, and the result is ``(q, scale, h)``."""
+    ``h = x + residual``, rounded to x's dtype, and the result is ``(q, scale, h)``.  ``eps`` 0 (a row of zeros
+    is NaN then) or at least 1e-37."""
     return ops.rms_norm_quant(x, weight, eps, residual, _choice(_MODES, "output", output))
 
 

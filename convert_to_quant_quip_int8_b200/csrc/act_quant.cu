@@ -223,15 +223,24 @@ __device__ __forceinline__ V over_row(V v, V* shared, int row_in_block, int warp
 __device__ __forceinline__ float add_f(float a, float b) { return a + b; }
 __device__ __forceinline__ uint32_t max_u(uint32_t a, uint32_t b) { return max(a, b); }
 
-// A row whose squares pass fp32's range is summed again with values 2^-80 of
-// theirs: the largest becomes 2^48.
+// A row whose squares pass fp32's range is summed again with values 2^-80 of theirs
+// (the largest becomes 2^48), one whose squares vanish with 2^95 times its values
+// (these are 2^-54 to 2^45 then).  That is looked for where eps does not cover them.
 constexpr float SMALLER = 8.271806125530277e-25f;  // 2^-80
+constexpr float LARGER = 3.961408125713217e28f;    // 2^95
+constexpr float EPS_COVERS = 1e-20f, VANISHED = 7.888609052210118e-31f;  // 2^-100
 
-__device__ __forceinline__ float root(const Args& p, float ss, bool smaller) {
-  const float m = smaller ? ss * p.inv_n : fmaf(ss, p.inv_n, p.eps);  // eps would vanish beside the former
+// What the values of a row with this sum of squares are multiplied by before they are
+// squared again; 1: nothing.
+__device__ __forceinline__ float again_with(const Args& p, float ss) {
+  return isinf(ss) ? SMALLER : ss < VANISHED && p.eps < EPS_COVERS ? LARGER : 1.0f;
+}
+// 1 / root mean square of values times `factor`
+__device__ __forceinline__ float root(const Args& p, float ss, float factor) {
+  const float m = fmaf(ss, p.inv_n, p.eps * factor * factor);
   float r = rsqrtf(m);
   if (m > 0.0f && m < 3e38f) r *= fmaf(-0.5f * m * r, r, 1.5f);  // one step of Newton's: half a unit
-  return smaller ? r * SMALLER : r;
+  return r;
 }
 
 // The maxima of neighbouring blocks, two at a time: scale bytes are as good as the
@@ -325,14 +334,17 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const __grid_constant_
 #pragma unroll
         for (int c = 0; c < CHUNKS; ++c) store_sum<T, WHOLE>(p, row, col0 + c * step, y[c]);
       ss = over_row(ss, sums[turn], mine, warps, add_f);
-      const bool smaller = isinf(ss);
-      if (smaller) {  // the whole row
+      const float factor = again_with(p, ss);
+      if (factor != 1.0f) {  // the whole row
         ss = 0.0f;
 #pragma unroll
-        for (int c = 0; c < CHUNKS; ++c) ss = squares(scaled(y[c], SMALLER), ss);
+        for (int c = 0; c < CHUNKS; ++c) {
+          y[c] = scaled(y[c], factor);
+          ss = squares(y[c], ss);
+        }
         ss = over_row(ss, again[turn], mine, warps, add_f);
       }
-      const float rstd = root(p, ss, smaller);
+      const float rstd = root(p, ss, factor);
 #pragma unroll
       for (int c = 0; c < CHUNKS; ++c) y[c] = normed(p, y[c], rstd, w[c]);
     }
@@ -356,7 +368,7 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_con
   constexpr int STEP = LONG_THREADS * 8;
   const int64_t row = blockIdx.x, col0 = threadIdx.x * 8;
   wait_for_last_kernel();
-  float rstd = 1.0f;
+  float factor = 1.0f, rstd = 1.0f;
   F8x y[1];
   if constexpr (OP == NORM) {
     float ss = 0.0f;
@@ -366,23 +378,23 @@ __global__ void __launch_bounds__(LONG_THREADS) long_row_kernel(const __grid_con
       if (p.sum) store_sum<T, false>(p, row, col, y[0]);
     }
     ss = over_row(ss, sums, 0, LONG_THREADS / 32, add_f);
-    const bool smaller = isinf(ss);  // the same for all threads
-    if (smaller) {
+    factor = again_with(p, ss);  // the same for all threads
+    if (factor != 1.0f) {
       ss = 0.0f;
       for (int64_t col = col0; col < p.n; col += STEP) {
         row_values<T, OP, false>(p, row, col, STEP, y);
-        ss = squares(scaled(y[0], SMALLER), ss);
+        ss = squares(scaled(y[0], factor), ss);
       }
       ss = over_row(ss, again, 0, LONG_THREADS / 32, add_f);
     }
-    rstd = root(p, ss, smaller);
+    rstd = root(p, ss, factor);
   }
   auto final_values = [&](int64_t col) {
     row_values<T, OP, false>(p, row, col, STEP, y);
     if constexpr (OP == NORM) {
       F8x w;
       if (p.weight) w = load_weight<false>(p, col);
-      y[0] = normed(p, y[0], rstd, w);
+      y[0] = normed(p, scaled(y[0], factor), rstd, w);
     }
   };
   uint32_t m = 0;
@@ -542,7 +554,7 @@ extern "C" int qi8_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int6
   QI8_REQUIRE(ld_x >= n && (!residual || ld_residual >= n) && (!sum_out || ld_sum >= n), QI8_ESHAPE,
               "row strides %lld, %lld and %lld for rows of %lld", (long long)ld_x, (long long)ld_residual,
               (long long)ld_sum, (long long)n);
-  QI8_REQUIRE(eps >= 0.0 && eps < 1e30, QI8_EINVAL, "eps %g", eps);
+  QI8_REQUIRE(eps == 0.0 || (eps >= 1e-37 && eps < 1e30), QI8_EINVAL, "eps %g: 0, or from 1e-37 to 1e30", eps);
   QI8_REQUIRE(!weight || aq::is_float(weight_dtype), QI8_EDTYPE, "weight dtype %d: bf16, f16 or f32", weight_dtype);
   if (rows == 0 || n == 0) return QI8_OK;
   QI8_REQUIRE(x && q_out && scale_out, QI8_EINVAL, "null pointer");
@@ -562,7 +574,7 @@ extern "C" int qi8_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int6
   p.rows = rows;
   p.n = n;
   p.blocks = f8_blocks(n);
-  p.eps = eps > 0.0 && eps < 1.2e-38 ? 1.2e-38f : (float)eps;  // one above 0 stays so: zero rows are zeros then
+  p.eps = (float)eps;
   p.inv_n = (float)(1.0 / (double)n);
   p.mode = mode;
   p.vec = rows_aligned(x, ld_x, size, 16) && (!residual || rows_aligned(residual, ld_residual, size, 16));

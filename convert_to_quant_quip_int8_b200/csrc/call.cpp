@@ -55,9 +55,10 @@ int64_t integer(PyObject* o) {
   return overflow ? -1 : v;
 }
 
-// On the current device, and nobody waits for its gradient or has given it a tangent.
+// On the current device, its memory as it reads, and nobody waits for its gradient or
+// has given it a tangent.
 bool plain(const at::Tensor& t, int device) {
-  return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == device &&
+  return t.is_cuda() && t.layout() == at::kStrided && t.get_device() == device && !t.is_neg() &&
          !(c10::GradMode::is_enabled() && t.requires_grad()) && !t._fw_grad(0).defined();
 }
 

@@ -62,7 +62,8 @@ int check_workspace(const void* workspace, int64_t have, int64_t need) {
 int check(int64_t M, int64_t K, int64_t N, int64_t ld_b, int64_t ld_out, int out_dtype, const void* bias,
           int bias_dtype) {
   QI8_REQUIRE(device_ok(), QI8_EUNSUPPORTED, "no sm_100 device current");
-  QI8_REQUIRE(M >= 0 && N >= 0 && K > 0 && M < (1ll << 31) && N < (1ll << 31) && K < (1ll << 31), QI8_ESHAPE,
+  constexpr int64_t MOST = (1ll << 31) - 4096;  // rounded up to whole tiles these are 32-bit numbers still
+  QI8_REQUIRE(M >= 0 && N >= 0 && K > 0 && M < MOST && N < MOST && K < MOST, QI8_ESHAPE,
               "product of %lld x %lld and %lld x %lld", (long long)M, (long long)K, (long long)N, (long long)K);
   QI8_REQUIRE(ld_b >= K && ld_out >= N, QI8_ESHAPE, "row strides %lld (weight) and %lld (result)", (long long)ld_b,
               (long long)ld_out);

@@ -691,6 +691,7 @@ def _float_code(dt: torch.dtype, what: str) -> int:
 def _strided_rows(x: torch.Tensor) -> Tuple[torch.Tensor, int]:
     """``x`` as rows with unit column stride, and their stride."""
     n = x.shape[-1]
+    x = x.resolve_neg()
     x2 = x if x.dim() == 2 else x.reshape(-1, n)
     if x2.shape[0] == 1 and (n <= 1 or x2.stride(1) == 1):
         return x2, max(n, 1)
@@ -784,7 +785,7 @@ def _f8_bias(bias: Optional[torch.Tensor], n: int) -> Tuple[Optional[torch.Tenso
     if bias is None:
         return None, None, 0
     assert bias.dim() == 1 and bias.shape[0] == n, f"Bias must be 1D with length {n}, got shape {tuple(bias.shape)}"
-    bias = bias.contiguous()
+    bias = bias.resolve_neg().contiguous()
     return bias, bias.data_ptr(), _float_code(bias.dtype, "bias")
 
 
@@ -880,13 +881,13 @@ def rms_norm_quant(x: torch.Tensor, weight: Optional[torch.Tensor] = None, eps: 
     w_ptr, w_dt = None, 0
     if weight is not None:
         assert weight.dim() == 1 and weight.shape[0] == n, f"weight of shape {tuple(weight.shape)}: expected [{n}]"
-        weight = weight.contiguous()
+        weight = weight.resolve_neg().contiguous()
         w_ptr, w_dt = weight.data_ptr(), _float_code(weight.dtype, "weight")
     if residual is not None:
         assert residual.shape == x.shape, f"residual of shape {tuple(residual.shape)} for {tuple(x.shape)}"
         if residual.dtype != x.dtype:
             raise TypeError(f"residual of {residual.dtype} for activations of {x.dtype}")
-    assert eps >= 0.0, f"eps {eps}"
+    assert eps == 0.0 or 1e-37 <= eps < 1e30, f"eps {eps}: 0, or from 1e-37 to 1e30"
     q, s = _quantized_out(x.shape, mode, dev)
     h = torch.empty(x.shape, dtype=x.dtype, device=dev) if residual is not None else None
     if q.numel():

@@ -511,12 +511,14 @@ QI8_API int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, int6
    and qi8_quant_rows' block mode truncate: twice the error).  QI8_Q_FP8: q_out
    e4m3, scale_out bytes [rows, ceil(n / 128)].  A scale whose block holds an
    infinity or a NaN is no finite number, and the block reads back as NaN.
-   Strides in elements of their tensor; q_out has row stride ld_q. */
+   Strides in elements of their tensor; q_out has row stride ld_q.  No output may
+   overlap an input or another output, here and in the fp8 entries above. */
 
 /* y = h * (mean(h^2) + eps)^-1/2 * weight with h = x + residual (residual or
    null), rounded to x's type and stored to sum_out (when not null); y is not
    rounded before it is quantized.  x, residual, sum_out of x_dtype (bf16 / f16
-   / f32), weight (or null: ones) [n] bf16 / f16 / f32. */
+   / f32), weight (or null: ones) [n] bf16 / f16 / f32; eps 0 (a row of zeros is
+   NaN then) or 1e-37 <= eps < 1e30. */
 QI8_API int qi8_rms_norm_quant(const void* x, int x_dtype, int64_t rows, int64_t n, int64_t ld_x,
                                const void* residual, int64_t ld_residual, const void* weight, int weight_dtype,
                                double eps, int mode, void* q_out, int64_t ld_q, void* scale_out, void* sum_out,

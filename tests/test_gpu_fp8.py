@@ -419,3 +419,30 @@ def test_layout_linear():
     assert torch.equal(F.linear(x, back, bias), expected)
     c.copy_(QuantizedTensor.from_float(w * 2, "BlockWiseFP8Layout", is_weight=True))
     assert torch.equal(F.linear(x, c), F8.fp8_linear(x, *F8.weight_quant_fp8(w * 2)))
+
+
+@pytest.mark.parametrize("m,ld", [(5, 1 << 30), (20, 1 << 28), (300, 1 << 24)])
+def test_codes_far_apart(m, ld):
+    # offsets beyond 32 bits in either operand
+    k, n = 400, 1000
+    a, a_s = F8.act_quant_fp8(randn(m, k, dtype=BF))
+    b, b_s = F8.weight_quant_fp8(randn(n, k, seed=1, dtype=BF))
+    far = torch.empty((m - 1) * ld + k, dtype=E4, device="cuda").as_strided((m, k), (ld, 1))
+    far.view(torch.uint8).copy_(a.view(torch.uint8))
+    assert torch.equal(F8.fp8_gemm(far, a_s, b, b_s), F8.fp8_gemm(a, a_s, b, b_s))
+    a2, a2_s = F8.act_quant_fp8(randn(n, k, seed=1, dtype=BF))
+    b2, b2_s = F8.weight_quant_fp8(randn(m, k, dtype=BF))
+    far.view(torch.uint8).copy_(b2.view(torch.uint8))
+    for t in (9, 100, n):
+        assert torch.equal(F8.fp8_gemm(a2[:t], a2_s[:t], far, b2_s), F8.fp8_gemm(a2[:t], a2_s[:t], b2, b2_s))
+
+
+@pytest.mark.parametrize("m,n,out", [(70000, 32768, BF), (128, 8388480, F32)])
+def test_results_beyond_32_bits(m, n, out):
+    k = 128 if m > 1000 else 16
+    a, a_s = F8.act_quant_fp8(randn(m, k, dtype=BF))
+    b, b_s = F8.weight_quant_fp8(randn(n, k, seed=1, dtype=BF))
+    y = F8.fp8_gemm(a, a_s, b, b_s, out_dtype=out)
+    rows, cols = slice(max(0, m - 300), m), slice(n - n % 128 - 128, n)
+    va, vb = values(a[rows], a_s[rows], 1), values(b[cols], b_s[cols.start // 128:], 128)
+    check_product(y[rows, cols], va, vb)

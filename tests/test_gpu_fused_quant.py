@@ -167,6 +167,63 @@ def test_norm_of_rows_out_of_the_ordinary(output, n):
     check_codes(q[rest], s[rest], y, DELTA * y.abs(), output)
 
 
+@pytest.mark.parametrize("output", ["fp8", "int8"])
+@pytest.mark.parametrize("n", [256, 12288, 40064])
+@pytest.mark.parametrize("eps", [0.0, 1e-37, 1e-30, 1e-12])
+def test_norm_of_small_rows_with_small_eps(n, eps, output):
+    x = randn(6, n, seed=n, dtype=F32)
+    for i, e in enumerate((-40, -60, -75, -100, -118, 50)):
+        x[i] *= 2.0 ** e
+    r = randn(6, n, seed=1, dtype=F32) * x.abs()
+    for res in (None, r):
+        got = FQ.rms_norm_quant(x, eps=eps, residual=res, output=output)
+        _, y = exact_norm(x, None, eps, res)
+        check_codes(got[0], got[1], y, DELTA * y.abs(), output)
+    q, s = FQ.rms_norm_quant(torch.zeros(2, n, device="cuda"), eps=eps, output=output)
+    v = F8.act_dequant_fp8(q, s, output_dtype=F32) if output == "fp8" else ops.dequant(q, s, L.QI8_S_ROW)
+    assert torch.isnan(v).all() if eps == 0 else (v == 0).all()
+
+
+def test_views_of_conjugates():
+    # the imaginary part of a conjugate is the stored one with a sign that is not in memory
+    z = torch.complex(randn(6, 256), randn(6, 256, seed=1))
+    v = z.conj().imag
+    assert v.is_neg()
+    c = torch.empty(6, 256, device="cuda").copy_(v)
+    for f in (lambda t: F8.act_quant_fp8(t), lambda t: F8.weight_quant_fp8(t),
+              lambda t: FQ.rms_norm_quant(t, t[0], residual=t), lambda t: FQ.gated_act_quant(t, t)):
+        assert all(torch.equal(a.double(), b.double()) for a, b in zip(f(v), f(c)))
+    w = F8.weight_quant_fp8(randn(32, 256))
+    assert torch.equal(F8.fp8_linear(v, *w, bias=v[0, :32]), F8.fp8_linear(c, *w, bias=c[0, :32]))
+
+
+def test_rows_far_apart():
+    # offsets beyond 32 bits: 5 rows 2^29 elements apart
+    ld, n = 1 << 29, 300
+    big = torch.empty(4 * ld + n, dtype=BF, device="cuda")
+    x = big.as_strided((5, n), (ld, 1))
+    x.copy_(randn(5, n, dtype=BF))
+    c = x.contiguous()
+    for a, b in ((FQ.rms_norm_quant(x, residual=x), FQ.rms_norm_quant(c, residual=c)),
+                 (FQ.gated_act_quant(x, x, output="int8"), FQ.gated_act_quant(c, c, output="int8")),
+                 (F8.act_quant_fp8(x), F8.act_quant_fp8(c)), (F8.weight_quant_fp8(x), F8.weight_quant_fp8(c))):
+        assert all(torch.equal(u.double(), v.double()) for u, v in zip(a, b))
+    w = F8.weight_quant_fp8(randn(40, n))
+    assert torch.equal(F8.fp8_linear(x, *w), F8.fp8_linear(c, *w))
+
+
+def test_more_than_32_bits_of_elements():
+    rows, n = 530000, 4224
+    x = torch.empty(rows, n, dtype=BF, device="cuda")
+    x[:4], x[-300:] = randn(4, n, dtype=BF), randn(300, n, seed=1, dtype=BF)
+    x[4:-300] = 1.0
+    tail = x[-300:].clone()
+    for f in (lambda t: FQ.rms_norm_quant(t, residual=t), lambda t: FQ.gated_act_quant(t, t),
+              lambda t: FQ.gated_act_quant(t, t, output="int8"), lambda t: F8.act_quant_fp8(t)):
+        got, want = f(x), f(tail)
+        assert all(torch.equal(u[-300:].double(), v.double()) for u, v in zip(got, want))
+
+
 def test_residual_sum_rounds_like_torch():
     x, r = randn(64, 512, scale=100.0, dtype=BF), randn(64, 512, seed=1, dtype=BF)
     assert torch.equal(FQ.rms_norm_quant(x, residual=r)[2], x + r)
@@ -295,8 +352,9 @@ def test_refusals():
         FQ.gated_act_quant(x, x.float())
     with pytest.raises(AssertionError):
         FQ.gated_act_quant(x, x[:, :100])
-    with pytest.raises(AssertionError):
-        FQ.rms_norm_quant(x, eps=-1.0)
+    for eps in (-1.0, 1e-40, float("nan"), float("inf")):
+        with pytest.raises(AssertionError, match="eps"):
+            FQ.rms_norm_quant(x, eps=eps)
     with pytest.raises(TypeError):
         FQ.rms_norm_quant(x.double())
     with pytest.raises(RuntimeError, match="backward"):
