@@ -33,14 +33,16 @@ bool is_float(int dtype) { return dtype == QI8_BF16 || dtype == QI8_F16 || dtype
 
 int64_t pitch(int64_t k) { return (k + 15) / 16 * 16; }
 
-// Workspace of one operand: nothing where its rows are aligned already.
+// Workspace of one operand: nothing where its rows are aligned already.  A single row
+// has no stride.
 int64_t copy_bytes(const uint8_t* q, int64_t rows, int64_t K, int64_t ld) {
-  return rows_aligned(q, ld, 1, 16) ? 0 : rows * pitch(K);
+  return rows_aligned(q, rows == 1 ? 0 : ld, 1, 16) ? 0 : rows * pitch(K);
 }
 
 // Brings an operand into the workspace where it has to be.
 int align_rows(const uint8_t*& q, int64_t rows, int64_t K, int64_t& ld, uint8_t*& workspace, cudaStream_t st) {
   const int64_t bytes = copy_bytes(q, rows, K, ld);
+  if (rows == 1) ld = pitch(K);
   if (bytes == 0) return QI8_OK;
   const int64_t blocks = (bytes / 16 + 255) / 256, most = (int64_t)sm_count() * 32;
   if (int rc = launch_early("repitch_kernel launch", repitch_kernel, dim3((unsigned)(blocks < most ? blocks : most)), 256,
@@ -128,7 +130,7 @@ extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, i
            bias_dtype, out_dtype};
   // Quantized by each block itself, the tokens cost a launch less, but every block the
   // work: 1 x 4096 x 4096 takes 6.1 us so and 6.7 with a kernel for it, two tokens 6.8 and
-  // 6.7, four 8.4 and 7.0.
+  // 6.7, four 8.4 and 7.0 (weights in L2).
   if (gemm_f8_rows_fits((int)M, (int)N, (int)K) && M * K <= 8192)
     return gemm_f8_rows(g, x, x_dtype, ld_x, false, st);
   if (int rc = quant_rows_f8(x, x_dtype, M, K, ld_x, q, f8g::pitch(K), s, st)) return rc;

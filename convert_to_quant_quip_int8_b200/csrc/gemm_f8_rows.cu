@@ -10,8 +10,10 @@
 // banks once.
 //
 // Against the tcgen05 kernel this one starts sooner (no tensor memory, maps or
-// scales to set up) and keeps every SM at work at any number of rows, but its steps
-// take 8.3 cycles for 16 rows and 8 tokens, too long for more than 16 of them.
+// scales to set up), but every block reads the tokens, up to eight, beside its 16
+// weight rows, and none shares its K with others.  1 x 4096 x 4096 with its quantization
+// takes 6.9 us with the weight from HBM, 5.8 to 6.7 from L2: launch, one latency of HBM
+// and the join of eight warps stand beside 2.6 us of reading.
 #include <cstdint>
 
 #include "f8.cuh"
@@ -21,10 +23,11 @@ namespace qi8 {
 namespace {
 namespace f8r {
 
-constexpr int ROWS = 16, WARPS = 8, COPIER = WARPS, THREADS = (WARPS + 1) * 32;
+constexpr int ROWS = 16, MOST_TOKENS = 8, WARPS = 8, COPIER = WARPS, THREADS = (WARPS + 1) * 32;
 constexpr int PIECE = WARPS * F8_BLOCK;           // columns of K per stage
 constexpr int PIECE_PITCH = PIECE + 16, STAGE = ROWS * PIECE_PITCH;
 constexpr int MAX_STAGES = 4, SMEM_MOST = 110 * 1024;  // two blocks per SM at least
+constexpr int STATIC_SMEM = 6000;                      // with what a block takes besides, rounded up
 
 struct Args {
   F8Gemm g;
@@ -67,10 +70,10 @@ __device__ __forceinline__ float2 both_scales(uint32_t a, uint32_t b) {
   return make_float2(__uint_as_float((uint32_t)(h + 127) << 23), __uint_as_float((uint32_t)(e - h + 127) << 23));
 }
 
-template <typename X, int NT>  // X uint8_t: codes; NT groups of eight tokens
+template <typename X>  // uint8_t: codes
 __global__ void __launch_bounds__(THREADS) gemm_f8_rows_kernel(const __grid_constant__ Args p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float part[WARPS][ROWS][8 * NT + 1];
+  __shared__ float part[WARPS][ROWS][MOST_TOKENS + 1];
   __shared__ __align__(16) uint8_t zeros[F8_BLOCK];
   __shared__ uint64_t bars[2 * MAX_STAGES];
   __shared__ int abort_word;
@@ -154,7 +157,7 @@ __global__ void __launch_bounds__(THREADS) gemm_f8_rows_kernel(const __grid_cons
     // nobody may be waiting any more, but what is on its way lands before the block exits
     for (int j = sent - p.stages; j < sent; ++j) drain_wait(full_bar(j % p.stages), (j / p.stages) & 1u);
   } else {
-    float acc[NT][4] = {};
+    float acc[4] = {};
     // rows and 16-byte halves of an A block: (0..7, 0), (8..15, 0), (0..7, 1), (8..15, 1)
     const uint32_t a_at = (uint32_t)((lane & 15) * PIECE_PITCH + warp * F8_BLOCK + (lane >> 4) * 16);
     const uint8_t* sw = p.g.sb + (int64_t)(n0 / F8_BLOCK) * KB;
@@ -176,24 +179,21 @@ __global__ void __launch_bounds__(THREADS) gemm_f8_rows_kernel(const __grid_cons
             for (int h = 0; h < 4; ++h)
               a[j][h] = below(a[j][h], kb * F8_BLOCK + 32 * j + 16 * (h >> 1) + 4 * (lane & 3), K);
         }
+        // lane l: token l % 8, 16 bytes l / 8 of 64
+        const int tok = lane & 7;
+        const uint32_t b_at = (tok < M ? smem_u32(codes + tok * p.x_pitch + kb * F8_BLOCK) : smem_u32(zeros)) + (lane >> 3) * 16;
+        uint32_t b[2][4];
+        ldmatrix4(b[0], b_at);
+        ldmatrix4(b[1], b_at + 64);
+        float d[4] = {0, 0, 0, 0};
 #pragma unroll
-        for (int t = 0; t < NT; ++t) {
-          // lane l: token l % 8, 16 bytes l / 8 of 64
-          const int tok = 8 * t + (lane & 7);
-          const uint32_t b_at = (tok < M ? smem_u32(codes + tok * p.x_pitch + kb * F8_BLOCK) : smem_u32(zeros)) + (lane >> 3) * 16;
-          uint32_t b[2][4];
-          ldmatrix4(b[0], b_at);
-          ldmatrix4(b[1], b_at + 64);
-          float d[4] = {0, 0, 0, 0};
+        for (int j = 0; j < 4; ++j) mma(d, a[j], b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
 #pragma unroll
-          for (int j = 0; j < 4; ++j) mma(d, a[j], b[j >> 1][2 * (j & 1)], b[j >> 1][2 * (j & 1) + 1]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            const int mine_t = 8 * t + 2 * (lane & 3) + u;
-            const float2 f = both_scales(mine_t < M ? scales[kb * M + mine_t] : 127u, w_scale);
-            acc[t][u] = fmaf(d[u] * f.y, f.x, acc[t][u]);
-            acc[t][u + 2] = fmaf(d[u + 2] * f.y, f.x, acc[t][u + 2]);
-          }
+        for (int u = 0; u < 2; ++u) {
+          const int t = 2 * (lane & 3) + u;
+          const float2 f = both_scales(t < M ? scales[kb * M + t] : 127u, w_scale);
+          acc[u] = fmaf(d[u] * f.y, f.x, acc[u]);
+          acc[u + 2] = fmaf(d[u + 2] * f.y, f.x, acc[u + 2]);
         }
       }
       __syncwarp();
@@ -201,9 +201,7 @@ __global__ void __launch_bounds__(THREADS) gemm_f8_rows_kernel(const __grid_cons
       if (++s == p.stages) s = 0, ph ^= 1u;
     }
 #pragma unroll
-    for (int t = 0; t < NT; ++t)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) part[warp][(lane >> 2) + 8 * (j >> 1)][8 * t + 2 * (lane & 3) + (j & 1)] = acc[t][j];
+    for (int j = 0; j < 4; ++j) part[warp][(lane >> 2) + 8 * (j >> 1)][2 * (lane & 3) + (j & 1)] = acc[j];
   }
   __syncthreads();
   for (int i = threadIdx.x; i < ROWS * M; i += THREADS) {
@@ -229,12 +227,12 @@ int stages_for(int M, int K, int KB, int* x_pitch, int* smem) {
   return tokens > SMEM_MOST || (stages < 2 && stages < pieces) ? 0 : stages;
 }
 
-template <typename X, int NT>
+template <typename X>
 int launch(const Args& p, int smem, cudaStream_t st) {
   static bool done[64];
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
-  auto kern = gemm_f8_rows_kernel<X, NT>;
+  auto kern = gemm_f8_rows_kernel<X>;
   if (dev >= 64 || !done[dev]) {
     QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST));
     if (dev < 64) done[dev] = true;
@@ -243,35 +241,32 @@ int launch(const Args& p, int smem, cudaStream_t st) {
                       p);
 }
 
-template <typename X>
-int launch_tokens(const Args& p, int smem, cudaStream_t st) {
-  return p.g.M <= 8 ? launch<X, 1>(p, smem, st) : launch<X, 2>(p, smem, st);
-}
-
 }  // namespace f8r
 }  // namespace
 
-// Up to where this kernel is the faster one (1 x 4096 x 4096: 6.1 us, on tcgen05 7.4;
-// 8 x 4096 x 4096 7.1 and 7.5, 16 x 4096 x 4096 10.3 and 7.7, 1 x 10240 x 4096 13.5 and
-// 11.3): every block reads the tokens beside its 16 weight rows, and from 9 tokens on
-// the steps take as long as the loads.  Nor does it split K, so that few rows of many
-// columns are left to the few SMs that their blocks fill (1 x 500 x 16384: 15 and 9 us).
+// Where this kernel is the faster one (cold weights, tcgen05 second): 2 x 4096 x 4096
+// 5.8 us and 6.8, 4 x 4096 x 4096 6.7 and 6.9, 8 x 4096 x 4096 7.9 and 6.9, 8 x 2560 x
+// 2560 5.6 and 6.1, 1 x 10240 x 2048 8.3 and 6.9, 4 x 2048 x 6144 7.2 and 6.4.  Tokens
+// beyond four cost it steps, many blocks their start, and it does not split K.  All
+// blocks have to run at once: 1 x 6144 x 4096 (three per SM) takes 7.6 us and 8.2, two
+// tokens (two per SM) 10.1 and 8.2.
 bool gemm_f8_rows_fits(int M, int N, int K) {
-  if (N < 148 * f8r::ROWS && K > 6 * f8r::PIECE) return false;
-  if (M > 16 || (int64_t)N * K / 16 * (16 + M) > (M > 8 ? 16000000 : 25500000)) return false;
+  if (M > 8 || N > 8192 || K > 5120 || (M > 4 && (K > 2560 || (int64_t)N * K > 10500000))) return false;
   int pitch, smem;
-  return f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) > 0;
+  if (f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) == 0) return false;
+  const int per_sm = 228 * 1024 / (smem + f8r::STATIC_SMEM);
+  return (N + f8r::ROWS - 1) / f8r::ROWS <= (per_sm < 7 ? per_sm : 7) * sm_count();
 }
 
 int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st) {
   f8r::Args p{g, x, ld_x, x && rows_aligned(x, ld_x, elem_size(x_dtype), 16), 0, 0, after_quant, device_status_ptr()};
   int smem = 0;
   p.stages = f8r::stages_for(g.M, g.K, g.KB, &p.x_pitch, &smem);
-  if (!x) return f8r::launch_tokens<uint8_t>(p, smem, st);
+  if (!x) return f8r::launch<uint8_t>(p, smem, st);
   switch (x_dtype) {
-    case QI8_BF16: return f8r::launch_tokens<__nv_bfloat16>(p, smem, st);
-    case QI8_F16: return f8r::launch_tokens<__half>(p, smem, st);
-    default: return f8r::launch_tokens<float>(p, smem, st);
+    case QI8_BF16: return f8r::launch<__nv_bfloat16>(p, smem, st);
+    case QI8_F16: return f8r::launch<__half>(p, smem, st);
+    default: return f8r::launch<float>(p, smem, st);
   }
 }
 

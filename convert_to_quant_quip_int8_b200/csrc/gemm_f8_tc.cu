@@ -7,6 +7,7 @@
 // itself: it takes one byte e + 127 per row and 32 columns of K from tensor
 // memory, so the four steps of a 128-block read the same byte.  The sums stay in
 // the accumulator over all of K.
+#include <cmath>
 #include <cstdint>
 
 #include "f8.cuh"
@@ -25,9 +26,10 @@ __host__ __device__ constexpr uint32_t idesc(int m, int n, uint32_t sf = 0) {
   return (sf << 4) | ((uint32_t)(n >> 3) << 17) | (1u << 23) | ((uint32_t)(m >> 4) << 24) | (sf << 29);
 }
 
-// Four scale bytes, K blocks kb .. kb + 3, of N rows (`row` gives the start of row i):
-// words where rows lie on whole ones, else byte by byte, out of the way of the
-// instruction cache.  Past the end: 0.
+// Four scale bytes, K blocks kb .. kb + 3, of N rows (`row` gives the start of row i).
+// words: rows and kb lie on whole words; else a word is shifted out of the two that it
+// begins and ends in (8 x 2560 x 2560, where four blocks share 20 K blocks, took 6.7 us
+// byte by byte, 6.1 so).  Past the row's end: any.
 template <int N, typename F>
 __device__ __forceinline__ void scale_words(uint32_t (&w)[N], F&& row, int kb, int KB, bool words) {
   if (words) {
@@ -36,10 +38,14 @@ __device__ __forceinline__ void scale_words(uint32_t (&w)[N], F&& row, int kb, i
   } else {
 #pragma unroll
     for (int i = 0; i < N; ++i) w[i] = 0;
-#pragma unroll 1
-    for (int b = 0; b < 4 && kb + b < KB; ++b)
+#pragma unroll 1  // little code beside that of the other case
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int i = 0; i < N; ++i) w[i] |= (uint32_t)__ldg(row(i) + kb + b) << (8 * b);
+      for (int i = 0; i < N; ++i) {
+        const uintptr_t at = reinterpret_cast<uintptr_t>(row(i) + kb), last = reinterpret_cast<uintptr_t>(row(i) + KB - 1);
+        const uint32_t v = __ldg(reinterpret_cast<const uint32_t*>((h == 0 ? at : min(at + 3, last)) & ~(uintptr_t)3));
+        w[i] = h == 0 ? v : __funnelshift_r(w[i], v, 8 * ((uint32_t)at & 3u));
+      }
   }
 }
 
@@ -50,12 +56,29 @@ __device__ __forceinline__ void tmem_st4(uint32_t addr, const uint32_t (&r)[4]) 
 }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// 32 results of one row from column n on, those before `end`.
-__device__ __forceinline__ void store32(const F8Gemm& g, int64_t m, int n, int end, const float (&y)[32]) {
-  const int64_t at = m * g.ld_out + n;
+// f(the result as what it holds).  Asked for once and not at each store: 100 x 10240 x
+// 4096 took 12.7 us else, 12.0 so.
+template <typename F>
+__device__ __forceinline__ void typed(const F8Gemm& g, F&& f) {
+  if (g.out_dtype == QI8_BF16) f(static_cast<__nv_bfloat16*>(g.out));
+  else if (g.out_dtype == QI8_F16) f(static_cast<__half*>(g.out));
+  else f(static_cast<float*>(g.out));
+}
+
+// 32 results `step` elements apart, the first `count` of them.
+template <typename T>
+__device__ __forceinline__ void store32(T* to, int64_t step, int count, const float (&y)[32]) {
+  if (count >= 32) {
 #pragma unroll
-  for (int j = 0; j < 32; ++j)
-    if (n + j < end) store_from_f32(g.out, g.out_dtype, at + j, y[j]);
+    for (int j = 0; j < 32; ++j) to[j * step] = Elem<T>::from_f32(y[j]);
+  } else {
+#pragma unroll
+    for (int h = 0; h < 32; h += 8)
+      if (h < count)
+#pragma unroll
+        for (int j = h; j < h + 8; ++j)
+          if (j < count) to[j * step] = Elem<T>::from_f32(y[j]);
+  }
 }
 
 // A warp's 32 rows (m0 on, lane = row) x 32 columns, all of them there, rows of the
@@ -113,7 +136,7 @@ __device__ __forceinline__ void store_tile(const F8Gemm& g, uint4* buf, int m0, 
 //   warps 0..7    epilogue (warp w: lanes 32 (w % 4), every other half)
 //   warps 8..11   scales: global memory -> tensor memory, four K blocks at a time
 //   warp 12       TMA producer
-//   warp 13       TMEM allocation; MMA issue (one thread of the even block)
+//   warp 13       TMEM allocation; MMA issue (the even block's)
 // Two accumulators of 256 columns and the scales do not fit 512 columns, so the
 // accumulators share 64: the epilogue reads those first, and the next tile's
 // MMAs wait for just that.  Tiles may have fewer features, where that fills the last
@@ -121,7 +144,9 @@ __device__ __forceinline__ void store_tile(const F8Gemm& g, uint4* buf, int m0, 
 // The issuing warp sets the pace: an MMA takes it 72 cycles, a wait 110, a commit
 // 60 to 100 (clock64), and the tensor cores, which queue about 14 MMAs, 128 cycles
 // for each.  A stage of one K block cost it 700 cycles per block, two blocks a stage
-// keep it below the 512 of the MMAs.
+// keep it below the 512 of the MMAs.  4096 x 10240 x 4096 with its quantization takes
+// 142 us alone (2420 TFLOP/s, 0.72 of twice the measured bf16 rate) and 154 us back to
+// back for seconds, where the board's 1 kW sets the clock: zeros take 107 us.
 namespace pair {
 
 constexpr int EPI_WARPS = 8, SCALE_WARP0 = 8, SCALE_WARPS = 4, PRODUCER = 12, ISSUER = 13;
@@ -392,7 +417,8 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
           for (int j = 0; j < 32; ++j) y[j] += my_bias[j];
         }
         if (p.vec_out && n + 32 <= end) store_tile(p.g, my_tile, m0, n, y);
-        else if (m0 + lane < p.g.M && n < end) store32(p.g, m0 + lane, n, end, y);
+        else if (m0 + lane < p.g.M && n < end)
+          typed(p.g, [&](auto* out) { store32(out + (int64_t)(m0 + lane) * p.g.ld_out + n, 1, end - n, y); });
       }
     }
   }
@@ -414,10 +440,15 @@ gemm_f8_pair_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_consta
 // weight that is read once fill the SMs; a cluster of `split` blocks may share a
 // tile's K and joins its fp32 sums through distributed shared memory in the order of
 // the ranks.  Roles of a block:
-//   warps 0..3  epilogue: TMEM -> registers -> out (thread = weight row)
-//   warps 4..7  scales: global memory -> tensor memory, four K blocks at a time
-//   warp 8      TMA producer: weight rows and tokens of one K block per stage
-//   warp 9      TMEM allocation, MMA issue (one thread)
+//   warps 0..3   epilogue: TMEM -> registers -> out (thread = weight row)
+//   warps 4..7   scales: global memory -> tensor memory, four K blocks at a time
+//   warp 8       TMA producer: weight rows and tokens, one or two K blocks per stage
+//   warps 9, 10  MMA issue, every other stage each; warp 9 TMEM allocation
+// Two issuers, because one takes 430 cycles for a K block's waits, MMAs and commits
+// however few the tokens.  16 x 10240 x 4096 takes 9.8 us (weights from HBM; 4.3 TB/s,
+// and 5.9 from one K block to the next: HBM), 100 x 10240 x 4096 11.9, where a block
+// reads 14 KB of tokens from L2 beside each 10 KB of weights and L2 sets the pace (0.27
+// us a K block against 0.22).  The rest is launch, first loads and the way out.
 namespace few {
 
 constexpr int BM = 128;
@@ -445,9 +476,6 @@ template <int KPS>
 __device__ __forceinline__ int first_issuer(int unit, int kn) { return (unit * ((kn + KPS - 1) / KPS)) & 1; }
 // tokens that each block of a split tile finishes
 __host__ __device__ constexpr int join_per(int bn, int split) { return ((bn + split - 1) / split + 3) & ~3; }
-// Their row's length in memory: an odd number of 16-byte pieces, so that eight rows
-// touch all banks.  (With 32 words a row the join of four blocks took 16 us.)
-__host__ __device__ constexpr int join_pitch(int bn, int split) { return join_per(bn, split) | 4; }
 
 __device__ __forceinline__ void mma(int one, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t sa, uint32_t sb,
                                     uint32_t accum) {
@@ -484,7 +512,7 @@ __device__ __forceinline__ void sums(uint32_t at, bool two, float (&y)[32]) {
   for (int j = 0; j < 32; ++j) y[j] = __uint_as_float(v[j]) + (two ? __uint_as_float(u[j]) : 0.0f);
 }
 
-template <int BN>
+template <int BN, bool SPLIT>
 __global__ void __launch_bounds__(THREADS, 1)
 gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB,
                    const __grid_constant__ Args p) {
@@ -509,7 +537,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   const uint32_t drain_bar = smem_u32(bars + BARS - 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int split = p.split, rank = split > 1 ? (int)cta_rank() : 0;
+  const int split = SPLIT ? p.split : 1, rank = SPLIT ? (int)cta_rank() : 0;
   if (threadIdx.x == 0) {
     for (int s = 0; s < p.stages; ++s) {
       mbar_init(full_bar(s), 1);
@@ -541,7 +569,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
   __syncthreads();
   tc_fence_after();
   // waited for where blocks first reach into one another's memory
-  if (split > 1) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+  if (SPLIT) asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
   wait_for_last_kernel();
   const uint32_t tmem = *tmem_slot;
   const int tiles = p.n_tiles * p.t_tiles;
@@ -678,7 +706,7 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
       const float bias = p.g.bias && n < p.g.N ? load_as_f32(p.g.bias, p.g.bias_dtype, n) : 0.0f;
       if (!warp_wait(tfull_bar(buf), (unit / ACCS) & 1, abort_flag, p.status, ST_F8_EPILOGUE, WAIT_LIMIT_NS)) break;
       tc_fence_after();
-      if (split == 1) {
+      if constexpr (!SPLIT) {
         const int t1 = min(p.bn, p.g.M - t0);
         // of a tile of one stage one accumulator has sums
         const int acc0 = (buf * ISSUERS + (kn > KPS ? 0 : first_issuer<KPS>(unit, kn))) * BN;
@@ -687,14 +715,10 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
           for (int c = 0; c < t1; c += 32) {
             float v[32];
             sums<BN>(lanes + (uint32_t)(acc0 + c), kn > KPS, v);
-            if (r < p.rows && n < p.g.N) {
-              const int64_t at = (int64_t)(t0 + c) * p.g.ld_out + n;
 #pragma unroll
-              for (int j = 0; j < 32; ++j) {
-                if (c + j >= t1) break;
-                store_from_f32(p.g.out, p.g.out_dtype, at + j * p.g.ld_out, v[j] + bias);
-              }
-            }
+            for (int j = 0; j < 32; ++j) v[j] += bias;
+            if (r < p.rows && n < p.g.N)
+              typed(p.g, [&](auto* out) { store32(out + (int64_t)(t0 + c) * p.g.ld_out + n, p.g.ld_out, t1 - c, v); });
           }
         tc_fence_before();
         __syncwarp();
@@ -703,17 +727,17 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     }
   }
 
-  if (split > 1) {
+  if constexpr (SPLIT) {
     // one tile per cluster
     __syncwarp();
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
     tc_fence_after();
     const int n0 = (tile0 % p.n_tiles) * p.rows, t0 = (tile0 / p.n_tiles) * p.bn, t1 = min(p.bn, p.g.M - t0);
-    const int per = join_per(p.bn, split), pitch = join_pitch(p.bn, split);
+    const int per = join_per(p.bn, split);
     if (warp < EPI_WARPS && __all_sync(0xffffffffu, !*abort_flag)) {
       const uint32_t lanes = tmem + ((uint32_t)(warp * 32) << 16);
       const int r = warp * 32 + lane;
-      // rank d finishes tokens [d per, (d + 1) per): sums as [source][row][pitch]
+      // rank d finishes tokens [d per, (d + 1) per): sums as [source][four tokens][row]
 #pragma unroll 1
       for (int c = 0; c < t1; c += 32) {
         float v[32];
@@ -723,8 +747,8 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
 #pragma unroll
           for (int j = 0; j < 32; j += 4) {
             if (c + j >= p.bn) break;  // past the last rank's
-            st_cluster_f32x4(mapa(base + (uint32_t)(p.join + ((rank * BM + r) * pitch + at) * 4), (uint32_t)d), v[j], v[j + 1],
-                             v[j + 2], v[j + 3]);
+            st_cluster_f32x4(mapa(base + (uint32_t)(p.join + ((rank * per + at) * BM + 4 * r) * 4), (uint32_t)d), v[j],
+                             v[j + 1], v[j + 2], v[j + 3]);
             if ((at += 4) >= per) at -= per, ++d;
           }
         }
@@ -735,23 +759,27 @@ gemm_f8_few_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constan
     cluster_sync();
     tc_fence_after();
     const float* part = reinterpret_cast<const float*>(sm + p.join);
-    for (int i = threadIdx.x; i < per / 4 * BM; i += THREADS) {  // four tokens of a row
-      const int r = i & (BM - 1), c = i / BM * 4;
-      const int t = rank * per + c, n = n0 + r;
-      if (t >= t1 || r >= p.rows || n >= p.g.N) continue;
-      float y[4] = {0, 0, 0, 0};
-      for (int s = 0; s < split; ++s) {
-        const float4 v = *reinterpret_cast<const float4*>(part + (s * BM + r) * pitch + c);
-        y[0] += v.x;
-        y[1] += v.y;
-        y[2] += v.z;
-        y[3] += v.w;
-      }
-      const float bias = p.g.bias ? load_as_f32(p.g.bias, p.g.bias_dtype, n) : 0.0f;
+    typed(p.g, [&](auto* out) {
+      using T = std::remove_pointer_t<decltype(out)>;
+      for (int i = threadIdx.x; i < per / 4 * BM; i += THREADS) {  // four tokens of a row
+        const int r = i & (BM - 1), c = i / BM * 4;
+        const int t = rank * per + c, n = n0 + r;
+        if (t >= t1 || r >= p.rows || n >= p.g.N) continue;
+        float y[4] = {0, 0, 0, 0};
+        for (int s = 0; s < split; ++s) {
+          const float4 v = *reinterpret_cast<const float4*>(part + (s * per + c) * BM + 4 * r);
+          y[0] += v.x;
+          y[1] += v.y;
+          y[2] += v.z;
+          y[3] += v.w;
+        }
+        const float bias = p.g.bias ? load_as_f32(p.g.bias, p.g.bias_dtype, n) : 0.0f;
+        T* to = out + (int64_t)(t0 + t) * p.g.ld_out + n;
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (t + j < t1) store_from_f32(p.g.out, p.g.out_dtype, (int64_t)(t0 + t + j) * p.g.ld_out + n, y[j] + bias);
-    }
+        for (int j = 0; j < 4; ++j)
+          if (t + j < t1) to[j * p.g.ld_out] = Elem<T>::from_f32(y[j] + bias);
+      }
+    });
   }
 
   __syncwarp();
@@ -814,12 +842,12 @@ int launch_pair(const F8Gemm& g, cudaStream_t st) {
                       pair::SMEM, 1, st, ma, mb, p);  // its clusters are in its attributes
 }
 
-template <int BN>
+template <int BN, bool SPLIT>
 int launch_few(const F8Gemm& g, int rows, int split, cudaStream_t st) {
   static bool done[64];
   int dev = 0;
   QI8_CUDA(cudaGetDevice(&dev));
-  auto kern = few::gemm_f8_few_kernel<BN>;
+  auto kern = few::gemm_f8_few_kernel<BN, SPLIT>;
   if (dev >= 64 || !done[dev]) {
     QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, few::SMEM));
     if (dev < 64) done[dev] = true;
@@ -828,7 +856,7 @@ int launch_few(const F8Gemm& g, int rows, int split, cudaStream_t st) {
   CUtensorMap ma, mb;
   if (int rc = code_map8(&ma, g.a, g.M, g.K, g.ld_a, bn)) return rc;
   if (int rc = code_map8(&mb, g.b, g.N, g.K, g.ld_b, rows)) return rc;
-  const int join = split > 1 ? split * few::BM * few::join_pitch(bn, split) * 4 : 0;
+  const int join = SPLIT ? split * few::BM * few::join_per(bn, split) * 4 : 0;
   int stages = (few::RING - join) / (few::kps(BN) * (rows + bn) * BK) / few::ISSUERS * few::ISSUERS;
   if (stages > few::MAX_STAGES) stages = few::MAX_STAGES;
   QI8_REQUIRE(stages >= few::ISSUERS, QI8_ESHAPE, "no room for two stages");
@@ -836,7 +864,7 @@ int launch_few(const F8Gemm& g, int rows, int split, cudaStream_t st) {
               word_rows(g.sb, g.KB), device_status_ptr()};
   const int64_t tiles = (int64_t)p.n_tiles * p.t_tiles;
   QI8_REQUIRE(tiles < (1 << 30), QI8_ESHAPE, "%lld output tiles", (long long)tiles);
-  const int64_t blocks = split > 1 ? tiles * split : tiles < sm_count() ? tiles : sm_count();
+  const int64_t blocks = SPLIT ? tiles * split : tiles < sm_count() ? tiles : sm_count();
   return launch_early("gemm_f8_few_kernel launch", kern, dim3((unsigned)blocks), few::THREADS, few::SMEM, split, st, ma, mb,
                       p);
 }
@@ -853,18 +881,20 @@ int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) {
   // empty: 100 x 32768 x 4096 takes 30.1 us so and 32.5 in those.
   const int64_t t_tiles = ((int64_t)g.M + 127) / 128, n_tiles = ((int64_t)g.N + 127) / 128;
   if (g.M > 128 && n_tiles * t_tiles > sms) return launch_pair(g, st);
-  // Blocks that share a tile's K: a K block takes about 0.19 us up to 64 tokens and 0.24
-  // with 128, the join 0.5 us and 0.012 for each token and block (fitted to 17 shapes of
-  // 9 to 700 tokens; 100 x 4096 x 4096 takes 12.5 us with whole tiles, 11.5 with two blocks
-  // each, 16 x 4096 x 4096 9.2 and, with four, 7.3).  Of clusters of two 74 run at once, of four
-  // 33, of eight 15; three blocks were never faster than two or four.
+  // Blocks that share a tile's K: a K block takes 0.21 us up to 64 tokens and 0.27 with
+  // 128, or what the weight takes from HBM, the join 1.4 us and 0.003 for each token and
+  // block.  Fitted to 21 shapes of 9 to 256 tokens, of which it misses the best choice in
+  // two, by 5 % at most: 16 x 4096 x 4096 takes 8.7 us with whole tiles, 7.4 with two
+  // blocks each and 7.0 with four, 100 x 4096 x 10240 21.7, 15.9 and 14.5, 100 x 8192 x
+  // 4096 12.2 and, with two, 13.4.  Of clusters of two 74 run at once, of four 33, of
+  // eight 15; three blocks were never faster than two or four.
   const int bn = (int)((g.M + t_tiles - 1) / t_tiles + 15) & ~15;
-  const double block_us = bn <= 64 ? 0.19 : 0.19 + 0.0008 * (bn - 64);
+  const double block_us = bn <= 64 ? 0.21 : 0.21 + 0.06 / 64 * (bn - 64), read_us = (double)g.N * g.K / 5.5e6;
   int split = 1, room = sms;
-  double best = g.KB * block_us;
+  double best = fmax(g.KB * block_us, read_us);
   for (int s : {2, 4, 8}) {
     const int there = s == 2 ? sms : s == 8 ? sms * 13 / 16 : sms * 57 / 64;
-    const double us = (g.KB + s - 1) / s * block_us + 0.5 + 0.012 * bn * s;
+    const double us = fmax((g.KB + s - 1) / s * block_us, read_us) + 1.4 + 0.003 * bn * s;
     if (s <= g.KB && n_tiles * t_tiles * s <= there && us < best) best = us, split = s, room = there;
   }
   // as few rows per tile as spread them over the SMs in as many waves
@@ -872,9 +902,9 @@ int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) {
   const int least = split > 1 ? 64 : 32;
   int rows = (int)(((int64_t)g.N + most - 1) / most + 15) & ~15;
   rows = rows < least ? least : rows > 128 ? 128 : rows;
-  if (bn <= 32) return launch_few<32>(g, rows, split, st);
-  if (bn <= 64) return launch_few<64>(g, rows, split, st);
-  return launch_few<128>(g, rows, split, st);
+  const auto launch = split > 1 ? bn <= 32 ? launch_few<32, true> : bn <= 64 ? launch_few<64, true> : launch_few<128, true>
+                      : bn <= 32 ? launch_few<32, false> : bn <= 64 ? launch_few<64, false> : launch_few<128, false>;
+  return launch(g, rows, split, st);
 }
 
 }  // namespace qi8

@@ -1,6 +1,7 @@
 // fp8 quantization with block scales (format: f8.cuh), and back.
 //
-// All three kernels move each byte once and are bound by HBM.
+// Both kernels move each byte once and are bound by HBM: quantizing a weight of 10240 x
+// 4096 bf16 takes 25.0 us (5.0 TB/s, 0.77 of the copy rate), 32768 x 4096 72.9 (5.5).
 #include <cstdint>
 
 #include "f8.cuh"
@@ -12,7 +13,8 @@ namespace f8q {
 constexpr int THREADS = 512, PASSES = F8_BLOCK * 16 / THREADS;
 
 // One 128 x 128 tile per thread block: 16 lanes by eight columns, 32 rows at a
-// time.  The tile stays in registers between its maximum and its codes.
+// time.  The tile stays in registers between its maximum and its codes.  (Blocks that
+// stay, with the next tile's loads under way, need 113 registers and took 28.3 us.)
 template <typename T>
 __global__ void __launch_bounds__(THREADS)
 weight_kernel(const T* __restrict__ w, int64_t N, int64_t K, int64_t ld_w, bool vec, uint8_t* __restrict__ q,
