@@ -7,6 +7,7 @@
     python benchmarks/microbench.py convert  # K4 QuIP conversion
     python benchmarks/microbench.py ldlq     # default converter: fp64 Hinv factorization, LDLQ pass
     python benchmarks/microbench.py int4     # 4-bit weights: quantization, linear, mixture of experts
+    python benchmarks/microbench.py fp8      # fp8 product, quantized norm and gate
     python benchmarks/microbench.py gemm_ksweep  # K2 plain GEMM over K at fixed M, N
 
 Each case is timed with CUDA events around one launch, median of ``--iters``
@@ -144,6 +145,35 @@ def int4_cases(run, dev):
     return res
 
 
+def fp8_cases(run, dev):
+    """fp8 and the producers of quantized activations at the sizes of a text encoder layer:
+    [us, GB/s of inputs and outputs], prompts [us, TFLOP/s]."""
+    res = {}
+    w = (torch.randn(10240, 4096, device=dev) * 0.02).to(torch.bfloat16)
+    us = run(lambda: ops.quant_weight_f8(w))
+    res["f8_quant_weight_10240x4096"] = [us, w.numel() * 3 / us / 1e3]
+    q, s = ops.quant_weight_f8(w)
+    one = ops.quant_weight_f8(w[:4096])
+    x = torch.randn(1, 4096, device=dev).to(torch.bfloat16)
+    us = run(lambda: ops.linear_f8(x, *one))
+    res["f8_linear_1x4096x4096"] = [us, one[0].numel() / us / 1e3]
+    for T in (16, 100, 512, 4096):
+        x = torch.randn(T, 4096, device=dev).to(torch.bfloat16)
+        a = ops.quant_rows_f8(x)
+        us = run(lambda: ops.gemm_f8(*a, q, s))
+        res[f"f8_gemm_{T}x10240x4096"] = [us, q.numel() / us / 1e3 if T < 512 else 2 * T * w.numel() / us / 1e6]
+    us = run(lambda: ops.quant_rows_f8(x))
+    res["f8_quant_rows_4096x4096"] = [us, x.numel() * 3 / us / 1e3]
+    r = torch.randn_like(x)
+    us = run(lambda: ops.rms_norm_quant(x, residual=r))
+    res["norm_f8_4096x4096"] = [us, x.numel() * 7 / us / 1e3]
+    g, u = (torch.randn(4096, 10240, device=dev).to(torch.bfloat16) for _ in range(2))
+    for name, act in (("silu", L.QI8_ACT_SILU), ("gelu", L.QI8_ACT_GELU), ("gelu_tanh", L.QI8_ACT_GELU_TANH)):
+        us = run(lambda: ops.gated_quant(g, u, act))
+        res[f"gated_{name}_f8_4096x10240"] = [us, g.numel() * 5 / us / 1e3]
+    return res
+
+
 def gemm_stack_cases(run, dev):
     """The stacks' largest GEMMs with per-row weight scales, bias and bf16
     output: Flux single-block linear1 (4608 x 3072 -> 21504) first, then the
@@ -252,7 +282,7 @@ def gemm_ksweep_cases(run, dev):
 
 CASES = {"rotate": rotate_cases, "quant": quant_cases, "gemm": gemm_cases, "gemm_stack": gemm_stack_cases,
          "gemm_tile": gemm_tile_cases,
-         "int4": int4_cases, "convert": convert_cases, "ldlq": ldlq_cases, "gemm_ksweep": gemm_ksweep_cases}
+         "int4": int4_cases, "fp8": fp8_cases, "convert": convert_cases, "ldlq": ldlq_cases, "gemm_ksweep": gemm_ksweep_cases}
 
 
 def main(argv=None):

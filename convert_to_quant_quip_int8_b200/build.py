@@ -120,7 +120,7 @@ def main(argv) -> None:
     try:
         print(build_call(force="--force" in argv, verbose=True))
     except (OSError, ImportError, subprocess.CalledProcessError) as e:
-        print(f"warning: the host-side shortcut was not built, the 4-bit operators do without it: {e}", file=sys.stderr)
+        print(f"warning: the host-side shortcut was not built, the 4-bit and fp8 operators do without it: {e}", file=sys.stderr)
 
 
 if __name__ == "__main__":

@@ -1,11 +1,11 @@
 // The common case of the 4-bit and fp8 operators' wrappers, without the
 // interpreter: a product for one token takes the GPU about 5 us and its Python
-// wrapper took the host 11 (4 bits) or 20 (fp8).  Each function checks that its arguments are what the kernels take as
-// they are (plain tensors on the current device, right types and shapes,
-// contiguous where that is needed, no gradient wanted), allocates the result and
-// calls the C ABI of libqi8.  For anything else, and for any error, it returns
-// None: the Python wrapper then goes its own way, which converts what can be
-// converted and raises what has to be raised.
+// wrapper took the host 11 (4 bits) or 20 (fp8), with this 5.  Each function checks
+// that its arguments are what the kernels take as they are (plain tensors on the
+// current device, right types and shapes, contiguous where that is needed, no
+// gradient wanted), allocates the result and calls the C ABI of libqi8.  For anything
+// else, and for any error, it returns None: the Python wrapper then goes its own way,
+// which converts what can be converted and raises what has to be raised.
 #include <Python.h>
 
 #include <ATen/ATen.h>
