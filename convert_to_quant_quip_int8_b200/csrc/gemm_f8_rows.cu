@@ -12,8 +12,8 @@
 // Against the tcgen05 kernel this one starts sooner (no tensor memory, maps or
 // scales to set up), but every block reads the tokens, up to eight, beside its 16
 // weight rows, and none shares its K with others.  1 x 4096 x 4096 with its quantization
-// takes 6.9 us with the weight from HBM, 5.8 to 6.7 from L2: launch, one latency of HBM
-// and the join of eight warps stand beside 2.6 us of reading.
+// takes 5.9 us with the weight from HBM: launch, one latency of HBM and the join of
+// eight warps stand beside 2.6 us of reading.
 #include <cstdint>
 
 #include "f8.cuh"
@@ -27,7 +27,7 @@ constexpr int ROWS = 16, MOST_TOKENS = 8, WARPS = 8, COPIER = WARPS, THREADS = (
 constexpr int PIECE = WARPS * F8_BLOCK;           // columns of K per stage
 constexpr int PIECE_PITCH = PIECE + 16, STAGE = ROWS * PIECE_PITCH;
 constexpr int MAX_STAGES = 4, SMEM_MOST = 110 * 1024;  // two blocks per SM at least
-constexpr int STATIC_SMEM = 6000;                      // with what a block takes besides, rounded up
+constexpr int SM_SMEM = 228 * 1024, STATIC_SMEM = 6000;                      // with what a block takes besides, rounded up
 
 struct Args {
   F8Gemm g;
@@ -234,18 +234,24 @@ int launch(const Args& p, int smem, cudaStream_t st) {
   QI8_CUDA(cudaGetDevice(&dev));
   auto kern = gemm_f8_rows_kernel<X>;
   if (dev >= 64 || !done[dev]) {
-    QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_MOST));
+    QI8_CUDA(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM_SMEM / 2));
     if (dev < 64) done[dev] = true;
   }
-  return launch_early("gemm_f8_rows_kernel launch", kern, dim3((unsigned)((p.g.N + ROWS - 1) / ROWS)), THREADS, smem, 1, st,
-                      p);
+  // Where most SMs take as many blocks as any, so much shared memory that no more fit:
+  // else some SMs get one more and others one less.  1 x 4096 x 4096 (256 blocks, of
+  // which three fit an SM) took 6.9 us so and takes 5.9; 2560 x 2560 (160 blocks) is 2 %
+  // faster without.
+  const int sms = sm_count(), blocks = (p.g.N + ROWS - 1) / ROWS, each = (blocks + sms - 1) / sms;
+  const int more = SM_SMEM / (each + 1);
+  if (smem < more && each * sms - blocks < sms / 2) smem = more;
+  return launch_early("gemm_f8_rows_kernel launch", kern, dim3((unsigned)blocks), THREADS, smem, 1, st, p);
 }
 
 }  // namespace f8r
 }  // namespace
 
-// Where this kernel is the faster one (cold weights, tcgen05 second): 2 x 4096 x 4096
-// 5.8 us and 6.8, 4 x 4096 x 4096 6.7 and 6.9, 8 x 4096 x 4096 7.9 and 6.9, 8 x 2560 x
+// Where this kernel is the faster one (cold weights, tcgen05 second): 1 x 4096 x 4096
+// 5.7 us and 6.7, 1 x 4096 x 5120 6.5 and 7.6, 2 x 4096 x 4096 5.8 and 6.8, 4 x 4096 x 4096 6.7 and 6.9, 8 x 4096 x 4096 7.9 and 6.9, 8 x 2560 x
 // 2560 5.6 and 6.1, 1 x 10240 x 2048 8.3 and 6.9, 4 x 2048 x 6144 7.2 and 6.4.  Tokens
 // beyond four cost it steps, many blocks their start, and it does not split K.  All
 // blocks have to run at once: 1 x 6144 x 4096 (three per SM) takes 7.6 us and 8.2, two
@@ -254,7 +260,7 @@ bool gemm_f8_rows_fits(int M, int N, int K) {
   if (M > 8 || N > 8192 || K > 5120 || (M > 4 && (K > 2560 || (int64_t)N * K > 10500000))) return false;
   int pitch, smem;
   if (f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) == 0) return false;
-  const int per_sm = 228 * 1024 / (smem + f8r::STATIC_SMEM);
+  const int per_sm = f8r::SM_SMEM / (smem + f8r::STATIC_SMEM);
   return (N + f8r::ROWS - 1) / f8r::ROWS <= (per_sm < 7 ? per_sm : 7) * sm_count();
 }
 
