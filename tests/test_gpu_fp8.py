@@ -446,3 +446,30 @@ def test_results_beyond_32_bits(m, n, out):
     rows, cols = slice(max(0, m - 300), m), slice(n - n % 128 - 128, n)
     va, vb = values(a[rows], a_s[rows], 1), values(b[cols], b_s[cols.start // 128:], 128)
     check_product(y[rows, cols], va, vb)
+
+
+@pytest.mark.parametrize("k", [31, 300, 2989])
+def test_a_single_row_has_no_stride(k):
+    lib = L.load()
+    for m, n in ((1, 70), (1, 1), (12, 1), (1, 5003)):
+        a, a_s = F8.act_quant_fp8(randn(m, k, dtype=BF))
+        b, b_s = F8.weight_quant_fp8(randn(n, k, seed=1, dtype=BF))
+        y = F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)
+        check_product(y, values(a, a_s, 1), values(b, b_s, 128))
+        assert torch.equal(F8.fp8_gemm(a.contiguous(), a_s, b, b_s, out_dtype=F32), y)
+        assert torch.equal(F8.fp8_gemm(a, a_s, b.contiguous(), b_s, out_dtype=F32), y)
+    one, many = torch.empty(k, dtype=E4, device="cuda"), torch.empty(2, k, dtype=E4, device="cuda")
+    assert lib.qi8_gemm_f8_workspace_bytes(one.data_ptr(), 1, k, k, one.data_ptr(), 1, k) == 0
+    assert lib.qi8_gemm_f8_workspace_bytes(many.data_ptr(), 2, k, k, one.data_ptr(), 1, k) == 2 * (-(-k // 16) * 16)
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 6144, 4096), (2, 6144, 4096), (3, 4096, 5120), (5, 2560, 2560), (8, 4096, 2560),
+                                   (9, 2560, 2560), (4, 8192, 1024), (4, 8208, 1024), (1, 500, 5248), (7, 1000, 2600),
+                                   (33, 700, 2560), (100, 4096, 10240), (60, 2048, 1300), (128, 1024, 8192)])
+def test_gemm_beside_the_borders_of_its_kernels(m, n, k):
+    a, b = wide(m, k, seed=m), wide(n, k, seed=n)
+    bias = randn(n, seed=5, dtype=HF)
+    (aq, a_s), (bq, b_s) = F8.act_quant_fp8(a), F8.weight_quant_fp8(b)
+    for out in (BF, F32):
+        check_product(F8.fp8_gemm(aq, a_s, bq, b_s, bias, out), values(aq, a_s, 1), values(bq, b_s, 128), bias)
+    assert torch.equal(F8.fp8_linear(a.to(BF), bq, b_s), F8.fp8_gemm(*F8.act_quant_fp8(a.to(BF)), bq, b_s))
