@@ -27,7 +27,8 @@ constexpr int ROWS = 16, MOST_TOKENS = 8, WARPS = 8, COPIER = WARPS, THREADS = (
 constexpr int PIECE = WARPS * F8_BLOCK;           // columns of K per stage
 constexpr int PIECE_PITCH = PIECE + 16, STAGE = ROWS * PIECE_PITCH;
 constexpr int MAX_STAGES = 4, SMEM_MOST = 110 * 1024;  // two blocks per SM at least
-constexpr int SM_SMEM = 228 * 1024, STATIC_SMEM = 6000;                      // with what a block takes besides, rounded up
+constexpr int SM_SMEM = 228 * 1024;
+constexpr int STATIC_SMEM = 6000;  // of a block beside its ring and tokens, rounded up
 
 struct Args {
   F8Gemm g;
@@ -251,11 +252,11 @@ int launch(const Args& p, int smem, cudaStream_t st) {
 }  // namespace
 
 // Where this kernel is the faster one (cold weights, tcgen05 second): 1 x 4096 x 4096
-// 5.7 us and 6.7, 1 x 4096 x 5120 6.5 and 7.6, 2 x 4096 x 4096 5.8 and 6.8, 4 x 4096 x 4096 6.7 and 6.9, 8 x 4096 x 4096 7.9 and 6.9, 8 x 2560 x
-// 2560 5.6 and 6.1, 1 x 10240 x 2048 8.3 and 6.9, 4 x 2048 x 6144 7.2 and 6.4.  Tokens
-// beyond four cost it steps, many blocks their start, and it does not split K.  All
-// blocks have to run at once: 1 x 6144 x 4096 (three per SM) takes 7.6 us and 8.2, two
-// tokens (two per SM) 10.1 and 8.2.
+// 5.7 us and 6.7, 1 x 4096 x 5120 6.5 and 7.6, 2 x 4096 x 4096 5.8 and 6.8, 4 x 4096 x
+// 4096 6.7 and 6.9, 8 x 4096 x 4096 7.9 and 6.9, 8 x 2560 x 2560 5.6 and 6.1, 1 x 10240 x
+// 2048 8.3 and 6.9, 4 x 2048 x 6144 7.2 and 6.4.  Tokens beyond four cost it steps, many
+// blocks their start, and it does not split K.  All blocks have to run at once: 1 x 6144
+// x 4096 (three per SM) takes 7.6 us and 8.2, two tokens (two per SM) 10.1 and 8.2.
 bool gemm_f8_rows_fits(int M, int N, int K) {
   if (M > 8 || N > 8192 || K > 5120 || (M > 4 && (K > 2560 || (int64_t)N * K > 10500000))) return false;
   int pitch, smem;
