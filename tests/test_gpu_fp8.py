@@ -473,3 +473,26 @@ def test_gemm_beside_the_borders_of_its_kernels(m, n, k):
     for out in (BF, F32):
         check_product(F8.fp8_gemm(aq, a_s, bq, b_s, bias, out), values(aq, a_s, 1), values(bq, b_s, 128), bias)
     assert torch.equal(F8.fp8_linear(a.to(BF), bq, b_s), F8.fp8_gemm(*F8.act_quant_fp8(a.to(BF)), bq, b_s))
+
+
+@pytest.mark.parametrize("m", [1, 60, 700])
+def test_beside_the_other_products_on_another_stream(m):
+    # both kinds of kernels hold tensor memory and most of an SM's shared memory
+    k, n = 1024, 2048
+    x = randn(m, k, dtype=BF)
+    w, w_s = F8.weight_quant_fp8(randn(n, k, seed=1, dtype=BF))
+    a, b = (torch.randint(-127, 128, s, dtype=torch.int8, device="cuda") for s in ((600, k), (n, k)))
+    w4, s4 = ops.quant_weight_i4(randn(n, k, seed=2, dtype=BF))
+    y8, y32, y4 = F8.fp8_linear(x, w, w_s), ops.gemm_i8(a, b, out_dtype=torch.int32), ops.gemm_w4(x, w4, s4)
+    torch.cuda.synchronize()
+    one, two = torch.cuda.Stream(), torch.cuda.Stream()
+    got = []
+    for _ in range(20):
+        with torch.cuda.stream(one):
+            got.append((F8.fp8_linear(x, w, w_s), y8))
+        with torch.cuda.stream(two):
+            got.append((ops.gemm_i8(a, b, out_dtype=torch.int32), y32))
+            got.append((ops.gemm_w4(x, w4, s4), y4))
+            got.append((F8.fp8_linear(x, w, w_s), y8))
+    torch.cuda.synchronize()
+    assert all(torch.equal(u, v) for u, v in got)
