@@ -131,16 +131,26 @@ __device__ __forceinline__ F8x combine(const Args& p, const Eight<T>& a, const E
 
 // `N` pieces of a row of each input, `step` columns apart, zero past the end: all
 // loads are issued before the first is used.
-template <typename T, int OP, int N, bool WHOLE>
+// LATE: rows that are not WHOLE are shifted in get(), which holds twice the registers
+// (gates with one scale per row: 2000 x 4099 takes 19 us so and 32 with shifts in
+// load(); the norm, whose registers are short, gains nothing).
+template <typename T, int OP, int N, bool WHOLE, bool LATE = false>
 struct Raw {
-  Eight<T> u[N], v[N];
+  static constexpr bool LOOSE = !WHOLE && LATE;
+  std::conditional_t<LOOSE, Loose<T>, Eight<T>> u[N], v[N];
 
   __device__ __forceinline__ void load(const Args& p, int64_t row, int64_t col, int step) {
     const T* a = static_cast<const T*>(p.x) + row * p.ld_x + col;
     const T* b = static_cast<const T*>(p.second) + row * p.ld_second + col;
     const bool two = OP != PLAIN && p.second;
     const int64_t left = p.n - col;  // columns from the first piece on
-    if constexpr (WHOLE) {
+    if constexpr (LOOSE) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) u[i].load(a - col, col + i * step, p.n);
+      if (two)
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i].load(b - col, col + i * step, p.n);
+    } else if constexpr (WHOLE) {
 #pragma unroll
       for (int i = 0; i < N; ++i) i * step < left ? u[i].load(a + i * step) : u[i].clear();
       if (two)
@@ -166,16 +176,25 @@ struct Raw {
       }
     }
   }
-  __device__ __forceinline__ void get(const Args& p, F8x (&y)[N]) const {
+  // of the row that was loaded last
+  __device__ __forceinline__ void get(const Args& p, int64_t row, int64_t col, int step, F8x (&y)[N]) const {
+    if constexpr (LOOSE) {
+      const T* a = static_cast<const T*>(p.x) + row * p.ld_x;
+      const T* b = static_cast<const T*>(p.second) + row * p.ld_second;
 #pragma unroll
-    for (int i = 0; i < N; ++i) y[i] = combine<T, OP>(p, u[i], v[i]);
+      for (int i = 0; i < N; ++i)
+        y[i] = combine<T, OP>(p, u[i].get(a, col + i * step, p.n), v[i].get(b, col + i * step, p.n));
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) y[i] = combine<T, OP>(p, u[i], v[i]);
+    }
   }
 };
 template <typename T, int OP, bool WHOLE, int N>
 __device__ __forceinline__ void row_values(const Args& p, int64_t row, int64_t col, int step, F8x (&y)[N]) {
   Raw<T, OP, N, WHOLE> raw;
   raw.load(p, row, col, step);
-  raw.get(p, y);
+  raw.get(p, row, col, step, y);
 }
 
 template <typename T, bool WHOLE>
@@ -316,16 +335,18 @@ __global__ void __launch_bounds__(ROW_THREADS) row_kernel(const __grid_constant_
   int64_t row = blockIdx.x * per + mine;
   wait_for_last_kernel();
   if (row >= p.rows) return;
-  Raw<T, OP, CHUNKS, WHOLE> raw;
-  raw.load(p, row, col0, step);
+  constexpr bool LATE = OP != NORM;
+  Raw<T, OP, CHUNKS, WHOLE, LATE> raw;
+  if (WHOLE || !LATE) raw.load(p, row, col0, step);
   F8x w[CHUNKS];
   if (OP == NORM && p.weight)
 #pragma unroll
     for (int c = 0; c < CHUNKS; ++c) w[c] = load_weight<WHOLE>(p, col0 + c * step);
   for (int turn = 0; row < p.rows; row += stride, turn ^= 1) {
     F8x y[CHUNKS];
-    raw.get(p, y);
-    if (row + stride < p.rows) raw.load(p, row + stride, col0, step);
+    if (!WHOLE && LATE) raw.load(p, row, col0, step);
+    raw.get(p, row, col0, step, y);
+    if ((WHOLE || !LATE) && row + stride < p.rows) raw.load(p, row + stride, col0, step);
     if constexpr (OP == NORM) {
       float ss = 0.0f;
 #pragma unroll

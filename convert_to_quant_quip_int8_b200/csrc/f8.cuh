@@ -159,6 +159,62 @@ struct Eight {
   }
 };
 
+// Bytes `off` (a multiple of the element's size, below 16) to off + 4 WORDS of a row of words.
+template <int WORDS>
+__device__ __forceinline__ void shift_out(uint32_t (&a)[WORDS + 4], uint32_t off, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < WORDS + 3; ++i) a[i] = off & 4u ? a[i + 1] : a[i];
+#pragma unroll
+  for (int i = 0; i < WORDS + 1; ++i) a[i] = off & 8u ? a[i + 2] : a[i];
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) w[i] = __funnelshift_r(a[i], a[i + 1], 8 * (off & 3u));
+}
+
+// Eight elements from column `col` of a row of n >= 1 on, wherever the row starts and
+// ends: the aligned 16 bytes that hold them are loaded, all of which hold an element of
+// the row, and shifted once they are there.  Columns from n on are zero.
+template <typename T>
+struct Loose {
+  static constexpr int CHUNKS = sizeof(T) / 2 + 1;
+  uint4 c[CHUNKS];
+
+  __device__ __forceinline__ void load(const T* row, int64_t col, int64_t n) {
+    if (col + 8 <= n) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(row + col);
+      const uint4* first = reinterpret_cast<const uint4*>(at & ~(uintptr_t)15);
+#pragma unroll
+      for (int i = 0; i + 1 < CHUNKS; ++i) c[i] = __ldg(first + i);
+      c[CHUNKS - 1] = __ldg(reinterpret_cast<const uint4*>((at + 15) & ~(uintptr_t)15) + (CHUNKS - 2));
+    } else {
+      const uintptr_t first = reinterpret_cast<uintptr_t>(row + min(col, n - 1)) & ~(uintptr_t)15;
+      const uintptr_t last = (reinterpret_cast<uintptr_t>(row + n) - 1) & ~(uintptr_t)15;
+#pragma unroll
+      for (int i = 0; i < CHUNKS; ++i) c[i] = __ldg(reinterpret_cast<const uint4*>(min(first + 16 * i, last)));
+    }
+  }
+  __device__ __forceinline__ Eight<T> get(const T* row, int64_t col, int64_t n) const {
+    constexpr int WORDS = 2 * sizeof(T);
+    uint32_t a[WORDS + 4];
+#pragma unroll
+    for (int i = 0; i < CHUNKS; ++i) {
+      a[4 * i] = c[i].x;
+      a[4 * i + 1] = c[i].y;
+      a[4 * i + 2] = c[i].z;
+      a[4 * i + 3] = c[i].w;
+    }
+    Eight<T> e;
+    shift_out<WORDS>(a, (uint32_t)(reinterpret_cast<uintptr_t>(row + col) & 15u), reinterpret_cast<uint32_t*>(e.v));
+    if (col + 8 > n) {
+      const int left = (int)max(n - col, (int64_t)0);
+      T* v = reinterpret_cast<T*>(e.v);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i >= left) v[i] = T(0.0f);
+    }
+    return e;
+  }
+};
+
 // The largest |value| as fp32 bits; NaN is above infinity.  One instruction for
 // two values.
 __device__ __forceinline__ uint32_t amax_bits(const F8x& f) {
