@@ -39,9 +39,18 @@ __device__ __forceinline__ float2 exp2_of(float2 x) {
   return e;
 }
 
-// x / (1 + 2^-t): 0 where 2^-t passes fp32, as it should be
-__device__ __forceinline__ float2 swish(float2 x, float2 minus_t) {
-  const float2 e = __fadd2_rn(exp2_of(minus_t), both(1.0f));
+// x / (1 + 2^m), given m - 7.  Quotient and denominator are taken 2^-7 times, since
+// __fdividef returns 0 for denominators above 2^126 while the result is a normal number
+// up to m = 132.6: so it is 0 only where it would be none.  (x under 2^-119 loses its
+// last bits instead.)  This is coarser than fp32 has to be: m's constant and its value
+// are rounded once each, which counts |m| ln 2 times, exp2 and the division are off by
+// 2 units each, in all at most (16 + 2 |m| ln 2) 2^-24 of the result: 1.6e-6 at x = -5, 8e-6
+// at x = -60, where a code is off by up to 2^-4 (e4m3) or 2^-8 (int8).  A second word of m
+// would cost as many instructions as exp2 itself.
+constexpr float SWISH_SHIFT = 7.0f, SWISH_SCALE = 0.0078125f;
+__device__ __forceinline__ float2 swish(float2 x, float2 m) {
+  const float2 e = __fadd2_rn(exp2_of(m), both(SWISH_SCALE));
+  x = __fmul2_rn(x, both(SWISH_SCALE));
   return make_float2(__fdividef(x.x, e.x), __fdividef(x.y, e.y));
 }
 
@@ -78,13 +87,13 @@ __device__ __forceinline__ F8x gate(const F8x& g, const F8x& up) {
     const float2 x = g.v[i];
     float2 a;
     if constexpr (ACT == QI8_ACT_SILU) {
-      a = swish(x, __fmul2_rn(x, both(-1.4426950408889634f)));  // -log2(e)
+      a = swish(x, __ffma2_rn(x, both(-1.4426950408889634f), both(-SWISH_SHIFT)));  // -log2(e)
     } else if constexpr (ACT == QI8_ACT_GELU) {
       a = gelu(x);
     } else {
       // 0.5 x (1 + tanh(u)) = x / (1 + exp(-2 u)), u = sqrt(2 / pi) (x + 0.044715 x^3)
       const float2 c = __ffma2_rn(__fmul2_rn(x, x), both(-0.10294324f), both(-2.3022082f));
-      a = swish(x, __fmul2_rn(x, c));
+      a = swish(x, __ffma2_rn(x, c, both(-SWISH_SHIFT)));
     }
     y.v[i] = __fmul2_rn(a, up.v[i]);
   }

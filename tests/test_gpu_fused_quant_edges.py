@@ -1,10 +1,14 @@
-"""GPU tests of the int8 read-back at the sizes where it goes another way."""
+"""GPU tests of the quantized gate at far values and of the int8 read-back of short rows."""
+
+import math
 
 import pytest
 import torch
 
 from convert_to_quant_quip_int8_b200 import _lib as L
 from convert_to_quant_quip_int8_b200 import ops
+from convert_to_quant_quip_int8_b200.comfy import fused_quant_kernels as FQ
+from test_gpu_fused_quant import check_codes, exact_gated, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -61,3 +65,43 @@ def test_one_scale_for_more_than_32_bits_of_values():
     s = torch.full((1,), 0.5, device="cuda")
     v = ops.dequant(q, s, L.QI8_S_SCALAR, out_dtype=BF)
     assert v[-1, -4:].tolist() == [0.5, 2.5, -3.0, 3.5] and v[0, 0] == 0.5 and (v[1234] == 0.5).all()
+
+
+# ------------------------------------------------------------- far gates
+def far_gated(g, u, act):
+    """exact_gated, where act itself may be small.  Up to t = 92.1 the quotient is taken, and its rounding off by 2^-149
+    at most, which counts |u| times; from there on act is under 2^-126 and may be 0."""
+    y, _ = exact_gated(g, u, act)
+    g, u = g.double(), u.double().abs()
+    t = -g if act == "silu" else -2 * math.sqrt(2 / math.pi) * (g + 0.044715 * g ** 3)
+    near = t < 92.1
+    # the argument's rounding counts |t| times, that of u in the tanh form four units
+    rel = 4 * (4 + t.abs() * (1 if act == "silu" else 4)) * 2.0 ** -24
+    return y, rel * y.abs() + torch.where(near, 2.0 ** -148, 2.0 ** -126) * u
+
+
+@pytest.mark.parametrize("output", ["fp8", "int8", "int8_block"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+def test_gates_as_far_as_results_are_normal_numbers(act, output):
+    # 1 + exp(t) passes 2^126 from t = 87.3 on, where act is a normal number down to t = 91.9 (silu) and 89.7 (tanh)
+    if act == "silu":
+        g = -torch.cat([torch.linspace(80, 91.8, 60), torch.tensor([87.5, 88.0, 88.5, 95.0, 300.0])])
+    else:
+        g = -torch.cat([torch.linspace(9.7, 10.1, 60), torch.tensor([10.02, 10.05, 10.4, 11.0, 300.0])])
+    g = g.cuda()[:, None].expand(-1, 256).contiguous()
+    u = randn(*g.shape, seed=1) * 1e30
+    q, s = FQ.gated_act_quant(g, u, activation=act, output=output)
+    check_codes(q, s, *far_gated(g, u, act), output)
+
+
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("output", ["fp8", "int8", "int8_block"])
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_gates_of_one_size(act, output, dtype, sign):
+    # each row's gates are near one value, so that its scale follows them into the tail
+    centre = torch.tensor([0.02, 0.3, 1.0, 2.0, 3.0, 4.0, 5.0, 6.0, 8.0, 10.0, 12.0])
+    g = sign * (centre.cuda()[:, None] * (1 + 0.02 * randn(11, 384, seed=2))).to(dtype)
+    u = randn(11, 384, seed=3, dtype=dtype) * (1.0 if dtype == HF else 2.0 ** 60)
+    q, s = FQ.gated_act_quant(g, u, activation=act, output=output)
+    check_codes(q, s, *far_gated(g, u, act), output)
