@@ -57,9 +57,11 @@ __device__ __forceinline__ float2 swish(float2 x, float2 m) {
 // x Phi(x) = max(x, 0) - |x| h, h = Phi(-|x|) = exp(-x^2 / 2) R(|x|).  R, half the
 // scaled complementary error function of |x| / sqrt(2), falls like 1 / |x|: t times a
 // polynomial in t = 1 / (1 + 0.27 |x|), fitted here by least squares weighted
-// towards the largest relative error, which is 2.3e-8 (with fp32's roundings h is off
-// by under 4e-7 of itself up to |x| = 3 and x Phi(x) by 2e-7 of x everywhere).  erff
-// has two cases, of which a warp meets both: 4096 x 10240 took 58 us with it.
+// towards the largest relative error, which is 4.2e-8 up to |x| = 10.  In fp32 h is off
+// by 6.2e-7 of itself up to |x| = 3 and 7.5e-6 at 12 if exp2 and the division were exact
+// (the rounding of x^2 counts x^2 / 2 times), with them by at most (32 + 2 x^2) 2^-24, and
+// x Phi(x) by 2e-7 of x.  erff has two cases, of which a warp meets both: 4096 x 10240
+// took 58 us with it.
 __device__ __forceinline__ float2 gelu(float2 x) {
   const float2 u = make_float2(fabsf(x.x), fabsf(x.y));
   const float2 d = __ffma2_rn(u, both(0.27f), both(1.0f));

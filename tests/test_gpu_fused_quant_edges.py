@@ -105,3 +105,21 @@ def test_gates_of_one_size(act, output, dtype, sign):
     u = randn(11, 384, seed=3, dtype=dtype) * (1.0 if dtype == HF else 2.0 ** 60)
     q, s = FQ.gated_act_quant(g, u, activation=act, output=output)
     check_codes(q, s, *far_gated(g, u, act), output)
+
+
+# The error of x Phi(x) = max(x, 0) - |x| h, h = exp(-x^2 / 2) t p(t), t = 1 / (1 + 0.27 |x|), in units of 2^-24: of
+# x^2 / 2 three (square, constant, product), which count x^2 / 2 times; exp2 four; t five, which count up to three
+# times in t p(t); p's steps five, the fit one, three products and the difference: under 32 + 2 x^2 of |x| h, and two
+# of the result.
+@pytest.mark.parametrize("dtype", [BF, HF, F32])
+@pytest.mark.parametrize("output", ["fp8", "int8", "int8_block"])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_gelu_of_gates_of_one_size(output, dtype, sign):
+    centre = torch.tensor([0.02, 0.3, 1.0, 2.0, 3.0, 4.0, 5.0, 6.0, 8.0, 10.0, 12.0])
+    g = sign * (centre.cuda()[:, None] * (1 + 0.02 * randn(11, 384, seed=2))).to(dtype)
+    u = randn(11, 384, seed=3, dtype=dtype) * (1.0 if dtype == HF else 2.0 ** 60)
+    q, s = FQ.gated_act_quant(g, u, activation="gelu", output=output)
+    y, _ = exact_gated(g, u, "gelu")
+    x = g.double().abs()
+    h = 0.5 * torch.special.erfc(x / math.sqrt(2))
+    check_codes(q, s, y, 2.0 ** -24 * ((32 + 2 * x * x) * x * h * u.double().abs() + 2 * y.abs()), output)
