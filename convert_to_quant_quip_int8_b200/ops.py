@@ -754,6 +754,8 @@ def quant_weight_f8(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     if pair is not None:
         return pair
     dev = _one_device(w)
+    with torch.no_grad():  # a parameter's gradient may be lost, a tangent not
+        _refuse_grad(w)
     dt = _float_code(w.dtype, "weights")
     assert w.dim() == 2, f"weight of shape {tuple(w.shape)}: expected [N, K]"
     n, k = w.shape
