@@ -237,7 +237,7 @@ def _device_transfer(qt, target_device, target_dtype=None):
         target_device = torch.device(target_device)
         if target_device != qt._qdata.device:
             params = _map_tensors(qt._layout_params, lambda v: v.to(device=target_device))
-            if target_dtype is not None:
+            if target_dtype is not None and target_dtype != qt.dtype:  # a transfer alone names the codes' type
                 params["orig_dtype"] = target_dtype
             return QuantizedTensor(qt._qdata.to(device=target_device), qt._layout_type, params)
     return qt

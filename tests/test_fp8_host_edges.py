@@ -7,6 +7,7 @@ import torch.autograd.forward_ad as fwd
 from convert_to_quant_quip_int8_b200 import ops
 from convert_to_quant_quip_int8_b200.comfy import fp8_kernels as F8
 from convert_to_quant_quip_int8_b200.comfy import fused_quant_kernels as FQ
+from convert_to_quant_quip_int8_b200.comfy.quant_ops import QuantizedTensor
 
 BF = torch.bfloat16
 
@@ -20,3 +21,11 @@ def test_tangents_are_refused(monkeypatch, grad):
         for f in (F8.weight_quant_fp8, F8.act_quant_fp8, FQ.rms_norm_quant, lambda t: FQ.gated_act_quant(x, t)):
             with pytest.raises(RuntimeError, match="forward mode"):
                 f(d)
+
+
+@pytest.mark.parametrize("layout,code", [("BlockWiseFP8Layout", torch.float8_e4m3fn), ("TensorWiseINT8Layout", torch.int8)])
+def test_a_transfer_keeps_the_type_that_is_dequantized_to(layout, code):
+    t = QuantizedTensor(torch.zeros(4, 256).to(code), layout, {"scale": torch.zeros(1), "orig_dtype": BF,
+                                                               "block_size": 128, "is_weight": True})
+    assert t.to("meta")._layout_params["orig_dtype"] == BF
+    assert t.to("meta", torch.float16)._layout_params["orig_dtype"] == torch.float16
