@@ -89,6 +89,11 @@ class QuantizedLayout:
         """The shape that the tensor shows: the one that ``dequantize`` returns, where a layout packs its data."""
         return qdata.shape
 
+    @staticmethod
+    def laid_out(qdata, layout_params):
+        """``qdata`` with the strides that the layout's operators read without a copy of their own."""
+        return qdata
+
 
 class QuantizedTensor(torch.Tensor):
     """Wrapper subclass holding quantized ``_qdata`` plus layout parameters."""
@@ -100,7 +105,7 @@ class QuantizedTensor(torch.Tensor):
                                                    dtype=qdata.dtype, requires_grad=False)
 
     def __init__(self, qdata, layout_type, layout_params):
-        self._qdata = qdata
+        self._qdata = getattr(LAYOUTS.get(layout_type), "laid_out", QuantizedLayout.laid_out)(qdata, layout_params)
         self._layout_type = layout_type
         self._layout_params = layout_params
 
@@ -485,6 +490,12 @@ class BlockWiseFP8Layout(QuantizedLayout):
     @staticmethod
     def dequantize(qdata, scale, block_size, is_weight=False, orig_dtype=None, output_dtype=None, **kwargs):
         return ops.dequant_f8(qdata, scale, 128 if is_weight else 1, output_dtype or orig_dtype)
+
+    @staticmethod
+    def laid_out(qdata, layout_params):
+        # a clone, a transfer or a reload makes a weight's codes contiguous, and each product would copy them to rows
+        # of whole 16 bytes again
+        return ops.aligned_codes(qdata) if layout_params.get("is_weight") and qdata.is_cuda else qdata
 
     @classmethod
     def get_plain_tensors(cls, qtensor):

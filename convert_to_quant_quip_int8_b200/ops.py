@@ -717,6 +717,14 @@ def _code_rows(q: torch.Tensor) -> Tuple[torch.Tensor, int]:
     return _strided_rows(q)
 
 
+def aligned_codes(q: torch.Tensor) -> torch.Tensor:
+    """``q`` [N, K] with rows that start on 16-byte boundaries, as the quantizers return them: itself, or a copy."""
+    if q.numel() == 0 or ((q.shape[1] == 1 or q.stride(1) == 1) and q.storage_offset() % 16 == 0
+                          and (q.shape[0] == 1 or q.stride(0) % 16 == 0)):
+        return q
+    return _new_codes(q.shape, q.dtype, q.device).copy_(q)
+
+
 def _check_f8(q: torch.Tensor, scale: torch.Tensor, tile: int) -> None:
     """``q`` e4m3 [..., n] with a scale per row and 128 columns, or [N, K] with 128 x 128 tiles."""
     if q.dtype != _F8 or scale.dtype != _E8:

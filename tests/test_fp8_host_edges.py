@@ -23,6 +23,21 @@ def test_tangents_are_refused(monkeypatch, grad):
                 f(d)
 
 
+def test_codes_get_rows_of_whole_16_bytes():
+    q = torch.arange(7 * 40, dtype=torch.uint8).view(7, 40)
+    for v in (q, q[:, 3:], q[:, :33], q[1:2, 5:], q.t(), q[:0], q[:, :0], q[:, 7:8]):
+        c = v.contiguous().view(torch.float8_e4m3fn)
+        for t in (c, v.view(torch.float8_e4m3fn)):
+            a = ops.aligned_codes(t)
+            assert a.shape == t.shape and torch.equal(a.view(torch.uint8), t.view(torch.uint8))
+            if a.numel():
+                assert a.storage_offset() % 16 == 0 and (a.shape[0] == 1 or a.stride(0) % 16 == 0)
+            assert ops.aligned_codes(a) is a
+    whole = torch.zeros(3, 48, dtype=torch.uint8).view(torch.float8_e4m3fn)
+    assert ops.aligned_codes(whole) is whole
+    assert ops.aligned_codes(whole[:, :33]).data_ptr() == whole.data_ptr()
+
+
 @pytest.mark.parametrize("layout,code", [("BlockWiseFP8Layout", torch.float8_e4m3fn), ("TensorWiseINT8Layout", torch.int8)])
 def test_a_transfer_keeps_the_type_that_is_dequantized_to(layout, code):
     t = QuantizedTensor(torch.zeros(4, 256).to(code), layout, {"scale": torch.zeros(1), "orig_dtype": BF,
