@@ -14,7 +14,8 @@ from typing import Dict, Optional, Tuple
 
 import torch
 
-BLOCK_BASED_FORMATS = ("int8_blockwise",)
+# formats whose scales cover a block or group of the size that is recorded
+BLOCK_BASED_FORMATS = ("int8_blockwise", "float8_blockwise", "int4_groupwise")
 
 
 def dict_to_tensor(data_dict: dict) -> torch.Tensor:

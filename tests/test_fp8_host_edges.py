@@ -7,7 +7,8 @@ import torch.autograd.forward_ad as fwd
 from convert_to_quant_quip_int8_b200 import ops
 from convert_to_quant_quip_int8_b200.comfy import fp8_kernels as F8
 from convert_to_quant_quip_int8_b200.comfy import fused_quant_kernels as FQ
-from convert_to_quant_quip_int8_b200.comfy.quant_ops import QuantizedTensor
+from convert_to_quant_quip_int8_b200.comfy.quant_ops import QUANT_ALGOS, QuantizedTensor
+from convert_to_quant_quip_int8_b200.utils import comfy_quant as CQ
 
 BF = torch.bfloat16
 
@@ -44,3 +45,10 @@ def test_a_transfer_keeps_the_type_that_is_dequantized_to(layout, code):
                                                                "block_size": 128, "is_weight": True})
     assert t.to("meta")._layout_params["orig_dtype"] == BF
     assert t.to("meta", torch.float16)._layout_params["orig_dtype"] == torch.float16
+
+
+def test_metadata_keeps_the_block_size():
+    for name, algo in QUANT_ALGOS.items():
+        size = algo.get("group_size", 128)
+        meta = CQ.tensor_to_dict(CQ.create_comfy_quant_tensor(name, block_size=size))
+        assert meta == ({"format": name, "group_size": size} if "group_size" in algo else {"format": name})
