@@ -884,16 +884,17 @@ int gemm_f8_tiles(const F8Gemm& g, cudaStream_t st) {
   // Blocks that share a tile's K: a K block takes 0.21 us up to 64 tokens and 0.27 with
   // 128, or what the weight takes from HBM, the join 1.4 us and 0.003 for each token and
   // block.  Fitted to 21 shapes of 9 to 256 tokens, of which it misses the best choice in
-  // two, by 5 % at most: 16 x 4096 x 4096 takes 8.7 us with whole tiles, 7.4 with two
-  // blocks each and 7.0 with four, 100 x 4096 x 10240 21.7, 15.9 and 14.5, 100 x 8192 x
-  // 4096 12.2 and, with two, 13.4.  Of clusters of two 74 run at once, of four 33, of
-  // eight 15; three blocks were never faster than two or four.
+  // two, by 5 % at most (64 x 4224 x 8192 and x 10240, beside them, by 6): 16 x 4096 x 4096
+  // takes 8.7 us with whole tiles, 7.4 with two blocks each and 7.0 with four, 100 x 4096 x
+  // 10240 21.7, 15.9 and 14.5, 100 x 8192 x 4096 12.2 and, with two, 13.4; 16 x 4224 x 4096
+  // 7.4 with two and 7.1 with four.  Of clusters of two 74 run at once on 148 SMs, of four
+  // 33, of eight 15; three blocks were never faster than two or four.
   const int bn = (int)((g.M + t_tiles - 1) / t_tiles + 15) & ~15;
   const double block_us = bn <= 64 ? 0.21 : 0.21 + 0.06 / 64 * (bn - 64), read_us = (double)g.N * g.K / 5.5e6;
   int split = 1, room = sms;
   double best = fmax(g.KB * block_us, read_us);
   for (int s : {2, 4, 8}) {
-    const int there = s == 2 ? sms : s == 8 ? sms * 13 / 16 : sms * 57 / 64;
+    const int there = s == 2 ? sms : s == 8 ? sms * 30 / 37 : sms * 33 / 37;
     const double us = fmax((g.KB + s - 1) / s * block_us, read_us) + 1.4 + 0.003 * bn * s;
     if (s <= g.KB && n_tiles * t_tiles * s <= there && us < best) best = us, split = s, room = there;
   }

@@ -8,7 +8,7 @@ from convert_to_quant_quip_int8_b200 import _lib as L
 from convert_to_quant_quip_int8_b200 import ops
 from convert_to_quant_quip_int8_b200.comfy import fp8_kernels as F8
 from convert_to_quant_quip_int8_b200.comfy.quant_ops import QuantizedTensor
-from test_gpu_fp8 import randn
+from test_gpu_fp8 import check_product, randn, values, wide
 
 pytestmark = pytest.mark.gpu
 
@@ -37,3 +37,15 @@ def test_copies_of_a_weight_keep_rows_that_products_take(k):
         assert torch.equal(F.linear(x, t), expected) and torch.equal(t.dequantize(), wq.dequantize())
     assert wq.detach()._qdata.data_ptr() == wq._qdata.data_ptr()
     assert wq.cpu()._qdata.is_contiguous()
+
+
+# as many tiles as clusters of four, or of two and eight, run at once, and one more
+@pytest.mark.parametrize("m", [9, 64, 100])
+@pytest.mark.parametrize("n,k", [(4224, 4096), (4225, 4096), (4160, 10240), (1920, 10240), (1921, 10240), (9472, 2048),
+                                 (9473, 2048)])
+def test_gemm_with_as_many_clusters_as_run_at_once(m, n, k):
+    a, a_s = F8.act_quant_fp8(wide(m, k, seed=m))
+    b, b_s = F8.weight_quant_fp8(wide(n, k, seed=n))
+    y = F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)
+    check_product(y, values(a, a_s, 1), values(b, b_s, 128))
+    assert all(torch.equal(y, F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)) for _ in range(3))
