@@ -49,3 +49,44 @@ def test_gemm_with_as_many_clusters_as_run_at_once(m, n, k):
     y = F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)
     check_product(y, values(a, a_s, 1), values(b, b_s, 128))
     assert all(torch.equal(y, F8.fp8_gemm(a, a_s, b, b_s, out_dtype=F32)) for _ in range(3))
+
+
+# ------------------------------------------------------- kernels in a chain
+# The one read before the wait for the last kernel: gemm_f8_rows_kernel copies its weight while the tokens' quantizer
+# runs.  Cases that get there (at most 8 tokens, more than 8192 values of x): 5 and 8 x 2048, 3 x 4096.  5 and 8 x 2100
+# with contiguous codes too, behind a kernel that brings the weight to rows of 16 bytes.  2 x 2048 quantizes in each
+# block and waits first, 9 x 2048 goes to the tcgen05 kernel.
+@pytest.mark.parametrize("m,k,contiguous", [(2, 2048, False), (5, 2048, False), (8, 2048, False), (3, 4096, False),
+                                            (5, 2100, True), (8, 2100, True), (3, 4090, True), (9, 2048, False),
+                                            (9, 2100, True)])
+def test_weights_written_just_before(m, k, contiguous):
+    n = 1500
+    xs, ws = [randn(m, k, seed=s, dtype=BF) for s in range(4)], [randn(n, k, seed=s, scale=0.05, dtype=BF) for s in range(4)]
+    ready = [F8.weight_quant_fp8(w) for w in ws]
+    if contiguous:
+        ready = [(q.contiguous(), s) for q, s in ready]
+    expected = [F8.fp8_linear(x, *w) for x, w in zip(xs, ready)]
+    torch.cuda.synchronize()
+    x, q, s = torch.empty_like(xs[0]), ready[0][0].clone(), ready[0][1].clone()
+    assert not contiguous or q.stride(0) % 16
+    got = []
+    for i in list(range(4)) * 6:
+        x.copy_(xs[i])
+        s.view(torch.uint8).copy_(ready[i][1].view(torch.uint8))
+        q.copy_(ready[i][0])  # the kernel before the product's first
+        got.append((F8.fp8_linear(x, q, s), expected[i]))
+        w, w_s = F8.weight_quant_fp8(ws[i])  # one that lets the next start early
+        got.append((F8.fp8_linear(x, w.contiguous() if contiguous else w, w_s), expected[i]))
+    # the same in a graph, where launches follow one another at once
+    g, outs = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(g):
+        for i in list(range(4)) * 3:
+            w, w_s = F8.weight_quant_fp8(ws[i])
+            q.view(torch.uint8).copy_(w.view(torch.uint8))
+            s.view(torch.uint8).copy_(w_s.view(torch.uint8))
+            outs.append((F8.fp8_linear(xs[i], w, w_s), expected[i]))
+            outs.append((F8.fp8_linear(xs[i], q, s), expected[i]))
+    for _ in range(5):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(y, e) for y, e in got + outs)
