@@ -90,3 +90,26 @@ def test_weights_written_just_before(m, k, contiguous):
         g.replay()
     torch.cuda.synchronize()
     assert all(torch.equal(y, e) for y, e in got + outs)
+
+
+# ------------------------------------------------------------------- sums
+@pytest.mark.parametrize("m,n,k", [(1, 300, 5120), (4, 300, 5120), (8, 300, 2560), (16, 300, 16384), (100, 520, 16384),
+                                   (128, 5000, 16384), (300, 5000, 16384)])
+def test_sums_keep_24_bits(m, n, k):
+    # odd codes from 9 to 15: products of 81 to 225 are whole numbers, as are sums of any order, which stay under 2^22
+    # and so are exact in fp32, and in nothing with fewer than 22 bits
+    g = torch.Generator().manual_seed(m)
+    a, b = (torch.randint(4, 8, s, generator=g).mul(2).add(1).float().cuda() for s in ((m, k), (n, k)))
+    one = [torch.full(s, 127, dtype=torch.uint8, device="cuda").view(torch.float8_e8m0fnu)
+           for s in ((m, -(-k // 128)), (-(-n // 128), -(-k // 128)))]
+    y = F8.fp8_gemm(a.to(torch.float8_e4m3fn), one[0], b.to(torch.float8_e4m3fn), one[1], out_dtype=F32)
+    want = a.double() @ b.double().T
+    assert want.max() < 2 ** 22 and torch.equal(y.double(), want)
+    # and beside a product 2^17 times as large as the others' sum: the accumulator's last bits count
+    a[:, 0], b[:, 0] = 448.0, 448.0
+    for side, t in ((0, a), (1, b)):
+        one[side].view(torch.uint8)[:, 0] = 127 + 2
+    a[:, 1:128], b[:, 1:128] = 0.0, 0.0
+    y = F8.fp8_gemm(a.to(torch.float8_e4m3fn), one[0], b.to(torch.float8_e4m3fn), one[1], out_dtype=F32)
+    want = 448.0 * 448.0 * 16 + a[:, 128:].double() @ b[:, 128:].double().T
+    assert want.max() < 2 ** 24 and torch.equal(y.double(), want)
