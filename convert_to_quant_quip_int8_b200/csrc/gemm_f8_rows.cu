@@ -26,9 +26,19 @@ namespace f8r {
 constexpr int ROWS = 16, MOST_TOKENS = 8, WARPS = 8, COPIER = WARPS, THREADS = (WARPS + 1) * 32;
 constexpr int PIECE = WARPS * F8_BLOCK;           // columns of K per stage
 constexpr int PIECE_PITCH = PIECE + 16, STAGE = ROWS * PIECE_PITCH;
-constexpr int MAX_STAGES = 4, SMEM_MOST = 110 * 1024;  // two blocks per SM at least
+constexpr int MAX_STAGES = 4;
 constexpr int SM_SMEM = 228 * 1024;
 constexpr int STATIC_SMEM = 6000;  // of a block beside its ring and tokens, rounded up
+// Largest K, up to four tokens and beyond (gemm_f8_rows_fits).
+constexpr int FEW_TOKENS = 4, FEW_K = 5120, MOST_K = 2560;
+
+// Bytes between tokens in shared memory, and of all of them with their scales.
+constexpr int pitch_for(int KB) { return KB * F8_BLOCK + 16; }
+constexpr int tokens_for(int M, int KB) { return M * (pitch_for(KB) + KB); }
+// Two blocks of any size share an SM.
+static_assert(MAX_STAGES * STAGE + tokens_for(FEW_TOKENS, FEW_K / F8_BLOCK) <= SM_SMEM / 2 - STATIC_SMEM &&
+                  MAX_STAGES * STAGE + tokens_for(MOST_TOKENS, MOST_K / F8_BLOCK) <= SM_SMEM / 2 - STATIC_SMEM,
+              "shared memory");
 
 struct Args {
   F8Gemm g;
@@ -216,17 +226,12 @@ __global__ void __launch_bounds__(THREADS) gemm_f8_rows_kernel(const __grid_cons
   }
 }
 
-// Stages beside the tokens in half of an SM's shared memory; under two: none.
-int stages_for(int M, int K, int KB, int* x_pitch, int* smem) {
-  *x_pitch = KB * F8_BLOCK + 16;
-  const int64_t tokens = (int64_t)M * (*x_pitch + KB);
-  const int64_t left = (SMEM_MOST - tokens) / STAGE;
+// Stages of the ring: as many as there are pieces of K, up to four.
+int stages_for(int K) {
   const int pieces = (K + PIECE - 1) / PIECE;
-  int stages = left > MAX_STAGES ? MAX_STAGES : (int)left;
-  if (stages > pieces) stages = pieces;
-  *smem = (int)(stages * STAGE + tokens);
-  return tokens > SMEM_MOST || (stages < 2 && stages < pieces) ? 0 : stages;
+  return pieces < MAX_STAGES ? pieces : MAX_STAGES;
 }
+int smem_for(int M, int K) { return stages_for(K) * STAGE + tokens_for(M, (int)f8_blocks(K)); }
 
 template <typename X>
 int launch(const Args& p, int smem, cudaStream_t st) {
@@ -258,17 +263,17 @@ int launch(const Args& p, int smem, cudaStream_t st) {
 // blocks their start, and it does not split K.  All blocks have to run at once: 1 x 6144
 // x 4096 (three per SM) takes 7.6 us and 8.2, two tokens (two per SM) 10.1 and 8.2.
 bool gemm_f8_rows_fits(int M, int N, int K) {
-  if (M > 8 || N > 8192 || K > 5120 || (M > 4 && (K > 2560 || (int64_t)N * K > 10500000))) return false;
-  int pitch, smem;
-  if (f8r::stages_for(M, K, (int)f8_blocks(K), &pitch, &smem) == 0) return false;
-  const int per_sm = f8r::SM_SMEM / (smem + f8r::STATIC_SMEM);
-  return (N + f8r::ROWS - 1) / f8r::ROWS <= (per_sm < 7 ? per_sm : 7) * sm_count();
+  using namespace f8r;
+  if (M > MOST_TOKENS || N > 8192 || K > FEW_K || (M > FEW_TOKENS && (K > MOST_K || (int64_t)N * K > 10500000)))
+    return false;
+  const int per_sm = SM_SMEM / (smem_for(M, K) + STATIC_SMEM);
+  return (N + ROWS - 1) / ROWS <= (per_sm < 7 ? per_sm : 7) * sm_count();
 }
 
 int gemm_f8_rows(const F8Gemm& g, const void* x, int x_dtype, int64_t ld_x, bool after_quant, cudaStream_t st) {
-  f8r::Args p{g, x, ld_x, x && rows_aligned(x, ld_x, elem_size(x_dtype), 16), 0, 0, after_quant, device_status_ptr()};
-  int smem = 0;
-  p.stages = f8r::stages_for(g.M, g.K, g.KB, &p.x_pitch, &smem);
+  f8r::Args p{g, x, ld_x, x && rows_aligned(x, ld_x, elem_size(x_dtype), 16), f8r::stages_for(g.K),
+              f8r::pitch_for(g.KB), after_quant, device_status_ptr()};
+  const int smem = f8r::smem_for(g.M, g.K);
   if (!x) return f8r::launch<uint8_t>(p, smem, st);
   switch (x_dtype) {
     case QI8_BF16: return f8r::launch<__nv_bfloat16>(p, smem, st);
