@@ -129,8 +129,9 @@ extern "C" int qi8_linear_f8(const void* x, int x_dtype, int64_t M, int64_t K, i
   F8Gemm g{q, b, s, b_scale, bias, out, f8g::pitch(K), ld_b, ld_out, (int)M, (int)N, (int)K, (int)f8_blocks(K),
            bias_dtype, out_dtype};
   // Quantized by each block itself, the tokens cost a launch less, but every block the
-  // work: 1 x 4096 x 4096 takes 5.9 us so and 7.0 with a kernel for it, two tokens 6.8 and
-  // 6.7, four 8.4 and 7.0 (these with weights in L2).
+  // work.  Features x K 4096 x 4096 (weights from HBM): one token 5.5 us so and 6.5 with a
+  // kernel for it, two 6.3 and 6.6, three 7.2 and 7.0; 4096 x 2048: four 4.8 and 5.0, six 5.6
+  // and 5.4; 4096 x 1024: eight 3.9 and 4.0 (8192 x 1024 5.4 and 5.3); 1024 x 512: 2.3 and 3.3.
   if (gemm_f8_rows_fits((int)M, (int)N, (int)K) && M * K <= 8192)
     return gemm_f8_rows(g, x, x_dtype, ld_x, false, st);
   if (int rc = quant_rows_f8(x, x_dtype, M, K, ld_x, q, f8g::pitch(K), s, st)) return rc;
