@@ -111,8 +111,16 @@ __device__ __forceinline__ float warp_max(float v) {
 // (barrier init, TMEM allocation, descriptor prefetch), and waits in
 // pdl_wait() -- before its first global-memory access -- until that kernel
 // has completed and its writes are visible.  Without the launch attribute
-// both are no-ops.  Off by default: on the Flux-shaped stack (one CUDA graph
-// of 456 launches) it measured 34.1 ms per forward against 32.9 ms without.
+// pdl_wait() is a no-op.  Off by default: on the Flux-shaped stack (one CUDA
+// graph of 456 launches) it measured 34.1 ms per forward against 32.9 ms without.
+//
+// The kernels of f8.cuh's launch_early always have the attribute, so that one
+// of them behind a kernel that calls pdl_launch_dependents() starts early,
+// whatever QI8_PDL says.  Two rules follow for any kernel that calls it.  It
+// has waited (or was launched without the attribute), so that all kernels
+// before it are done when the next one starts; and it has allocated its tensor
+// memory, since the next one may take all 512 columns of an SM and keep them
+// until this kernel is done.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 // Lets the next kernel on the stream be scheduled (it still waits in pdl_wait).
 __device__ __forceinline__ void pdl_launch_dependents() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
