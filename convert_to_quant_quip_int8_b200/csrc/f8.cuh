@@ -78,6 +78,17 @@ struct F8x {
   float2 v[4];
 };
 
+// Bytes `off` (a multiple of the element's size, below 16) to off + 4 WORDS of a row of words.
+template <int WORDS>
+__device__ __forceinline__ void shift_out(uint32_t (&a)[WORDS + 4], uint32_t off, uint32_t* w) {
+#pragma unroll
+  for (int i = 0; i < WORDS + 3; ++i) a[i] = off & 4u ? a[i + 1] : a[i];
+#pragma unroll
+  for (int i = 0; i < WORDS + 1; ++i) a[i] = off & 8u ? a[i + 2] : a[i];
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) w[i] = __funnelshift_r(a[i], a[i + 1], 8 * (off & 3u));
+}
+
 // The same as they lie in memory.
 template <typename T>
 struct Eight {
@@ -103,13 +114,7 @@ struct Eight {
       a[4 * i + 2] = c.z;
       a[4 * i + 3] = c.w;
     }
-#pragma unroll
-    for (int i = 0; i < WORDS + 3; ++i) a[i] = off & 4u ? a[i + 1] : a[i];
-#pragma unroll
-    for (int i = 0; i < WORDS + 1; ++i) a[i] = off & 8u ? a[i + 2] : a[i];
-    uint32_t* w = reinterpret_cast<uint32_t*>(v);
-#pragma unroll
-    for (int i = 0; i < WORDS; ++i) w[i] = __funnelshift_r(a[i], a[i + 1], 8 * (off & 3u));
+    shift_out<WORDS>(a, off, reinterpret_cast<uint32_t*>(v));
   }
   // From column `col` on, zero from n on.
   __device__ __forceinline__ void load_some(const T* row, int64_t col, int64_t n) {
@@ -158,17 +163,6 @@ struct Eight {
     }
   }
 };
-
-// Bytes `off` (a multiple of the element's size, below 16) to off + 4 WORDS of a row of words.
-template <int WORDS>
-__device__ __forceinline__ void shift_out(uint32_t (&a)[WORDS + 4], uint32_t off, uint32_t* w) {
-#pragma unroll
-  for (int i = 0; i < WORDS + 3; ++i) a[i] = off & 4u ? a[i + 1] : a[i];
-#pragma unroll
-  for (int i = 0; i < WORDS + 1; ++i) a[i] = off & 8u ? a[i + 2] : a[i];
-#pragma unroll
-  for (int i = 0; i < WORDS; ++i) w[i] = __funnelshift_r(a[i], a[i + 1], 8 * (off & 3u));
-}
 
 // Eight elements from column `col` of a row of n >= 1 on, wherever the row starts and
 // ends: the aligned 16 bytes that hold them are loaded, all of which hold an element of
