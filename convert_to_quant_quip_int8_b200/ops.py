@@ -873,6 +873,8 @@ def _quantized_out(shape: tuple, mode: int, dev) -> Tuple[torch.Tensor, torch.Te
     assert mode == L.QI8_Q_TOKEN or n % 128 == 0, \
         f"Last dimension size must be divisible by block_size (block_size=128), got {n}"
     s = torch.empty(*shape[:-1], 1 if mode == L.QI8_Q_TOKEN else n // 128, dtype=torch.float32, device=dev)
+    if n == 0:
+        s.fill_(1e-30)  # rows of no columns: the least scale, and no kernel to write it
     return torch.empty(shape, dtype=torch.int8, device=dev), s
 
 

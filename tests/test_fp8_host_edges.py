@@ -52,3 +52,13 @@ def test_metadata_keeps_the_block_size():
         size = algo.get("group_size", 128)
         meta = CQ.tensor_to_dict(CQ.create_comfy_quant_tensor(name, block_size=size))
         assert meta == ({"format": name, "group_size": size} if "group_size" in algo else {"format": name})
+
+
+def test_rows_of_no_columns_have_the_least_scale(monkeypatch):
+    monkeypatch.setattr(ops, "_one_device", lambda *t: torch.device("cpu"))  # nothing is launched
+    torch.full((3 * 5,), 7.0)  # memory that a fresh tensor may get
+    x = torch.empty(3, 5, 0, dtype=BF)
+    for got in (FQ.rms_norm_quant(x, output="int8"), FQ.gated_act_quant(x, x, output="int8")):
+        assert got[0].shape == x.shape and got[1].shape == (3, 5, 1) and (got[1] == torch.tensor(1e-30)).all()
+    for output in ("fp8", "int8_block"):
+        assert FQ.gated_act_quant(x, x, output=output)[1].shape == (3, 5, 0)
