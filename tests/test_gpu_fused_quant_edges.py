@@ -8,6 +8,7 @@ import torch
 from convert_to_quant_quip_int8_b200 import _lib as L
 from convert_to_quant_quip_int8_b200 import ops
 from convert_to_quant_quip_int8_b200.comfy import fused_quant_kernels as FQ
+from convert_to_quant_quip_int8_b200.comfy.quant_ops import QuantizedTensor
 from test_gpu_fused_quant import check_codes, exact_gated, randn
 
 pytestmark = pytest.mark.gpu
@@ -123,3 +124,20 @@ def test_gelu_of_gates_of_one_size(output, dtype, sign):
     x = g.double().abs()
     h = 0.5 * torch.special.erfc(x / math.sqrt(2))
     check_codes(q, s, y, 2.0 ** -24 * ((32 + 2 * x * x) * x * h * u.double().abs() + 2 * y.abs()), output)
+
+
+# ------------------------------------------------- outputs into int8 layouts
+@pytest.mark.parametrize("rows", [1, 130])
+def test_block_outputs_go_into_linear_layers(rows):
+    x, w = randn(rows, 512, dtype=BF), randn(256, 512, seed=1, scale=0.05, dtype=BF)
+    bias = randn(256, seed=2, dtype=BF)
+    for layout, output in (("BlockWiseINT8Layout", "int8_block"), ("BlockWiseFP8Layout", "fp8")):
+        wq = QuantizedTensor.from_float(w, layout, is_weight=True)
+        q, s = FQ.rms_norm_quant(x, output=output)
+        a = QuantizedTensor(q, layout, {"scale": s, "block_size": 128, "is_weight": False, "orig_dtype": x.dtype})
+        y = torch.nn.functional.linear(a, wq, bias)
+        va, vw = a.dequantize().double(), wq.dequantize().double()
+        # a and w are rounded to bf16 where they are read back, y once; the sums are fp32
+        total = va.abs() @ vw.abs().T + bias.double().abs()
+        assert y.dtype == BF
+        assert ((y.double() - va @ vw.T - bias.double()).abs() <= (3 * 2.0 ** -8 + 2.0 ** -14) * total).all()
