@@ -718,9 +718,10 @@ def _code_rows(q: torch.Tensor) -> Tuple[torch.Tensor, int]:
 
 
 def aligned_codes(q: torch.Tensor) -> torch.Tensor:
-    """``q`` [N, K] with rows that start on 16-byte boundaries, as the quantizers return them: itself, or a copy."""
-    if q.numel() == 0 or ((q.shape[1] == 1 or q.stride(1) == 1) and q.storage_offset() % 16 == 0
-                          and (q.shape[0] == 1 or q.stride(0) % 16 == 0)):
+    """``q`` [..., K] with rows that start on 16-byte boundaries, as the quantizers return them: itself, or a copy."""
+    steps = (step for size, step in zip(q.shape[:-1], q.stride()) if size != 1)
+    if q.numel() == 0 or ((q.shape[-1] == 1 or q.stride(-1) == 1) and q.storage_offset() % 16 == 0
+                          and all(step % 16 == 0 for step in steps)):
         return q
     return _new_codes(q.shape, q.dtype, q.device).copy_(q)
 

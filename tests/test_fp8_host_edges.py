@@ -34,6 +34,9 @@ def test_codes_get_rows_of_whole_16_bytes():
             if a.numel():
                 assert a.storage_offset() % 16 == 0 and (a.shape[0] == 1 or a.stride(0) % 16 == 0)
             assert ops.aligned_codes(a) is a
+    for v in (q[0], q.view(7, 2, 20), q.view(7, 1, 40)[:, :, :7], q[0, 3:]):  # no weights, but no error here either
+        t = v.view(torch.float8_e4m3fn)
+        assert torch.equal(ops.aligned_codes(t).view(torch.uint8), v)
     whole = torch.zeros(3, 48, dtype=torch.uint8).view(torch.float8_e4m3fn)
     assert ops.aligned_codes(whole) is whole
     assert ops.aligned_codes(whole[:, :33]).data_ptr() == whole.data_ptr()
